@@ -351,6 +351,111 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
                   int32_t* token, void* workspace, size_t workspace_bytes, int dtype,
                   void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged KV cache.  No counterpart in the reference, whose cache is one array per
+ * layer (smollm2_triton/model.py:190-225); positions and arithmetic are those
+ * of tl_rope_kv_append and tl_attention_decode above.
+ * A layer's K (and V) is a pool of n_pages pages (n_kv_head, page_size, d_k),
+ * given by {page, head, row} element strides; page_size is a power of two from
+ * 16 to 1024.  page_table is (batch, max_pages) int32: position t of sequence b
+ * lies in page page_table[b][t / page_size], row t % page_size.  An entry
+ * outside [0, n_pages) names no page: nothing is written to its positions, and
+ * they are hidden from every query.  max_pages * page_size fits in int32 (in
+ * 2^30 for tl_paged_attention_prefill).
+ *
+ * tl_paged_kv_append: token s < n_new of sequence b (s < new_lens[b] where new_lens
+ * is not NULL) goes to position cache_lens[b] + s: k_new and v_new into the pages,
+ * q to q_out (the same layout and address: in place; otherwise the two may not
+ * overlap; q NULL: none), q and k after rotary positions.  cos / sin tables are
+ * (rope_rows, rotary / 2) fp32; the first `rotary` (even) features of a head are
+ * turned in pairs (i, i + rotary / 2), or (2 i, 2 i + 1) where interleaved != 0; the
+ * rest are copied.  cos NULL: no positions.  A token past the table of pages,
+ * past rope_rows, or without a page writes nothing, its q_out row included.
+ * Sequences that share a page may not append to it in one call.
+ * Strides: q, q_out, k_new, v_new {batch, seq, head}; any even d_k.
+ *
+ * tl_paged_attention_decode: one query per sequence, q / o (batch, n_head, d_k)
+ * {batch, head}, over L = min(cache_lens[b] + len_add, max_pages * page_size)
+ * positions; with window > 0 it sees only the last `window` of them and the first
+ * `sinks`.  A sequence that sees nothing gives zeros.  Hidden positions are not
+ * read.  Two launches; the workspace (tl_paged_decode_workspace_bytes, 16-byte
+ * aligned) holds partial results and needs no initialisation.  d_k 64 or 128,
+ * rows aligned to d_k / 16 elements.
+ *
+ * tl_paged_attention_prefill: n_new queries per sequence (new_lens[b] where it is
+ * not NULL; rows behind them are left as they were), query i at position
+ * cache_lens[b] + i, over the pages (their own positions appended before), with
+ * the same window.  q / o (batch, n_new, n_head, d_k) {batch, head, seq}.
+ * tl_window_attention: the same over K / V (batch, n_kv_head, seq_k, d_k)
+ * {batch, head, seq}, query i at position seq_k - seq_q + i.
+ * Both: window = 0 is plain causal attention; a row that sees no key gives zeros;
+ * d_k 64 or 128, rows of q, k and v 16-byte aligned; o may not overlap q, k or v.
+ * A NaN or infinity in a V row makes NaN of the rows that are computed in one
+ * tile with it, seen or not, as a product with a zero weight does.
+ *
+ * tl_copy_pages: page host_dst[i] = page host_src[i], i < count, in every cache of
+ * the list (page_bytes bytes at page_stride_bytes * page of each base, all three
+ * multiples of 16).  The lists are host memory and travel with the launch: they may be
+ * released at once, and a captured graph keeps them.  A page that is a destination
+ * twice, or a source and a destination, ends up with either content.
+ * tl_write_i32: dst[host_index[i]] = host_value[i] on the device, by value likewise
+ * (page table entries, lengths); an index twice: either value.
+ * ------------------------------------------------------------------------- */
+int tl_paged_kv_append(const void* q, void* q_out, const void* k_new, const void* v_new,
+                       void* k_pages, void* v_pages, const int32_t* page_table, int max_pages,
+                       int n_pages, int page_size, const int32_t* cache_lens,
+                       const int32_t* new_lens, const float* cos_table, const float* sin_table,
+                       int rope_rows, int rotary, int interleaved, int batch, int n_new,
+                       int n_head, int n_kv_head, int d_k, const int64_t* q_strides,
+                       const int64_t* q_out_strides, const int64_t* k_new_strides,
+                       const int64_t* v_new_strides, const int64_t* k_page_strides,
+                       const int64_t* v_page_strides, int dtype, void* stream);
+size_t tl_paged_decode_workspace_bytes(int n_head, int n_kv_head, int d_k);
+int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_pages,
+                              const int32_t* page_table, int max_pages, int n_pages,
+                              int page_size, const int32_t* cache_lens, int len_add, int window,
+                              int sinks, void* o, void* workspace, size_t workspace_bytes,
+                              int batch, int n_head, int n_kv_head, int d_k,
+                              const int64_t* q_strides, const int64_t* k_page_strides,
+                              const int64_t* v_page_strides, const int64_t* o_strides,
+                              float sm_scale, int dtype, void* stream);
+int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v_pages,
+                               const int32_t* page_table, int max_pages, int n_pages,
+                               int page_size, const int32_t* cache_lens, const int32_t* new_lens,
+                               void* o, int batch, int n_new, int n_head, int n_kv_head, int d_k,
+                               const int64_t* q_strides, const int64_t* k_page_strides,
+                               const int64_t* v_page_strides, const int64_t* o_strides,
+                               float sm_scale, int window, int sinks, int dtype, void* stream);
+int tl_window_attention(const void* q, const void* k, const void* v, void* o, int batch,
+                        int n_head, int n_kv_head, int seq_q, int seq_k, int d_k,
+                        const int64_t* q_strides, const int64_t* k_strides,
+                        const int64_t* v_strides, const int64_t* o_strides, float sm_scale,
+                        int window, int sinks, int dtype, void* stream);
+int tl_copy_pages(void* const* caches, int n_caches, int64_t page_bytes,
+                  int64_t page_stride_bytes, int n_pages, const int32_t* host_src,
+                  const int32_t* host_dst, int count, void* stream);
+int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
+                 const int32_t* host_value, int count, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search's selection.  No counterpart in the reference (it samples:
+ * smollm2_triton/model.py:566-584).  logits (batch * beams, vocab) with
+ * row_stride >= vocab, scores (batch, beams) fp32: of every batch item's
+ * beams * vocab continuations, scored scores[b][j] + log softmax(logits[b, j])[v] (ordered
+ * in 64 bits, written in 32), the `select` best, best first, ties to the lowest
+ * j * vocab + v: score, parent beam j and token v, each (batch, select).
+ * A logit of -inf is no continuation; nor is any of a beam whose score is not
+ * finite or whose logits hold NaN, +inf or only -inf.  Where fewer are left the rest get
+ * -inf, -1, -1.  beams <= 64, select <= tl_beam_max_select() (64), vocab <= 262144,
+ * batch * beams <= 65535.  The workspace (16-byte aligned) needs no initialisation.
+ * ------------------------------------------------------------------------- */
+int tl_beam_max_select(void);
+size_t tl_beam_select_workspace_bytes(int batch, int beams, int vocab);
+int tl_beam_select(const void* logits, const float* scores, int batch, int beams, int vocab,
+                   int64_t row_stride, int select, float* out_scores, int32_t* out_parents,
+                   int32_t* out_tokens, void* workspace, size_t workspace_bytes, int dtype,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

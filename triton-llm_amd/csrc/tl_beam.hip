@@ -1,0 +1,367 @@
+// Beam search's selection: of the J V continuations of every batch item's J beams the n best,
+//   score(j, v) = s_j + x_jv - log sum_u exp x_ju,
+// best first, ties to the lowest j V + v.  The reference has no beam search; it stands beside
+// the sampler that replaces its _sample (smollm2_triton/model.py:566-584).
+//
+// Scores are ordered in 64 bits: neighbours of different beams may differ by less than a 32-bit step of
+// their size.  x - max and exp are 32-bit (the argument of exp2 carried in two words, so that its
+// rounding does not grow with the distance from the maximum), their sum 64.
+//
+// Bytes: every logit is read once, by beam_scan, a workgroup a segment of a row, which leaves
+//   * the segment's maximum and its sum of exp against it;
+//   * the maximum of every group of 64 entries.
+// beam_finish, a workgroup a batch item, has everything else from those.  A group's best score is
+// base_j + its maximum, base_j = s_j - log-sum-exp.  The groups are dealt to 64 classes; the n-th largest
+// of the classes' best (n <= 64) is a bound that n continuations reach, so only groups that reach it are
+// read again, and their entries that reach it are the candidates: about n for scattered
+// scores.  A candidate's rank is the number of better ones.  Where the candidates outgrow their place
+// (thousands of ties, a row in descending order) every wave walks its groups in order instead and
+// keeps its 64 best in its lanes; those are the candidates then.
+#include "tl_common.h"
+
+#include <limits.h>
+#include <math.h>
+
+namespace {
+
+constexpr int kST = 256;                 // threads of beam_scan
+constexpr int kPer = 8;                  // entries of a thread
+constexpr int kSeg = kST * kPer;         // entries of a segment
+constexpr int kGrp = 64;                 // entries of a group: 8 threads
+constexpr int kFT = 1024;                // threads of beam_finish
+constexpr int kFW = kFT / 64;
+constexpr int kMaxVocab = 262144;
+constexpr int kMaxBeams = 64;
+constexpr int kMaxSelect = 64;
+constexpr int kMaxCand = 3072;           // candidates in LDS
+constexpr int kMaxList = 2048;           // groups that are read again
+
+struct BeamParams {
+  const void* logits;
+  int64_t row_stride;
+  const float* scores;
+  int batch, beams, vocab, select;
+  int n_seg, n_grp;
+  float* gmax;    // [rows][n_grp]
+  float* smax;    // [rows][n_seg]
+  double* ssum;   // [rows][n_seg]
+  float* out_scores;
+  int32_t* out_parents;
+  int32_t* out_tokens;
+};
+
+// Rows of odd length start anywhere: these loads ask for an element's alignment only.
+typedef uint32_t words16 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t words32 __attribute__((ext_vector_type(4), aligned(4)));
+
+size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
+
+// exp(x - m) for x <= m; 0 where it is under the smallest 32-bit number, NaN for NaN.
+__device__ __forceinline__ float exp_below(float x, float m) {
+  constexpr float kL = 1.44269504f, kLlo = 1.92596303e-8f;  // log2 e in two words
+  const float d = x - m;
+  const float hi = d * kL;
+  const float lo = fmaf(d, kL, -hi) + d * kLlo;
+  const float e = fast_exp2(hi);
+  return d < -110.f ? 0.f : fmaf(e * 0.693147181f, lo, e);
+}
+
+__device__ __forceinline__ double shfl_xor_d(double x, int off) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t a = __shfl_xor((uint32_t)u, off), b = __shfl_xor((uint32_t)(u >> 32), off);
+  return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
+}
+__device__ __forceinline__ double shfl_d(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t a = __shfl((uint32_t)u, lane), b = __shfl((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kST) void beam_scan_kernel(BeamParams p) {
+  using B = typename T::bits;
+  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x;
+  const B* x = (const B*)p.logits + (int64_t)row * p.row_stride;
+  const int i0 = seg * kSeg + tid * kPer;
+  float v[kPer];
+  if (i0 + kPer <= p.vocab) {
+    if constexpr (T::size == 2) {
+      const words16 w = *(const words16*)(x + i0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    } else {
+      const words32 a = *(const words32*)(x + i0), b = *(const words32*)(x + i0 + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = __uint_as_float(a[i]);
+        v[4 + i] = __uint_as_float(b[i]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = i0 + i < p.vocab ? to_f32<T>(x[i0 + i]) : -INFINITY;
+  }
+  float m = v[0];
+#pragma unroll
+  for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
+#pragma unroll
+  for (int off = 1; off < 8; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+  if ((tid & 7) == 0 && i0 < p.vocab) p.gmax[(int64_t)row * p.n_grp + i0 / kGrp] = m;
+#pragma unroll
+  for (int off = 8; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+  __shared__ float s_m[kST / 64];
+  __shared__ double s_s[kST / 64];
+  if ((tid & 63) == 0) s_m[tid >> 6] = m;
+  __syncthreads();
+  m = s_m[0];
+#pragma unroll
+  for (int w = 1; w < kST / 64; ++w) m = fmaxf(m, s_m[w]);
+  // a segment of -inf alone has no mass; NaN in it comes through the maximum as -inf
+  const float base = m == -INFINITY ? 0.f : m;
+  float e = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) e += exp_below(v[i], base);
+  double s = e;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
+  if ((tid & 63) == 0) s_s[tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) {
+#pragma unroll
+    for (int w = 1; w < kST / 64; ++w) s += s_s[w];
+    p.smax[(int64_t)row * p.n_seg + seg] = m;
+    p.ssum[(int64_t)row * p.n_seg + seg] = s;
+  }
+}
+
+struct Cand {
+  double v;
+  int i;  // j V + v
+};
+__device__ __forceinline__ bool better(double va, int ia, double vb, int ib) {
+  return va > vb || (va == vb && ia < ib);
+}
+
+// One step of a bitonic network: lanes a distance `off` apart, the better of the two to the lower
+// lane where `down`.
+__device__ __forceinline__ void exchange(Cand& c, int lane, int off, bool down) {
+  const double v = shfl_xor_d(c.v, off);
+  const int i = __shfl_xor(c.i, off);
+  const bool lower = (lane & off) == 0;
+  const bool mine = better(c.v, c.i, v, i);
+  if (mine != (lower == down)) c.v = v, c.i = i;
+}
+__device__ __forceinline__ void sort64(Cand& c, int lane) {  // best in lane 0
+  for (int size = 2; size <= 64; size <<= 1)
+    for (int off = size >> 1; off > 0; off >>= 1) exchange(c, lane, off, (lane & size) == 0);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
+  using B = typename T::bits;
+  const int item = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int J = p.beams, n = p.select;
+  __shared__ double s_base[kMaxBeams];
+  __shared__ double s_best[kFT];
+  __shared__ double s_bound;
+  __shared__ int s_n_list, s_n_cand;
+  __shared__ int s_list[kMaxList];
+  __shared__ double s_cv[kMaxCand];
+  __shared__ int s_ci[kMaxCand];
+
+  if (tid == 0) s_n_list = s_n_cand = 0;
+  // base_j = s_j - log-sum-exp of the row; -inf where either has no value, and such a beam has no
+  // continuations
+  for (int j = wave; j < J; j += kFW) {
+    const int64_t row = (int64_t)item * J + j;
+    const float* sm = p.smax + row * p.n_seg;
+    const double* ss = p.ssum + row * p.n_seg;
+    float m = -INFINITY;
+    for (int i = lane; i < p.n_seg; i += 64) m = fmaxf(m, sm[i]);
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+    double s = 0.;
+    for (int i = lane; i < p.n_seg; i += 64) {
+      const double part = ss[i];
+      s += sm[i] == -INFINITY ? part : part * exp((double)sm[i] - (double)m);  // (a NaN's sum comes through)
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
+    if (lane == 0) {
+      const double base = (double)p.scores[row] - ((double)m + log(s));
+      s_base[j] = base > -INFINITY && base < INFINITY ? base : -INFINITY;
+    }
+  }
+  __syncthreads();
+
+  // the bound: n-th best of the 64 classes' best
+  const int groups = J * p.n_grp;  // row-major over (beam, group)
+  const float* gmax = p.gmax + (int64_t)item * groups;
+  auto group_best = [&](int g) { return s_base[g / p.n_grp] + (double)gmax[g]; };
+  double best = -INFINITY;
+  for (int g = tid; g < groups; g += kFT) best = fmax(best, group_best(g));
+  s_best[tid] = best;
+  __syncthreads();
+  if (wave == 0) {
+    Cand c{-INFINITY, lane};
+    for (int w = 0; w < kFW; ++w) c.v = fmax(c.v, s_best[w * 64 + lane]);
+    sort64(c, lane);
+    const double bound = shfl_d(c.v, n - 1);
+    if (lane == 0) s_bound = bound;
+  }
+  __syncthreads();
+  const double bound = s_bound;
+
+  auto entry = [&](int g, double& v, int& i) {  // this lane's entry of group g
+    const int j = g / p.n_grp, at = (g - j * p.n_grp) * kGrp + lane;
+    v = -INFINITY;
+    i = INT_MAX;
+    if (at < p.vocab) {
+      v = s_base[j] + (double)to_f32<T>(((const B*)p.logits)[((int64_t)item * J + j) * p.row_stride + at]);
+      i = j * p.vocab + at;
+    }
+  };
+  for (int g = tid; g < groups; g += kFT) {
+    const double v = group_best(g);
+    if (v >= bound && v > -INFINITY) {
+      const int at = atomicAdd(&s_n_list, 1);
+      if (at < kMaxList) s_list[at] = g;
+    }
+  }
+  __syncthreads();
+  const int n_list = s_n_list;
+  if (n_list <= kMaxList) {
+    for (int w = wave; w < n_list; w += kFW) {
+      double v;
+      int i;
+      entry(s_list[w], v, i);
+      if (v >= bound && v > -INFINITY) {
+        const int at = atomicAdd(&s_n_cand, 1);
+        if (at < kMaxCand) s_cv[at] = v, s_ci[at] = i;
+      }
+    }
+  }
+  __syncthreads();
+  int n_cand = s_n_cand;
+  if (n_list > kMaxList || n_cand > kMaxCand) {
+    __syncthreads();
+    if (tid == 0) s_n_cand = 0;
+    __syncthreads();
+    Cand kept{-INFINITY, INT_MAX};  // this wave's 64 best so far, best in lane 0
+    for (int g = wave; g < groups; g += kFW) {
+      const double gv = group_best(g);
+      const double worst = shfl_d(kept.v, 63);
+      if (!(gv >= bound && gv > -INFINITY && gv >= worst)) continue;
+      Cand c;
+      entry(g, c.v, c.i);
+      if (!(c.v > -INFINITY)) c.v = -INFINITY, c.i = INT_MAX;
+      const int wi = __shfl(kept.i, 63);
+      if (!__any(better(c.v, c.i, worst, wi))) continue;
+      sort64(c, lane);
+      // the better of i-th best and (63 - i)-th best are the 64 best of both, in a bitonic order
+      const double rv = shfl_d(c.v, 63 - lane);
+      const int ri = __shfl(c.i, 63 - lane);
+      if (better(rv, ri, kept.v, kept.i)) kept.v = rv, kept.i = ri;
+      for (int off = 32; off > 0; off >>= 1) exchange(kept, lane, off, true);
+    }
+    if (kept.v > -INFINITY) {
+      const int at = atomicAdd(&s_n_cand, 1);
+      s_cv[at] = kept.v, s_ci[at] = kept.i;  // at most 16 waves of 64
+    }
+    __syncthreads();
+    n_cand = s_n_cand;
+  }
+  static_assert(kMaxCand >= kFW * 64, "every wave's best fit");
+
+  const int64_t o = (int64_t)item * n;
+  for (int c = tid; c < n_cand; c += kFT) {
+    const double v = s_cv[c];
+    const int i = s_ci[c];
+    int rank = 0;
+    for (int k = 0; k < n_cand; ++k) rank += better(s_cv[k], s_ci[k], v, i) ? 1 : 0;
+    if (rank < n) {
+      p.out_scores[o + rank] = (float)v;
+      p.out_parents[o + rank] = i / p.vocab;
+      p.out_tokens[o + rank] = i - i / p.vocab * p.vocab;
+    }
+  }
+  // fewer continuations than asked for
+  for (int r = n_cand + tid; r < n; r += kFT) {
+    p.out_scores[o + r] = -INFINITY;
+    p.out_parents[o + r] = -1;
+    p.out_tokens[o + r] = -1;
+  }
+}
+
+int n_segments(int vocab) { return (vocab + kSeg - 1) / kSeg; }
+int n_groups(int vocab) { return (vocab + kGrp - 1) / kGrp; }
+
+size_t ws_layout(int64_t rows, int vocab, char* base, BeamParams* p) {
+  const size_t R = (size_t)rows, S = (size_t)n_segments(vocab), G = (size_t)n_groups(vocab);
+  const size_t gb = align256(R * G * 4), mb = align256(R * S * 4), sb = align256(R * S * 8);
+  if (p) {
+    p->gmax = (float*)base;
+    p->smax = (float*)(base + gb);
+    p->ssum = (double*)(base + gb + mb);
+  }
+  return gb + mb + sb;
+}
+
+template <typename T>
+int launch_beam(const BeamParams& p, hipStream_t st) {
+  hipLaunchKernelGGL(beam_scan_kernel<T>, dim3(p.n_seg, p.batch * p.beams), dim3(kST), 0, st, p);
+  const int e = tl_launch_status();
+  if (e) return e;
+  hipLaunchKernelGGL(beam_finish_kernel<T>, dim3(p.batch), dim3(kFT), 0, st, p);
+  return tl_launch_status();
+}
+
+bool beam_sizes_ok(int batch, int beams, int vocab, int select) {
+  return batch > 0 && beams > 0 && beams <= kMaxBeams && (int64_t)batch * beams <= 65535 && vocab > 0 &&
+         vocab <= kMaxVocab && select > 0 && select <= kMaxSelect;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tl_beam_max_select(void) { return kMaxSelect; }
+
+size_t tl_beam_select_workspace_bytes(int batch, int beams, int vocab) {
+  if (!beam_sizes_ok(batch, beams, vocab, 1)) return 0;
+  return ws_layout((int64_t)batch * beams, vocab, nullptr, nullptr);
+}
+
+int tl_beam_select(const void* logits, const float* scores, int batch, int beams, int vocab, int64_t row_stride,
+                   int select, float* out_scores, int32_t* out_parents, int32_t* out_tokens, void* workspace,
+                   size_t workspace_bytes, int dtype, void* stream) {
+  if (batch == 0 || select == 0) return 0;
+  if (!logits || !scores || !out_scores || !out_parents || !out_tokens || !workspace || batch < 0 || beams < 1 ||
+      vocab < 1 || select < 0 || row_stride < vocab || ((uintptr_t)workspace & 15))
+    return TL_ERR_INVALID;
+  if (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16) return TL_ERR_INVALID;
+  if (!beam_sizes_ok(batch, beams, vocab, select)) return TL_ERR_UNSUPPORTED;
+  if (workspace_bytes < tl_beam_select_workspace_bytes(batch, beams, vocab)) return TL_ERR_INVALID;
+  BeamParams p{};
+  p.logits = logits;
+  p.row_stride = row_stride;
+  p.scores = scores;
+  p.batch = batch;
+  p.beams = beams;
+  p.vocab = vocab;
+  p.select = select;
+  p.n_seg = n_segments(vocab);
+  p.n_grp = n_groups(vocab);
+  ws_layout((int64_t)batch * beams, vocab, (char*)workspace, &p);
+  p.out_scores = out_scores;
+  p.out_parents = out_parents;
+  p.out_tokens = out_tokens;
+  hipStream_t st = tl_resolve_stream(stream);
+  switch (dtype) {
+    case TL_DTYPE_F32: return launch_beam<F32>(p, st);
+    case TL_DTYPE_F16: return launch_beam<F16>(p, st);
+    default: return launch_beam<BF16>(p, st);
+  }
+}
+
+}  // extern "C"

@@ -1,0 +1,815 @@
+// The paged KV cache: what writes it (paged_append), reads it for one new token a
+// sequence (paged_decode, paged_combine) and copies its pages (copy_pages).
+//
+// The reference keeps one contiguous cache per sequence on the host
+// (smollm2_triton/model.py:190-225) and has no pages; positions, RoPE and attention
+// semantics are those of rope_kv_append and attention_decode here.
+#include "tl_paged.h"
+
+#include <math.h>
+
+using namespace tlpg;
+
+namespace {
+
+// ---------------------------------------------------------------------------------
+// Append: rotary positions on q and k, k and v into the pages.
+//
+//   half         (x_i, x_{i + r/2}) -> (x_i c - x_{i + r/2} s, x_{i + r/2} c + x_i s)
+//   interleaved  (x_{2i}, x_{2i+1}) likewise;   i < r / 2, r rotated features of d_k
+//
+// with c, s the tables' entry i of row `position`.  Products and sums are rounded one by
+// one in fp32 and once to the storage type (as rope_kv_append's are, whose bits this gives).
+// Bytes only: every row is read and written once.
+// ---------------------------------------------------------------------------------
+enum { kNoRope = 0, kHalf = 1, kInterleaved = 2 };
+
+struct AppendParams {
+  const void* q;
+  void* qo;
+  const void* kn;
+  const void* vn;
+  void* kp;
+  void* vp;
+  PageMap pm;
+  const int32_t* lens;
+  const int32_t* new_lens;  // NULL: n_new for every sequence
+  const float* cos_t;
+  const float* sin_t;
+  int rope_rows, rot_half;
+  int batch, n_new, n_head, n_kv, d_k;
+  int64_t q_sb, q_ss, q_sh;
+  int64_t qo_sb, qo_ss, qo_sh;
+  int64_t kn_sb, kn_ss, kn_sh;
+  int64_t vn_sb, vn_ss, vn_sh;
+  int64_t kp_sp, kp_sh, kp_sr;
+  int64_t vp_sp, vp_sh, vp_sr;
+};
+
+// Where token s of sequence b goes; false: it is not written (see the header).
+__device__ __forceinline__ bool token_place(const AppendParams& p, int b, int s, bool rope, int& pos, int& page) {
+  if (p.new_lens && s >= p.new_lens[b]) return false;
+  const int64_t at = (int64_t)p.lens[b] + s;
+  if (at < 0 || (at >> p.pm.shift) >= p.pm.max_pages || (rope && at >= p.rope_rows)) return false;
+  pos = (int)at;
+  page = p.pm.table[(int64_t)b * p.pm.max_pages + (pos >> p.pm.shift)];
+  return (unsigned)page < (unsigned)p.pm.n_pages;
+}
+
+// Row r of token (b, s) -- its n_head q rows, then n_kv k rows, then n_kv v rows -- as
+// source and destination addresses.
+template <typename B>
+__device__ __forceinline__ void token_row(const AppendParams& p, int b, int s, int pos, int page, int r, const B*& src,
+                                          B*& dst) {
+  const int row = pos & ((1 << p.pm.shift) - 1);
+  if (r < p.n_head) {
+    src = (const B*)p.q + b * p.q_sb + s * p.q_ss + r * p.q_sh;
+    dst = (B*)p.qo + b * p.qo_sb + s * p.qo_ss + r * p.qo_sh;
+  } else if (r < p.n_head + p.n_kv) {
+    const int h = r - p.n_head;
+    src = (const B*)p.kn + b * p.kn_sb + s * p.kn_ss + h * p.kn_sh;
+    dst = (B*)p.kp + page * p.kp_sp + h * p.kp_sh + row * p.kp_sr;
+  } else {
+    const int h = r - p.n_head - p.n_kv;
+    src = (const B*)p.vn + b * p.vn_sb + s * p.vn_ss + h * p.vn_sh;
+    dst = (B*)p.vp + page * p.vp_sp + h * p.vp_sh + row * p.vp_sr;
+  }
+}
+
+// One element pair a thread: any even d_k, any strides.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
+  using B = typename T::bits;
+  const int pairs = p.d_k / 2, rows = p.n_head + 2 * p.n_kv;
+  const int64_t tid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (tid >= (int64_t)p.batch * p.n_new * rows * pairs) return;
+  const int i = (int)(tid % pairs);
+  const int64_t t = tid / pairs;
+  const int r = (int)(t % rows);
+  const int64_t tok = t / rows;
+  const int b = (int)(tok / p.n_new), s = (int)(tok % p.n_new);
+  int pos, page;
+  if (!token_place(p, b, s, MODE != kNoRope, pos, page)) return;
+  const B* src;
+  B* dst;
+  token_row(p, b, s, pos, page, r, src, dst);
+  int x = 2 * i, y = 2 * i + 1;
+  if (MODE == kHalf && i < p.rot_half) x = i, y = i + p.rot_half;
+  const B sx = src[x], sy = src[y];
+  if (MODE != kNoRope && i < p.rot_half && r < p.n_head + p.n_kv) {
+    const int64_t at = (int64_t)pos * p.rot_half + i;
+    float ox, oy;
+    rope_rotate_pair(to_f32<T>(sx), to_f32<T>(sy), p.cos_t[at], p.sin_t[at], ox, oy);
+    dst[x] = from_f32<T>(ox);
+    dst[y] = from_f32<T>(oy);
+  } else {
+    dst[x] = sx;
+    dst[y] = sy;
+  }
+}
+
+template <typename T>
+int launch_append(const AppendParams& p, int mode, hipStream_t st) {
+  const int64_t total = (int64_t)p.batch * p.n_new * (p.n_head + 2 * p.n_kv) * (p.d_k / 2);
+  const int64_t blocks = (total + 255) / 256;
+  if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)blocks), block(256);
+  if (mode == kHalf) hipLaunchKernelGGL((paged_append_kernel<T, kHalf>), grid, block, 0, st, p);
+  else if (mode == kInterleaved) hipLaunchKernelGGL((paged_append_kernel<T, kInterleaved>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((paged_append_kernel<T, kNoRope>), grid, block, 0, st, p);
+  return tl_launch_status();
+}
+
+// ---------------------------------------------------------------------------------
+// One new token a sequence over its pages: o = softmax(scale q . K^T over the keys it
+// sees) V, the softmax's running maximum m and sum l kept in fp32 (log2 domain):
+//   m' = max(m, s),  l' = l 2^(m - m') + 2^(s - m'),  acc' = acc 2^(m - m') + 2^(s - m') v
+// and two states joined as (max m, sum l_i 2^(m_i - m), sum acc_i 2^(m_i - m)).
+//
+// Work.  The blocks of 16 positions that a sequence's query sees (all of them, or a
+// window's and the sinks') are laid end to end, (sequence, pair, block), a pair being one KV head with up to
+// 8 of its query heads, and cut into equal shares, a workgroup each, whatever the lengths.
+// A share may end inside a pair and go on in the next; each piece is a segment.  A pair inside one
+// share is finished there; else each segment leaves (m, l, acc) in the workspace, and
+// paged_combine joins them.  A share has at most one segment of a pair that began before it
+// (slot 0) and one of a pair that goes on after it (slot 1), so the workspace is two
+// slots a workgroup, whatever batch and length are.
+// ---------------------------------------------------------------------------------
+constexpr int kDecThreads = 256;
+constexpr int kDecWaves = kDecThreads / 64;
+constexpr int kMaxShares = 2048;  // workgroups at most: bounds the workspace
+constexpr int kMinShare = 4;      // blocks of a share at least: one for each wave
+constexpr float kRescaleLog2 = 8.f;
+constexpr int kAuxNontemporal = 2;  // buffer-load cache policy: nt
+constexpr uint32_t kPastEnd = 0x7FFFFF00u;  // an offset that every resource here ends before
+
+struct DecodeParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  const int32_t* lens;
+  PageMap pm;
+  float* ws_ml;   // [share][2][heads_per_pair][2]
+  float* ws_acc;  // [share][2][heads_per_pair][D]
+  void* o;
+  int len_add, window, sinks;
+  int batch, n_head, n_kv, group;
+  int heads_per_pair, n_pairs, n_shares;
+  int64_t q_sb, q_sh, o_sb, o_sh;
+  int64_t k_sp, k_sh, v_sp, v_sh;     // page and head strides in elements
+  uint32_t k_row_bytes, v_row_bytes;  // row strides in bytes
+  float scale_log2;
+};
+
+// What sequence b's query sees: len positions, `lo` the window's first; n blocks, the
+// first ns of them from the sequence's start on, the others from block wb on.
+struct Seen {
+  int len, lo, n, ns, wb;
+};
+__device__ __forceinline__ Seen seen_of(const DecodeParams& p, int b) {
+  Seen s;
+  int64_t len = (int64_t)p.lens[b] + p.len_add;
+  const int64_t cap = (int64_t)p.pm.max_pages << p.pm.shift;
+  len = len < 0 ? 0 : len > cap ? cap : len;
+  s.len = (int)len;
+  const int nb = (int)((len + kBlk - 1) >> kBlkShift);
+  s.lo = p.window > 0 && s.len > p.window ? s.len - p.window : 0;
+  s.ns = s.n = nb;
+  s.wb = 0;
+  if (s.lo > 0) {
+    const int sb = min(nb, (int)(((int64_t)p.sinks + kBlk - 1) >> kBlkShift));
+    const int wb = s.lo >> kBlkShift;
+    if (wb > sb) {
+      s.ns = sb;
+      s.wb = wb;
+      s.n = sb + nb - wb;
+    }
+  }
+  return s;
+}
+
+__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d);
+    if (lane >= d) x += y;
+  }
+  return x;
+}
+
+// Blocks of every pair of sequences [0, b) and of all sequences.
+__device__ __forceinline__ void blocks_before(const DecodeParams& p, int b, int lane, int64_t& before, int64_t& total) {
+  int64_t t = 0, u = 0;
+  for (int i = lane; i < p.batch; i += 64) {
+    const int64_t n = seen_of(p, i).n;
+    t += n;
+    u += i < b ? n : 0;
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    t += __shfl_xor(t, off);
+    u += __shfl_xor(u, off);
+  }
+  total = uni(t) * p.n_pairs;
+  before = uni(u) * p.n_pairs;
+}
+
+// Blocks of a share: an even part, whole rounds of the waves.
+__device__ __forceinline__ int64_t share_blocks(const DecodeParams& p, int64_t total) {
+  int64_t r = (total + p.n_shares - 1) / p.n_shares;
+  r = r < kMinShare ? kMinShare : r;
+  return (r + kDecWaves - 1) / kDecWaves * kDecWaves;
+}
+
+// The sequence that owns row r of the flattened blocks (r < total), and its first row.
+__device__ __forceinline__ int owner_of(const DecodeParams& p, int64_t r, int lane, int64_t& start) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const int64_t n = b0 + lane < p.batch ? (int64_t)seen_of(p, b0 + lane).n * p.n_pairs : 0;
+    const int64_t incl = base + wave_scan(n, lane);
+    const uint64_t hit = __ballot(incl > r);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      start = uni(__shfl(incl - n, l));
+      return uni(b0 + l);
+    }
+    base = uni(__shfl(incl, 63));
+  }
+  start = base;
+  return p.batch - 1;  // not reached for r < total
+}
+
+template <int W>
+struct Slice {
+  uint32_t w[W];
+};
+
+template <int W>
+__device__ __forceinline__ void load_slice(Slice<W>& s, __amdgpu_buffer_rsrc_t r, uint32_t voff) {
+  if constexpr (W == 2) {
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, voff, 0, kAuxNontemporal));
+    s.w[0] = a.x;
+    s.w[1] = a.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const u32x4 a =
+          __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff + 16 * i, 0, kAuxNontemporal));
+      s.w[4 * i + 0] = a.x;
+      s.w[4 * i + 1] = a.y;
+      s.w[4 * i + 2] = a.z;
+      s.w[4 * i + 3] = a.w;
+    }
+  }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ float dot_slice(const Slice<W>& q, const Slice<W>& k) {
+  float d = 0.f;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (T::code == TL_DTYPE_BF16)
+      d = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, q.w[i]), __builtin_bit_cast(bf16x2, k.w[i]), d,
+                                          false);
+    else if constexpr (T::code == TL_DTYPE_F16)
+      d = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, q.w[i]), __builtin_bit_cast(f16x2, k.w[i]), d, false);
+    else
+      d = fmaf(__uint_as_float(q.w[i]), __uint_as_float(k.w[i]), d);
+  }
+  return d;
+}
+
+// Buffer resource of one block of 16 rows, from wave-uniform values.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const char* base, uint32_t bytes) {
+  const int64_t a = uni((int64_t)(uintptr_t)base);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)a, (short)0, (int)bytes, kBufRsrcWord3);
+}
+
+// 16 lanes read a row, a wave 4 rows a load and a block of 16 positions in 4; wave w takes
+// blocks w, w + 4, ... of the segment.
+template <typename T, int D, int G>
+__global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams p) {
+  constexpr int EPL = D / 16;           // elements of a lane's slice of a row
+  constexpr int W = EPL * T::size / 4;  // its 32-bit words
+  constexpr int U = 4;                  // rows of a block that a lane reads
+  constexpr int NW = kDecWaves;
+  using B = typename T::bits;
+  const int lane = threadIdx.x & 63;
+  const int wave = uni((int)threadIdx.x >> 6);
+  const int sub = lane & 15, rowg = lane >> 4;
+  const int n_chunks = p.n_pairs / p.n_kv;
+  __shared__ float s_m[NW][G], s_l[NW][G];
+  __shared__ float s_acc[NW][G][D];
+  const uint32_t lane_bytes = sub * (EPL * T::size);
+
+  // Blocks [v0, v1) of the Seen blocks of pair `pair` of sequence b.
+  auto segment = [&](const int b, const Seen& sn, const int pair, const int v0, const int v1, const bool whole,
+                     const int slot) {
+    const int hkv = pair / n_chunks;
+    const int hq0 = hkv * p.group + (pair - hkv * n_chunks) * G;
+    const int n_g = min(G, hkv * p.group + p.group - hq0);
+    Slice<W> qs[G];
+    float m[G], l[G], acc[G][EPL];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint32_t* src =
+          (const uint32_t*)((const B*)p.q + b * p.q_sb + (int64_t)min(hq0 + g, hq0 + n_g - 1) * p.q_sh + sub * EPL);
+#pragma unroll
+      for (int i = 0; i < W; ++i) qs[g].w[i] = g < n_g ? src[i] : 0u;
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) acc[g][e] = 0.f;
+    }
+    const int32_t* row = p.pm.table + (int64_t)b * p.pm.max_pages;
+    const int shift = p.pm.shift;
+    auto block_at = [&](int v) { return v < sn.ns ? v : v - sn.ns + sn.wb; };
+
+    int pages = 0;  // lane i: the page of this wave's block (it & ~63) + i
+    int it = 0;
+    for (int v = v0 + wave; v < v1; v += NW, ++it) {
+      if ((it & 63) == 0) {
+        const int mine = v + NW * lane;
+        pages = mine < v1 ? row[block_at(mine) >> (shift - kBlkShift)] : -1;
+      }
+      const int page = __builtin_amdgcn_readlane(pages, it & 63);
+      const bool there = (unsigned)page < (unsigned)p.pm.n_pages;
+      const int pos0 = block_at(v) << kBlkShift;
+      const int in_page = pos0 & ((1 << shift) - 1);
+      const int64_t id = there ? page : 0;
+      const auto krs = block_rsrc((const char*)p.k + (id * p.k_sp + hkv * p.k_sh) * T::size + (int64_t)in_page * p.k_row_bytes,
+                                  there ? 15 * p.k_row_bytes + D * T::size : 0);
+      const auto vrs = block_rsrc((const char*)p.v + (id * p.v_sp + hkv * p.v_sh) * T::size + (int64_t)in_page * p.v_row_bytes,
+                                  there ? 15 * p.v_row_bytes + D * T::size : 0);
+      Slice<W> kr[U], vr[U];
+      bool seen[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = 4 * u + rowg;
+        const int pos = pos0 + r;
+        // hidden rows may hold anything (NaN among it): they are not read, and read as zeros
+        seen[u] = there && pos < sn.len && (pos >= sn.lo || pos < p.sinks);
+        load_slice(kr[u], krs, seen[u] ? r * p.k_row_bytes + lane_bytes : kPastEnd);
+        load_slice(vr[u], vrs, seen[u] ? r * p.v_row_bytes + lane_bytes : kPastEnd);
+      }
+      float s[G][U];
+      bool grow = false;
+      float mb[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float d = row16_sum(dot_slice<T>(qs[g], kr[u])) * p.scale_log2;
+          s[g][u] = seen[u] ? d : -INFINITY;
+        }
+        mb[g] = fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3]));
+        grow |= mb[g] > m[g] + kRescaleLog2;
+      }
+      // the maximum moves only when a score passes it by 2^8 (it only bounds the exponents)
+      if (__any(grow)) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float mn = fmaxf(m[g], mb[g]);
+          const float a = fast_exp2(m[g] - (mn == -INFINITY ? 0.f : mn));
+          m[g] = mn;
+          l[g] *= a;
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[g][e] *= a;
+        }
+      }
+      float pu[G][U];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float base = m[g] == -INFINITY ? 0.f : m[g];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          pu[g][u] = fast_exp2(s[g][u] - base);
+          l[g] += pu[g][u];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float vf[EPL];
+        if constexpr (T::size == 4) {
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) vf[i] = __uint_as_float(vr[u].w[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < W; ++i) unpack2<T>(vr[u].w[i], vf[2 * i], vf[2 * i + 1]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int e = 0; e < EPL; ++e) acc[g][e] = fmaf(pu[g][u], vf[e], acc[g][e]);
+      }
+    }
+
+    // join the wave's four rows of a load, then the waves
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float m2 = __shfl_xor(m[g], off), l2 = __shfl_xor(l[g], off);
+        const float mn = fmaxf(m[g], m2);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float w1 = fast_exp2(m[g] - base), w2 = fast_exp2(m2 - base);
+        m[g] = mn;
+        l[g] = l[g] * w1 + l2 * w2;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) acc[g][e] = acc[g][e] * w1 + __shfl_xor(acc[g][e], off) * w2;
+      }
+    }
+    __syncthreads();  // the last segment's sums have been read
+    if (lane < 16) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (lane == 0) {
+          s_m[wave][g] = m[g];
+          s_l[wave][g] = l[g];
+        }
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) s_acc[wave][g][sub * EPL + e] = acc[g][e];
+      }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < n_g * D; idx += kDecThreads) {
+      const int g = idx / D, d = idx - g * D;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w][g]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float a = 0.f, ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float wt = fast_exp2(s_m[w][g] - base);
+        a += s_acc[w][g][d] * wt;
+        ls += s_l[w][g] * wt;
+      }
+      if (whole) {
+        ((B*)p.o)[b * p.o_sb + (int64_t)(hq0 + g) * p.o_sh + d] = from_f32<T>(ls == 0.f ? 0.f : a / ls);
+      } else {
+        const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * G + g;
+        p.ws_acc[at * D + d] = a;
+        if (d == 0) {
+          p.ws_ml[at * 2] = mx;
+          p.ws_ml[at * 2 + 1] = ls;
+        }
+      }
+    }
+  };
+
+  int64_t before, total;
+  blocks_before(p, 0, lane, before, total);
+  const int64_t rpb = uni(share_blocks(p, total));
+  const int64_t r0 = (int64_t)blockIdx.x * rpb;
+  if (r0 >= total) return;
+  const int64_t r1 = r0 + rpb < total ? r0 + rpb : total;
+  for (int64_t r = r0; r < r1;) {
+    int64_t seq0;
+    const int b = owner_of(p, r, lane, seq0);
+    Seen sn = seen_of(p, b);
+    const int pair = uni((int)((r - seq0) / sn.n));
+    const int64_t pair0 = seq0 + (int64_t)pair * sn.n;
+    const int v0 = (int)(r - pair0);
+    const int v1 = (int)((r1 - pair0) < sn.n ? (r1 - pair0) : sn.n);
+    segment(b, sn, pair, v0, v1, v0 == 0 && v1 == sn.n, v0 == 0 ? 1 : 0);
+    r = pair0 + v1;
+  }
+}
+
+// One wave a (sequence, query head): join the shares of its pair.  A pair inside one share
+// is finished already; a sequence that sees nothing gets zeros here.
+template <typename T, int D>
+__global__ __launch_bounds__(64) void paged_combine_kernel(DecodeParams p) {
+  constexpr int NJ = D / 64;
+  using B = typename T::bits;
+  const int hq = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
+  const Seen sn = seen_of(p, b);
+  B* o = (B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh;
+  if (sn.n == 0) {
+    for (int d = lane; d < D; d += 64) o[d] = 0;
+    return;
+  }
+  int64_t before, total;
+  blocks_before(p, b, lane, before, total);
+  const int64_t rpb = share_blocks(p, total);
+  const int hkv = hq / p.group, in = hq - hkv * p.group;
+  const int pair = hkv * (p.n_pairs / p.n_kv) + in / p.heads_per_pair;
+  const int g = in % p.heads_per_pair;
+  const int64_t pair0 = before + (int64_t)pair * sn.n;
+  const int64_t first = pair0 / rpb;
+  const int parts = (int)((pair0 + sn.n - 1) / rpb - first) + 1;
+  if (parts == 1) return;
+  auto at = [&](int s) { return ((first + s) * 2 + (s == 0 ? 1 : 0)) * p.heads_per_pair + g; };
+  float mx = -INFINITY;
+  for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, p.ws_ml[at(s) * 2]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float ls = 0.f, a[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) a[j] = 0.f;
+  for (int s = 0; s < parts; ++s) {
+    const int64_t i = at(s);
+    const float w = fast_exp2(p.ws_ml[i * 2] - base);
+    ls += p.ws_ml[i * 2 + 1] * w;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) a[j] = fmaf(p.ws_acc[i * D + lane + 64 * j], w, a[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = from_f32<T>(ls == 0.f ? 0.f : a[j] / ls);
+}
+
+// Blocks that one sequence's query can see at most.
+int64_t most_blocks(int64_t cap, int window, int sinks) {
+  int64_t n = (cap + kBlk - 1) / kBlk;
+  if (window > 0) {
+    const int64_t w = (int64_t)window / kBlk + 2 + ((int64_t)sinks + kBlk - 1) / kBlk;
+    n = n < w ? n : w;
+  }
+  return n;
+}
+
+int heads_per_pair(int n_head, int n_kv) { return n_head / n_kv < 8 ? n_head / n_kv : 8; }
+
+size_t ws_ml_bytes(int hpp) { return (size_t)kMaxShares * 2 * hpp * 2 * sizeof(float); }
+
+template <typename T, int D, int G>
+int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
+  static int per_cu = 0;
+  if (per_cu == 0) {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_decode_kernel<T, D, G>, kDecThreads, 0) != hipSuccess ||
+        n <= 0)
+      n = 1;
+    per_cu = n;
+  }
+  int64_t shares = (int64_t)per_cu * tl_device_cus();
+  shares = shares < kMaxShares ? shares : kMaxShares;
+  const int64_t full = (most + kMinShare - 1) / kMinShare;
+  p.n_shares = (int)(shares < full ? shares : full);
+  hipLaunchKernelGGL((paged_decode_kernel<T, D, G>), dim3(p.n_shares), dim3(kDecThreads), 0, st, p);
+  const int e = tl_launch_status();
+  if (e) return e;
+  hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(p.n_head, p.batch), dim3(64), 0, st, p);
+  return tl_launch_status();
+}
+
+template <typename T, int D>
+int launch_decode_d(DecodeParams& p, int64_t most, hipStream_t st) {
+  switch (p.heads_per_pair) {
+    case 1: return launch_decode_g<T, D, 1>(p, most, st);
+    case 2: return launch_decode_g<T, D, 2>(p, most, st);
+    case 3: return launch_decode_g<T, D, 3>(p, most, st);
+    case 4: return launch_decode_g<T, D, 4>(p, most, st);
+    case 5: return launch_decode_g<T, D, 5>(p, most, st);
+    case 6: return launch_decode_g<T, D, 6>(p, most, st);
+    case 7: return launch_decode_g<T, D, 7>(p, most, st);
+    default: return launch_decode_g<T, D, 8>(p, most, st);
+  }
+}
+
+template <typename T>
+int launch_decode(DecodeParams& p, int d_k, int64_t most, hipStream_t st) {
+  return d_k == 64 ? launch_decode_d<T, 64>(p, most, st) : launch_decode_d<T, 128>(p, most, st);
+}
+
+// ---------------------------------------------------------------------------------
+// Page copies.  Bases and pairs ride in the kernel's argument: no upload, and a captured
+// graph keeps them.  They are read from the argument segment with scalar loads (an index into
+// the by-value argument would copy the arrays into registers).
+// ---------------------------------------------------------------------------------
+constexpr int kCopyBases = 64, kCopyPairs = 256;
+constexpr int kCopyBytes = 16384;  // of a page, a workgroup
+
+struct CopyParams {
+  uint64_t base[kCopyBases];
+  int2 pair[kCopyPairs];  // (source, destination)
+  int64_t page_stride;    // bytes
+  int page_bytes, n_pairs, pieces;
+};
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(CopyParams p) {
+  typedef const __attribute__((address_space(4))) char* kchar;
+  typedef const __attribute__((address_space(4))) uint64_t* ku64;
+  const kchar args = (kchar)__builtin_amdgcn_kernarg_segment_ptr();
+  const int piece = blockIdx.x, pair = blockIdx.y, cache = blockIdx.z;
+  const uint64_t base = *(ku64)(args + offsetof(CopyParams, base) + 8 * cache);
+  const uint64_t sd = *(ku64)(args + offsetof(CopyParams, pair) + 8 * pair);
+  const int src = (int)(uint32_t)sd, dst = (int)(uint32_t)(sd >> 32);
+  const int lo = piece * kCopyBytes, hi = min(p.page_bytes, lo + kCopyBytes);
+  const char* s = (const char*)base + src * p.page_stride;
+  char* d = (char*)base + dst * p.page_stride;
+  for (int i = lo + threadIdx.x * 16; i < hi; i += 256 * 16) *(u32x4*)(d + i) = *(const u32x4*)(s + i);
+}
+
+// Entries of an int32 array on the device, by value.
+struct WriteParams {
+  int2 at[kCopyPairs];  // (index, value)
+  int32_t* dst;
+  int n;
+};
+
+__global__ __launch_bounds__(256) void write_i32_kernel(WriteParams p) {
+  typedef const __attribute__((address_space(4))) char* kchar;
+  typedef const __attribute__((address_space(4))) int* kint;
+  const kchar args = (kchar)__builtin_amdgcn_kernarg_segment_ptr();
+  if ((int)threadIdx.x >= p.n) return;
+  const kint at = (kint)(args + offsetof(WriteParams, at) + 8 * threadIdx.x);
+  p.dst[at[0]] = at[1];
+}
+
+bool known_dtype(int dtype) { return dtype == TL_DTYPE_F32 || dtype == TL_DTYPE_F16 || dtype == TL_DTYPE_BF16; }
+
+// Bytes from a tensor's first element to behind its last, outer dims (n, stride) in elements.
+size_t span_bytes(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t inner, int esize) {
+  return (size_t)((n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + inner) * esize;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tl_paged_kv_append(const void* q, void* q_out, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                       const int32_t* page_table, int max_pages, int n_pages, int page_size,
+                       const int32_t* cache_lens, const int32_t* new_lens, const float* cos_table,
+                       const float* sin_table, int rope_rows, int rotary, int interleaved, int batch, int n_new,
+                       int n_head, int n_kv_head, int d_k, const int64_t* q_strides, const int64_t* q_out_strides,
+                       const int64_t* k_new_strides, const int64_t* v_new_strides, const int64_t* k_page_strides,
+                       const int64_t* v_page_strides, int dtype, void* stream) {
+  if (batch == 0 || n_new == 0) return 0;
+  if (!k_new || !v_new || !k_pages || !v_pages || !page_table || !cache_lens || batch < 0 || n_new < 0 || n_head < 0 ||
+      n_kv_head < 1 || d_k < 2 || (d_k & 1) || max_pages < 1 || n_pages < 1 || !k_new_strides || !v_new_strides ||
+      !k_page_strides || !v_page_strides || !known_dtype(dtype))
+    return TL_ERR_INVALID;
+  const int shift = page_shift(page_size);
+  if (shift < 0 || ((int64_t)max_pages << shift) > INT32_MAX) return TL_ERR_INVALID;
+  if ((cos_table == nullptr) != (sin_table == nullptr)) return TL_ERR_INVALID;
+  if (cos_table && (rope_rows < 0 || rotary < 2 || (rotary & 1) || rotary > d_k)) return TL_ERR_INVALID;
+  const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
+  AppendParams p{};
+  if (q && n_head > 0) {
+    if (!q_out || !q_strides || !q_out_strides) return TL_ERR_INVALID;
+    if (q == q_out) {
+      for (int i = 0; i < 3; ++i)
+        if (q_strides[i] != q_out_strides[i]) return TL_ERR_INVALID;
+    } else if (tl_overlap(q, span_bytes(batch, q_strides[0], n_new, q_strides[1], n_head, q_strides[2], d_k, esize),
+                          q_out, span_bytes(batch, q_out_strides[0], n_new, q_out_strides[1], n_head, q_out_strides[2],
+                                            d_k, esize))) {
+      return TL_ERR_INVALID;
+    }
+    p.n_head = cos_table || q != q_out ? n_head : 0;  // nothing to do in place without positions
+    p.q = q;
+    p.qo = q_out;
+    p.q_sb = q_strides[0], p.q_ss = q_strides[1], p.q_sh = q_strides[2];
+    p.qo_sb = q_out_strides[0], p.qo_ss = q_out_strides[1], p.qo_sh = q_out_strides[2];
+  }
+  p.kn = k_new;
+  p.vn = v_new;
+  p.kp = k_pages;
+  p.vp = v_pages;
+  p.pm = PageMap{page_table, max_pages, n_pages, shift};
+  p.lens = cache_lens;
+  p.new_lens = new_lens;
+  p.cos_t = cos_table;
+  p.sin_t = sin_table;
+  p.rope_rows = rope_rows;
+  p.rot_half = cos_table ? rotary / 2 : 0;
+  p.batch = batch;
+  p.n_new = n_new;
+  p.n_kv = n_kv_head;
+  p.d_k = d_k;
+  p.kn_sb = k_new_strides[0], p.kn_ss = k_new_strides[1], p.kn_sh = k_new_strides[2];
+  p.vn_sb = v_new_strides[0], p.vn_ss = v_new_strides[1], p.vn_sh = v_new_strides[2];
+  p.kp_sp = k_page_strides[0], p.kp_sh = k_page_strides[1], p.kp_sr = k_page_strides[2];
+  p.vp_sp = v_page_strides[0], p.vp_sh = v_page_strides[1], p.vp_sr = v_page_strides[2];
+  const int mode = !cos_table ? kNoRope : interleaved ? kInterleaved : kHalf;
+  hipStream_t st = tl_resolve_stream(stream);
+  switch (dtype) {
+    case TL_DTYPE_F32: return launch_append<F32>(p, mode, st);
+    case TL_DTYPE_F16: return launch_append<F16>(p, mode, st);
+    default: return launch_append<BF16>(p, mode, st);
+  }
+}
+
+size_t tl_paged_decode_workspace_bytes(int n_head, int n_kv_head, int d_k) {
+  if (n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head || d_k <= 0) return 0;
+  const int hpp = heads_per_pair(n_head, n_kv_head);
+  return ws_ml_bytes(hpp) + (size_t)kMaxShares * 2 * hpp * d_k * sizeof(float);
+}
+
+int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                              int max_pages, int n_pages, int page_size, const int32_t* cache_lens, int len_add,
+                              int window, int sinks, void* o, void* workspace, size_t workspace_bytes, int batch,
+                              int n_head, int n_kv_head, int d_k, const int64_t* q_strides,
+                              const int64_t* k_page_strides, const int64_t* v_page_strides, const int64_t* o_strides,
+                              float sm_scale, int dtype, void* stream) {
+  if (batch == 0 || n_head == 0) return 0;
+  if (!q || !k_pages || !v_pages || !page_table || !cache_lens || !o || !workspace || batch < 0 || n_head < 0 ||
+      n_kv_head < 1 || n_head % n_kv_head || max_pages < 1 || n_pages < 1 || window < 0 || sinks < 0 || !q_strides ||
+      !k_page_strides || !v_page_strides || !o_strides || !known_dtype(dtype) || ((uintptr_t)workspace & 15))
+    return TL_ERR_INVALID;
+  const int shift = page_shift(page_size);
+  const int64_t cap = (int64_t)max_pages << (shift < 0 ? 0 : shift);
+  if (shift < 0 || cap > INT32_MAX) return TL_ERR_INVALID;
+  if (d_k != 64 && d_k != 128) return TL_ERR_UNSUPPORTED;
+  if (batch > 65535) return TL_ERR_UNSUPPORTED;  // the combine's grid
+  if (workspace_bytes < tl_paged_decode_workspace_bytes(n_head, n_kv_head, d_k)) return TL_ERR_INVALID;
+  // a lane reads d_k / 16 elements of a row in 8- or 16-byte words, a block of 16 rows with 32-bit offsets
+  const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
+  const int64_t slice = d_k / 16;
+  const int64_t strides[] = {q_strides[0], q_strides[1], k_page_strides[0], k_page_strides[1], k_page_strides[2],
+                             v_page_strides[0], v_page_strides[1], v_page_strides[2]};
+  for (int64_t s : strides)
+    if (s < 0 || s % slice) return TL_ERR_UNSUPPORTED;
+  if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % (uintptr_t)(slice * esize)) return TL_ERR_UNSUPPORTED;
+  if (k_page_strides[2] > (1 << 24) || v_page_strides[2] > (1 << 24)) return TL_ERR_UNSUPPORTED;
+  DecodeParams p{};
+  p.q = q;
+  p.k = k_pages;
+  p.v = v_pages;
+  p.lens = cache_lens;
+  p.pm = PageMap{page_table, max_pages, n_pages, shift};
+  p.o = o;
+  p.len_add = len_add;
+  p.window = window;
+  p.sinks = sinks;
+  p.batch = batch;
+  p.n_head = n_head;
+  p.n_kv = n_kv_head;
+  p.group = n_head / n_kv_head;
+  p.heads_per_pair = heads_per_pair(n_head, n_kv_head);
+  p.n_pairs = n_kv_head * ((p.group + p.heads_per_pair - 1) / p.heads_per_pair);
+  p.ws_ml = (float*)workspace;
+  p.ws_acc = (float*)((char*)workspace + ws_ml_bytes(p.heads_per_pair));
+  p.q_sb = q_strides[0], p.q_sh = q_strides[1];
+  p.o_sb = o_strides[0], p.o_sh = o_strides[1];
+  p.k_sp = k_page_strides[0], p.k_sh = k_page_strides[1];
+  p.v_sp = v_page_strides[0], p.v_sh = v_page_strides[1];
+  p.k_row_bytes = (uint32_t)(k_page_strides[2] * esize);
+  p.v_row_bytes = (uint32_t)(v_page_strides[2] * esize);
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  const int64_t most = most_blocks(cap, window, sinks) * batch * p.n_pairs;
+  hipStream_t st = tl_resolve_stream(stream);
+  switch (dtype) {
+    case TL_DTYPE_F32: return launch_decode<F32>(p, d_k, most, st);
+    case TL_DTYPE_F16: return launch_decode<F16>(p, d_k, most, st);
+    default: return launch_decode<BF16>(p, d_k, most, st);
+  }
+}
+
+int tl_copy_pages(void* const* caches, int n_caches, int64_t page_bytes, int64_t page_stride_bytes, int n_pages,
+                  const int32_t* host_src, const int32_t* host_dst, int count, void* stream) {
+  if (n_caches == 0 || count == 0) return 0;
+  if (!caches || !host_src || !host_dst || n_caches < 0 || count < 0 || n_pages < 1 || page_bytes < 16 ||
+      page_bytes % 16 || page_bytes > INT32_MAX || page_stride_bytes < page_bytes || page_stride_bytes % 16)
+    return TL_ERR_INVALID;
+  for (int c = 0; c < n_caches; ++c)
+    if (!caches[c] || ((uintptr_t)caches[c] & 15)) return TL_ERR_INVALID;
+  for (int i = 0; i < count; ++i)
+    if (host_src[i] < 0 || host_src[i] >= n_pages || host_dst[i] < 0 || host_dst[i] >= n_pages) return TL_ERR_INVALID;
+  hipStream_t st = tl_resolve_stream(stream);
+  CopyParams p;
+  p.page_stride = page_stride_bytes;
+  p.page_bytes = (int)page_bytes;
+  p.pieces = (int)((page_bytes + kCopyBytes - 1) / kCopyBytes);
+  for (int c0 = 0; c0 < n_caches; c0 += kCopyBases) {
+    const int nc = n_caches - c0 < kCopyBases ? n_caches - c0 : kCopyBases;
+    for (int c = 0; c < kCopyBases; ++c) p.base[c] = (uint64_t)(uintptr_t)caches[c0 + (c < nc ? c : 0)];
+    for (int i0 = 0; i0 < count; i0 += kCopyPairs) {
+      p.n_pairs = count - i0 < kCopyPairs ? count - i0 : kCopyPairs;
+      for (int i = 0; i < kCopyPairs; ++i) {
+        const int j = i0 + (i < p.n_pairs ? i : 0);
+        p.pair[i] = make_int2(host_src[j], host_dst[j]);
+      }
+      hipLaunchKernelGGL(copy_pages_kernel, dim3(p.pieces, p.n_pairs, nc), dim3(256), 0, st, p);
+      const int e = tl_launch_status();
+      if (e) return e;
+    }
+  }
+  return 0;
+}
+
+int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index, const int32_t* host_value, int count,
+                 void* stream) {
+  if (count == 0) return 0;
+  if (!dst || !host_index || !host_value || count < 0) return TL_ERR_INVALID;
+  for (int i = 0; i < count; ++i)
+    if (host_index[i] < 0 || host_index[i] >= dst_count) return TL_ERR_INVALID;
+  hipStream_t st = tl_resolve_stream(stream);
+  WriteParams p;
+  p.dst = dst;
+  for (int i0 = 0; i0 < count; i0 += kCopyPairs) {
+    p.n = count - i0 < kCopyPairs ? count - i0 : kCopyPairs;
+    for (int i = 0; i < kCopyPairs; ++i) {
+      const int j = i0 + (i < p.n ? i : 0);
+      p.at[i] = make_int2(host_index[j], host_value[j]);
+    }
+    hipLaunchKernelGGL(write_i32_kernel, dim3(1), dim3(256), 0, st, p);
+    const int e = tl_launch_status();
+    if (e) return e;
+  }
+  return 0;
+}
+
+}  // extern "C"

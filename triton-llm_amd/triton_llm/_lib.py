@@ -25,6 +25,7 @@ _c_size = ctypes.c_size_t
 _c_float = ctypes.c_float
 _vp = ctypes.c_void_p
 _i64p = ctypes.POINTER(ctypes.c_int64)
+_i32p = ctypes.POINTER(ctypes.c_int32)
 
 # name -> (restype, argtypes).  Kept in the order of include/triton_llm_hip.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -111,6 +112,38 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tl_sample_workspace_bytes": (_c_size, [_c_int, _c_int]),
     "tl_sample": (_c_int, [_vp, _c_int, _c_int, _c_i64, _c_float, _c_int, _vp, _vp, _vp, _c_size, _c_int, _vp]),
     "tl_sample_row": (_c_int, [_vp, _c_int, _c_float, _c_int, ctypes.c_double, _vp, _vp, _c_size, _c_int, _vp]),
+    "tl_paged_kv_append": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp,
+         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _c_int, _vp],
+    ),
+    "tl_paged_decode_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "tl_paged_attention_decode": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _c_int, _vp, _vp, _c_size,
+         _c_int, _c_int, _c_int, _c_int,
+         _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _vp],
+    ),
+    "tl_paged_attention_prefill": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp,
+         _c_int, _c_int, _c_int, _c_int, _c_int,
+         _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
+    ),
+    "tl_window_attention": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
+    ),
+    "tl_copy_pages": (
+        _c_int, [ctypes.POINTER(_vp), _c_int, _c_i64, _c_i64, _c_int, _i32p, _i32p, _c_int, _vp]),
+    "tl_write_i32": (_c_int, [_vp, _c_i64, _i32p, _i32p, _c_int, _vp]),
+    "tl_beam_max_select": (_c_int, []),
+    "tl_beam_select_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "tl_beam_select": (
+        _c_int,
+        [_vp, _vp, _c_int, _c_int, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_size, _c_int, _vp]),
 }
 
 _lib: ctypes.CDLL | None = None

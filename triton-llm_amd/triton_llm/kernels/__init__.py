@@ -6,7 +6,9 @@ ziliangpeng/triton-llm: ``attention``, ``attention_gqa``, ``precompute_cos_sin``
 (flash prefill, KV-cache append, split-K decode) and the model step's other
 layers: the projection ``gemm``, ``rms_norm`` (plus the fused
 ``add_rms_norm``), ``swiglu`` and ``add``, and on-device next-token
-``sample`` / ``sample_rows`` (the models' ``_sample``).  The reference's gelu,
+``sample`` / ``sample_rows`` (the models' ``_sample``).  Serving many sequences
+adds the cache in pages (append, attention, page copies), attention through a
+sliding window, and beam search's selection.  The reference's gelu,
 layer_norm, softmax and embedding kernels (GPT-2 and host-side pieces) are
 outside this library's scope.
 """
@@ -27,6 +29,17 @@ from .decode import (
     decode_workspace,
     rope_kv_append,
 )
+from .paged import (
+    allocate_kv_pages,
+    copy_kv_pages,
+    paged_attention_decode,
+    paged_attention_prefill,
+    paged_decode_workspace,
+    paged_kv_append,
+    write_i32,
+)
+from .window import window_attention, window_attention_strided
+from .beam import beam_select
 
 __all__ = [
     "attention",
@@ -49,4 +62,14 @@ __all__ = [
     "add",
     "sample",
     "sample_rows",
+    "allocate_kv_pages",
+    "paged_kv_append",
+    "paged_attention_decode",
+    "paged_decode_workspace",
+    "paged_attention_prefill",
+    "copy_kv_pages",
+    "write_i32",
+    "window_attention",
+    "window_attention_strided",
+    "beam_select",
 ]

@@ -1,0 +1,57 @@
+"""Causal attention through a sliding window with sinks (additive API).
+
+``window_attention`` is :func:`~triton_llm.kernels.flash.flash_attention` with a
+bounded view: a query at position p sees the keys ``p - window < j <= p`` and the first
+``sinks`` keys of the sequence; ``window = 0`` sees every ``j <= p``.  Positions are
+bottom-right aligned, query i at ``seq_k - seq_q + i`` (attention_gqa.py:97 of the
+reference, which has no windows); a query before position 0 sees nothing and gives
+zeros.  Keys outside of every row's view are not read.
+
+:func:`~triton_llm.kernels.paged.paged_attention_prefill` is the same over a cache in pages.
+"""
+
+from __future__ import annotations
+
+from triton_llm import _lib, gpu
+from ._common import contiguous_strides, default_scale, launch, same_dtype, vp
+from .paged import check_window
+
+
+def window_attention_strided(q, k, v, out, *, batch, n_head, n_kv_head, seq_q, seq_k, d_k, q_strides, k_strides,
+                             v_strides, o_strides, window, sinks=0, sm_scale=None):
+    """The kernel on raw layouts given by {batch, head, seq} element strides."""
+    if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head:
+        raise ValueError(f"n_head ({n_head}) must be a positive multiple of n_kv_head ({n_kv_head})")
+    if d_k not in (64, 128):
+        raise ValueError(f"window attention supports d_k in (64, 128), got {d_k}")
+    check_window(window, sinks)
+    code = same_dtype(q, k, v, out)
+    if batch == 0 or seq_q == 0:
+        return out
+    if seq_k == 0:
+        raise ValueError("seq_k must be >= 1")
+    if sm_scale is None:
+        sm_scale = default_scale(d_k)
+    launch(gpu.runtime().tl_window_attention, vp(q), vp(k), vp(v), vp(out), batch, n_head, n_kv_head, seq_q, seq_k,
+           d_k, _lib.strides(*q_strides), _lib.strides(*k_strides), _lib.strides(*v_strides),
+           _lib.strides(*o_strides), float(sm_scale), int(window), int(sinks), code, None, what="window_attention")
+    return out
+
+
+def window_attention(q, k, v, window: int, sinks: int = 0, sm_scale: float | None = None, out=None):
+    """q ``(batch, n_head, seq_q, d_k)``, k/v ``(batch, n_kv_head, seq_k, d_k)``, contiguous; returns out like q."""
+    if len(q.shape) != 4 or len(k.shape) != 4 or k.shape != v.shape:
+        raise ValueError(f"expected q (B,Hq,Sq,D) and k/v (B,Hkv,Sk,D), got {q.shape}, {k.shape}, {v.shape}")
+    batch, n_head, seq_q, d_k = q.shape
+    kb, n_kv, seq_k, kd = k.shape
+    if kb != batch or kd != d_k:
+        raise ValueError(f"q {q.shape} and k {k.shape} disagree on batch or d_k")
+    if out is None:
+        out = gpu.allocate(q.shape, q.dtype)
+    elif out.shape != q.shape:
+        raise ValueError(f"out shape {out.shape} != q shape {q.shape}")
+    qs = contiguous_strides(q.shape)[:3]
+    ks = contiguous_strides(k.shape)[:3]
+    return window_attention_strided(q, k, v, out, batch=batch, n_head=n_head, n_kv_head=n_kv, seq_q=seq_q,
+                                    seq_k=seq_k, d_k=d_k, q_strides=qs, k_strides=ks, v_strides=ks, o_strides=qs,
+                                    window=window, sinks=sinks, sm_scale=sm_scale)
