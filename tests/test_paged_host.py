@@ -256,3 +256,10 @@ def test_c_beam_refuses():
     ws = lib.tl_beam_select_workspace_bytes
     assert ws(0, 1, 10) == ws(1, 65, 10) == ws(1, 1, 0) == ws(1, 1, 300000) == 0
     assert ws(2, 4, 128256) >= 8 * 2004 * 4
+
+
+def test_beam_refuses_sizes_the_kernels_do_not_take():
+    for logits, scores, n in [((65, 10), (1, 65), 4), ((4, 300000), (1, 4), 4), ((4, 100), (1, 4), 65),
+                              ((80000, 10), (40000, 2), 4)]:
+        with pytest.raises(ValueError, match="is not supported"):
+            beam_select(fake(logits), fake(scores), n)

@@ -10,11 +10,12 @@ returned best first.  The sequences' states follow their parents by a change of 
 
 from __future__ import annotations
 
+import functools
 import math
 
 import numpy as np
 
-from triton_llm import gpu
+from triton_llm import _lib, gpu
 from ._common import launch, scratch, vp
 
 __all__ = ["beam_select", "max_select"]
@@ -22,7 +23,32 @@ __all__ = ["beam_select", "max_select"]
 
 def max_select() -> int:
     """Most continuations a call selects per batch item."""
-    return int(gpu.runtime().tl_beam_max_select())
+    return int(_lib.load().tl_beam_max_select())
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(scores, logits, n_select):
+    """(batch, beams, vocab, n_select, workspace bytes) of a call by its shapes."""
+    if len(scores) != 2:
+        raise ValueError(f"scores must be float32 (batch, beams), got {scores}")
+    batch, beams = scores
+    if len(logits) < 2 or logits[-1] <= 0:
+        raise ValueError(f"logits must be (batch * beams, vocab) with vocab > 0, got {logits}")
+    vocab = logits[-1]
+    if math.prod(logits[:-1]) != batch * beams:
+        raise ValueError(f"logits {logits} do not hold {batch} x {beams} rows")
+    n_select = 2 * beams if n_select is None else int(n_select)
+    if n_select < 0:
+        raise ValueError(f"n_select must be >= 0, got {n_select}")
+    need = 0
+    if batch and n_select:
+        lib = _lib.load()
+        need = lib.tl_beam_select_workspace_bytes(batch, beams, vocab)
+        if need == 0 or n_select > lib.tl_beam_max_select():
+            raise ValueError(f"selecting {n_select} of {batch} x {beams} rows of vocab {vocab} is not supported "
+                             f"(n_select <= {lib.tl_beam_max_select()}, beams <= 64, batch * beams <= 65535, "
+                             f"vocab <= 262144)")
+    return batch, beams, vocab, n_select, need
 
 
 def beam_select(logits_dev, scores_dev, n_select: int | None = None, out=None, workspace=None):
@@ -35,33 +61,18 @@ def beam_select(logits_dev, scores_dev, n_select: int | None = None, out=None, w
     +inf or nothing but -inf, has no continuations, and a logit of -inf is none;
     where fewer are left the rest are ``(-inf, -1, -1)``.  No synchronisation.
     """
-    if len(scores_dev.shape) != 2 or scores_dev.dtype != np.float32:
-        raise ValueError(f"scores must be float32 (batch, beams), got {gpu.dtype_name(scores_dev.dtype)} "
-                         f"{scores_dev.shape}")
-    batch, beams = scores_dev.shape
-    if len(logits_dev.shape) < 2 or logits_dev.shape[-1] <= 0:
-        raise ValueError(f"logits must be (batch * beams, vocab) with vocab > 0, got {logits_dev.shape}")
-    vocab = logits_dev.shape[-1]
-    if math.prod(logits_dev.shape[:-1]) != batch * beams:
-        raise ValueError(f"logits {logits_dev.shape} do not hold {batch} x {beams} rows")
+    if scores_dev.dtype.char != "f":
+        raise ValueError(f"scores must be float32 (batch, beams), got {gpu.dtype_name(scores_dev.dtype)}")
     code = gpu.dtype_code(logits_dev.dtype)
-    n_select = 2 * beams if n_select is None else int(n_select)
-    if n_select < 0:
-        raise ValueError(f"n_select must be >= 0, got {n_select}")
+    batch, beams, vocab, n_select, need = _plan(scores_dev.shape, logits_dev.shape, n_select)
     shape = (batch, n_select)
     if out is None:
         out = tuple(gpu.allocate(shape, t) for t in (np.float32, np.int32, np.int32))
-    elif (len(out) != 3 or any(tuple(o.shape) != shape for o in out)
-          or [gpu.dtype_name(o.dtype) for o in out] != ["float32", "int32", "int32"]):
+    elif len(out) != 3 or any(o.shape != shape or o.dtype.char != c for o, c in zip(out, "fii")):
         raise ValueError(f"out must be float32, int32 and int32 tensors of shape {shape}")
     if batch == 0 or n_select == 0:
         return out
-    lib = gpu.runtime()
-    need = lib.tl_beam_select_workspace_bytes(batch, beams, vocab)
-    if need == 0 or n_select > max_select():
-        raise ValueError(f"selecting {n_select} of {batch} x {beams} rows of vocab {vocab} is not supported "
-                         f"(n_select <= {max_select()}, beams <= 64, batch * beams <= 65535, vocab <= 262144)")
     ws = scratch(need, workspace, key="beam")
-    launch(lib.tl_beam_select, vp(logits_dev), vp(scores_dev), batch, beams, vocab, vocab, n_select, vp(out[0]),
-           vp(out[1]), vp(out[2]), vp(ws), ws.nbytes, code, None, what="beam_select")
+    launch(gpu.runtime().tl_beam_select, vp(logits_dev), vp(scores_dev), batch, beams, vocab, vocab, n_select,
+           vp(out[0]), vp(out[1]), vp(out[2]), vp(ws), ws.nbytes, code, None, what="beam_select")
     return out

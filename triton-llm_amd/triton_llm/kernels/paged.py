@@ -26,7 +26,9 @@ and the first ``sinks`` of the sequence; 0 means all up to its own.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+import operator
 
 import numpy as np
 
@@ -52,30 +54,40 @@ def allocate_kv_pages(n_pages: int, n_kv_head: int, page_size: int, d_k: int, dt
     return alloc(shape, dtype), alloc(shape, dtype)
 
 
-def _check_pool(k_pages, v_pages):
-    if len(k_pages.shape) != 4 or k_pages.shape != v_pages.shape:
+# The checks of shapes and what follows from them (strides as the C entries take them) are kept
+# per combination of shapes: a decode step of a serving loop comes with the same ones every time, and
+# putting them together costs more than the launch.  Types are checked in every call.
+
+def _is_int32(t) -> bool:
+    return t.dtype.char == "i"
+
+
+def _check_pool(k_shape, v_shape):
+    if len(k_shape) != 4 or k_shape != v_shape:
         raise ValueError(f"k_pages/v_pages must be matching 4-D (n_pages, n_kv_head, page_size, d_k), "
-                         f"got {k_pages.shape} and {v_pages.shape}")
-    if min(k_pages.shape) <= 0:
-        raise ValueError(f"pool dims must be positive, got {k_pages.shape}")
-    _check_page_size(k_pages.shape[2])
-    return k_pages.shape
+                         f"got {k_shape} and {v_shape}")
+    if min(k_shape) <= 0:
+        raise ValueError(f"pool dims must be positive, got {k_shape}")
+    _check_page_size(k_shape[2])
+    return k_shape
 
 
-def _check_table(page_table, cache_lens, page_size, most):
-    if gpu.dtype_name(page_table.dtype) != "int32" or len(page_table.shape) != 2 or page_table.shape[1] < 1:
-        raise ValueError(f"page_table must be int32 (batch, max_pages), got {gpu.dtype_name(page_table.dtype)} "
-                         f"{page_table.shape}")
-    batch, max_pages = page_table.shape
+def _check_table(table_shape, lens_shape, new_lens_shape, page_size, most):
+    if len(table_shape) != 2 or table_shape[1] < 1:
+        raise ValueError(f"page_table must be int32 (batch, max_pages), got {table_shape}")
+    batch, max_pages = table_shape
     if max_pages * page_size > most:
         raise ValueError(f"{max_pages} pages of {page_size} exceed {most} positions")
-    _check_lens("cache_lens", cache_lens, batch)
+    for name, shape in (("cache_lens", lens_shape), ("new_lens", new_lens_shape)):
+        if shape is not None and shape != (batch,):
+            raise ValueError(f"{name} must be int32 of shape ({batch},), got {shape}")
     return batch, max_pages
 
 
-def _check_lens(name, lens, batch):
-    if gpu.dtype_name(lens.dtype) != "int32" or tuple(lens.shape) != (batch,):
-        raise ValueError(f"{name} must be int32 of shape ({batch},), got {gpu.dtype_name(lens.dtype)} {lens.shape}")
+def _check_int32(page_table, cache_lens, new_lens=None):
+    for name, t in (("page_table", page_table), ("cache_lens", cache_lens), ("new_lens", new_lens)):
+        if t is not None and not _is_int32(t):
+            raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
 
 
 def _check_heads(n_head, n_kv_head, n_kv, d_k):
@@ -95,10 +107,48 @@ def check_window(window: int, sinks: int) -> None:
 def _same_output(out, q):
     if out is None:
         return gpu.allocate(q.shape, q.dtype)
-    if tuple(out.shape) != tuple(q.shape) or gpu.dtype_name(out.dtype) != gpu.dtype_name(q.dtype):
+    if out.shape != q.shape or (out.dtype is not q.dtype and gpu.dtype_name(out.dtype) != gpu.dtype_name(q.dtype)):
         raise ValueError(f"out must be like q, {q.shape} {gpu.dtype_name(q.dtype)}, got {out.shape} "
                          f"{gpu.dtype_name(out.dtype)}")
     return out
+
+
+def _shape(t):
+    return None if t is None else t.shape
+
+
+@functools.lru_cache(maxsize=1024)
+def _append_plan(pool, v_pool, table, lens, new_lens, k, v, q, cos, sin):
+    """Strides and sizes of an append by its shapes: the C entry's arguments in their order."""
+    n_pages, n_kv, page_size, d_k = _check_pool(pool, v_pool)
+    batch, max_pages = _check_table(table, lens, new_lens, page_size, (1 << 31) - 1)
+    if len(k) not in (3, 4):
+        raise ValueError(f"k_new must be 3-D or 4-D, got {k}")
+    n_new = 1 if len(k) == 3 else k[1]
+    want = (batch, n_kv, d_k) if len(k) == 3 else (batch, n_new, n_kv, d_k)
+    if k != want:
+        raise ValueError(f"k_new shape {k} is not {want} (table {table}, pool {pool})")
+    if v != want:
+        raise ValueError(f"v_new shape {v} != k_new shape {k}")
+    if d_k % 2:
+        raise ValueError(f"d_k must be even, got {d_k}")
+    n_head = 0
+    if q is not None:
+        if len(q) != len(want) or q[:-2] != want[:-2] or q[-1] != d_k:
+            raise ValueError(f"q shape {q} does not match k_new {k}")
+        n_head = q[-2]
+        if n_head <= 0 or n_head % n_kv:
+            raise ValueError(f"n_head ({n_head}) must be a positive multiple of n_kv_head ({n_kv})")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos_dev and sin_dev must both be given or both be None")
+    if cos is not None and (cos != sin or len(cos) != 2 or not 1 <= cos[1] <= d_k // 2):
+        raise ValueError(f"cos/sin tables must be float32 (rows, r // 2) with r <= {d_k}, got {cos} and {sin}")
+    rows, rotary = (0, 0) if cos is None else (cos[0], 2 * cos[1])
+    q_str = _lib.strides(n_new * n_head * d_k, n_head * d_k, d_k)
+    kv_str = _lib.strides(n_new * n_kv * d_k, n_kv * d_k, d_k)
+    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
+    return ((max_pages, n_pages, page_size), (rows, rotary),
+            (batch, n_new, n_head, n_kv, d_k, q_str, q_str, kv_str, kv_str, p_str, p_str))
 
 
 def paged_kv_append(q_dev, k_new, v_new, k_pages, v_pages, page_table, cache_lens, cos_dev=None, sin_dev=None,
@@ -115,48 +165,22 @@ def paged_kv_append(q_dev, k_new, v_new, k_pages, v_pages, page_table, cache_len
     are skipped, q row and all.  Sequences that share a page may not append to it in
     one call.
     """
-    n_pages, n_kv, page_size, d_k = _check_pool(k_pages, v_pages)
-    batch, max_pages = _check_table(page_table, cache_lens, page_size, (1 << 31) - 1)
-    if len(k_new.shape) not in (3, 4):
-        raise ValueError(f"k_new must be 3-D or 4-D, got {k_new.shape}")
-    n_new = 1 if len(k_new.shape) == 3 else k_new.shape[1]
-    want = (batch, n_kv, d_k) if len(k_new.shape) == 3 else (batch, n_new, n_kv, d_k)
-    if tuple(k_new.shape) != want:
-        raise ValueError(f"k_new shape {k_new.shape} is not {want} (table {page_table.shape}, pool {k_pages.shape})")
-    if tuple(v_new.shape) != want:
-        raise ValueError(f"v_new shape {v_new.shape} != k_new shape {k_new.shape}")
-    if d_k % 2:
-        raise ValueError(f"d_k must be even, got {d_k}")
-    n_head = 0
-    if q_dev is not None:
-        if len(q_dev.shape) != len(want) or q_dev.shape[:-2] != want[:-2] or q_dev.shape[-1] != d_k:
-            raise ValueError(f"q shape {q_dev.shape} does not match k_new {k_new.shape}")
-        n_head = q_dev.shape[-2]
-        if n_head <= 0 or n_head % n_kv:
-            raise ValueError(f"n_head ({n_head}) must be a positive multiple of n_kv_head ({n_kv})")
+    _check_int32(page_table, cache_lens, new_lens)
+    pages, tables, sizes = _append_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
+                                        _shape(new_lens), k_new.shape, v_new.shape, _shape(q_dev), _shape(cos_dev),
+                                        _shape(sin_dev))
+    if q_dev is None:
+        if q_out is not None:
+            raise ValueError("q_out is given without q_dev")
+        code = same_dtype(k_new, v_new, k_pages, v_pages)
+    else:
         q_out = q_dev if q_out is None else _same_output(q_out, q_dev)
-    elif q_out is not None:
-        raise ValueError("q_out is given without q_dev")
-    tensors = [k_new, v_new, k_pages, v_pages] + ([q_dev, q_out] if q_dev is not None else [])
-    code = same_dtype(*tensors)
-    if new_lens is not None:
-        _check_lens("new_lens", new_lens, batch)
-    if (cos_dev is None) != (sin_dev is None):
-        raise ValueError("cos_dev and sin_dev must both be given or both be None")
-    rows = rotary = 0
-    if cos_dev is not None:
-        if (cos_dev.shape != sin_dev.shape or len(cos_dev.shape) != 2 or not 1 <= cos_dev.shape[1] <= d_k // 2
-                or cos_dev.dtype != np.float32 or sin_dev.dtype != np.float32):
-            raise ValueError(f"cos/sin tables must be float32 (rows, r // 2) with r <= {d_k}, got {cos_dev.shape} "
-                             f"and {sin_dev.shape}")
-        rows, rotary = cos_dev.shape[0], 2 * cos_dev.shape[1]
-    q_str = _lib.strides(n_new * n_head * d_k, n_head * d_k, d_k)
-    kv_str = _lib.strides(n_new * n_kv * d_k, n_kv * d_k, d_k)
-    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
+        code = same_dtype(k_new, v_new, k_pages, v_pages, q_dev)
+    if cos_dev is not None and not cos_dev.dtype.char == sin_dev.dtype.char == "f":
+        raise ValueError(f"cos/sin tables must be float32, got {cos_dev.dtype} and {sin_dev.dtype}")
     launch(gpu.runtime().tl_paged_kv_append, vp(q_dev), vp(q_out), vp(k_new), vp(v_new), vp(k_pages), vp(v_pages),
-           vp(page_table), max_pages, n_pages, page_size, vp(cache_lens), vp(new_lens), vp(cos_dev), vp(sin_dev),
-           rows, rotary, 1 if interleaved else 0, batch, n_new, n_head, n_kv, d_k, q_str, q_str, kv_str, kv_str,
-           p_str, p_str, code, None, what="paged_kv_append")
+           vp(page_table), *pages, vp(cache_lens), vp(new_lens), vp(cos_dev), vp(sin_dev), *tables,
+           1 if interleaved else 0, *sizes, code, None, what="paged_kv_append")
     return q_out
 
 
@@ -168,6 +192,31 @@ def paged_decode_workspace(batch: int, n_head: int, n_kv_head: int, max_ctx: int
     return gpu.allocate((gpu.runtime().tl_paged_decode_workspace_bytes(n_head, n_kv_head, d_k),), np.uint8)
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_plan(pool, v_pool, table, lens, new_lens, q, n_head, n_kv_head, window, sinks, prefill):
+    """Strides and sizes of an attention call by its shapes."""
+    n_pages, n_kv, page_size, d_k = _check_pool(pool, v_pool)
+    batch, max_pages = _check_table(table, lens, new_lens, page_size, 1 << 30 if prefill else (1 << 31) - 1)
+    _check_heads(n_head, n_kv_head, n_kv, d_k)
+    check_window(window, sinks)
+    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
+    pages = (max_pages, n_pages, page_size)
+    if prefill:
+        if len(q) != 4 or q[0] != batch or q[2:] != (n_head, d_k):
+            raise ValueError(f"q shape {q} is not (batch={batch}, n_new, n_head={n_head}, d_k={d_k})")
+        q_str = _lib.strides(q[1] * n_head * d_k, d_k, n_head * d_k)  # {batch, head, seq}
+        return pages, (batch, q[1], n_head, n_kv_head, d_k, q_str, p_str, p_str, q_str)
+    if math.prod(q) != batch * n_head * d_k:
+        raise ValueError(f"q shape {q} is not (batch={batch}, n_head={n_head}, d_k={d_k})")
+    q_str = _lib.strides(n_head * d_k, d_k)
+    return pages, (batch, n_head, n_kv_head, d_k, q_str, p_str, p_str, q_str)
+
+
+@functools.lru_cache(maxsize=64)
+def _decode_workspace_bytes(n_head: int, n_kv_head: int, d_k: int) -> int:
+    return _lib.load().tl_paged_decode_workspace_bytes(n_head, n_kv_head, d_k)
+
+
 def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_head: int, n_kv_head: int,
                            sm_scale: float | None = None, len_add: int = 0, window: int = 0, sinks: int = 0,
                            out=None, workspace=None):
@@ -176,23 +225,18 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
     Query head h reads KV head ``h // (n_head // n_kv_head)``.  A sequence without
     visible positions gives zeros.  Hidden positions are not read.
     """
-    n_pages, n_kv, page_size, d_k = _check_pool(k_pages, v_pages)
-    batch, max_pages = _check_table(page_table, cache_lens, page_size, (1 << 31) - 1)
-    _check_heads(n_head, n_kv_head, n_kv, d_k)
-    check_window(window, sinks)
-    if math.prod(q_dev.shape) != batch * n_head * d_k:
-        raise ValueError(f"q shape {q_dev.shape} is not (batch={batch}, n_head={n_head}, d_k={d_k})")
+    _check_int32(page_table, cache_lens)
+    pages, sizes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape, None,
+                                   q_dev.shape, n_head, n_kv_head, window, sinks, False)
     code = same_dtype(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
+    d_k = k_pages.shape[3]
     if sm_scale is None:
         sm_scale = default_scale(d_k)
-    lib = gpu.runtime()
-    ws = scratch(lib.tl_paged_decode_workspace_bytes(n_head, n_kv_head, d_k), workspace, key="paged_decode")
-    qo = _lib.strides(n_head * d_k, d_k)
-    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
-    launch(lib.tl_paged_attention_decode, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), max_pages, n_pages,
-           page_size, vp(cache_lens), int(len_add), int(window), int(sinks), vp(out), vp(ws), ws.nbytes, batch,
-           n_head, n_kv_head, d_k, qo, p_str, p_str, qo, float(sm_scale), code, None, what="paged_attention_decode")
+    ws = scratch(_decode_workspace_bytes(n_head, n_kv_head, d_k), workspace, key="paged_decode")
+    launch(gpu.runtime().tl_paged_attention_decode, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), *pages,
+           vp(cache_lens), int(len_add), int(window), int(sinks), vp(out), vp(ws), ws.nbytes, *sizes, float(sm_scale), code, None,
+           what="paged_attention_decode")
     return out
 
 
@@ -203,24 +247,16 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
     The new tokens' own k and v are appended before.  ``new_lens`` as in :func:`paged_kv_append`: rows
     behind a sequence's tokens are left as they were.
     """
-    n_pages, n_kv, page_size, d_k = _check_pool(k_pages, v_pages)
-    batch, max_pages = _check_table(page_table, cache_lens, page_size, 1 << 30)
-    _check_heads(n_head, n_kv_head, n_kv, d_k)
-    check_window(window, sinks)
-    if len(q_dev.shape) != 4 or q_dev.shape[0] != batch or tuple(q_dev.shape[2:]) != (n_head, d_k):
-        raise ValueError(f"q shape {q_dev.shape} is not (batch={batch}, n_new, n_head={n_head}, d_k={d_k})")
-    n_new = q_dev.shape[1]
+    _check_int32(page_table, cache_lens, new_lens)
+    pages, sizes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
+                                   _shape(new_lens), q_dev.shape, n_head, n_kv_head, window, sinks, True)
     code = same_dtype(q_dev, k_pages, v_pages)
-    if new_lens is not None:
-        _check_lens("new_lens", new_lens, batch)
     out = _same_output(out, q_dev)
     if sm_scale is None:
-        sm_scale = default_scale(d_k)
-    q_str = _lib.strides(n_new * n_head * d_k, d_k, n_head * d_k)  # {batch, head, seq}
-    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
-    launch(gpu.runtime().tl_paged_attention_prefill, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), max_pages,
-           n_pages, page_size, vp(cache_lens), vp(new_lens), vp(out), batch, n_new, n_head, n_kv_head, d_k, q_str,
-           p_str, p_str, q_str, float(sm_scale), int(window), int(sinks), code, None, what="paged_attention_prefill")
+        sm_scale = default_scale(k_pages.shape[3])
+    launch(gpu.runtime().tl_paged_attention_prefill, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), *pages,
+           vp(cache_lens), vp(new_lens), vp(out), *sizes, float(sm_scale), int(window), int(sinks), code, None,
+           what="paged_attention_prefill")
     return out
 
 
@@ -233,46 +269,58 @@ def copy_kv_pages(caches, src, dst) -> None:
     synchronises, and a captured graph replays the same copies.
     """
     caches = list(caches)
-    src, dst = (np.asarray(list(x), dtype=np.int64) for x in (src, dst))
-    if src.shape != dst.shape:
-        raise ValueError(f"{src.size} source pages, {dst.size} destinations")
-    if not caches or src.size == 0:
+    src, dst = _numbers(src), _numbers(dst)
+    n = len(src)
+    if n != len(dst):
+        raise ValueError(f"{n} source pages, {len(dst)} destinations")
+    if not caches or n == 0:
         return
-    shape, dtype = tuple(caches[0].shape), gpu.dtype_name(caches[0].dtype)
+    shape, dtype = caches[0].shape, caches[0].dtype
     if len(shape) != 4 or min(shape) <= 0:
         raise ValueError(f"pools must be 4-D (n_pages, n_kv_head, page_size, d_k), got {shape}")
     _check_page_size(shape[2])
+    gpu.dtype_code(dtype)
     for c in caches:
-        if tuple(c.shape) != shape or gpu.dtype_name(c.dtype) != dtype:
-            raise ValueError(f"pools differ: {shape} {dtype} and {c.shape} {gpu.dtype_name(c.dtype)}")
-    if min(src.min(), dst.min()) < 0 or max(src.max(), dst.max()) >= shape[0]:
+        if c.shape != shape or (c.dtype is not dtype and gpu.dtype_name(c.dtype) != gpu.dtype_name(dtype)):
+            raise ValueError(f"pools differ: {shape} {gpu.dtype_name(dtype)} and {c.shape} {gpu.dtype_name(c.dtype)}")
+    if min(src) < 0 or min(dst) < 0 or max(src) >= shape[0] or max(dst) >= shape[0]:
         raise ValueError(f"page numbers must be in [0, {shape[0]})")
-    if np.unique(dst).size != dst.size:
+    to = set(dst)
+    if len(to) != n:
         raise ValueError("a page is a destination twice")
-    if np.intersect1d(src, dst).size:
+    if not to.isdisjoint(src):
         raise ValueError("a page is source and destination")
-    page_bytes = math.prod(shape[1:]) * caches[0].dtype.itemsize
-    bases = (ctypes.c_void_p * len(caches))(*[c.data_ptr() for c in caches])
-    pairs = [(ctypes.c_int32 * src.size)(*x.tolist()) for x in (src, dst)]
-    launch(gpu.runtime().tl_copy_pages, bases, len(caches), page_bytes, page_bytes, shape[0], *pairs, src.size, None,
-           what="copy_kv_pages")
+    page_bytes = shape[1] * shape[2] * shape[3] * dtype.itemsize
+    bases = (ctypes.c_void_p * len(caches))(*[c.ptr.value for c in caches])
+    launch(gpu.runtime().tl_copy_pages, bases, len(caches), page_bytes, page_bytes, shape[0], (ctypes.c_int32 * n)(*src),
+           (ctypes.c_int32 * n)(*dst), n, None, what="copy_kv_pages")
+
+
+def _numbers(x) -> list:
+    """Whole numbers of a sequence or array, as a list of int."""
+    if isinstance(x, np.ndarray):
+        if x.dtype.kind not in "iu":
+            raise ValueError(f"expected whole numbers, got {x.dtype}")
+        return x.ravel().tolist()
+    return [operator.index(i) for i in x]
 
 
 def write_i32(dst, index, value) -> None:
     """``dst.flat[index[i]] = value[i]`` for a device int32 tensor, the values on the host: no
     upload, no synchronisation (page table entries, lengths).  Indices must be distinct."""
-    if gpu.dtype_name(dst.dtype) != "int32":
+    if not _is_int32(dst):
         raise ValueError(f"dst must be int32, got {gpu.dtype_name(dst.dtype)}")
-    index, value = (np.asarray(x, dtype=np.int64).ravel() for x in (index, value))
-    if index.size != value.size:
-        raise ValueError(f"{index.size} indices, {value.size} values")
-    if index.size == 0:
+    index, value = _numbers(index), _numbers(value)
+    n = len(index)
+    if n != len(value):
+        raise ValueError(f"{n} indices, {len(value)} values")
+    if n == 0:
         return
-    if index.min() < 0 or index.max() >= dst.size:
+    if min(index) < 0 or max(index) >= dst.size:
         raise ValueError(f"indices must be in [0, {dst.size})")
-    if np.unique(index).size != index.size:
+    if len(set(index)) != n:
         raise ValueError("an index is given twice")
-    if value.min() < -(1 << 31) or value.max() >= 1 << 31:
+    if min(value) < -(1 << 31) or max(value) >= 1 << 31:
         raise ValueError("values must fit in int32")
-    pairs = [(ctypes.c_int32 * index.size)(*x.tolist()) for x in (index, value)]
-    launch(gpu.runtime().tl_write_i32, vp(dst), dst.size, *pairs, index.size, None, what="write_i32")
+    launch(gpu.runtime().tl_write_i32, vp(dst), dst.size, (ctypes.c_int32 * n)(*index), (ctypes.c_int32 * n)(*value), n,
+           None, what="write_i32")
