@@ -108,16 +108,139 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   }
 }
 
+// 16 bytes of a row at once.  A row is cut into pairs of 16-byte chunks, thread j of a row's d_k / 2 / VEC
+// taking one pair: in the half layout the two chunks that are turned into each other, behind the turned features
+// and in the other layouts two neighbours (an interleaved chunk is turned in itself).  A thread takes
+// rows g, g + R, ... of its token and loads its angles once for all of them.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void paged_append_vec_kernel(AppendParams p, int R) {
+  using B = typename T::bits;
+  constexpr int VEC = 16 / T::size;
+  constexpr int UNROLL = 4;
+  const int per_row = p.d_k / (2 * VEC);
+  const int64_t tid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per_tok = per_row * R;
+  if (tid >= (int64_t)p.batch * p.n_new * per_tok) return;
+  const int64_t tok = tid / per_tok;
+  const int rest = (int)(tid - tok * per_tok);
+  const int g = rest / per_row, j = rest - g * per_row;
+  const int b = (int)(tok / p.n_new), s = (int)(tok - (int64_t)b * p.n_new);
+  int pos, page;
+  if (!token_place(p, b, s, MODE != kNoRope, pos, page)) return;
+
+  const int turned = MODE == kHalf ? p.rot_half / VEC : 0;  // pairs of chunks that turn into each other
+  const bool across = MODE == kHalf && j < turned;
+  const int ca = across ? j : MODE == kHalf ? 2 * turned + 2 * (j - turned) : 2 * j;
+  const int cb = across ? j + turned : ca + 1;
+  const bool in_a = MODE == kInterleaved && ca * VEC < 2 * p.rot_half;
+  const bool in_b = MODE == kInterleaved && cb * VEC < 2 * p.rot_half;
+  // angles: across, VEC of them at j VEC; inside, VEC / 2 a chunk at ca VEC / 2
+  float c[VEC], sn[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) c[i] = 1.f, sn[i] = 0.f;
+  if (MODE != kNoRope && (across || in_a)) {
+    const int64_t at = (int64_t)pos * p.rot_half + j * VEC;
+    const int n = across || in_b ? VEC : VEC / 2;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < n) c[i] = p.cos_t[at + i], sn[i] = p.sin_t[at + i];
+  }
+  auto unpack = [](const u32x4& w, float (&f)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (T::size == 4) f[i] = __uint_as_float(w[i]);
+      else unpack2<T>(w[i], f[2 * i], f[2 * i + 1]);
+    }
+  };
+  auto pack = [](const float (&f)[VEC]) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (T::size == 4) w[i] = __float_as_uint(f[i]);
+      else w[i] = (uint32_t)from_f32<T>(f[2 * i]) | ((uint32_t)from_f32<T>(f[2 * i + 1]) << 16);
+    }
+    return w;
+  };
+  const int rows = p.n_head + 2 * p.n_kv, rot_rows = p.n_head + p.n_kv;
+  for (int r = g; r < rows; r += UNROLL * R) {
+    u32x4 wa[UNROLL], wb[UNROLL];
+    B* out[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (r + u * R < rows) {
+        const B* src;
+        token_row(p, b, s, pos, page, r + u * R, src, out[u]);
+        wa[u] = *(const u32x4*)(src + ca * VEC);
+        wb[u] = *(const u32x4*)(src + cb * VEC);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      if (r + u * R < rows) {
+        u32x4 oa = wa[u], ob = wb[u];
+        if (MODE != kNoRope && r + u * R < rot_rows && (across || in_a)) {
+          float x[VEC], y[VEC];
+          unpack(wa[u], x);
+          unpack(wb[u], y);
+          if (MODE == kHalf) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) rope_rotate_pair(x[i], y[i], c[i], sn[i], x[i], y[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+              rope_rotate_pair(x[2 * i], x[2 * i + 1], c[i], sn[i], x[2 * i], x[2 * i + 1]);
+              if (in_b) rope_rotate_pair(y[2 * i], y[2 * i + 1], c[VEC / 2 + i], sn[VEC / 2 + i], y[2 * i], y[2 * i + 1]);
+            }
+          }
+          oa = pack(x);
+          if (MODE == kHalf || in_b) ob = pack(y);
+        }
+        *(u32x4*)(out[u] + ca * VEC) = oa;
+        *(u32x4*)(out[u] + cb * VEC) = ob;
+      }
+    }
+  }
+}
+
+// Whether every row can be moved in whole 16-byte chunks, turned features ending at a chunk's end.
+template <typename T>
+bool append_vec_ok(const AppendParams& p, int mode) {
+  constexpr int VEC = 16 / T::size;
+  if (p.d_k % (2 * VEC)) return false;
+  if (mode == kHalf && p.rot_half % VEC) return false;
+  if (mode == kInterleaved && (2 * p.rot_half) % VEC) return false;
+  const int64_t st[] = {p.kn_sb, p.kn_ss, p.kn_sh, p.vn_sb, p.vn_ss, p.vn_sh, p.kp_sp, p.kp_sh, p.kp_sr,
+                        p.vp_sp, p.vp_sh, p.vp_sr, p.q_sb,  p.q_ss,  p.q_sh,  p.qo_sb, p.qo_ss, p.qo_sh};
+  for (int64_t x : st)
+    if (x % VEC) return false;
+  return !(((uintptr_t)p.q | (uintptr_t)p.qo | (uintptr_t)p.kn | (uintptr_t)p.vn | (uintptr_t)p.kp | (uintptr_t)p.vp) & 15);
+}
+
+template <typename T, int MODE>
+int launch_append_mode(const AppendParams& p, hipStream_t st) {
+  const int rows = p.n_head + 2 * p.n_kv;
+  if (append_vec_ok<T>(p, MODE)) {
+    // A decoded token: a thread a chunk pair.  Prompts: about 2^18 threads, each with several rows
+    // for one load of its angles.
+    const int64_t lanes = (int64_t)p.batch * p.n_new * (p.d_k / (2 * (16 / T::size)));
+    int64_t groups = ((int64_t)1 << 18) / lanes;
+    groups = groups < 1 ? 1 : groups > rows ? rows : groups;
+    const int64_t blocks = (lanes * groups + 255) / 256;
+    if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((paged_append_vec_kernel<T, MODE>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)groups);
+    return tl_launch_status();
+  }
+  const int64_t blocks = ((int64_t)p.batch * p.n_new * rows * (p.d_k / 2) + 255) / 256;
+  if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((paged_append_kernel<T, MODE>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+  return tl_launch_status();
+}
+
 template <typename T>
 int launch_append(const AppendParams& p, int mode, hipStream_t st) {
-  const int64_t total = (int64_t)p.batch * p.n_new * (p.n_head + 2 * p.n_kv) * (p.d_k / 2);
-  const int64_t blocks = (total + 255) / 256;
-  if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)blocks), block(256);
-  if (mode == kHalf) hipLaunchKernelGGL((paged_append_kernel<T, kHalf>), grid, block, 0, st, p);
-  else if (mode == kInterleaved) hipLaunchKernelGGL((paged_append_kernel<T, kInterleaved>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((paged_append_kernel<T, kNoRope>), grid, block, 0, st, p);
-  return tl_launch_status();
+  return mode == kHalf          ? launch_append_mode<T, kHalf>(p, st)
+         : mode == kInterleaved ? launch_append_mode<T, kInterleaved>(p, st)
+                                : launch_append_mode<T, kNoRope>(p, st);
 }
 
 // ---------------------------------------------------------------------------------
