@@ -390,6 +390,10 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * {batch, head, seq}, query i at position seq_k - seq_q + i.
  * Both: window = 0 is plain causal attention; a row that sees no key gives zeros;
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; o may not overlap q, k or v.
+ * With few rows the keys are shared by several workgroups, whose results lie in the
+ * workspace (tl_window_workspace_bytes bytes, 16-byte aligned, most_keys = seq_k, or
+ * max_pages * page_size; no initialisation) and are joined by a second launch;
+ * given less (NULL: none) the call runs in one.  Either is deterministic.
  * A NaN or infinity in a V row makes NaN of the rows that are computed in one
  * tile with it, seen or not, as a product with a zero weight does.
  *
@@ -422,12 +426,15 @@ int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_
 int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v_pages,
                                const int32_t* page_table, int max_pages, int n_pages,
                                int page_size, const int32_t* cache_lens, const int32_t* new_lens,
-                               void* o, int batch, int n_new, int n_head, int n_kv_head, int d_k,
+                               void* o, void* workspace, size_t workspace_bytes, int batch,
+                               int n_new, int n_head, int n_kv_head, int d_k,
                                const int64_t* q_strides, const int64_t* k_page_strides,
                                const int64_t* v_page_strides, const int64_t* o_strides,
                                float sm_scale, int window, int sinks, int dtype, void* stream);
-int tl_window_attention(const void* q, const void* k, const void* v, void* o, int batch,
-                        int n_head, int n_kv_head, int seq_q, int seq_k, int d_k,
+size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q, int most_keys,
+                                 int d_k, int window, int sinks, int dtype);
+int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace,
+                        size_t workspace_bytes, int batch, int n_head, int n_kv_head, int seq_q, int seq_k, int d_k,
                         const int64_t* q_strides, const int64_t* k_strides,
                         const int64_t* v_strides, const int64_t* o_strides, float sm_scale,
                         int window, int sinks, int dtype, void* stream);

@@ -193,13 +193,13 @@ def test_c_decode_refuses():
 
 
 def c_window(q=PTR, sq=8, sk=8, heads=(4, 2), d_k=64, qs=S3, ks=S3, window=0, sinks=0, dtype=BF16, batch=1):
-    return _lib.load().tl_window_attention(q, PTR, PTR, PTR, batch, *heads, sq, sk, d_k, qs, ks, S3, S3, 0.1, window,
+    return _lib.load().tl_window_attention(q, PTR, PTR, PTR, None, 0, batch, *heads, sq, sk, d_k, qs, ks, S3, S3, 0.1, window,
                                            sinks, dtype, None)
 
 
 def c_prefill(table=PTR, lens=PTR, max_pages=4, n_pages=9, page=16, n_new=5, batch=1, **kw):
     q, d_k = kw.get("q", PTR), kw.get("d_k", 64)
-    return _lib.load().tl_paged_attention_prefill(q, PTR, PTR, table, max_pages, n_pages, page, lens, None, PTR, batch,
+    return _lib.load().tl_paged_attention_prefill(q, PTR, PTR, table, max_pages, n_pages, page, lens, None, PTR, None, 0, batch,
                                                   n_new, 4, 2, d_k, S3, S3, S3, S3, 0.1, 0, 0, BF16, None)
 
 

@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kBM = 128;  // query rows of a workgroup
+constexpr int kMinShare = 4;  // key tiles of a part at least
 constexpr float kRescaleLog2 = 8.f;
 
 struct WinParams {
@@ -39,6 +40,9 @@ struct WinParams {
   const int32_t* new_lens;
   int batch, n_head, n_kv, group, seq_q, seq_k, n_qt;
   int window, sinks;
+  int share, n_parts;  // key tiles of a part at least, parts of a row tile at most
+  int vec_out;         // o's rows take 4 elements at once
+  float* ws;           // [tile][part] of partial results (n_parts > 1)
   int64_t q_sb, q_sh, q_ss;
   int64_t k_sb, k_sh, k_ss;
   int64_t v_sb, v_sh, v_ss;
@@ -76,24 +80,40 @@ struct Tile16 {
   struct Q {
     frag f[NKS];
   };
-  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int h) {
+  // sign: flips of the values' sign bits
+  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int h, uint32_t sign) {
+    sign |= sign >> 16;
 #pragma unroll
     for (int ks = 0; ks < NKS; ++ks) {
       u32x4 x = u32x4{0u, 0u, 0u, 0u};
       if (there) x = *(const u32x4*)(row + 32 * ks + 16 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] ^= sign;
       q.f[ks] = __builtin_bit_cast(frag, x);
     }
   }
+  // Operands are read kAhead MFMAs ahead; the barriers keep the compiler from reading them all at
+  // once, which their registers do not allow at d_k 128.
+  static constexpr int kAhead = 4;
   static __device__ __forceinline__ void scores(f32x16 (&s)[NMB], const Q& q, const char* kt, int lq, int h) {
+    constexpr int NG = NMB * NKS;
+    const char* row = kt + lq * ROWB;
+    const int sw = (h ^ k_swz<T, D>(lq)) << 4;
+    u32x4 f[NG];
+    auto fetch = [&](int g) __attribute__((always_inline)) {
+      f[g] = *(const u32x4*)(row + 32 * (g % NMB) * ROWB + (sw ^ ((g / NMB) << 5)));
+    };
 #pragma unroll
-    for (int mb = 0; mb < NMB; ++mb) {
+    for (int g = 0; g < kAhead; ++g) fetch(g);
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < NKS; ++ks) {
-        const u32x4 a = *(const u32x4*)(kt + (32 * mb + lq) * ROWB + (((2 * ks + h) ^ k_swz<T, D>(lq)) << 4));
-        s[mb] = M::mma(__builtin_bit_cast(frag, a), q.f[ks], s[mb]);
-      }
+    for (int g = 0; g < NG; ++g) {
+      if (g + kAhead < NG) fetch(g + kAhead);
+      s[g % NMB] = M::mma(__builtin_bit_cast(frag, f[g]), q.f[g / NMB], s[g % NMB]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   // s holds the probabilities; they are rounded to the storage type here (at most half a step
@@ -101,25 +121,33 @@ struct Tile16 {
   static __device__ __forceinline__ void values(f32x16 (&o)[NDB], const f32x16 (&s)[NMB], const char* vt, int lane) {
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
-    const auto* lds = (const __attribute__((address_space(3))) char*)vt;
-    const int g = lane >> 4, e = (lane >> 2) & 3, c = lane & 3;
+    constexpr int NG = 2 * NMB * NDB;
+    const int g16 = lane >> 4, e = (lane >> 2) & 3, c = lane & 3;
+    const auto* lds = (const __attribute__((address_space(3))) char*)vt + (4 * (g16 >> 1) + e) * ROWB + 8 * (c & 1);
+    const int sw = ((2 * (g16 & 1) + (c >> 1)) ^ v_swz<T, D>(e)) << 4;
+    u32x4 f[NG];
+    u32x4 pw[2 * NMB];
+    auto fetch = [&](int g) __attribute__((always_inline)) {
+      const auto* at = lds + 16 * (g / NDB) * ROWB + (sw ^ ((g % NDB) << 6));
+      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at));
+      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * ROWB)));
+      f[g] = u32x4{a.x, a.y, b.x, b.y};
+    };
 #pragma unroll
-    for (int tt = 0; tt < 2 * NMB; ++tt) {
-      u32x4 pw;
+    for (int g = 0; g < kAhead; ++g) fetch(g);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x[2] = {s[tt >> 1][8 * (tt & 1) + 2 * j], s[tt >> 1][8 * (tt & 1) + 2 * j + 1]};
-        pw[j] = pack2<T>(x);
+    for (int g = 0; g < NG; ++g) {
+      const int tt = g / NDB, db = g % NDB;
+      if (db == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x[2] = {s[tt >> 1][8 * (tt & 1) + 2 * j], s[tt >> 1][8 * (tt & 1) + 2 * j + 1]};
+          pw[tt][j] = pack2<T>(x);
+        }
       }
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const int chunk = 4 * db + 2 * (g & 1) + (c >> 1);
-        const int off = (16 * tt + 4 * (g >> 1) + e) * ROWB + ((chunk ^ v_swz<T, D>(e)) << 4) + 8 * (c & 1);
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(lds + off));
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(lds + off + 8 * ROWB));
-        const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-        o[db] = M::mma(__builtin_bit_cast(frag, u32x4{a.x, a.y, b.x, b.y}), __builtin_bit_cast(frag, pw), o[db]);
-      }
+      if (g + kAhead < NG) fetch(g + kAhead);
+      o[db] = M::mma(__builtin_bit_cast(frag, f[g]), __builtin_bit_cast(frag, pw[tt]), o[db]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -130,13 +158,13 @@ struct Tile32 {
   struct Q {
     float f[D / 2];  // features h D / 2 .. of the row
   };
-  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int h) {
+  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int h, uint32_t sign) {
 #pragma unroll
     for (int c = 0; c < D / 8; ++c) {
-      f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (there) x = *(const f32x4*)(row + h * (D * 2) + 16 * c);
+      u32x4 x = u32x4{0u, 0u, 0u, 0u};
+      if (there) x = *(const u32x4*)(row + h * (D * 2) + 16 * c);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) q.f[4 * c + i] = x[i];
+      for (int i = 0; i < 4; ++i) q.f[4 * c + i] = __uint_as_float(x[i] ^ sign);
     }
   }
   static __device__ __forceinline__ void scores(f32x16 (&s)[NMB], const Q& q, const char* kt, int lq, int h) {
@@ -170,6 +198,72 @@ struct Tile<F16, D> : Tile16<F16, D> {};
 template <int D>
 struct Tile<F32, D> : Tile32<D> {};
 
+// Where a sequence's query rows stand: token i at position base + i, nq tokens, no key from `end` on.
+struct Rows {
+  int base, nq, end;
+};
+template <bool PAGED>
+__device__ __forceinline__ Rows rows_of(const WinParams& p, int b) {
+  Rows r;
+  if constexpr (PAGED) {
+    constexpr int kFar = 1 << 30;
+    r.base = min(max(p.lens[b], -kFar), kFar);
+    r.nq = p.new_lens ? min(max(p.new_lens[b], 0), p.seq_q) : p.seq_q;
+    r.end = min(r.base + r.nq, p.pm.max_pages << p.pm.shift);
+  } else {
+    r.base = p.seq_k - p.seq_q;
+    r.nq = p.seq_q;
+    r.end = p.seq_k;
+  }
+  return r;
+}
+
+// The key tiles of row tile qt: ns of the sinks', then those from t0 on; in how many parts.
+struct Keys {
+  int ns, t0, tiles, parts, end;
+  __device__ __forceinline__ int key0(int t) const { return t < ns ? t : t - ns + t0; }  // in tiles
+};
+template <int BN>
+__device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int qt) {
+  Keys k{0, 0, 0, 1, r.end};
+  const int p0 = r.base + qt * kBM / p.group;
+  const int p1 = min(r.base + min((qt * kBM + kBM - 1) / p.group + 1, r.nq), r.end) - 1;  // last key any row sees
+  if (p1 < 0) return k;
+  if (p.window > 0) {
+    k.t0 = max(p0 - p.window + 1, 0) / BN;
+    k.ns = (min(p.sinks, p1 + 1) + BN - 1) / BN;
+    if (k.t0 <= k.ns) k.ns = k.t0 = 0;
+  }
+  k.tiles = k.ns + p1 / BN - k.t0 + 1;
+  if (p.n_parts > 1) k.parts = min(p.n_parts, (k.tiles + p.share - 1) / p.share);
+  return k;
+}
+
+// Four neighbouring outputs, rounded to nearest even.
+template <typename T>
+__device__ __forceinline__ void store4(typename T::bits* d, float a, float b, float c, float e, int vec) {
+  if constexpr (T::size == 4) {
+    if (vec) {
+      *(f32x4*)d = f32x4{a, b, c, e};
+    } else {
+      d[0] = __float_as_uint(a), d[1] = __float_as_uint(b), d[2] = __float_as_uint(c), d[3] = __float_as_uint(e);
+    }
+  } else {
+    const float x[2] = {a, b}, y[2] = {c, e};
+    const uint32_t lo = pack2<T>(x), hi = pack2<T>(y);
+    if (vec) {
+      *(u32x2*)d = u32x2{lo, hi};
+    } else {
+      d[0] = (uint16_t)lo, d[1] = (uint16_t)(lo >> 16), d[2] = (uint16_t)hi, d[3] = (uint16_t)(hi >> 16);
+    }
+  }
+}
+
+// A part's results: 32 rows a wave, each wave's m and l (by row) and then its O^T, the registers as
+// they lie in the lanes.
+template <int D>
+constexpr size_t part_floats() { return (size_t)4 * (64 + 64 * (D / 2)); }
+
 template <typename T, int D, bool PAGED>
 __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   using TL = Tile<T, D>;
@@ -187,54 +281,35 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];  // (K, V) twice
 
   // Workgroups are dealt to the 8 XCDs in turn; XCD x takes a contiguous range of (sequence, KV head,
-  // query head, tile), so that few KV heads share its L2.
-  const int n_items = p.batch * p.n_head * p.n_qt;
+  // row tile, part), so that few KV heads share its L2.
+  const int n_tiles = p.batch * p.n_kv * p.n_qt;
+  const int n_items = n_tiles * p.n_parts;
   const int per = (n_items + 7) / 8;
   const int item = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
   if ((int)(blockIdx.x / 8) >= per || item >= n_items) return;
-  const int head = item / p.n_qt;
-  const int qt = p.n_qt - 1 - (item - head * p.n_qt);  // the longest rows first
-  const int b = head / p.n_head;
-  const int hq = head - b * p.n_head;
-  const int hkv = hq / p.group;
+  const int tile = item / p.n_parts, part = item - tile * p.n_parts;
+  const int kvh = tile / p.n_qt;
+  const int qt = p.n_qt - 1 - (tile - kvh * p.n_qt);  // the longest rows first
+  const int b = kvh / p.n_kv;
+  const int hkv = kvh - b * p.n_kv;
+  const Rows rw = rows_of<PAGED>(p, b);
+  const Keys ks = keys_of<BN>(p, rw, qt);
+  if (qt * kBM >= rw.nq * p.group || part >= ks.parts) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)threadIdx.x >> 6);
   const int lq = lane & 31, h = lane >> 5;
 
-  int base, nq, key_end;  // position of row 0, rows, keys behind which nothing is read
-  if constexpr (PAGED) {
-    constexpr int kFar = 1 << 30;
-    base = min(max(p.lens[b], -kFar), kFar);
-    nq = p.new_lens ? min(max(p.new_lens[b], 0), p.seq_q) : p.seq_q;
-    key_end = min(base + nq, p.pm.max_pages << p.pm.shift);
-  } else {
-    base = p.seq_k - p.seq_q;
-    nq = p.seq_q;
-    key_end = p.seq_k;
-  }
-  if (qt * kBM >= nq) return;
-
-  // the key tiles: ns of the sinks, then from t0 on
-  const int p0 = base + qt * kBM;
-  const int p1 = min(base + min(qt * kBM + kBM, nq), key_end) - 1;  // last key any row sees
-  int ns = 0, t0 = 0, nt = 0;
-  if (p1 >= 0) {
-    const int te = p1 / BN;
-    if (p.window > 0) {
-      t0 = max(p0 - p.window + 1, 0) / BN;
-      ns = (min(p.sinks, p1 + 1) + BN - 1) / BN;
-      if (t0 <= ns) ns = t0 = 0;
-    }
-    nt = ns + te - t0 + 1;
-  }
-  auto tile_key0 = [&](int t) { return (t < ns ? t : t - ns + t0) * BN; };
-
-  const int row = qt * kBM + 32 * wave + lq;  // this lane's query row
-  const int pos = base + row;
-  const bool there = row < nq;
+  // this lane's row: query head hkv * group + row % group of token row / group
+  const int row = qt * kBM + 32 * wave + lq;
+  const int tok = row / p.group;
+  const int hq = hkv * p.group + (row - tok * p.group);
+  const bool there = tok < rw.nq;
+  const int pos = rw.base + tok;
   typename TL::Q q;
-  TL::load_q(q, (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh + (int64_t)min(row, nq - 1) * p.q_ss), there, h);
+  TL::load_q(q, (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh + (int64_t)tok * p.q_ss), there && p.scale_log2 != 0.f,
+             h, p.scale_log2 < 0.f ? 0x80000000u : 0u);
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
 
   // ---- tile loads --------------------------------------------------------------
   const uint32_t k_row = (uint32_t)(p.k_ss * T::size), v_row = (uint32_t)(p.v_ss * T::size);
@@ -251,30 +326,32 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   auto tile_pages = [&](int t) {
     int id = -1;
     if constexpr (PAGED) {
-      const int e = (tile_key0(t) + kBlk * lane) >> p.pm.shift;
+      const int e = (ks.key0(t) * BN + kBlk * lane) >> p.pm.shift;
       if (lane < BN / kBlk && e < p.pm.max_pages) id = table[e];
       if ((unsigned)id >= (unsigned)p.pm.n_pages) id = -1;
     }
     return id;
   };
-  // Rows past key_end, and rows of pages that are not there, read as zeros.
-  auto load_tile = [&](int t, int buf, int pages) {
-    const int pos0 = tile_key0(t) + wave * WROWS;
-    int rows = min(max(key_end - pos0, 0), WROWS);
-    const char *kb, *vb;
+  // Rows past the last key, and rows of pages that are not there, read as zeros.
+  const char* const kbase = (const char*)((const B*)p.k + (PAGED ? 0 : b * p.k_sb) + hkv * p.k_sh);
+  const char* const vbase = (const char*)((const B*)p.v + (PAGED ? 0 : b * p.v_sb) + hkv * p.v_sh);
+  auto load_tile = [&](int t, int buf, int pages) __attribute__((always_inline)) {
+    const int pos0 = ks.key0(t) * BN + wave * WROWS;
+    int rows = min(max(ks.end - pos0, 0), WROWS);
+    int64_t ka, va;
     if constexpr (PAGED) {
       const int id = __builtin_amdgcn_readlane(pages, (wave * WROWS) / kBlk);
       const int in = pos0 & ((1 << p.pm.shift) - 1);
       if (id < 0) rows = 0;
       const int64_t at = id < 0 ? 0 : id;
-      kb = (const char*)((const B*)p.k + at * p.k_sb + hkv * p.k_sh + in * p.k_ss);
-      vb = (const char*)((const B*)p.v + at * p.v_sb + hkv * p.v_sh + in * p.v_ss);
+      ka = at * p.k_sb * T::size + (int64_t)in * k_row;
+      va = at * p.v_sb * T::size + (int64_t)in * v_row;
     } else {
-      kb = (const char*)((const B*)p.k + b * p.k_sb + hkv * p.k_sh + pos0 * p.k_ss);
-      vb = (const char*)((const B*)p.v + b * p.v_sb + hkv * p.v_sh + pos0 * p.v_ss);
+      ka = (int64_t)pos0 * k_row;
+      va = (int64_t)pos0 * v_row;
     }
-    const i32x4 rk = uniform_rsrc(kb, rows ? (rows - 1) * k_row + ROWB : 0);
-    const i32x4 rv = uniform_rsrc(vb, rows ? (rows - 1) * v_row + ROWB : 0);
+    const i32x4 rk = uniform_rsrc(kbase + ka, rows ? (rows - 1) * k_row + ROWB : 0);
+    const i32x4 rv = uniform_rsrc(vbase + va, rows ? (rows - 1) * v_row + ROWB : 0);
     const uint32_t la = lds0 + buf * 2 * TILEB + wave * WROWS * ROWB;
 #pragma unroll
     for (int i = 0; i < NDMA; ++i) lds_dma16(rk, koff[i], la + i * 1024);
@@ -289,60 +366,46 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  const int wp0 = uni(base + qt * kBM + 32 * wave);  // this wave's first position
-  const int wp1 = min(wp0 + 31, base + nq - 1);
-  const bool wave_rows = qt * kBM + 32 * wave < nq;
+  // this wave's first and last position
+  const int row0 = qt * kBM + 32 * wave;
+  const int wp0 = uni(rw.base + row0 / p.group);
+  const int wp1 = uni(rw.base + min((row0 + 31) / p.group, rw.nq - 1));
+  const bool wave_rows = row0 < rw.nq * p.group;
 
-  int pages = nt > 0 ? tile_pages(0) : -1;
-  if (nt > 0) load_tile(0, 0, pages);
-  int next_pages = nt > 1 ? tile_pages(1) : -1;
-  for (int t = 0; t < nt; ++t) {
-    wait_vmcnt<0>();  // this wave's rows of tile t are in LDS
-    lds_barrier();    // everybody's are, and tile t - 1 has been read
-    const int there_now = pages;
-    if (t + 1 < nt) {
-      load_tile(t + 1, (t + 1) & 1, next_pages);
-      pages = next_pages;
-      if (t + 2 < nt) next_pages = tile_pages(t + 2);
-    }
-    const int k0 = tile_key0(t);
-    // does any row of this wave see a key of the tile, and does every row see all of them
-    const bool any = wave_rows && k0 <= wp1 && (p.window <= 0 || k0 + BN - 1 > wp0 - p.window || k0 < p.sinks);
-    if (!any) continue;
-    uint32_t gone = 0;  // blocks that have no page
-    if constexpr (PAGED) gone = (uint32_t)__ballot(there_now < 0) & ((1u << (BN / kBlk)) - 1);
-    const bool all = k0 + BN - 1 <= wp0 && k0 + BN <= key_end && gone == 0 &&
-                     (p.window <= 0 || k0 > wp1 - p.window || k0 + BN <= p.sinks);
-    const char* kt = smem + (t & 1) * 2 * TILEB;
-    const char* vt = kt + TILEB;
+  // One key tile: scores, softmax, O^T.  all: every row sees every key.
+  auto step = [&](int k0, const char* kt, uint32_t gone, bool all) __attribute__((always_inline)) {
     f32x16 s[NMB];
     TL::scores(s, q, kt, lq, h);
     if (!all) {
+      asm volatile("");  // a branch: as selects the tests would run for every tile
+      // key k0 + kl + 4 h of this lane is seen if kl <= hi and (kl > lo or kl < sk)
+      const int off = k0 + 4 * h;
+      const int hi = min(pos, ks.end - 1) - off;
+      const int lo = p.window > 0 ? pos - p.window - off : -BN - 1;
+      const int sk = p.sinks - off;
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int key = k0 + 32 * mb + 8 * (r >> 2) + 4 * h + (r & 3);
-          const bool seen = key_seen(key, pos, p.window, p.sinks) && key < key_end && !((gone >> (2 * mb + (r >> 3))) & 1);
-          s[mb][r] = seen ? s[mb][r] : -INFINITY;
+          const int kl = 32 * mb + 8 * (r >> 2) + (r & 3);
+          s[mb][r] = kl <= hi && (kl > lo || kl < sk) ? s[mb][r] : -INFINITY;
         }
+      if (gone) {
+        asm volatile("");
+#pragma unroll
+        for (int mb = 0; mb < NMB; ++mb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if ((gone >> (2 * mb + (r >> 3))) & 1) s[mb][r] = -INFINITY;
+      }
     }
-    float mx = -INFINITY;
+    float mx = s[0][0];
 #pragma unroll
     for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mb][r]);
-    mx = tlp::max_xor32(mx) * p.scale_log2;
-    // a negative scale turns the order round: the maximum is then the smallest score's
-    if (p.scale_log2 < 0.f) {
-      float mn = INFINITY;
-#pragma unroll
-      for (int mb = 0; mb < NMB; ++mb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mn = fminf(mn, s[mb][r] == -INFINITY ? INFINITY : s[mb][r]);
-      mx = -tlp::max_xor32(-mn);
-      mx = mx == INFINITY ? -INFINITY : mx * p.scale_log2;
-    }
+    mx = tlp::max_xor32(mx) * scale;
+    // the maximum moves only when a score passes it by 2^8 (it only bounds the exponents)
     if (__any(mx > m + kRescaleLog2)) {
       const float mn = fmaxf(m, mx);
       const float a = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
@@ -358,39 +421,151 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float x = s[mb][r];
-        const float e = fast_exp2(fmaf(x, p.scale_log2, -shift));
-        s[mb][r] = all || x != -INFINITY ? e : 0.f;
+        s[mb][r] = fast_exp2(fmaf(s[mb][r], scale, -shift));
         l += s[mb][r];
       }
-    TL::values(o, s, vt, lane);
+    TL::values(o, s, kt + TILEB, lane);
+  };
+
+  const int t_lo = (int)((int64_t)ks.tiles * part / ks.parts), t_hi = (int)((int64_t)ks.tiles * (part + 1) / ks.parts);
+  int pages = t_lo < t_hi ? tile_pages(t_lo) : -1;
+  if (t_lo < t_hi) load_tile(t_lo, 0, pages);
+  int next_pages = t_lo + 1 < t_hi ? tile_pages(t_lo + 1) : -1;
+  for (int t = t_lo; t < t_hi; ++t) {
+    wait_vmcnt<0>();  // this wave's rows of tile t are in LDS
+    lds_barrier();    // everybody's are, and tile t - 1 has been read
+    const int buf = (t - t_lo) & 1;
+    const int these = pages;
+    if (t + 1 < t_hi) {
+      load_tile(t + 1, buf ^ 1, next_pages);
+      pages = next_pages;
+      if (t + 2 < t_hi) next_pages = tile_pages(t + 2);
+    }
+    const int k0 = ks.key0(t) * BN;
+    // does any row of this wave see a key of the tile, and does every row see all of them
+    const bool any = wave_rows && k0 <= wp1 && (p.window <= 0 || k0 + BN - 1 > wp0 - p.window || k0 < p.sinks);
+    if (!any) continue;
+    uint32_t gone = 0;  // blocks that have no page
+    if constexpr (PAGED) gone = (uint32_t)__ballot(these < 0) & ((1u << (BN / kBlk)) - 1);
+    const bool all = k0 + BN - 1 <= wp0 && k0 + BN <= ks.end && gone == 0 &&
+                     (p.window <= 0 || k0 > wp1 - p.window || k0 + BN <= p.sinks);
+    const char* kt = smem + buf * 2 * TILEB;
+    step(k0, kt, gone, all);
   }
 
   l = tlp::sum_xor32(l);
+  if (ks.parts > 1) {
+    float* w = p.ws + (size_t)item * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
+    if (h == 0) {
+      w[2 * lq] = m;
+      w[2 * lq + 1] = l;
+    }
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        *(f32x4*)(w + 64 + (4 * db + a) * 256 + 4 * lane) =
+            f32x4{o[db][4 * a], o[db][4 * a + 1], o[db][4 * a + 2], o[db][4 * a + 3]};
+    return;
+  }
   if (!there) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)row * p.o_ss;
+  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)tok * p.o_ss;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int d = 32 * db + 8 * a + 4 * h;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[d + i] = from_f32<T>(o[db][4 * a + i] * inv);
-    }
+    for (int a = 0; a < 4; ++a)
+      store4<T>(out + 32 * db + 8 * a + 4 * h, o[db][4 * a] * inv, o[db][4 * a + 1] * inv, o[db][4 * a + 2] * inv,
+                o[db][4 * a + 3] * inv, p.vec_out);
 }
+
+// Joins the parts of a row tile: the same lanes that wrote them.
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
+  using B = typename T::bits;
+  constexpr int BN = tile_keys<T>();
+  const int tile = blockIdx.x, db = blockIdx.y;
+  const int kvh = tile / p.n_qt;
+  const int qt = p.n_qt - 1 - (tile - kvh * p.n_qt);
+  const int b = kvh / p.n_kv;
+  const int hkv = kvh - b * p.n_kv;
+  const Rows rw = rows_of<PAGED>(p, b);
+  const Keys ks = keys_of<BN>(p, rw, qt);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, h = lane >> 5;
+  const int row = qt * kBM + 32 * wave + lq;
+  const int tok = row / p.group;
+  if (tok >= rw.nq || ks.parts <= 1) return;
+  const int hq = hkv * p.group + (row - tok * p.group);
+  const float* w = p.ws + (size_t)tile * p.n_parts * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
+  float m = -INFINITY;
+  for (int i = 0; i < ks.parts; ++i) m = fmaxf(m, w[i * part_floats<D>() + 2 * lq]);
+  const float shift = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f32x4 o[4];
+#pragma unroll
+  for (int a = 0; a < 4; ++a) o[a] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < ks.parts; ++i) {
+    const float* wi = w + i * part_floats<D>();
+    const float2 ml = *(const float2*)(wi + 2 * lq);
+    const float f = fast_exp2(ml.x - shift);
+    l = fmaf(ml.y, f, l);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      const f32x4 x = *(const f32x4*)(wi + 64 + (4 * db + a) * 256 + 4 * lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[a][e] = fmaf(x[e], f, o[a][e]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)tok * p.o_ss;
+#pragma unroll
+  for (int a = 0; a < 4; ++a)
+    store4<T>(out + 32 * db + 8 * a + 4 * h, o[a][0] * inv, o[a][1] * inv, o[a][2] * inv, o[a][3] * inv, p.vec_out);
+}
+
+// Key tiles that one row tile can have at most.
+int64_t most_tiles(int64_t keys, int window, int sinks, int group, int bn) {
+  int64_t n = (keys + bn - 1) / bn;
+  if (window > 0) {
+    const int64_t w = ((int64_t)window + kBM / group + 1) / bn + 2 + ((int64_t)sinks + bn - 1) / bn;
+    n = n < w ? n : w;
+  }
+  return n < 1 ? 1 : n;
+}
+
+// Parts of a row tile's keys.  Where the row tiles fill the device there is one; else the key tiles are shared
+// so that there are about as many workgroups as run at once, kMinShare key tiles each at least.
+void plan_parts(WinParams& p, int64_t keys, int d_k, int esize) {
+  const int bn = esize == 2 ? 64 : 32;
+  const int64_t most = most_tiles(keys, p.window, p.sinks, p.group, bn);
+  const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
+  const int64_t slots = (int64_t)tl_device_cus() * 2;
+  int64_t share = (tiles * most + slots - 1) / slots;
+  share = share < kMinShare ? kMinShare : share;
+  const int64_t parts = (most + share - 1) / share;
+  p.share = (int)share;
+  p.n_parts = tiles >= slots || parts < 2 ? 1 : (int)parts;
+}
+
+size_t part_bytes(int d_k) { return (d_k == 64 ? part_floats<64>() : part_floats<128>()) * sizeof(float); }
 
 template <typename T, int D>
 int launch_window(const WinParams& p, bool paged, hipStream_t st) {
-  const int64_t items = (int64_t)p.batch * p.n_head * p.n_qt;
+  const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
+  const int64_t items = tiles * p.n_parts;
   if (items > (1 << 30)) return TL_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)((items + 7) / 8 * 8));
   if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
+  int e = tl_launch_status();
+  if (e || p.n_parts == 1) return e;
+  const dim3 join((unsigned)tiles, D / 32);
+  if (paged) hipLaunchKernelGGL((window_join_kernel<T, D, true>), join, dim3(kThreads), 0, st, p);
+  else hipLaunchKernelGGL((window_join_kernel<T, D, false>), join, dim3(kThreads), 0, st, p);
   return tl_launch_status();
 }
 
-int window_entry(WinParams& p, bool paged, int d_k, const int64_t* qs, const int64_t* ks, const int64_t* vs,
+int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t workspace_bytes, int d_k, const int64_t* qs, const int64_t* ks, const int64_t* vs,
                  const int64_t* os, float sm_scale, int dtype, void* stream) {
   if (!p.q || !p.k || !p.v || !p.o || !qs || !ks || !vs || !os || p.batch < 0 || p.n_head < 0 || p.n_kv < 1 ||
       p.n_head % p.n_kv || p.seq_q < 0 || p.window < 0 || p.sinks < 0)
@@ -412,8 +587,17 @@ int window_entry(WinParams& p, bool paged, int d_k, const int64_t* qs, const int
   p.v_sb = vs[0], p.v_sh = vs[1], p.v_ss = vs[2];
   p.o_sb = os[0], p.o_sh = os[1], p.o_ss = os[2];
   p.group = p.n_head / p.n_kv;
-  p.n_qt = (p.seq_q + kBM - 1) / kBM;
+  if ((int64_t)p.seq_q * p.group > (1 << 30)) return TL_ERR_UNSUPPORTED;
+  p.n_qt = (p.seq_q * p.group + kBM - 1) / kBM;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.vec_out = ((uintptr_t)p.o % (4 * esize)) == 0 && os[0] % 4 == 0 && os[1] % 4 == 0 && os[2] % 4 == 0;
+  plan_parts(p, keys, d_k, esize);
+  if (p.n_parts > 1) {
+    // without room for the parts the call runs whole
+    const size_t need = (size_t)p.batch * p.n_kv * p.n_qt * p.n_parts * part_bytes(d_k);
+    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) p.n_parts = 1;
+    p.ws = (float*)workspace;
+  }
   hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
     case TL_DTYPE_F32: return d_k == 64 ? launch_window<F32, 64>(p, paged, st) : launch_window<F32, 128>(p, paged, st);
@@ -426,7 +610,24 @@ int window_entry(WinParams& p, bool paged, int d_k, const int64_t* qs, const int
 
 extern "C" {
 
-int tl_window_attention(const void* q, const void* k, const void* v, void* o, int batch, int n_head, int n_kv_head,
+size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q, int most_keys, int d_k, int window,
+                                 int sinks, int dtype) {
+  if (batch < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || seq_q < 1 || seq_q > (1 << 29) || most_keys < 1 ||
+      window < 0 || sinks < 0 || (d_k != 64 && d_k != 128) || (int64_t)seq_q * (n_head / n_kv_head) > (1 << 30) ||
+      (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16))
+    return 0;
+  WinParams p{};
+  p.batch = batch;
+  p.n_kv = n_kv_head;
+  p.group = n_head / n_kv_head;
+  p.n_qt = (seq_q * p.group + kBM - 1) / kBM;
+  p.window = window;
+  p.sinks = sinks;
+  plan_parts(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2);
+  return p.n_parts == 1 ? 0 : (size_t)batch * n_kv_head * p.n_qt * p.n_parts * part_bytes(d_k);
+}
+
+int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace, size_t workspace_bytes, int batch, int n_head, int n_kv_head,
                         int seq_q, int seq_k, int d_k, const int64_t* q_strides, const int64_t* k_strides,
                         const int64_t* v_strides, const int64_t* o_strides, float sm_scale, int window, int sinks,
                         int dtype, void* stream) {
@@ -444,12 +645,12 @@ int tl_window_attention(const void* q, const void* k, const void* v, void* o, in
   p.seq_k = seq_k;
   p.window = window;
   p.sinks = sinks;
-  return window_entry(p, false, d_k, q_strides, k_strides, v_strides, o_strides, sm_scale, dtype, stream);
+  return window_entry(p, false, seq_k, workspace, workspace_bytes, d_k, q_strides, k_strides, v_strides, o_strides, sm_scale, dtype, stream);
 }
 
 int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                int max_pages, int n_pages, int page_size, const int32_t* cache_lens,
-                               const int32_t* new_lens, void* o, int batch, int n_new, int n_head, int n_kv_head,
+                               const int32_t* new_lens, void* o, void* workspace, size_t workspace_bytes, int batch, int n_new, int n_head, int n_kv_head,
                                int d_k, const int64_t* q_strides, const int64_t* k_page_strides,
                                const int64_t* v_page_strides, const int64_t* o_strides, float sm_scale, int window,
                                int sinks, int dtype, void* stream) {
@@ -472,7 +673,7 @@ int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v
   p.seq_q = n_new;
   p.window = window;
   p.sinks = sinks;
-  return window_entry(p, true, d_k, q_strides, k_page_strides, v_page_strides, o_strides, sm_scale, dtype, stream);
+  return window_entry(p, true, (int64_t)max_pages << shift, workspace, workspace_bytes, d_k, q_strides, k_page_strides, v_page_strides, o_strides, sm_scale, dtype, stream);
 }
 
 }  // extern "C"

@@ -127,13 +127,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "tl_paged_attention_prefill": (
         _c_int,
-        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp, _vp, _c_size,
          _c_int, _c_int, _c_int, _c_int, _c_int,
          _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
     ),
+    "tl_window_workspace_bytes": (
+        _c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "tl_window_attention": (
         _c_int,
-        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+        [_vp, _vp, _vp, _vp, _vp, _c_size, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
          _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
     ),
     "tl_copy_pages": (

@@ -205,7 +205,9 @@ def _attention_plan(pool, v_pool, table, lens, new_lens, q, n_head, n_kv_head, w
         if len(q) != 4 or q[0] != batch or q[2:] != (n_head, d_k):
             raise ValueError(f"q shape {q} is not (batch={batch}, n_new, n_head={n_head}, d_k={d_k})")
         q_str = _lib.strides(q[1] * n_head * d_k, d_k, n_head * d_k)  # {batch, head, seq}
-        return pages, (batch, q[1], n_head, n_kv_head, d_k, q_str, p_str, p_str, q_str)
+        ws = [_lib.load().tl_window_workspace_bytes(batch, n_head, n_kv_head, q[1], max_pages * page_size, d_k, window,
+                                                    sinks, code) for code in range(3)]  # by dtype code
+        return pages, (batch, q[1], n_head, n_kv_head, d_k, q_str, p_str, p_str, q_str), ws
     if math.prod(q) != batch * n_head * d_k:
         raise ValueError(f"q shape {q} is not (batch={batch}, n_head={n_head}, d_k={d_k})")
     q_str = _lib.strides(n_head * d_k, d_k)
@@ -241,21 +243,23 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
 
 
 def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_head: int, n_kv_head: int,
-                            new_lens=None, sm_scale: float | None = None, window: int = 0, sinks: int = 0, out=None):
+                            new_lens=None, sm_scale: float | None = None, window: int = 0, sinks: int = 0, out=None,
+                            workspace=None):
     """Queries ``(batch, n_new, n_head, d_k)`` at positions ``cache_lens[b] + i`` over the pages.
 
     The new tokens' own k and v are appended before.  ``new_lens`` as in :func:`paged_kv_append`: rows
     behind a sequence's tokens are left as they were.
     """
     _check_int32(page_table, cache_lens, new_lens)
-    pages, sizes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
-                                   _shape(new_lens), q_dev.shape, n_head, n_kv_head, window, sinks, True)
+    pages, sizes, ws_bytes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
+                                             _shape(new_lens), q_dev.shape, n_head, n_kv_head, window, sinks, True)
     code = same_dtype(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
+    ws = scratch(ws_bytes[code], workspace, key="window")
     if sm_scale is None:
         sm_scale = default_scale(k_pages.shape[3])
     launch(gpu.runtime().tl_paged_attention_prefill, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), *pages,
-           vp(cache_lens), vp(new_lens), vp(out), *sizes, float(sm_scale), int(window), int(sinks), code, None,
+           vp(cache_lens), vp(new_lens), vp(out), vp(ws), ws.nbytes if ws is not None else 0, *sizes, float(sm_scale), int(window), int(sinks), code, None,
            what="paged_attention_prefill")
     return out
 

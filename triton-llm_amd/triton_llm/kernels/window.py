@@ -12,13 +12,20 @@ zeros.  Keys outside of every row's view are not read.
 
 from __future__ import annotations
 
+import functools
+
 from triton_llm import _lib, gpu
-from ._common import contiguous_strides, default_scale, launch, same_dtype, vp
+from ._common import contiguous_strides, default_scale, launch, same_dtype, scratch, vp
 from .paged import check_window
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes) -> int:
+    return _lib.load().tl_window_workspace_bytes(*sizes)
+
+
 def window_attention_strided(q, k, v, out, *, batch, n_head, n_kv_head, seq_q, seq_k, d_k, q_strides, k_strides,
-                             v_strides, o_strides, window, sinks=0, sm_scale=None):
+                             v_strides, o_strides, window, sinks=0, sm_scale=None, workspace=None):
     """The kernel on raw layouts given by {batch, head, seq} element strides."""
     if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head:
         raise ValueError(f"n_head ({n_head}) must be a positive multiple of n_kv_head ({n_kv_head})")
@@ -32,13 +39,14 @@ def window_attention_strided(q, k, v, out, *, batch, n_head, n_kv_head, seq_q, s
         raise ValueError("seq_k must be >= 1")
     if sm_scale is None:
         sm_scale = default_scale(d_k)
-    launch(gpu.runtime().tl_window_attention, vp(q), vp(k), vp(v), vp(out), batch, n_head, n_kv_head, seq_q, seq_k,
+    ws = scratch(_workspace_bytes(batch, n_head, n_kv_head, seq_q, seq_k, d_k, window, sinks, code), workspace, key="window")
+    launch(gpu.runtime().tl_window_attention, vp(q), vp(k), vp(v), vp(out), vp(ws), ws.nbytes if ws is not None else 0, batch, n_head, n_kv_head, seq_q, seq_k,
            d_k, _lib.strides(*q_strides), _lib.strides(*k_strides), _lib.strides(*v_strides),
            _lib.strides(*o_strides), float(sm_scale), int(window), int(sinks), code, None, what="window_attention")
     return out
 
 
-def window_attention(q, k, v, window: int, sinks: int = 0, sm_scale: float | None = None, out=None):
+def window_attention(q, k, v, window: int, sinks: int = 0, sm_scale: float | None = None, out=None, workspace=None):
     """q ``(batch, n_head, seq_q, d_k)``, k/v ``(batch, n_kv_head, seq_k, d_k)``, contiguous; returns out like q."""
     if len(q.shape) != 4 or len(k.shape) != 4 or k.shape != v.shape:
         raise ValueError(f"expected q (B,Hq,Sq,D) and k/v (B,Hkv,Sk,D), got {q.shape}, {k.shape}, {v.shape}")
@@ -54,4 +62,4 @@ def window_attention(q, k, v, window: int, sinks: int = 0, sm_scale: float | Non
     ks = contiguous_strides(k.shape)[:3]
     return window_attention_strided(q, k, v, out, batch=batch, n_head=n_head, n_kv_head=n_kv, seq_q=seq_q,
                                     seq_k=seq_k, d_k=d_k, q_strides=qs, k_strides=ks, v_strides=ks, o_strides=qs,
-                                    window=window, sinks=sinks, sm_scale=sm_scale)
+                                    window=window, sinks=sinks, sm_scale=sm_scale, workspace=workspace)
