@@ -41,6 +41,7 @@ struct WinParams {
   int batch, n_head, n_kv, group, seq_q, seq_k, n_qt;
   int window, sinks;
   int share, n_parts;  // key tiles of a part at least, parts of a row tile at most
+  int q_step, n_lvl, xcd_groups;  // how workgroups are dealt (window_fwd_kernel)
   int vec_out;         // o's rows take 4 elements at once
   float* ws;           // [tile][part] of partial results (n_parts > 1)
   int64_t q_sb, q_sh, q_ss;
@@ -95,6 +96,9 @@ struct Tile16 {
   // Operands are read kAhead MFMAs ahead; the barriers keep the compiler from reading them all at
   // once, which their registers do not allow at d_k 128.
   static constexpr int kAhead = 4;
+  // The sum of a row's weights.  At d_k 64 the vector unit is the limit and the matrix unit half idle: there it is one
+  // more MFMA per 16 keys, ones . P^T, of the rounded weights (4 x 500 rows on prefixes, fp16: 51.4 -> 47.8 us).
+  static constexpr bool kSumMfma = D == 64;
   static __device__ __forceinline__ void scores(f32x16 (&s)[NMB], const Q& q, const char* kt, int lq, int h) {
     constexpr int NG = NMB * NKS;
     const char* row = kt + lq * ROWB;
@@ -118,7 +122,7 @@ struct Tile16 {
   }
   // s holds the probabilities; they are rounded to the storage type here (at most half a step
   // each, as the causal prefill does), the sum l is of the unrounded ones.
-  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], const f32x16 (&s)[NMB], const char* vt, int lane) {
+  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt, int lane) {
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
     constexpr int NG = 2 * NMB * NDB;
@@ -147,6 +151,10 @@ struct Tile16 {
       }
       if (g + kAhead < NG) fetch(g + kAhead);
       o[db] = M::mma(__builtin_bit_cast(frag, f[g]), __builtin_bit_cast(frag, pw[tt]), o[db]);
+      if (kSumMfma && db == 0) {
+        const frag ones = __builtin_bit_cast(frag, u32x4{T::one_pair, T::one_pair, T::one_pair, T::one_pair});
+        la = M::mma(ones, __builtin_bit_cast(frag, pw[tt]), la);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -155,6 +163,7 @@ struct Tile16 {
 template <int D>
 struct Tile32 {
   static constexpr int ROWB = D * 4, NDB = D / 32, NMB = 1;
+  static constexpr bool kSumMfma = false;
   struct Q {
     float f[D / 2];  // features h D / 2 .. of the row
   };
@@ -177,7 +186,7 @@ struct Tile32 {
       for (int i = 0; i < 4; ++i) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], q.f[4 * c + i], s[0], 0, 0, 0);
     }
   }
-  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], const f32x16 (&s)[NMB], const char* vt, int lane) {
+  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt, int lane) {
     const int lq = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -280,18 +289,20 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];  // (K, V) twice
 
-  // Workgroups are dealt to the 8 XCDs in turn; XCD x takes a contiguous range of (sequence, KV head,
-  // row tile, part), so that few KV heads share its L2.
-  const int n_tiles = p.batch * p.n_kv * p.n_qt;
-  const int n_items = n_tiles * p.n_parts;
-  const int per = (n_items + 7) / 8;
-  const int item = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
-  if ((int)(blockIdx.x / 8) >= per || item >= n_items) return;
-  const int tile = item / p.n_parts, part = item - tile * p.n_parts;
-  const int kvh = tile / p.n_qt;
-  const int qt = p.n_qt - 1 - (tile - kvh * p.n_qt);  // the longest rows first
+  // Workgroups are dealt to the 8 XCDs in turn.  The work is cut into groups, (sequence, KV head) x part
+  // of the keys x every q_step-th row tile, a multiple of 8 of them dealt to the XCDs in turn, so that
+  // an XCD's L2 holds the keys of few groups and sequences of unequal length spread over the
+  // XCDs.  Within an XCD the longest rows come first.
+  const int xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+  const int lvl = at / p.xcd_groups;
+  const int grp = (at - lvl * p.xcd_groups) * 8 + xcd;
+  const int unit_part = grp / p.q_step;
+  const int qt = (p.n_lvl - 1 - lvl) * p.q_step + (grp - unit_part * p.q_step);
+  const int kvh = unit_part / p.n_parts, part = unit_part - kvh * p.n_parts;
+  if (qt >= p.n_qt || kvh >= p.batch * p.n_kv) return;
   const int b = kvh / p.n_kv;
   const int hkv = kvh - b * p.n_kv;
+  const int tile = kvh * p.n_qt + qt;
   const Rows rw = rows_of<PAGED>(p, b);
   const Keys ks = keys_of<BN>(p, rw, qt);
   if (qt * kBM >= rw.nq * p.group || part >= ks.parts) return;
@@ -365,6 +376,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
   float m = -INFINITY, l = 0.f;
+  f32x16 la;  // kSumMfma: the row's sum in every register
+#pragma unroll
+  for (int r = 0; r < 16; ++r) la[r] = 0.f;
 
   // this wave's first and last position
   const int row0 = qt * kBM + 32 * wave;
@@ -399,11 +413,13 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
             if ((gone >> (2 * mb + (r >> 3))) & 1) s[mb][r] = -INFINITY;
       }
     }
+    // IEEE maximum: one v_maximum3_f32 for two scores, where fmaxf first quiets its operands
     float mx = s[0][0];
 #pragma unroll
     for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[mb][r]);
+      for (int r = 0; r < 16; r += 2)
+        mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, s[mb][r]), s[mb][r + 1]);
     mx = tlp::max_xor32(mx) * scale;
     // the maximum moves only when a score passes it by 2^8 (it only bounds the exponents)
     if (__any(mx > m + kRescaleLog2)) {
@@ -411,6 +427,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
       const float a = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
       l *= a;
+      if constexpr (TL::kSumMfma) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) la[r] *= a;
+      }
 #pragma unroll
       for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -422,9 +442,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[mb][r] = fast_exp2(fmaf(s[mb][r], scale, -shift));
-        l += s[mb][r];
+        if (!TL::kSumMfma) l += s[mb][r];
       }
-    TL::values(o, s, kt + TILEB, lane);
+    TL::values(o, la, s, kt + TILEB, lane);
   };
 
   const int t_lo = (int)((int64_t)ks.tiles * part / ks.parts), t_hi = (int)((int64_t)ks.tiles * (part + 1) / ks.parts);
@@ -453,9 +473,9 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     step(k0, kt, gone, all);
   }
 
-  l = tlp::sum_xor32(l);
+  l = TL::kSumMfma ? la[0] : tlp::sum_xor32(l);
   if (ks.parts > 1) {
-    float* w = p.ws + (size_t)item * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
+    float* w = p.ws + ((size_t)tile * p.n_parts + part) * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
     if (h == 0) {
       w[2 * lq] = m;
       w[2 * lq + 1] = l;
@@ -486,7 +506,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
   constexpr int BN = tile_keys<T>();
   const int tile = blockIdx.x, db = blockIdx.y;
   const int kvh = tile / p.n_qt;
-  const int qt = p.n_qt - 1 - (tile - kvh * p.n_qt);
+  const int qt = tile - kvh * p.n_qt;
   const int b = kvh / p.n_kv;
   const int hkv = kvh - b * p.n_kv;
   const Rows rw = rows_of<PAGED>(p, b);
@@ -536,10 +556,12 @@ int64_t most_tiles(int64_t keys, int window, int sinks, int group, int bn) {
 // Parts of a row tile's keys.  Where the row tiles fill the device there is one; else the key tiles are shared
 // so that there are about as many workgroups as run at once, kMinShare key tiles each at least.
 void plan_parts(WinParams& p, int64_t keys, int d_k, int esize) {
+  // workgroups that run on a CU at once: by registers at d_k 128, by LDS at d_k 64
+  const int per_cu = d_k == 64 ? 4 : 2;
   const int bn = esize == 2 ? 64 : 32;
   const int64_t most = most_tiles(keys, p.window, p.sinks, p.group, bn);
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
-  const int64_t slots = (int64_t)tl_device_cus() * 2;
+  const int64_t slots = (int64_t)tl_device_cus() * per_cu;
   int64_t share = (tiles * most + slots - 1) / slots;
   share = share < kMinShare ? kMinShare : share;
   const int64_t parts = (most + share - 1) / share;
@@ -550,11 +572,15 @@ void plan_parts(WinParams& p, int64_t keys, int d_k, int esize) {
 size_t part_bytes(int d_k) { return (d_k == 64 ? part_floats<64>() : part_floats<128>()) * sizeof(float); }
 
 template <typename T, int D>
-int launch_window(const WinParams& p, bool paged, hipStream_t st) {
+int launch_window(WinParams& p, bool paged, hipStream_t st) {
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
-  const int64_t items = tiles * p.n_parts;
-  if (items > (1 << 30)) return TL_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8));
+  if (tiles * p.n_parts > (1 << 27)) return TL_ERR_UNSUPPORTED;
+  const int64_t unit_parts = (int64_t)p.batch * p.n_kv * p.n_parts;
+  p.q_step = 8;  // unit_parts * q_step is a multiple of 8
+  while (p.q_step > 1 && unit_parts % (16 / p.q_step) == 0) p.q_step /= 2;
+  p.n_lvl = (p.n_qt + p.q_step - 1) / p.q_step;
+  p.xcd_groups = (int)(unit_parts * p.q_step / 8);
+  const dim3 grid((unsigned)(8 * p.xcd_groups * p.n_lvl));
   if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
   int e = tl_launch_status();
