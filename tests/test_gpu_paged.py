@@ -99,6 +99,13 @@ def run_decode(dtype, Hq, Hkv, D, page, lens, window, sinks, len_add=0, scale=No
     P.check(f"decode {dtype} {Hq}/{Hkv} d{D} page {page} window {window} sinks {sinks}", P.back(out, dtype), want, tol)
 
 
+@pytest.fixture(params=["pair", "shares"])
+def mode(request, monkeypatch):
+    """Short caches take a workgroup a (sequence, KV head), others equal shares of all blocks; the override sends
+    every call through the shares."""
+    P.H.set_override(monkeypatch, "TRITON_LLM_HIP_DECODE_SHARES", 1 if request.param == "shares" else None)
+
+
 SHORT = [0, 1, 15, 16, 17, 31, 33, 64, 100, 255, 257]
 
 
@@ -106,17 +113,17 @@ SHORT = [0, 1, 15, 16, 17, 31, 33, 64, 100, 255, 257]
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("page,window,sinks", [(16, 0, 0), (32, 20, 3), (256, 1, 0), (16, 64, 16), (64, 50, 40),
                                                (16, 16, 1 << 30), (1024, 1 << 30, 0), (16, 33, 17)])
-def test_decode_lengths(dtype, D, page, window, sinks):
+def test_decode_lengths(mode, dtype, D, page, window, sinks):
     run_decode(dtype, 6, 2, D, page, SHORT, window, sinks)
 
 
 @pytest.mark.parametrize("Hq,Hkv", [(1, 1), (4, 2), (4, 1), (5, 1), (6, 1), (14, 2), (8, 1), (12, 1), (17, 1), (9, 9)])
 @pytest.mark.parametrize("dtype,D", [("bfloat16", 128), ("float32", 64), ("float16", 64), ("float32", 128)])
-def test_decode_groups(Hq, Hkv, dtype, D):
+def test_decode_groups(mode, Hq, Hkv, dtype, D):
     run_decode(dtype, Hq, Hkv, D, 16, [3, 200, 0, 90], 0, 0)
 
 
-def test_decode_many_sequences_and_len_add():
+def test_decode_many_sequences_and_len_add(mode):
     rng = np.random.default_rng(5)
     run_decode("bfloat16", 4, 2, 64, 16, rng.integers(0, 90, 150), 0, 0, len_add=1)
     run_decode("float16", 4, 2, 64, 32, rng.integers(-3, 60, 65), 25, 2, len_add=-2)
@@ -128,12 +135,12 @@ def test_decode_long_and_past_the_table():
     run_decode("float16", 2, 1, 64, 16, [1 << 30, 40, -7], 0, 0, max_pages=5)  # lengths end where the table does
 
 
-def test_decode_scales():
+def test_decode_scales(mode):
     for scale in (-0.2, 0.0, 4.0):
         run_decode("float16", 2, 1, 64, 16, [40, 3], 0, 0, scale=scale)
 
 
-def test_decode_pages_that_are_not_there():
+def test_decode_pages_that_are_not_there(mode):
     def edit(table, n_pages):
         table[0, 1], table[0, 4], table[2, :] = -1, n_pages, 2 ** 31 - 1
         table[1, 0] = -2 ** 31
@@ -143,6 +150,7 @@ def test_decode_pages_that_are_not_there():
 
 def test_decode_fewer_compute_units(monkeypatch):
     """Shares of many blocks: pairs begin and end inside them, and over several."""
+    P.H.set_override(monkeypatch, "TRITON_LLM_HIP_DECODE_SHARES", 1)
     for cus in (1, 3):
         P.H.set_override(monkeypatch, "TRITON_LLM_HIP_MAX_CUS", cus)
         run_decode("bfloat16", 6, 2, 64, 16, [700, 0, 1300, 5, 64], 0, 0)

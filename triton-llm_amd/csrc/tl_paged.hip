@@ -8,6 +8,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 using namespace tlpg;
 
 namespace {
@@ -262,6 +264,8 @@ constexpr int kDecThreads = 256;
 constexpr int kDecWaves = kDecThreads / 64;
 constexpr int kMaxShares = 2048;  // workgroups at most: bounds the workspace
 constexpr int kMinShare = 4;      // blocks of a share at least: one for each wave
+constexpr int64_t kPairMaxBytes = 384ll << 10;
+constexpr int64_t kPairMaxAll = 64ll << 20;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kAuxNontemporal = 2;  // buffer-load cache policy: nt
 constexpr uint32_t kPastEnd = 0x7FFFFF00u;  // an offset that every resource here ends before
@@ -311,55 +315,41 @@ __device__ __forceinline__ Seen seen_of(const DecodeParams& p, int b) {
   return s;
 }
 
-__device__ __forceinline__ int64_t wave_scan(int64_t x, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t y = __shfl_up(x, d);
-    if (lane >= d) x += y;
-  }
+__device__ __forceinline__ bool row_seen(const Seen& s, int sinks, int pos) {
+  return pos < s.len && (pos >= s.lo || pos < sinks);
+}
+
+// Sums over the lanes up to and with each, by DPP moves: rows of 16 first, then row to row.
+__device__ __forceinline__ int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // row_shr:1
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15 into rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31 into rows 2 and 3
   return x;
 }
 
-// Blocks of every pair of sequences [0, b) and of all sequences.
-__device__ __forceinline__ void blocks_before(const DecodeParams& p, int b, int lane, int64_t& before, int64_t& total) {
-  int64_t t = 0, u = 0;
-  for (int i = lane; i < p.batch; i += 64) {
-    const int64_t n = seen_of(p, i).n;
-    t += n;
-    u += i < b ? n : 0;
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) {
-    t += __shfl_xor(t, off);
-    u += __shfl_xor(u, off);
-  }
-  total = uni(t) * p.n_pairs;
-  before = uni(u) * p.n_pairs;
+// The flattened blocks of the sequences b0 .. b0 + 63: lane i's sequence has n a pair, and all up to and
+// with it have `incl` behind `base`.
+struct SeqBlocks {
+  int n, incl;
+};
+__device__ __forceinline__ SeqBlocks seq_blocks(const DecodeParams& p, int b0, int base, int lane) {
+  SeqBlocks s;
+  s.n = b0 + lane < p.batch ? seen_of(p, b0 + lane).n : 0;
+  s.incl = base + wave_scan(s.n * p.n_pairs);
+  return s;
 }
 
 // Blocks of a share: an even part, whole rounds of the waves.
-__device__ __forceinline__ int64_t share_blocks(const DecodeParams& p, int64_t total) {
-  int64_t r = (total + p.n_shares - 1) / p.n_shares;
+__device__ __forceinline__ int share_blocks(const DecodeParams& p, int total) {
+  int r = (int)(((unsigned)total + p.n_shares - 1) / p.n_shares);
   r = r < kMinShare ? kMinShare : r;
   return (r + kDecWaves - 1) / kDecWaves * kDecWaves;
-}
-
-// The sequence that owns row r of the flattened blocks (r < total), and its first row.
-__device__ __forceinline__ int owner_of(const DecodeParams& p, int64_t r, int lane, int64_t& start) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const int64_t n = b0 + lane < p.batch ? (int64_t)seen_of(p, b0 + lane).n * p.n_pairs : 0;
-    const int64_t incl = base + wave_scan(n, lane);
-    const uint64_t hit = __ballot(incl > r);
-    if (hit) {
-      const int l = __ffsll((unsigned long long)hit) - 1;
-      start = uni(__shfl(incl - n, l));
-      return uni(b0 + l);
-    }
-    base = uni(__shfl(incl, 63));
-  }
-  start = base;
-  return p.batch - 1;  // not reached for r < total
 }
 
 template <int W>
@@ -367,17 +357,18 @@ struct Slice {
   uint32_t w[W];
 };
 
+// A row's slice at byte offset voff + soff of a block (soff the same on every lane).
 template <int W>
-__device__ __forceinline__ void load_slice(Slice<W>& s, __amdgpu_buffer_rsrc_t r, uint32_t voff) {
+__device__ __forceinline__ void load_slice(Slice<W>& s, __amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff) {
   if constexpr (W == 2) {
-    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, voff, 0, kAuxNontemporal));
+    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, voff, soff, kAuxNontemporal));
     s.w[0] = a.x;
     s.w[1] = a.y;
   } else {
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) {
       const u32x4 a =
-          __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff + 16 * i, 0, kAuxNontemporal));
+          __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff + 16 * i, soff, kAuxNontemporal));
       s.w[4 * i + 0] = a.x;
       s.w[4 * i + 1] = a.y;
       s.w[4 * i + 2] = a.z;
@@ -402,20 +393,29 @@ __device__ __forceinline__ float dot_slice(const Slice<W>& q, const Slice<W>& k)
   return d;
 }
 
+// Wave priority by what is done of the share: without it a CU's oldest workgroup runs ahead of its youngest, and
+// equal shares end far apart.
+__device__ __forceinline__ void set_progress_priority(int done, int share) {
+  const int q = 4 * done / share;
+  if (q <= 0) __builtin_amdgcn_s_setprio(3);
+  else if (q == 1) __builtin_amdgcn_s_setprio(2);
+  else if (q == 2) __builtin_amdgcn_s_setprio(1);
+  else __builtin_amdgcn_s_setprio(0);
+}
+
 // Buffer resource of one block of 16 rows, from wave-uniform values.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const char* base, uint32_t bytes) {
   const int64_t a = uni((int64_t)(uintptr_t)base);
   return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)a, (short)0, (int)bytes, kBufRsrcWord3);
 }
 
-// 16 lanes read a row, a wave 4 rows a load and a block of 16 positions in 4; wave w takes
-// blocks w, w + 4, ... of the segment.
-template <typename T, int D, int G>
-__global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams p) {
+// 16 lanes read a row, a wave 4 rows a load and a block of 16 positions in 4; wave w takes blocks
+// w, w + NW, ... of the segment, NB of them at a time.  PAIR: a workgroup takes a whole pair (see pair_mode).
+template <typename T, int D, int G, int NW, int NB, bool PAIR>
+__global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
   constexpr int EPL = D / 16;           // elements of a lane's slice of a row
   constexpr int W = EPL * T::size / 4;  // its 32-bit words
   constexpr int U = 4;                  // rows of a block that a lane reads
-  constexpr int NW = kDecWaves;
   using B = typename T::bits;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)threadIdx.x >> 6);
@@ -423,11 +423,13 @@ __global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams 
   const int n_chunks = p.n_pairs / p.n_kv;
   __shared__ float s_m[NW][G], s_l[NW][G];
   __shared__ float s_acc[NW][G][D];
-  const uint32_t lane_bytes = sub * (EPL * T::size);
+  const uint32_t k_lane = rowg * p.k_row_bytes + sub * (EPL * T::size);
+  const uint32_t v_lane = rowg * p.v_row_bytes + sub * (EPL * T::size);
 
-  // Blocks [v0, v1) of the Seen blocks of pair `pair` of sequence b.
+  // Blocks [v0, v1) of the Seen blocks of pair `pair` of sequence b; r0 of share blocks of the workgroup's
+  // share are done before.
   auto segment = [&](const int b, const Seen& sn, const int pair, const int v0, const int v1, const bool whole,
-                     const int slot) {
+                     const int slot, const int done, const int share) {
     const int hkv = pair / n_chunks;
     const int hq0 = hkv * p.group + (pair - hkv * n_chunks) * G;
     const int n_g = min(G, hkv * p.group + p.group - hq0);
@@ -447,48 +449,78 @@ __global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams 
     const int32_t* row = p.pm.table + (int64_t)b * p.pm.max_pages;
     const int shift = p.pm.shift;
     auto block_at = [&](int v) { return v < sn.ns ? v : v - sn.ns + sn.wb; };
+    const char* const kh = (const char*)p.k + hkv * p.k_sh * T::size;
+    const char* const vh = (const char*)p.v + hkv * p.v_sh * T::size;
 
     int pages = 0;  // lane i: the page of this wave's block (it & ~63) + i
     int it = 0;
-    for (int v = v0 + wave; v < v1; v += NW, ++it) {
+    for (int v = v0 + wave; v < v1; v += NW * NB, it += NB) {
       if ((it & 63) == 0) {
         const int mine = v + NW * lane;
         pages = mine < v1 ? row[block_at(mine) >> (shift - kBlkShift)] : -1;
       }
-      const int page = __builtin_amdgcn_readlane(pages, it & 63);
-      const bool there = (unsigned)page < (unsigned)p.pm.n_pages;
-      const int pos0 = block_at(v) << kBlkShift;
-      const int in_page = pos0 & ((1 << shift) - 1);
-      const int64_t id = there ? page : 0;
-      const auto krs = block_rsrc((const char*)p.k + (id * p.k_sp + hkv * p.k_sh) * T::size + (int64_t)in_page * p.k_row_bytes,
-                                  there ? 15 * p.k_row_bytes + D * T::size : 0);
-      const auto vrs = block_rsrc((const char*)p.v + (id * p.v_sp + hkv * p.v_sh) * T::size + (int64_t)in_page * p.v_row_bytes,
-                                  there ? 15 * p.v_row_bytes + D * T::size : 0);
-      Slice<W> kr[U], vr[U];
-      bool seen[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = 4 * u + rowg;
-        const int pos = pos0 + r;
-        // hidden rows may hold anything (NaN among it): they are not read, and read as zeros
-        seen[u] = there && pos < sn.len && (pos >= sn.lo || pos < p.sinks);
-        load_slice(kr[u], krs, seen[u] ? r * p.k_row_bytes + lane_bytes : kPastEnd);
-        load_slice(vr[u], vrs, seen[u] ? r * p.v_row_bytes + lane_bytes : kPastEnd);
+      if constexpr (!PAIR) {
+        if ((it & 3) == 0) set_progress_priority(done + it * NW, share);
       }
-      float s[G][U];
+      Slice<W> kr[NB][U], vr[NB][U];
+      bool full[NB];
+      int pos0[NB];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int vi = v + i * NW;
+        const int page = __builtin_amdgcn_readlane(pages, (it + i) & 63);  // -1 past the segment
+        const bool there = (unsigned)page < (unsigned)p.pm.n_pages;
+        pos0[i] = block_at(vi) << kBlkShift;
+        const int in_page = pos0[i] & ((1 << shift) - 1);
+        const int64_t id = there ? page : 0;
+        const auto krs = block_rsrc(kh + id * p.k_sp * T::size + (int64_t)in_page * p.k_row_bytes,
+                                    there ? 15 * p.k_row_bytes + D * T::size : 0);
+        const auto vrs = block_rsrc(vh + id * p.v_sp * T::size + (int64_t)in_page * p.v_row_bytes,
+                                    there ? 15 * p.v_row_bytes + D * T::size : 0);
+        full[i] = there && pos0[i] + kBlk <= sn.len && (pos0[i] >= sn.lo || pos0[i] + kBlk <= p.sinks);
+        if (!there) pos0[i] = sn.len;  // hidden throughout
+        if (full[i]) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) load_slice(kr[i][u], krs, k_lane, 4 * u * p.k_row_bytes);
+#pragma unroll
+          for (int u = 0; u < U; ++u) load_slice(vr[i][u], vrs, v_lane, 4 * u * p.v_row_bytes);
+        } else {
+          // hidden rows may hold anything (NaN among it): they are not read, and count as zeros
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const bool seen = row_seen(sn, p.sinks, pos0[i] + 4 * u + rowg);
+            load_slice(kr[i][u], krs, seen ? k_lane + 4 * u * p.k_row_bytes : kPastEnd, 0);
+            load_slice(vr[i][u], vrs, seen ? v_lane + 4 * u * p.v_row_bytes : kPastEnd, 0);
+          }
+        }
+      }
+      float s[G][NB * U];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int g = 0; g < G; ++g) s[g][i * U + u] = row16_sum(dot_slice<T>(qs[g], kr[i][u])) * p.scale_log2;
+        if (!full[i]) {
+          asm volatile("");
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const bool seen = row_seen(sn, p.sinks, pos0[i] + 4 * u + rowg);
+#pragma unroll
+            for (int g = 0; g < G; ++g) s[g][i * U + u] = seen ? s[g][i * U + u] : -INFINITY;
+          }
+        }
+      }
+      // the maximum moves only when a score passes it by 2^8 (it only bounds the exponents)
       bool grow = false;
       float mb[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
+        mb[g] = s[g][0];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float d = row16_sum(dot_slice<T>(qs[g], kr[u])) * p.scale_log2;
-          s[g][u] = seen[u] ? d : -INFINITY;
-        }
-        mb[g] = fmaxf(fmaxf(s[g][0], s[g][1]), fmaxf(s[g][2], s[g][3]));
+        for (int u = 1; u < NB * U; ++u) mb[g] = fmaxf(mb[g], s[g][u]);
         grow |= mb[g] > m[g] + kRescaleLog2;
       }
-      // the maximum moves only when a score passes it by 2^8 (it only bounds the exponents)
       if (__any(grow)) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -500,31 +532,32 @@ __global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams 
           for (int e = 0; e < EPL; ++e) acc[g][e] *= a;
         }
       }
-      float pu[G][U];
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float base = m[g] == -INFINITY ? 0.f : m[g];
 #pragma unroll
+        for (int u = 0; u < NB * U; ++u) {
+          s[g][u] = fast_exp2(s[g][u] - base);
+          l[g] += s[g][u];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
         for (int u = 0; u < U; ++u) {
-          pu[g][u] = fast_exp2(s[g][u] - base);
-          l[g] += pu[g][u];
+          float vf[EPL];
+          if constexpr (T::size == 4) {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) vf[e] = __uint_as_float(vr[i][u].w[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < W; ++e) unpack2<T>(vr[i][u].w[e], vf[2 * e], vf[2 * e + 1]);
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) acc[g][e] = fmaf(s[g][i * U + u], vf[e], acc[g][e]);
         }
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float vf[EPL];
-        if constexpr (T::size == 4) {
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) vf[i] = __uint_as_float(vr[u].w[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < W; ++i) unpack2<T>(vr[u].w[i], vf[2 * i], vf[2 * i + 1]);
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int e = 0; e < EPL; ++e) acc[g][e] = fmaf(pu[g][u], vf[e], acc[g][e]);
-      }
     }
 
     // join the wave's four rows of a load, then the waves
@@ -555,7 +588,7 @@ __global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams 
       }
     }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < n_g * D; idx += kDecThreads) {
+    for (int idx = threadIdx.x; idx < n_g * D; idx += 64 * NW) {
       const int g = idx / D, d = idx - g * D;
       float mx = -INFINITY;
 #pragma unroll
@@ -581,64 +614,113 @@ __global__ __launch_bounds__(kDecThreads) void paged_decode_kernel(DecodeParams 
     }
   };
 
-  int64_t before, total;
-  blocks_before(p, 0, lane, before, total);
-  const int64_t rpb = uni(share_blocks(p, total));
-  const int64_t r0 = (int64_t)blockIdx.x * rpb;
-  if (r0 >= total) return;
-  const int64_t r1 = r0 + rpb < total ? r0 + rpb : total;
-  for (int64_t r = r0; r < r1;) {
-    int64_t seq0;
-    const int b = owner_of(p, r, lane, seq0);
-    Seen sn = seen_of(p, b);
-    const int pair = uni((int)((r - seq0) / sn.n));
-    const int64_t pair0 = seq0 + (int64_t)pair * sn.n;
-    const int v0 = (int)(r - pair0);
-    const int v1 = (int)((r1 - pair0) < sn.n ? (r1 - pair0) : sn.n);
-    segment(b, sn, pair, v0, v1, v0 == 0 && v1 == sn.n, v0 == 0 ? 1 : 0);
-    r = pair0 + v1;
+  if constexpr (PAIR) {
+    const int b = (int)blockIdx.x / p.n_pairs;
+    const Seen sn = seen_of(p, b);
+    segment(b, sn, (int)blockIdx.x - b * p.n_pairs, 0, sn.n, true, 0, 0, 0);
+  } else {
+    // up to 64 sequences stay in the lanes; of more every look-up walks the lengths again
+    SeqBlocks sb = seq_blocks(p, 0, 0, lane);
+    int total = uni(__builtin_amdgcn_readlane(sb.incl, 63));
+    for (int b0 = 64; b0 < p.batch; b0 += 64)
+      total = uni(__builtin_amdgcn_readlane(seq_blocks(p, b0, total, lane).incl, 63));
+    const int rpb = uni(share_blocks(p, total));
+    const int64_t first = (int64_t)blockIdx.x * rpb;
+    if (first >= total) return;
+    const int r0 = (int)first, r1 = (int)min((int64_t)total, first + rpb);
+    for (int r = r0; r < r1;) {
+      int b0 = 0;
+      SeqBlocks s = sb;
+      while (b0 + 64 < p.batch && uni(__builtin_amdgcn_readlane(s.incl, 63)) <= r) {
+        b0 += 64;
+        s = seq_blocks(p, b0, uni(__builtin_amdgcn_readlane(s.incl, 63)), lane);
+      }
+      const int li = __ffsll((unsigned long long)__ballot(s.incl > r)) - 1;
+      const int b = uni(b0 + li);
+      const int n = uni(__builtin_amdgcn_readlane(s.n, uni(li)));
+      const int seq0 = uni(__builtin_amdgcn_readlane(s.incl, uni(li))) - n * p.n_pairs;
+      const Seen sn = seen_of(p, b);
+      const int pair = (r - seq0) / n;
+      const int pair0 = seq0 + pair * n;
+      const int v0 = r - pair0, v1 = min(r1 - pair0, n);
+      segment(b, sn, pair, v0, v1, v0 == 0 && v1 == n, v0 == 0 ? 1 : 0, r - r0, r1 - r0);
+      r = pair0 + v1;
+    }
   }
 }
 
 // One wave a (sequence, query head): join the shares of its pair.  A pair inside one share
-// is finished already; a sequence that sees nothing gets zeros here.
+// is finished already; a sequence that sees nothing gets zeros here.  All latency: lane s holds share s's
+// (m, l), accumulators are read eight shares at a time.
 template <typename T, int D>
 __global__ __launch_bounds__(64) void paged_combine_kernel(DecodeParams p) {
-  constexpr int NJ = D / 64;
+  constexpr int NJ = D / 64, R = 8;
   using B = typename T::bits;
   const int hq = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
-  const Seen sn = seen_of(p, b);
   B* o = (B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh;
-  if (sn.n == 0) {
-    for (int d = lane; d < D; d += 64) o[d] = 0;
+  int total = 0, before = 0, n = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const SeqBlocks s = seq_blocks(p, b0, total, lane);
+    if (b >= b0 && b < b0 + 64) {
+      n = uni(__builtin_amdgcn_readlane(s.n, b - b0));
+      before = uni(__builtin_amdgcn_readlane(s.incl, b - b0)) - n * p.n_pairs;
+    }
+    total = uni(__builtin_amdgcn_readlane(s.incl, 63));
+  }
+  if (n == 0) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = 0;
     return;
   }
-  int64_t before, total;
-  blocks_before(p, b, lane, before, total);
-  const int64_t rpb = share_blocks(p, total);
+  const int rpb = uni(share_blocks(p, total));
   const int hkv = hq / p.group, in = hq - hkv * p.group;
   const int pair = hkv * (p.n_pairs / p.n_kv) + in / p.heads_per_pair;
   const int g = in % p.heads_per_pair;
-  const int64_t pair0 = before + (int64_t)pair * sn.n;
-  const int64_t first = pair0 / rpb;
-  const int parts = (int)((pair0 + sn.n - 1) / rpb - first) + 1;
+  const int pair0 = before + pair * n;
+  const int first = pair0 / rpb;
+  const int parts = (pair0 + n - 1) / rpb - first + 1;
   if (parts == 1) return;
   auto at = [&](int s) { return ((first + s) * 2 + (s == 0 ? 1 : 0)) * p.heads_per_pair + g; };
-  float mx = -INFINITY;
-  for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, p.ws_ml[at(s) * 2]);
+  auto load = [&](int s0, float (&r)[R][NJ]) {
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) r[k][j] = s0 + k < parts ? p.ws_acc[(int64_t)at(s0 + k) * D + lane + 64 * j] : 0.f;
+  };
+  float r[R][NJ];
+  load(0, r);
+  const float2* ml = (const float2*)p.ws_ml;
+  const float2 e0 = lane < parts ? ml[at(lane)] : make_float2(-INFINITY, 0.f);
+  float mx = e0.x;
+  for (int s = lane + 64; s < parts; s += 64) mx = fmaxf(mx, ml[at(s)].x);
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
   const float base = mx == -INFINITY ? 0.f : mx;
-  float ls = 0.f, a[NJ];
+  float ls = 0.f, wl = 0.f, a[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) a[j] = 0.f;
-  for (int s = 0; s < parts; ++s) {
-    const int64_t i = at(s);
-    const float w = fast_exp2(p.ws_ml[i * 2] - base);
-    ls += p.ws_ml[i * 2 + 1] * w;
+  for (int s0 = 0; s0 < parts; s0 += R) {
+    if ((s0 & 63) == 0) {
+      const int s = s0 + lane;
+      const float2 e = s0 == 0 ? e0 : s < parts ? ml[at(s)] : make_float2(-INFINITY, 0.f);
+      wl = s < parts ? fast_exp2(e.x - base) : 0.f;
+      ls += e.y * wl;
+    }
+    float rn[R][NJ];
+    if (s0 + R < parts) load(s0 + R, rn);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) a[j] = fmaf(p.ws_acc[i * D + lane + 64 * j], w, a[j]);
+    for (int k = 0; k < R; ++k) {
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wl), (s0 + k) & 63));
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) a[j] = fmaf(r[k][j], w, a[j]);
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) r[k][j] = rn[k][j];
   }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) ls += __shfl_xor(ls, off);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = from_f32<T>(ls == 0.f ? 0.f : a[j] / ls);
 }
@@ -657,12 +739,25 @@ int heads_per_pair(int n_head, int n_kv) { return n_head / n_kv < 8 ? n_head / n
 
 size_t ws_ml_bytes(int hpp) { return (size_t)kMaxShares * 2 * hpp * 2 * sizeof(float); }
 
+// A workgroup for each pair, which finishes it: no partial results, one launch.  Taken where the longest pair
+// there can be is short (pair_bytes of K and V) and the pairs are few bytes in all.
+bool pair_mode(const DecodeParams& p, int64_t pair_bytes) {
+  return !tl_overrides.decode_shares && pair_bytes <= kPairMaxBytes && pair_bytes * p.batch * p.n_pairs <= kPairMaxAll;
+}
+
 template <typename T, int D, int G>
 int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
+  const int64_t pair_bytes = most / ((int64_t)p.batch * p.n_pairs) * kBlk * 2 * D * T::size;
+  if (pair_mode(p, pair_bytes)) {
+    // 16 waves while a lane's state fits the 128 registers of a 1024-thread workgroup
+    constexpr int NW = D * G * T::size <= 512 ? 16 : 8;
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, G, NW, 2, true>), dim3(p.batch * p.n_pairs), dim3(64 * NW), 0, st, p);
+    return tl_launch_status();
+  }
   static int per_cu = 0;
   if (per_cu == 0) {
     int n = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_decode_kernel<T, D, G>, kDecThreads, 0) != hipSuccess ||
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_decode_kernel<T, D, G, kDecWaves, 1, false>, kDecThreads, 0) != hipSuccess ||
         n <= 0)
       n = 1;
     per_cu = n;
@@ -671,7 +766,7 @@ int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
   shares = shares < kMaxShares ? shares : kMaxShares;
   const int64_t full = (most + kMinShare - 1) / kMinShare;
   p.n_shares = (int)(shares < full ? shares : full);
-  hipLaunchKernelGGL((paged_decode_kernel<T, D, G>), dim3(p.n_shares), dim3(kDecThreads), 0, st, p);
+  hipLaunchKernelGGL((paged_decode_kernel<T, D, G, kDecWaves, 1, false>), dim3(p.n_shares), dim3(kDecThreads), 0, st, p);
   const int e = tl_launch_status();
   if (e) return e;
   hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(p.n_head, p.batch), dim3(64), 0, st, p);
@@ -873,6 +968,7 @@ int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_
   p.v_row_bytes = (uint32_t)(v_page_strides[2] * esize);
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   const int64_t most = most_blocks(cap, window, sinks) * batch * p.n_pairs;
+  if (most > INT32_MAX) return TL_ERR_UNSUPPORTED;  // blocks are counted in 32 bits
   hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
     case TL_DTYPE_F32: return launch_decode<F32>(p, d_k, most, st);
