@@ -266,6 +266,8 @@ constexpr int kMaxShares = 2048;  // workgroups at most: bounds the workspace
 constexpr int kMinShare = 4;      // blocks of a share at least: one for each wave
 constexpr int64_t kPairMaxBytes = 384ll << 10;
 constexpr int64_t kPairMaxAll = 64ll << 20;
+constexpr int64_t kPairFewBytes = 128ll << 10;
+constexpr int kPairMany = 64;
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kAuxNontemporal = 2;  // buffer-load cache policy: nt
 constexpr uint32_t kPastEnd = 0x7FFFFF00u;  // an offset that every resource here ends before
@@ -333,23 +335,67 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// The flattened blocks of the sequences b0 .. b0 + 63: lane i's sequence has n a pair, and all up to and
-// with it have `incl` behind `base`.
-struct SeqBlocks {
-  int n, incl;
+// How the blocks are dealt.  Even shares of the flattened blocks, whole rounds of the waves, where the pairs are many;
+// a share may then hold the end of one pair and the beginning of the next.  Where that costs a share at most two
+// rounds of the waves, every pair is cut by itself into parts of `share` blocks instead, so that no workgroup runs one
+// short segment after another: 8 pairs of 100 positions (d_k 128, bf16) 13.6 -> 10.0 us, 64 of 500 17.2 -> 14.2; 512 pairs
+// of 10000, where the parts would be twice the shares, 441 as shares and 486 as parts.
+// unit(n): what a pair of n blocks counts, blocks or parts; incl: those of sequences 0 .. lane, for all pairs.
+struct Layout {
+  bool padded;
+  int share, total;
+  int n, incl;  // lane's sequence (of the first 64)
+  __device__ __forceinline__ int unit(int blocks) const { return padded ? (blocks + share - 1) / share : blocks; }
 };
-__device__ __forceinline__ SeqBlocks seq_blocks(const DecodeParams& p, int b0, int base, int lane) {
-  SeqBlocks s;
-  s.n = b0 + lane < p.batch ? seen_of(p, b0 + lane).n : 0;
-  s.incl = base + wave_scan(s.n * p.n_pairs);
-  return s;
+__device__ __forceinline__ int last_lane(int x) { return uni(__builtin_amdgcn_readlane(x, 63)); }
+__device__ __forceinline__ int blocks_at(const DecodeParams& p, int b) { return b < p.batch ? seen_of(p, b).n : 0; }
+
+__device__ __forceinline__ Layout layout_of(const DecodeParams& p, int lane) {
+  Layout y;
+  y.n = blocks_at(p, lane);
+  y.incl = wave_scan(y.n * p.n_pairs);
+  y.total = last_lane(y.incl);
+  for (int b0 = 64; b0 < p.batch; b0 += 64) y.total += last_lane(wave_scan(blocks_at(p, b0 + lane) * p.n_pairs));
+  const int pairs = p.batch * p.n_pairs;
+  auto share_of = [&](int shares) {
+    const int r = max((int)(((unsigned)y.total + shares - 1) / shares), kMinShare);
+    return (r + kDecWaves - 1) / kDecWaves * kDecWaves;
+  };
+  y.share = share_of(p.n_shares);
+  y.padded = 2 * pairs <= p.n_shares && share_of(p.n_shares - pairs) <= y.share + 2 * kDecWaves;
+  if (y.padded) y.share = share_of(p.n_shares - pairs);
+  if (y.padded) {
+    y.incl = wave_scan(y.unit(y.n) * p.n_pairs);
+    y.total = last_lane(y.incl);
+    for (int b0 = 64; b0 < p.batch; b0 += 64) y.total += last_lane(wave_scan(y.unit(blocks_at(p, b0 + lane)) * p.n_pairs));
+  }
+  return y;
 }
 
-// Blocks of a share: an even part, whole rounds of the waves.
-__device__ __forceinline__ int share_blocks(const DecodeParams& p, int total) {
-  int r = (int)(((unsigned)total + p.n_shares - 1) / p.n_shares);
-  r = r < kMinShare ? kMinShare : r;
-  return (r + kDecWaves - 1) / kDecWaves * kDecWaves;
+// The sequence that unit r < total belongs to, and its first unit.
+struct Owner {
+  int b, first;
+};
+__device__ __forceinline__ Owner owner_of(const DecodeParams& p, const Layout& y, int r, int lane) {
+  int b0 = 0, n = y.unit(y.n) * p.n_pairs, incl = y.incl;
+  while (b0 + 64 < p.batch && last_lane(incl) <= r) {
+    const int base = last_lane(incl);
+    b0 += 64;
+    n = y.unit(blocks_at(p, b0 + lane)) * p.n_pairs;
+    incl = base + wave_scan(n);
+  }
+  const int li = uni(__ffsll((unsigned long long)__ballot(incl > r)) - 1);
+  return Owner{b0 + li, uni(__builtin_amdgcn_readlane(incl - n, li))};
+}
+// The first unit of sequence b.
+__device__ __forceinline__ int first_of(const DecodeParams& p, const Layout& y, int b, int lane) {
+  int base = 0, n = y.unit(y.n) * p.n_pairs, incl = y.incl;
+  for (int b0 = 64; b0 <= b; b0 += 64) {
+    base = last_lane(incl);
+    n = y.unit(blocks_at(p, b0 + lane)) * p.n_pairs;
+    incl = base + wave_scan(n);
+  }
+  return uni(__builtin_amdgcn_readlane(incl - n, b & 63));
 }
 
 template <int W>
@@ -393,6 +439,12 @@ __device__ __forceinline__ float dot_slice(const Slice<W>& q, const Slice<W>& k)
   return d;
 }
 
+// Blocks of a wave at a time in a pair's workgroup, whose waves are few: a block's K and V take D * size / 8
+// registers.
+template <typename T, int D>
+constexpr int kPairBlocks = D * T::size == 512 ? 1 : 2;
+constexpr int kPairWaves = 8;
+
 // Wave priority by what is done of the share: without it a CU's oldest workgroup runs ahead of its youngest, and
 // equal shares end far apart.
 __device__ __forceinline__ void set_progress_priority(int done, int share) {
@@ -409,17 +461,20 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const char* base, u
   return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)a, (short)0, (int)bytes, kBufRsrcWord3);
 }
 
-// 16 lanes read a row, a wave 4 rows a load and a block of 16 positions in 4; wave w takes blocks
+// 16 lanes read a row, a wave 4 rows a load and a block in 4 loads of K and 4 of V; wave w takes blocks
 // w, w + NW, ... of the segment, NB of them at a time.  PAIR: a workgroup takes a whole pair (see pair_mode).
+// (8 lanes with 16-byte loads for rows of 128 bytes were slower: 32 sequences, 15 / 5 heads, d_k 64, 1000 positions
+// 15.2 -> 17.0 us as pairs, 17.7 -> 18.9 as shares.)
 template <typename T, int D, int G, int NW, int NB, bool PAIR>
 __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
-  constexpr int EPL = D / 16;           // elements of a lane's slice of a row
+  constexpr int LPR = 16, RPL = 4;      // lanes of a row, rows of a load
+  constexpr int EPL = D / LPR;          // elements of a lane's slice of a row
   constexpr int W = EPL * T::size / 4;  // its 32-bit words
-  constexpr int U = 4;                  // rows of a block that a lane reads
+  constexpr int U = kBlk / RPL;         // rows of a block that a lane reads
   using B = typename T::bits;
   const int lane = threadIdx.x & 63;
   const int wave = uni((int)threadIdx.x >> 6);
-  const int sub = lane & 15, rowg = lane >> 4;
+  const int sub = lane & (LPR - 1), rowg = lane / LPR;
   const int n_chunks = p.n_pairs / p.n_kv;
   __shared__ float s_m[NW][G], s_l[NW][G];
   __shared__ float s_acc[NW][G][D];
@@ -453,22 +508,16 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
     const char* const vh = (const char*)p.v + hkv * p.v_sh * T::size;
 
     int pages = 0;  // lane i: the page of this wave's block (it & ~63) + i
-    int it = 0;
-    for (int v = v0 + wave; v < v1; v += NW * NB, it += NB) {
-      if ((it & 63) == 0) {
-        const int mine = v + NW * lane;
-        pages = mine < v1 ? row[block_at(mine) >> (shift - kBlkShift)] : -1;
-      }
-      if constexpr (!PAIR) {
-        if ((it & 3) == 0) set_progress_priority(done + it * NW, share);
-      }
-      Slice<W> kr[NB][U], vr[NB][U];
-      bool full[NB];
-      int pos0[NB];
+    // The wave's blocks it .. it + N - 1, from v on NW apart.
+    auto blocks = [&](const int v, const int it, auto count) __attribute__((always_inline)) {
+      constexpr int N = decltype(count)::value;
+      Slice<W> kr[N][U], vr[N][U];
+      bool full[N];
+      int pos0[N];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
+      for (int i = 0; i < N; ++i) {
         const int vi = v + i * NW;
-        const int page = __builtin_amdgcn_readlane(pages, (it + i) & 63);  // -1 past the segment
+        const int page = __builtin_amdgcn_readlane(pages, (it + i) & 63);
         const bool there = (unsigned)page < (unsigned)p.pm.n_pages;
         pos0[i] = block_at(vi) << kBlkShift;
         const int in_page = pos0[i] & ((1 << shift) - 1);
@@ -481,22 +530,22 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
         if (!there) pos0[i] = sn.len;  // hidden throughout
         if (full[i]) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) load_slice(kr[i][u], krs, k_lane, 4 * u * p.k_row_bytes);
+          for (int u = 0; u < U; ++u) load_slice(kr[i][u], krs, k_lane, RPL * u * p.k_row_bytes);
 #pragma unroll
-          for (int u = 0; u < U; ++u) load_slice(vr[i][u], vrs, v_lane, 4 * u * p.v_row_bytes);
+          for (int u = 0; u < U; ++u) load_slice(vr[i][u], vrs, v_lane, RPL * u * p.v_row_bytes);
         } else {
           // hidden rows may hold anything (NaN among it): they are not read, and count as zeros
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const bool seen = row_seen(sn, p.sinks, pos0[i] + 4 * u + rowg);
-            load_slice(kr[i][u], krs, seen ? k_lane + 4 * u * p.k_row_bytes : kPastEnd, 0);
-            load_slice(vr[i][u], vrs, seen ? v_lane + 4 * u * p.v_row_bytes : kPastEnd, 0);
+            const bool seen = row_seen(sn, p.sinks, pos0[i] + RPL * u + rowg);
+            load_slice(kr[i][u], krs, seen ? k_lane + RPL * u * p.k_row_bytes : kPastEnd, 0);
+            load_slice(vr[i][u], vrs, seen ? v_lane + RPL * u * p.v_row_bytes : kPastEnd, 0);
           }
         }
       }
-      float s[G][NB * U];
+      float s[G][N * U];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
+      for (int i = 0; i < N; ++i) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -505,7 +554,7 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
           asm volatile("");
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            const bool seen = row_seen(sn, p.sinks, pos0[i] + 4 * u + rowg);
+            const bool seen = row_seen(sn, p.sinks, pos0[i] + RPL * u + rowg);
 #pragma unroll
             for (int g = 0; g < G; ++g) s[g][i * U + u] = seen ? s[g][i * U + u] : -INFINITY;
           }
@@ -518,7 +567,7 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
       for (int g = 0; g < G; ++g) {
         mb[g] = s[g][0];
 #pragma unroll
-        for (int u = 1; u < NB * U; ++u) mb[g] = fmaxf(mb[g], s[g][u]);
+        for (int u = 1; u < N * U; ++u) mb[g] = fmaxf(mb[g], s[g][u]);
         grow |= mb[g] > m[g] + kRescaleLog2;
       }
       if (__any(grow)) {
@@ -536,13 +585,13 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
       for (int g = 0; g < G; ++g) {
         const float base = m[g] == -INFINITY ? 0.f : m[g];
 #pragma unroll
-        for (int u = 0; u < NB * U; ++u) {
+        for (int u = 0; u < N * U; ++u) {
           s[g][u] = fast_exp2(s[g][u] - base);
           l[g] += s[g][u];
         }
       }
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float vf[EPL];
@@ -558,11 +607,31 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
 #pragma unroll
             for (int e = 0; e < EPL; ++e) acc[g][e] = fmaf(s[g][i * U + u], vf[e], acc[g][e]);
         }
+    };
+    int v = v0 + wave, it = 0;
+    auto look_up = [&]() __attribute__((always_inline)) {
+      if ((it & 63) == 0) {
+        const int mine = v + NW * lane;
+        pages = mine < v1 ? row[block_at(mine) >> (shift - kBlkShift)] : -1;
+      }
+    };
+    if constexpr (NB > 1) {
+      for (; v + NW * (NB - 1) < v1; v += NW * NB, it += NB) {
+        look_up();
+        blocks(v, it, std::integral_constant<int, NB>{});
+      }
+    }
+    for (; v < v1; v += NW, ++it) {
+      look_up();
+      if constexpr (!PAIR) {
+        if ((it & 3) == 0) set_progress_priority(done + it * NW, share);
+      }
+      blocks(v, it, std::integral_constant<int, 1>{});
     }
 
-    // join the wave's four rows of a load, then the waves
+    // join the rows of a load, then the waves
 #pragma unroll
-    for (int off = 16; off <= 32; off <<= 1) {
+    for (int off = LPR; off <= 32; off <<= 1) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const float m2 = __shfl_xor(m[g], off), l2 = __shfl_xor(l[g], off);
@@ -576,7 +645,7 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
       }
     }
     __syncthreads();  // the last segment's sums have been read
-    if (lane < 16) {
+    if (lane < LPR) {
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         if (lane == 0) {
@@ -619,31 +688,30 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
     const Seen sn = seen_of(p, b);
     segment(b, sn, (int)blockIdx.x - b * p.n_pairs, 0, sn.n, true, 0, 0, 0);
   } else {
-    // up to 64 sequences stay in the lanes; of more every look-up walks the lengths again
-    SeqBlocks sb = seq_blocks(p, 0, 0, lane);
-    int total = uni(__builtin_amdgcn_readlane(sb.incl, 63));
-    for (int b0 = 64; b0 < p.batch; b0 += 64)
-      total = uni(__builtin_amdgcn_readlane(seq_blocks(p, b0, total, lane).incl, 63));
-    const int rpb = uni(share_blocks(p, total));
-    const int64_t first = (int64_t)blockIdx.x * rpb;
-    if (first >= total) return;
-    const int r0 = (int)first, r1 = (int)min((int64_t)total, first + rpb);
+    const Layout lay = layout_of(p, lane);
+    if (lay.padded) {
+      // one segment a workgroup: part blockIdx.x - first of its pair
+      const int w = (int)blockIdx.x;
+      if (w >= lay.total) return;
+      const Owner own = owner_of(p, lay, w, lane);
+      const Seen sn = seen_of(p, own.b);
+      const int parts = (sn.n + lay.share - 1) / lay.share;
+      const int pair = (w - own.first) / parts;
+      const int part = (w - own.first) - pair * parts;
+      const int v0 = part * lay.share, v1 = min(v0 + lay.share, sn.n);
+      segment(own.b, sn, pair, v0, v1, parts == 1, part == 0 ? 1 : 0, 0, v1 - v0);
+      return;
+    }
+    const int64_t first = (int64_t)blockIdx.x * lay.share;
+    if (first >= lay.total) return;
+    const int r0 = (int)first, r1 = (int)min((int64_t)lay.total, first + lay.share);
     for (int r = r0; r < r1;) {
-      int b0 = 0;
-      SeqBlocks s = sb;
-      while (b0 + 64 < p.batch && uni(__builtin_amdgcn_readlane(s.incl, 63)) <= r) {
-        b0 += 64;
-        s = seq_blocks(p, b0, uni(__builtin_amdgcn_readlane(s.incl, 63)), lane);
-      }
-      const int li = __ffsll((unsigned long long)__ballot(s.incl > r)) - 1;
-      const int b = uni(b0 + li);
-      const int n = uni(__builtin_amdgcn_readlane(s.n, uni(li)));
-      const int seq0 = uni(__builtin_amdgcn_readlane(s.incl, uni(li))) - n * p.n_pairs;
-      const Seen sn = seen_of(p, b);
-      const int pair = (r - seq0) / n;
-      const int pair0 = seq0 + pair * n;
-      const int v0 = r - pair0, v1 = min(r1 - pair0, n);
-      segment(b, sn, pair, v0, v1, v0 == 0 && v1 == n, v0 == 0 ? 1 : 0, r - r0, r1 - r0);
+      const Owner own = owner_of(p, lay, r, lane);
+      const Seen sn = seen_of(p, own.b);
+      const int pair = (r - own.first) / sn.n;
+      const int pair0 = own.first + pair * sn.n;
+      const int v0 = r - pair0, v1 = min(r1 - pair0, sn.n);
+      segment(own.b, sn, pair, v0, v1, v0 == 0 && v1 == sn.n, v0 == 0 ? 1 : 0, r - r0, r1 - r0);
       r = pair0 + v1;
     }
   }
@@ -658,28 +726,27 @@ __global__ __launch_bounds__(64) void paged_combine_kernel(DecodeParams p) {
   using B = typename T::bits;
   const int hq = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
   B* o = (B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh;
-  int total = 0, before = 0, n = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    const SeqBlocks s = seq_blocks(p, b0, total, lane);
-    if (b >= b0 && b < b0 + 64) {
-      n = uni(__builtin_amdgcn_readlane(s.n, b - b0));
-      before = uni(__builtin_amdgcn_readlane(s.incl, b - b0)) - n * p.n_pairs;
-    }
-    total = uni(__builtin_amdgcn_readlane(s.incl, 63));
-  }
-  if (n == 0) {
+  const Seen sn = seen_of(p, b);
+  if (sn.n == 0) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = 0;
     return;
   }
-  const int rpb = uni(share_blocks(p, total));
+  const Layout lay = layout_of(p, lane);
   const int hkv = hq / p.group, in = hq - hkv * p.group;
   const int pair = hkv * (p.n_pairs / p.n_kv) + in / p.heads_per_pair;
   const int g = in % p.heads_per_pair;
-  const int pair0 = before + pair * n;
-  const int first = pair0 / rpb;
-  const int parts = (pair0 + n - 1) / rpb - first + 1;
-  if (parts == 1) return;
+  int parts, first;
+  if (lay.padded) {
+    parts = (sn.n + lay.share - 1) / lay.share;
+    if (parts == 1) return;
+    first = first_of(p, lay, b, lane) + pair * parts;
+  } else {
+    const int pair0 = first_of(p, lay, b, lane) + pair * sn.n;
+    first = pair0 / lay.share;
+    parts = (pair0 + sn.n - 1) / lay.share - first + 1;
+    if (parts == 1) return;
+  }
   auto at = [&](int s) { return ((first + s) * 2 + (s == 0 ? 1 : 0)) * p.heads_per_pair + g; };
   auto load = [&](int s0, float (&r)[R][NJ]) {
 #pragma unroll
@@ -740,18 +807,20 @@ int heads_per_pair(int n_head, int n_kv) { return n_head / n_kv < 8 ? n_head / n
 size_t ws_ml_bytes(int hpp) { return (size_t)kMaxShares * 2 * hpp * 2 * sizeof(float); }
 
 // A workgroup for each pair, which finishes it: no partial results, one launch.  Taken where the longest pair
-// there can be is short (pair_bytes of K and V) and the pairs are few bytes in all.
+// there can be (pair_bytes of K and V) is short: one CU streams it.  us a call as pairs / as shares, 250 KB a pair,
+// 16 bits: 5 pairs 13.2 / 9.6, 40 pairs 13.5 / 12.3, 64 (d_k 128) 12.9 / 14.2, 96 (MHA) 10.5 / 13.7, 160 15.2 / 17.7; 350 KB: 32
+// 15.1 / 12.9, 128 16.4 / 17.8, 24 (fp32) 12.5 / 11.4; 126 KB: 320 13.9 / 17.8; 50 KB: 8 7.0 / 10.0, 128 7.7 / 10.8.
 bool pair_mode(const DecodeParams& p, int64_t pair_bytes) {
-  return !tl_overrides.decode_shares && pair_bytes <= kPairMaxBytes && pair_bytes * p.batch * p.n_pairs <= kPairMaxAll;
+  const int64_t pairs = (int64_t)p.batch * p.n_pairs;
+  return !tl_overrides.decode_shares && pair_bytes <= kPairMaxBytes && pair_bytes * pairs <= kPairMaxAll &&
+         (pair_bytes <= kPairFewBytes || pairs >= kPairMany);
 }
 
 template <typename T, int D, int G>
 int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
   const int64_t pair_bytes = most / ((int64_t)p.batch * p.n_pairs) * kBlk * 2 * D * T::size;
   if (pair_mode(p, pair_bytes)) {
-    // 16 waves while a lane's state fits the 128 registers of a 1024-thread workgroup
-    constexpr int NW = D * G * T::size <= 512 ? 16 : 8;
-    hipLaunchKernelGGL((paged_decode_kernel<T, D, G, NW, 2, true>), dim3(p.batch * p.n_pairs), dim3(64 * NW), 0, st, p);
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, G, kPairWaves, kPairBlocks<T, D>, true>), dim3(p.batch * p.n_pairs), dim3(64 * kPairWaves), 0, st, p);
     return tl_launch_status();
   }
   static int per_cu = 0;
@@ -764,7 +833,10 @@ int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
   }
   int64_t shares = (int64_t)per_cu * tl_device_cus();
   shares = shares < kMaxShares ? shares : kMaxShares;
-  const int64_t full = (most + kMinShare - 1) / kMinShare;
+  // never more than the parts there can be; twice the pairs at least, where the device holds as many, so that the
+  // pairs are cut one by one
+  const int64_t pairs = (int64_t)p.batch * p.n_pairs;
+  const int64_t full = (most + kMinShare - 1) / kMinShare + pairs;
   p.n_shares = (int)(shares < full ? shares : full);
   hipLaunchKernelGGL((paged_decode_kernel<T, D, G, kDecWaves, 1, false>), dim3(p.n_shares), dim3(kDecThreads), 0, st, p);
   const int e = tl_launch_status();
