@@ -7,16 +7,16 @@
 // their size.  x - max and exp are 32-bit (the argument of exp2 carried in two words, so that its
 // rounding does not grow with the distance from the maximum), their sum 64.
 //
-// Bytes: every logit is read once, by beam_scan, a workgroup a segment of a row, which leaves
+// Bytes: every logit is read once, by beam_scan, a wave a segment of 1024 entries of a row, which leaves
 //   * the segment's maximum and its sum of exp against it;
 //   * the maximum of every group of 64 entries.
-// beam_finish, a workgroup a batch item, has everything else from those.  A group's best score is
-// base_j + its maximum, base_j = s_j - log-sum-exp.  The groups are dealt to 64 classes; the n-th largest
-// of the classes' best (n <= 64) is a bound that n continuations reach, so only groups that reach it are
-// read again, and their entries that reach it are the candidates: about n for scattered
-// scores.  A candidate's rank is the number of better ones.  Where the candidates outgrow their place
-// (thousands of ties, a row in descending order) every wave walks its groups in order instead and
-// keeps its 64 best in its lanes; those are the candidates then.
+// beam_finish, a workgroup a batch item, has everything else from those.  The best score in a unit (a segment, or
+// a group where the segments are few) is base_j + its maximum, base_j = s_j - log-sum-exp.  The units are
+// dealt to 64 classes; the n-th largest of the classes' best (n <= 64) is a bound that n continuations reach,
+// so only units that reach it are read again, and their entries that reach it are the
+// candidates: about n for scattered scores.  A candidate's rank is the number of better ones.  Where the
+// candidates are many (ties, rows in order) every wave walks its units in order instead and keeps its 64 best in
+// its lanes; those are the candidates then.  beam_finish is latency alone: dependent steps on one CU.
 #include "tl_common.h"
 
 #include <limits.h>
@@ -25,16 +25,19 @@
 namespace {
 
 constexpr int kST = 256;                 // threads of beam_scan
-constexpr int kPer = 8;                  // entries of a thread
-constexpr int kSeg = kST * kPer;         // entries of a segment
-constexpr int kGrp = 64;                 // entries of a group: 8 threads
+constexpr int kVec = 8;                  // neighbouring entries of a lane
+constexpr int kVecs = 2;                 // of those a lane has in a segment
+constexpr int kSeg = 64 * kVec * kVecs;  // entries of a segment, a wave's
+constexpr int kGrp = 64;                 // entries of a group: 8 lanes
 constexpr int kFT = 1024;                // threads of beam_finish
 constexpr int kFW = kFT / 64;
 constexpr int kMaxVocab = 262144;
 constexpr int kMaxBeams = 64;
 constexpr int kMaxSelect = 64;
-constexpr int kMaxCand = 3072;           // candidates in LDS
-constexpr int kMaxList = 2048;           // groups that are read again
+constexpr int kMaxCand = 1024;           // candidates that are ranked
+constexpr int kAtOnce = 4;               // units of a thread that are read together
+constexpr int kMaxList = 1024;           // units that are read again
+constexpr int kUnitsAPlace = 4;          // segments a place in the selection, below which groups are the units
 
 struct BeamParams {
   const void* logits;
@@ -42,6 +45,7 @@ struct BeamParams {
   const float* scores;
   int batch, beams, vocab, select;
   int n_seg, n_grp;
+  int unit, n_units;  // entries of a unit, units of a row
   float* gmax;    // [rows][n_grp]
   float* smax;    // [rows][n_seg]
   double* ssum;   // [rows][n_seg]
@@ -56,14 +60,37 @@ typedef uint32_t words32 __attribute__((ext_vector_type(4), aligned(4)));
 
 size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 
-// exp(x - m) for x <= m; 0 where it is under the smallest 32-bit number, NaN for NaN.
+// exp(x - m) for x <= m; 0 where it is under the smallest 32-bit number, NaN for NaN (the IEEE maximum
+// passes it on).
 __device__ __forceinline__ float exp_below(float x, float m) {
   constexpr float kL = 1.44269504f, kLlo = 1.92596303e-8f;  // log2 e in two words
-  const float d = x - m;
+  const float d = __builtin_elementwise_maximum(x - m, -126.f);
   const float hi = d * kL;
-  const float lo = fmaf(d, kL, -hi) + d * kLlo;
+  const float lo = fmaf(d, kLlo, fmaf(d, kL, -hi));
   const float e = fast_exp2(hi);
-  return d < -110.f ? 0.f : fmaf(e * 0.693147181f, lo, e);
+  return fmaf(e * 0.693147181f, lo, e);
+}
+
+// kVec neighbouring entries of a row from i on, -inf behind its end.
+template <typename T>
+__device__ __forceinline__ void load_vec(float (&v)[kVec], const typename T::bits* x, int i, int vocab) {
+  if (i + kVec <= vocab) {
+    if constexpr (T::size == 2) {
+      const words16 w = *(const words16*)(x + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) unpack2<T>(w[e], v[2 * e], v[2 * e + 1]);
+    } else {
+      const words32 a = *(const words32*)(x + i), b = *(const words32*)(x + i + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = __uint_as_float(a[e]);
+        v[4 + e] = __uint_as_float(b[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = i + e < vocab ? to_f32<T>(x[i + e]) : -INFINITY;
+  }
 }
 
 __device__ __forceinline__ double shfl_xor_d(double x, int off) {
@@ -77,58 +104,51 @@ __device__ __forceinline__ double shfl_d(double x, int lane) {
   return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
 }
 
+// Lane i's value, i the same on every lane.
+__device__ __forceinline__ double lane_d(double x, int i) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t a = __builtin_amdgcn_readlane((uint32_t)u, i), b = __builtin_amdgcn_readlane((uint32_t)(u >> 32), i);
+  return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
+}
+
 template <typename T>
 __global__ __launch_bounds__(kST) void beam_scan_kernel(BeamParams p) {
   using B = typename T::bits;
-  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.y, lane = threadIdx.x & 63;
+  const int seg = blockIdx.x * (kST / 64) + (threadIdx.x >> 6);
+  if (seg >= p.n_seg) return;
   const B* x = (const B*)p.logits + (int64_t)row * p.row_stride;
-  const int i0 = seg * kSeg + tid * kPer;
-  float v[kPer];
-  if (i0 + kPer <= p.vocab) {
-    if constexpr (T::size == 2) {
-      const words16 w = *(const words16*)(x + i0);
+  float v[kVecs][kVec];
+  const int i0 = seg * kSeg + lane * kVec;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
-    } else {
-      const words32 a = *(const words32*)(x + i0), b = *(const words32*)(x + i0 + 4);
+  for (int k = 0; k < kVecs; ++k) load_vec<T>(v[k], x, i0 + k * 64 * kVec, p.vocab);
+  float m = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = __uint_as_float(a[i]);
-        v[4 + i] = __uint_as_float(b[i]);
-      }
-    }
-  } else {
+  for (int k = 0; k < kVecs; ++k) {
+    float g = v[k][0];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = i0 + i < p.vocab ? to_f32<T>(x[i0 + i]) : -INFINITY;
+    for (int e = 1; e < kVec; ++e) g = fmaxf(g, v[k][e]);
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1) g = fmaxf(g, __shfl_xor(g, off));
+    const int i = i0 + k * 64 * kVec;
+    if ((lane & 7) == 0 && i < p.vocab) p.gmax[(int64_t)row * p.n_grp + i / kGrp] = g;
+    m = fmaxf(m, g);
   }
-  float m = v[0];
-#pragma unroll
-  for (int i = 1; i < kPer; ++i) m = fmaxf(m, v[i]);
-#pragma unroll
-  for (int off = 1; off < 8; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-  if ((tid & 7) == 0 && i0 < p.vocab) p.gmax[(int64_t)row * p.n_grp + i0 / kGrp] = m;
 #pragma unroll
   for (int off = 8; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-  __shared__ float s_m[kST / 64];
-  __shared__ double s_s[kST / 64];
-  if ((tid & 63) == 0) s_m[tid >> 6] = m;
-  __syncthreads();
-  m = s_m[0];
-#pragma unroll
-  for (int w = 1; w < kST / 64; ++w) m = fmaxf(m, s_m[w]);
   // a segment of -inf alone has no mass; NaN in it comes through the maximum as -inf
   const float base = m == -INFINITY ? 0.f : m;
-  float e = 0.f;
+  double s = 0.;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) e += exp_below(v[i], base);
-  double s = e;
+  for (int k = 0; k < kVecs; ++k) {
+    float e = 0.f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) e += exp_below(v[k][i], base);
+    s += e;
+  }
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
-  if ((tid & 63) == 0) s_s[tid >> 6] = s;
-  __syncthreads();
-  if (tid == 0) {
-#pragma unroll
-    for (int w = 1; w < kST / 64; ++w) s += s_s[w];
+  if (lane == 0) {
     p.smax[(int64_t)row * p.n_seg + seg] = m;
     p.ssum[(int64_t)row * p.n_seg + seg] = s;
   }
@@ -169,6 +189,11 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   __shared__ double s_cv[kMaxCand];
   __shared__ int s_ci[kMaxCand];
 
+  const int U = p.n_units;
+  const float* umax = (p.unit == kGrp ? p.gmax : p.smax) + (int64_t)item * J * U;
+  float um[kAtOnce];  // the first of this thread's units, on their way during the sums
+#pragma unroll
+  for (int k = 0; k < kAtOnce; ++k) um[k] = tid + k * kFT < J * U ? umax[tid + k * kFT] : -INFINITY;
   if (tid == 0) s_n_list = s_n_cand = 0;
   // base_j = s_j - log-sum-exp of the row; -inf where either has no value, and such a beam has no
   // continuations
@@ -195,25 +220,42 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   __syncthreads();
 
   // the bound: n-th best of the 64 classes' best
-  const int groups = J * p.n_grp;  // row-major over (beam, group)
-  const float* gmax = p.gmax + (int64_t)item * groups;
-  auto group_best = [&](int g) { return s_base[g / p.n_grp] + (double)gmax[g]; };
   double best = -INFINITY;
-  for (int g = tid; g < groups; g += kFT) best = fmax(best, group_best(g));
+#pragma unroll
+  for (int k = 0; k < kAtOnce; ++k)
+    if (tid + k * kFT < J * U) best = fmax(best, s_base[(tid + k * kFT) / U] + (double)um[k]);
+  for (int u = tid + kAtOnce * kFT; u < J * U; u += kFT) best = fmax(best, s_base[u / U] + (double)umax[u]);
   s_best[tid] = best;
   __syncthreads();
   if (wave == 0) {
-    Cand c{-INFINITY, lane};
-    for (int w = 0; w < kFW; ++w) c.v = fmax(c.v, s_best[w * 64 + lane]);
-    sort64(c, lane);
-    const double bound = shfl_d(c.v, n - 1);
-    if (lane == 0) s_bound = bound;
+    double c = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFW; ++w) c = fmax(c, s_best[w * 64 + lane]);
+    int rank = 0;  // of this class
+    for (int i = 0; i < 64; ++i) rank += better(lane_d(c, i), i, c, lane) ? 1 : 0;
+    if (rank == n - 1) s_bound = c;
   }
   __syncthreads();
   const double bound = s_bound;
+  auto reaches = [&](double v) { return v >= bound && v > -INFINITY; };
 
-  auto entry = [&](int g, double& v, int& i) {  // this lane's entry of group g
-    const int j = g / p.n_grp, at = (g - j * p.n_grp) * kGrp + lane;
+  if (reaches(best)) {
+    auto list = [&](int u, float x) {
+      if (reaches(s_base[u / U] + (double)x)) {
+        const int at = atomicAdd(&s_n_list, 1);
+        if (at < kMaxList) s_list[at] = u;
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (tid + k * kFT < J * U) list(tid + k * kFT, um[k]);
+    for (int u = tid + kAtOnce * kFT; u < J * U; u += kFT) list(u, umax[u]);
+  }
+  __syncthreads();
+  const int n_list = s_n_list;
+  // this lane's entry 64 c + lane of unit u (of beam u / U)
+  auto entry = [&](int u, int c, double& v, int& i) __attribute__((always_inline)) {
+    const int j = u / U, at = (u - j * U) * p.unit + c * 64 + lane;
     v = -INFINITY;
     i = INT_MAX;
     if (at < p.vocab) {
@@ -221,24 +263,38 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
       i = j * p.vocab + at;
     }
   };
-  for (int g = tid; g < groups; g += kFT) {
-    const double v = group_best(g);
-    if (v >= bound && v > -INFINITY) {
-      const int at = atomicAdd(&s_n_list, 1);
-      if (at < kMaxList) s_list[at] = g;
-    }
-  }
-  __syncthreads();
-  const int n_list = s_n_list;
-  if (n_list <= kMaxList) {
+  auto push = [&](double v, int i) {
+    const int at = atomicAdd(&s_n_cand, 1);
+    if (at < kMaxCand) s_cv[at] = v, s_ci[at] = i;
+  };
+  if (n_list <= kMaxList && p.unit == kSeg) {
+    // a wave a segment, read as beam_scan does
     for (int w = wave; w < n_list; w += kFW) {
+      const int u = s_list[w], j = u / U, at = (u - j * U) * kSeg + lane * kVec;
+      const double base = s_base[j];
+      float x[kVecs][kVec];
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k)
+        load_vec<T>(x[k], (const B*)p.logits + ((int64_t)item * J + j) * p.row_stride, at + k * 64 * kVec, p.vocab);
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        float m = x[k][0];
+#pragma unroll
+        for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[k][e]);
+        if (!reaches(base + (double)m)) continue;
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const double v = base + (double)x[k][e];
+          if (reaches(v)) push(v, j * p.vocab + at + k * 64 * kVec + e);
+        }
+      }
+    }
+  } else if (n_list <= kMaxList) {
+    for (int w = wave; w < n_list; w += kFW) {  // a wave a group
       double v;
       int i;
-      entry(s_list[w], v, i);
-      if (v >= bound && v > -INFINITY) {
-        const int at = atomicAdd(&s_n_cand, 1);
-        if (at < kMaxCand) s_cv[at] = v, s_ci[at] = i;
-      }
+      entry(s_list[w], 0, v, i);
+      if (reaches(v)) push(v, i);
     }
   }
   __syncthreads();
@@ -248,21 +304,21 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
     if (tid == 0) s_n_cand = 0;
     __syncthreads();
     Cand kept{-INFINITY, INT_MAX};  // this wave's 64 best so far, best in lane 0
-    for (int g = wave; g < groups; g += kFW) {
-      const double gv = group_best(g);
-      const double worst = shfl_d(kept.v, 63);
-      if (!(gv >= bound && gv > -INFINITY && gv >= worst)) continue;
-      Cand c;
-      entry(g, c.v, c.i);
-      if (!(c.v > -INFINITY)) c.v = -INFINITY, c.i = INT_MAX;
-      const int wi = __shfl(kept.i, 63);
-      if (!__any(better(c.v, c.i, worst, wi))) continue;
-      sort64(c, lane);
-      // the better of i-th best and (63 - i)-th best are the 64 best of both, in a bitonic order
-      const double rv = shfl_d(c.v, 63 - lane);
-      const int ri = __shfl(c.i, 63 - lane);
-      if (better(rv, ri, kept.v, kept.i)) kept.v = rv, kept.i = ri;
-      for (int off = 32; off > 0; off >>= 1) exchange(kept, lane, off, true);
+    for (int u = wave; u < J * U; u += kFW) {
+      const double uv = s_base[u / U] + (double)umax[u];
+      if (!(reaches(uv) && uv >= lane_d(kept.v, 63))) continue;
+      for (int c = 0; c < p.unit / 64; ++c) {
+        Cand x;
+        entry(u, c, x.v, x.i);
+        if (!(x.v > -INFINITY)) x.v = -INFINITY, x.i = INT_MAX;
+        if (!__any(better(x.v, x.i, lane_d(kept.v, 63), __builtin_amdgcn_readlane(kept.i, 63)))) continue;
+        sort64(x, lane);
+        // the better of i-th best and (63 - i)-th best are the 64 best of both, in a bitonic order
+        const double rv = shfl_d(x.v, 63 - lane);
+        const int ri = __shfl(x.i, 63 - lane);
+        if (better(rv, ri, kept.v, kept.i)) kept.v = rv, kept.i = ri;
+        for (int off = 32; off > 0; off >>= 1) exchange(kept, lane, off, true);
+      }
     }
     if (kept.v > -INFINITY) {
       const int at = atomicAdd(&s_n_cand, 1);
@@ -309,7 +365,7 @@ size_t ws_layout(int64_t rows, int vocab, char* base, BeamParams* p) {
 
 template <typename T>
 int launch_beam(const BeamParams& p, hipStream_t st) {
-  hipLaunchKernelGGL(beam_scan_kernel<T>, dim3(p.n_seg, p.batch * p.beams), dim3(kST), 0, st, p);
+  hipLaunchKernelGGL(beam_scan_kernel<T>, dim3((p.n_seg + kST / 64 - 1) / (kST / 64), p.batch * p.beams), dim3(kST), 0, st, p);
   const int e = tl_launch_status();
   if (e) return e;
   hipLaunchKernelGGL(beam_finish_kernel<T>, dim3(p.batch), dim3(kFT), 0, st, p);
@@ -352,6 +408,10 @@ int tl_beam_select(const void* logits, const float* scores, int batch, int beams
   p.select = select;
   p.n_seg = n_segments(vocab);
   p.n_grp = n_groups(vocab);
+  // segments where they are several for each place, so that few of them reach the bound and no class is empty
+  const bool segments = (int64_t)beams * p.n_seg >= kUnitsAPlace * select && (int64_t)beams * p.n_seg >= 64;
+  p.unit = segments ? kSeg : kGrp;
+  p.n_units = segments ? p.n_seg : p.n_grp;
   ws_layout((int64_t)batch * beams, vocab, (char*)workspace, &p);
   p.out_scores = out_scores;
   p.out_parents = out_parents;
