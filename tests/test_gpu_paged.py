@@ -309,3 +309,38 @@ def test_captured_step_replays():
             step(eager)  # eager work on the same workspace
             for n, x in want.items():
                 np.testing.assert_array_equal(gpu.to_host(s[n]).view(np.uint8), x.view(np.uint8), err_msg=f"{n} replay {i}")
+
+
+@pytest.mark.parametrize("dtype,D,batch,cus", [("bfloat16", 64, 70, None), ("float32", 64, 70, 200), ("float16", 128, 3, 2), ("bfloat16", 64, 5, 7)])
+def test_prefill_divided_keys(monkeypatch, dtype, D, batch, cus):
+    """Few rows on long and short prefixes: the keys are shared by workgroups, sequences without tokens among them."""
+    P.H.set_override(monkeypatch, "TRITON_LLM_HIP_MAX_CUS", cus)
+    rng = np.random.default_rng(batch)
+    Hq, Hkv, page, n_new = 2, 1, 32, 5
+    lens = rng.integers(0, 1500, batch).astype(np.int32)
+    lens[::7] = 0
+    new = rng.integers(0, n_new + 1, batch).astype(np.int32)
+    new[0] = n_new
+    total = lens + new
+    max_pages = 50
+    n_pages = sum(-(-int(t) // page) for t in total) + 2
+    table = P.shuffled_table(rng, total, page, max_pages, n_pages)
+    keep = [np.arange(max_pages * page) < t for t in total]
+    kp, vp = (P.pool_with(rng, table, keep, (n_pages, Hkv, page, D), dtype) for _ in range(2))
+    q = P.values(rng, (batch, n_new, Hq, D), dtype)
+    before = P.values(rng, q.shape, dtype)
+    kp_d, vp_d = P.dev(kp, dtype), P.dev(vp, dtype)
+    for window, sinks in ((0, 0), (700, 5)):
+        out = P.dev(before, dtype)
+        paged_attention_prefill(P.dev(q, dtype), kp_d, vp_d, P.int32(table), P.int32(lens), Hq, Hkv, new_lens=P.int32(new),
+                                window=window, sinks=sinks, out=out)
+        got = P.back(out, dtype)
+        for b in range(batch):
+            n, m = int(lens[b]), int(new[b])
+            np.testing.assert_array_equal(got[b, m:], on.from_storage(before[b, m:], dtype))
+            if m == 0:
+                continue
+            k, there = op.gather(on.from_storage(kp, dtype), table[b], n + m)
+            v, _ = op.gather(on.from_storage(vp, dtype), table[b], n + m)
+            want, tol = P.rows_want(q[b, :m].transpose(1, 0, 2), k, v, n + np.arange(m), there, window, sinks, D ** -0.5, dtype)
+            P.check(f"divided {dtype} sequence {b} {n}+{m} window {window}", got[b, :m].transpose(1, 0, 2), want, tol)

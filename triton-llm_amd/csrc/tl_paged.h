@@ -11,6 +11,8 @@
 
 #include "tl_common.h"
 
+#include <type_traits>
+
 namespace tlpg {
 
 constexpr int kBlk = 16;  // positions of a block
@@ -41,5 +43,21 @@ __device__ __forceinline__ int64_t uni(int64_t x) {
   const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
+
+// Sums over the lanes up to and with each, by DPP moves: rows of 16 first, then row to row.
+__device__ __forceinline__ int wave_scan(int x) {
+  auto add = [&](auto ctrl, auto rows) {
+    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // row_shr:1
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15 into rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+__device__ __forceinline__ int last_lane(int x) { return uni(__builtin_amdgcn_readlane(x, 63)); }
 
 }  // namespace tlpg

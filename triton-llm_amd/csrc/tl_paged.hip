@@ -321,20 +321,6 @@ __device__ __forceinline__ bool row_seen(const Seen& s, int sinks, int pos) {
   return pos < s.len && (pos >= s.lo || pos < sinks);
 }
 
-// Sums over the lanes up to and with each, by DPP moves: rows of 16 first, then row to row.
-__device__ __forceinline__ int wave_scan(int x) {
-  auto add = [&](auto ctrl, auto rows) {
-    x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
-  };
-  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // row_shr:1
-  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
-  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
-  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
-  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15 into rows 1 and 3
-  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31 into rows 2 and 3
-  return x;
-}
-
 // How the blocks are dealt.  Even shares of the flattened blocks, whole rounds of the waves, where the pairs are many;
 // a share may then hold the end of one pair and the beginning of the next.  Where that costs a share at most two
 // rounds of the waves, every pair is cut by itself into parts of `share` blocks instead, so that no workgroup runs one
@@ -347,7 +333,6 @@ struct Layout {
   int n, incl;  // lane's sequence (of the first 64)
   __device__ __forceinline__ int unit(int blocks) const { return padded ? (blocks + share - 1) / share : blocks; }
 };
-__device__ __forceinline__ int last_lane(int x) { return uni(__builtin_amdgcn_readlane(x, 63)); }
 __device__ __forceinline__ int blocks_at(const DecodeParams& p, int b) { return b < p.batch ? seen_of(p, b).n : 0; }
 
 __device__ __forceinline__ Layout layout_of(const DecodeParams& p, int lane) {

@@ -40,10 +40,10 @@ struct WinParams {
   const int32_t* new_lens;
   int batch, n_head, n_kv, group, seq_q, seq_k, n_qt;
   int window, sinks;
-  int share, n_parts;  // key tiles of a part at least, parts of a row tile at most
+  int slots;           // workgroups that the keys are shared by; 0: a row tile's keys are not divided
   int q_step, n_lvl, xcd_groups;  // how workgroups are dealt (window_fwd_kernel)
   int vec_out;         // o's rows take 4 elements at once
-  float* ws;           // [tile][part] of partial results (n_parts > 1)
+  float* ws;           // partial results by part (slots > 0)
   int64_t q_sb, q_sh, q_ss;
   int64_t k_sb, k_sh, k_ss;
   int64_t v_sb, v_sh, v_ss;
@@ -227,14 +227,14 @@ __device__ __forceinline__ Rows rows_of(const WinParams& p, int b) {
   return r;
 }
 
-// The key tiles of row tile qt: ns of the sinks', then those from t0 on; in how many parts.
+// The key tiles of row tile qt: ns of the sinks', then those from t0 on.
 struct Keys {
-  int ns, t0, tiles, parts, end;
+  int ns, t0, tiles, end;
   __device__ __forceinline__ int key0(int t) const { return t < ns ? t : t - ns + t0; }  // in tiles
 };
 template <int BN>
 __device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int qt) {
-  Keys k{0, 0, 0, 1, r.end};
+  Keys k{0, 0, 0, r.end};
   const int p0 = r.base + qt * kBM / p.group;
   const int p1 = min(r.base + min((qt * kBM + kBM - 1) / p.group + 1, r.nq), r.end) - 1;  // last key any row sees
   if (p1 < 0) return k;
@@ -244,8 +244,64 @@ __device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int q
     if (k.t0 <= k.ns) k.ns = k.t0 = 0;
   }
   k.tiles = k.ns + p1 / BN - k.t0 + 1;
-  if (p.n_parts > 1) k.parts = min(p.n_parts, (k.tiles + p.share - 1) / p.share);
   return k;
+}
+
+// How divided keys are dealt.  Every sequence's row tiles have the same number of parts, as its last one needs for
+// `share` key tiles a part, and its parts, by (KV head, part, row tile), stand behind those of the sequences before it.  Only
+// the device knows the lengths, so only it can make the parts about `slots`, equally long, without gaps between
+// them: with a grid by the longest lengths that there could be, workgroups without work stood among the
+// others, and 4 x 500 rows on prefixes of 2875 to 3835 (of at most 4608) took 47.8 us.
+struct Deal {
+  int share, total;
+  int n, incl;  // parts of lane's sequence, and of all up to it (of the first 64)
+};
+struct Seq {
+  int tiles, keys;  // row tiles, key tiles of the last of them
+  __device__ __forceinline__ int parts(int share) const { return max(1, (keys + share - 1) / share); }
+};
+template <int BN, bool PAGED>
+__device__ __forceinline__ Seq seq_at(const WinParams& p, int b) {
+  if (b >= p.batch) return Seq{0, 0};
+  const Rows r = rows_of<PAGED>(p, b);
+  const int tiles = (r.nq * p.group + kBM - 1) / kBM;
+  return Seq{tiles, tiles ? min(keys_of<BN>(p, r, tiles - 1).tiles, 1 << 20) : 0};
+}
+template <int BN, bool PAGED>
+__device__ __forceinline__ Deal deal_of(const WinParams& p, int lane) {
+  // the sums are over few row tiles (the host divides no others), of at most 2^20 key tiles
+  Deal d;
+  const Seq s = seq_at<BN, PAGED>(p, lane);
+  int work = last_lane(wave_scan(s.tiles * s.keys)), tiles = last_lane(wave_scan(s.tiles));
+  for (int b0 = 64; b0 < p.batch; b0 += 64) {
+    const Seq t = seq_at<BN, PAGED>(p, b0 + lane);
+    work += last_lane(wave_scan(t.tiles * t.keys));
+    tiles += last_lane(wave_scan(t.tiles));
+  }
+  // a sequence's last part is short: as many parts more than shares as there are row tiles
+  const int aim = max(p.slots - tiles * p.n_kv, p.slots / 2);
+  d.share = max((int)(((int64_t)work * p.n_kv + aim - 1) / aim), kMinShare);
+  d.n = s.tiles * s.parts(d.share) * p.n_kv;
+  d.incl = wave_scan(d.n);
+  d.total = last_lane(d.incl);
+  for (int b0 = 64; b0 < p.batch; b0 += 64) {
+    const Seq t = seq_at<BN, PAGED>(p, b0 + lane);
+    d.total += last_lane(wave_scan(t.tiles * t.parts(d.share) * p.n_kv));
+  }
+  return d;
+}
+// The parts before lane's sequence of the 64 from b0 on, and its own.
+template <int BN, bool PAGED>
+__device__ __forceinline__ int parts_before(const WinParams& p, const Deal& d, int b0, int lane, int& own) {
+  int n = d.n, incl = d.incl;
+  for (int b = 64; b <= b0; b += 64) {
+    const int base = last_lane(incl);
+    const Seq t = seq_at<BN, PAGED>(p, b + lane);
+    n = t.tiles * t.parts(d.share) * p.n_kv;
+    incl = base + wave_scan(n);
+  }
+  own = n;
+  return incl - n;
 }
 
 // Four neighbouring outputs, rounded to nearest even.
@@ -289,25 +345,44 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 
   __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];  // (K, V) twice
 
-  // Workgroups are dealt to the 8 XCDs in turn.  The work is cut into groups, (sequence, KV head) x part
-  // of the keys x every q_step-th row tile, a multiple of 8 of them dealt to the XCDs in turn, so that
-  // an XCD's L2 holds the keys of few groups and sequences of unequal length spread over the
-  // XCDs.  Within an XCD the longest rows come first.
+  const int lane = threadIdx.x & 63;
+  // Workgroups are dealt to the 8 XCDs in turn, and an XCD's L2 should hold the keys of few (sequence, KV head)s.
+  // Undivided: these are cut into every q_step-th row tile, so that a multiple of 8 groups is dealt to the XCDs;
+  // within an XCD the longest rows come first.  Divided: an XCD takes a contiguous range of the parts.
   const int xcd = blockIdx.x % 8, at = blockIdx.x / 8;
-  const int lvl = at / p.xcd_groups;
-  const int grp = (at - lvl * p.xcd_groups) * 8 + xcd;
-  const int unit_part = grp / p.q_step;
-  const int qt = (p.n_lvl - 1 - lvl) * p.q_step + (grp - unit_part * p.q_step);
-  const int kvh = unit_part / p.n_parts, part = unit_part - kvh * p.n_parts;
-  if (qt >= p.n_qt || kvh >= p.batch * p.n_kv) return;
-  const int b = kvh / p.n_kv;
-  const int hkv = kvh - b * p.n_kv;
-  const int tile = kvh * p.n_qt + qt;
+  int b, hkv, qt, part = 0, parts = 1, place = 0;
+  if (p.slots > 0) {
+    const Deal d = deal_of<BN, PAGED>(p, lane);
+    const int per = (d.total + 7) / 8;
+    place = xcd * per + at;
+    if (at >= per || place >= d.total) return;
+    int b0 = 0, own, before = parts_before<BN, PAGED>(p, d, 0, lane, own);
+    while (last_lane(before + own) <= place) {
+      b0 += 64;
+      before = parts_before<BN, PAGED>(p, d, b0, lane, own);
+    }
+    const int li = uni(__ffsll((unsigned long long)__ballot(before + own > place)) - 1);
+    b = b0 + li;
+    const Seq s = seq_at<BN, PAGED>(p, b);
+    const int in = place - uni(__builtin_amdgcn_readlane(before, li));
+    parts = s.parts(d.share);
+    hkv = in / (parts * s.tiles);
+    const int r = in - hkv * parts * s.tiles;
+    part = r / s.tiles;
+    qt = s.tiles - 1 - (r - part * s.tiles);
+  } else {
+    const int lvl = at / p.xcd_groups;
+    const int grp = (at - lvl * p.xcd_groups) * 8 + xcd;
+    const int kvh = grp / p.q_step;
+    qt = (p.n_lvl - 1 - lvl) * p.q_step + (grp - kvh * p.q_step);
+    if (qt >= p.n_qt || kvh >= p.batch * p.n_kv) return;
+    b = kvh / p.n_kv;
+    hkv = kvh - b * p.n_kv;
+  }
   const Rows rw = rows_of<PAGED>(p, b);
   const Keys ks = keys_of<BN>(p, rw, qt);
-  if (qt * kBM >= rw.nq * p.group || part >= ks.parts) return;
+  if (qt * kBM >= rw.nq * p.group) return;
 
-  const int lane = threadIdx.x & 63;
   const int wave = uni((int)threadIdx.x >> 6);
   const int lq = lane & 31, h = lane >> 5;
 
@@ -447,7 +522,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     TL::values(o, la, s, kt + TILEB, lane);
   };
 
-  const int t_lo = (int)((int64_t)ks.tiles * part / ks.parts), t_hi = (int)((int64_t)ks.tiles * (part + 1) / ks.parts);
+  const int t_lo = (int)((int64_t)ks.tiles * part / parts), t_hi = (int)((int64_t)ks.tiles * (part + 1) / parts);
   int pages = t_lo < t_hi ? tile_pages(t_lo) : -1;
   if (t_lo < t_hi) load_tile(t_lo, 0, pages);
   int next_pages = t_lo + 1 < t_hi ? tile_pages(t_lo + 1) : -1;
@@ -474,8 +549,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   }
 
   l = TL::kSumMfma ? la[0] : tlp::sum_xor32(l);
-  if (ks.parts > 1) {
-    float* w = p.ws + ((size_t)tile * p.n_parts + part) * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
+  if (parts > 1) {
+    float* w = p.ws + (size_t)place * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
     if (h == 0) {
       w[2 * lq] = m;
       w[2 * lq + 1] = l;
@@ -505,27 +580,34 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
   using B = typename T::bits;
   constexpr int BN = tile_keys<T>();
   const int tile = blockIdx.x, db = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, h = lane >> 5;
   const int kvh = tile / p.n_qt;
   const int qt = tile - kvh * p.n_qt;
   const int b = kvh / p.n_kv;
   const int hkv = kvh - b * p.n_kv;
-  const Rows rw = rows_of<PAGED>(p, b);
-  const Keys ks = keys_of<BN>(p, rw, qt);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lq = lane & 31, h = lane >> 5;
+  const Seq s = seq_at<BN, PAGED>(p, b);
+  if (qt >= s.tiles) return;
+  const Deal d = deal_of<BN, PAGED>(p, lane);
+  const int parts = s.parts(d.share);
+  if (parts <= 1) return;
+  int own;
+  const int before = uni(__builtin_amdgcn_readlane(parts_before<BN, PAGED>(p, d, b & ~63, lane, own), b & 63));
   const int row = qt * kBM + 32 * wave + lq;
   const int tok = row / p.group;
-  if (tok >= rw.nq || ks.parts <= 1) return;
+  if (tok >= rows_of<PAGED>(p, b).nq) return;
   const int hq = hkv * p.group + (row - tok * p.group);
-  const float* w = p.ws + (size_t)tile * p.n_parts * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
+  const float* w = p.ws + ((size_t)before + hkv * parts * s.tiles + (s.tiles - 1 - qt)) * part_floats<D>() +
+                   (size_t)wave * (64 + 64 * (D / 2));
+  const size_t step = (size_t)s.tiles * part_floats<D>();  // from part to part
   float m = -INFINITY;
-  for (int i = 0; i < ks.parts; ++i) m = fmaxf(m, w[i * part_floats<D>() + 2 * lq]);
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, w[i * step + 2 * lq]);
   const float shift = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   f32x4 o[4];
 #pragma unroll
   for (int a = 0; a < 4; ++a) o[a] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < ks.parts; ++i) {
-    const float* wi = w + i * part_floats<D>();
+  for (int i = 0; i < parts; ++i) {
+    const float* wi = w + i * step;
     const float2 ml = *(const float2*)(wi + 2 * lq);
     const float f = fast_exp2(ml.x - shift);
     l = fmaf(ml.y, f, l);
@@ -553,38 +635,35 @@ int64_t most_tiles(int64_t keys, int window, int sinks, int group, int bn) {
   return n < 1 ? 1 : n;
 }
 
-// Parts of a row tile's keys.  Where the row tiles fill the device there is one; else the key tiles are shared
-// so that there are about as many workgroups as run at once, kMinShare key tiles each at least.
-void plan_parts(WinParams& p, int64_t keys, int d_k, int esize) {
-  // workgroups that run on a CU at once: by registers at d_k 128, by LDS at d_k 64
-  const int per_cu = d_k == 64 ? 4 : 2;
+// Whether the keys of the row tiles are divided, and by how many workgroups: where the row tiles alone would not fill
+// the device and a row tile can have several parts.  fp32 is bound by its matrix products, which one workgroup a CU
+// keeps busy; the 16-bit kernels take as many as fit.  Returns the most parts there can be (0: undivided).
+int64_t plan_slots(WinParams& p, int64_t keys, int d_k, int esize) {
   const int bn = esize == 2 ? 64 : 32;
   const int64_t most = most_tiles(keys, p.window, p.sinks, p.group, bn);
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
-  const int64_t slots = (int64_t)tl_device_cus() * per_cu;
-  int64_t share = (tiles * most + slots - 1) / slots;
-  share = share < kMinShare ? kMinShare : share;
-  const int64_t parts = (most + share - 1) / share;
-  p.share = (int)share;
-  p.n_parts = tiles >= slots || parts < 2 ? 1 : (int)parts;
+  const int64_t slots = (int64_t)tl_device_cus() * (esize == 4 ? 1 : d_k == 64 ? 3 : 2);
+  p.slots = tiles >= slots || most < 2 * kMinShare ? 0 : (int)slots;
+  const int64_t parts = tiles * ((most + kMinShare - 1) / kMinShare);
+  return !p.slots ? 0 : parts < 2 * slots + tiles ? parts : 2 * slots + tiles;
 }
 
 size_t part_bytes(int d_k) { return (d_k == 64 ? part_floats<64>() : part_floats<128>()) * sizeof(float); }
 
 template <typename T, int D>
-int launch_window(WinParams& p, bool paged, hipStream_t st) {
+int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) {
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
-  if (tiles * p.n_parts > (1 << 27)) return TL_ERR_UNSUPPORTED;
-  const int64_t unit_parts = (int64_t)p.batch * p.n_kv * p.n_parts;
-  p.q_step = 8;  // unit_parts * q_step is a multiple of 8
-  while (p.q_step > 1 && unit_parts % (16 / p.q_step) == 0) p.q_step /= 2;
+  if (tiles > (1 << 27)) return TL_ERR_UNSUPPORTED;
+  const int64_t units = (int64_t)p.batch * p.n_kv;
+  p.q_step = 8;  // units * q_step is a multiple of 8
+  while (p.q_step > 1 && units % (16 / p.q_step) == 0) p.q_step /= 2;
   p.n_lvl = (p.n_qt + p.q_step - 1) / p.q_step;
-  p.xcd_groups = (int)(unit_parts * p.q_step / 8);
-  const dim3 grid((unsigned)(8 * p.xcd_groups * p.n_lvl));
+  p.xcd_groups = (int)(units * p.q_step / 8);
+  const dim3 grid(p.slots > 0 ? (unsigned)((most_parts + 7) / 8 * 8) : (unsigned)(8 * p.xcd_groups * p.n_lvl));
   if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
   int e = tl_launch_status();
-  if (e || p.n_parts == 1) return e;
+  if (e || p.slots == 0) return e;
   const dim3 join((unsigned)tiles, D / 32);
   if (paged) hipLaunchKernelGGL((window_join_kernel<T, D, true>), join, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_join_kernel<T, D, false>), join, dim3(kThreads), 0, st, p);
@@ -617,18 +696,17 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
   p.n_qt = (p.seq_q * p.group + kBM - 1) / kBM;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.vec_out = ((uintptr_t)p.o % (4 * esize)) == 0 && os[0] % 4 == 0 && os[1] % 4 == 0 && os[2] % 4 == 0;
-  plan_parts(p, keys, d_k, esize);
-  if (p.n_parts > 1) {
-    // without room for the parts the call runs whole
-    const size_t need = (size_t)p.batch * p.n_kv * p.n_qt * p.n_parts * part_bytes(d_k);
-    if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)) p.n_parts = 1;
+  const int64_t most_parts = plan_slots(p, keys, d_k, esize);
+  if (p.slots > 0) {
+    // without room for the parts the keys stay undivided
+    if (!workspace || workspace_bytes < (size_t)most_parts * part_bytes(d_k) || ((uintptr_t)workspace & 15)) p.slots = 0;
     p.ws = (float*)workspace;
   }
   hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
-    case TL_DTYPE_F32: return d_k == 64 ? launch_window<F32, 64>(p, paged, st) : launch_window<F32, 128>(p, paged, st);
-    case TL_DTYPE_F16: return d_k == 64 ? launch_window<F16, 64>(p, paged, st) : launch_window<F16, 128>(p, paged, st);
-    default: return d_k == 64 ? launch_window<BF16, 64>(p, paged, st) : launch_window<BF16, 128>(p, paged, st);
+    case TL_DTYPE_F32: return d_k == 64 ? launch_window<F32, 64>(p, paged, most_parts, st) : launch_window<F32, 128>(p, paged, most_parts, st);
+    case TL_DTYPE_F16: return d_k == 64 ? launch_window<F16, 64>(p, paged, most_parts, st) : launch_window<F16, 128>(p, paged, most_parts, st);
+    default: return d_k == 64 ? launch_window<BF16, 64>(p, paged, most_parts, st) : launch_window<BF16, 128>(p, paged, most_parts, st);
   }
 }
 
@@ -649,8 +727,7 @@ size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q
   p.n_qt = (seq_q * p.group + kBM - 1) / kBM;
   p.window = window;
   p.sinks = sinks;
-  plan_parts(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2);
-  return p.n_parts == 1 ? 0 : (size_t)batch * n_kv_head * p.n_qt * p.n_parts * part_bytes(d_k);
+  return (size_t)plan_slots(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2) * part_bytes(d_k);
 }
 
 int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace, size_t workspace_bytes, int batch, int n_head, int n_kv_head,
