@@ -39,9 +39,10 @@ struct WinParams {
   const int32_t* lens;
   const int32_t* new_lens;
   int batch, n_head, n_kv, group, seq_q, seq_k, n_qt;
+  uint32_t group_magic;  // row / group = mulhi(row, group_magic) for the rows there are (group > 1)
   int window, sinks;
   int slots;           // workgroups that the keys are shared by; 0: a row tile's keys are not divided
-  int q_step, n_lvl, xcd_groups;  // how workgroups are dealt (window_fwd_kernel)
+  int q_shift, n_lvl, xcd_groups;  // how workgroups are dealt (window_fwd_kernel)
   int vec_out;         // o's rows take 4 elements at once
   float* ws;           // partial results by part (slots > 0)
   int64_t q_sb, q_sh, q_ss;
@@ -207,6 +208,12 @@ struct Tile<F16, D> : Tile16<F16, D> {};
 template <int D>
 struct Tile<F32, D> : Tile32<D> {};
 
+// The token of a row.  Integer divisions are long dependent chains, and what runs before a short call's first
+// load counts: this one is a multiplication.
+__device__ __forceinline__ int token_of(const WinParams& p, int row) {
+  return p.group == 1 ? row : (int)__umulhi((uint32_t)row, p.group_magic);
+}
+
 // Where a sequence's query rows stand: token i at position base + i, nq tokens, no key from `end` on.
 struct Rows {
   int base, nq, end;
@@ -235,8 +242,8 @@ struct Keys {
 template <int BN>
 __device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int qt) {
   Keys k{0, 0, 0, r.end};
-  const int p0 = r.base + qt * kBM / p.group;
-  const int p1 = min(r.base + min((qt * kBM + kBM - 1) / p.group + 1, r.nq), r.end) - 1;  // last key any row sees
+  const int p0 = r.base + token_of(p, qt * kBM);
+  const int p1 = min(r.base + min(token_of(p, qt * kBM + kBM - 1) + 1, r.nq), r.end) - 1;  // last key any row sees
   if (p1 < 0) return k;
   if (p.window > 0) {
     k.t0 = max(p0 - p.window + 1, 0) / BN;
@@ -280,7 +287,8 @@ __device__ __forceinline__ Deal deal_of(const WinParams& p, int lane) {
   }
   // a sequence's last part is short: as many parts more than shares as there are row tiles
   const int aim = max(p.slots - tiles * p.n_kv, p.slots / 2);
-  d.share = max((int)(((int64_t)work * p.n_kv + aim - 1) / aim), kMinShare);
+  // rounded up past the 32-bit quotient's error
+  d.share = max((int)((float)work * (float)p.n_kv * __builtin_amdgcn_rcpf((float)aim) * 1.00001f) + 1, kMinShare);
   d.n = s.tiles * s.parts(d.share) * p.n_kv;
   d.incl = wave_scan(d.n);
   d.total = last_lane(d.incl);
@@ -347,7 +355,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 
   const int lane = threadIdx.x & 63;
   // Workgroups are dealt to the 8 XCDs in turn, and an XCD's L2 should hold the keys of few (sequence, KV head)s.
-  // Undivided: these are cut into every q_step-th row tile, so that a multiple of 8 groups is dealt to the XCDs;
+  // Undivided: these are cut into every 2^q_shift-th row tile, so that a multiple of 8 groups is dealt to the XCDs;
   // within an XCD the longest rows come first.  Divided: an XCD takes a contiguous range of the parts.
   const int xcd = blockIdx.x % 8, at = blockIdx.x / 8;
   int b, hkv, qt, part = 0, parts = 1, place = 0;
@@ -366,17 +374,17 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     const Seq s = seq_at<BN, PAGED>(p, b);
     const int in = place - uni(__builtin_amdgcn_readlane(before, li));
     parts = s.parts(d.share);
-    hkv = in / (parts * s.tiles);
+    hkv = (int)((unsigned)in / (unsigned)(parts * s.tiles));
     const int r = in - hkv * parts * s.tiles;
-    part = r / s.tiles;
+    part = (int)((unsigned)r / (unsigned)s.tiles);
     qt = s.tiles - 1 - (r - part * s.tiles);
   } else {
-    const int lvl = at / p.xcd_groups;
+    const int lvl = (int)((unsigned)at / (unsigned)p.xcd_groups);
     const int grp = (at - lvl * p.xcd_groups) * 8 + xcd;
-    const int kvh = grp / p.q_step;
-    qt = (p.n_lvl - 1 - lvl) * p.q_step + (grp - kvh * p.q_step);
+    const int kvh = grp >> p.q_shift;
+    qt = ((p.n_lvl - 1 - lvl) << p.q_shift) + (grp - (kvh << p.q_shift));
     if (qt >= p.n_qt || kvh >= p.batch * p.n_kv) return;
-    b = kvh / p.n_kv;
+    b = (int)((unsigned)kvh / (unsigned)p.n_kv);
     hkv = kvh - b * p.n_kv;
   }
   const Rows rw = rows_of<PAGED>(p, b);
@@ -388,7 +396,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 
   // this lane's row: query head hkv * group + row % group of token row / group
   const int row = qt * kBM + 32 * wave + lq;
-  const int tok = row / p.group;
+  const int tok = token_of(p, row);
   const int hq = hkv * p.group + (row - tok * p.group);
   const bool there = tok < rw.nq;
   const int pos = rw.base + tok;
@@ -457,8 +465,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 
   // this wave's first and last position
   const int row0 = qt * kBM + 32 * wave;
-  const int wp0 = uni(rw.base + row0 / p.group);
-  const int wp1 = uni(rw.base + min((row0 + 31) / p.group, rw.nq - 1));
+  const int wp0 = uni(rw.base + token_of(p, row0));
+  const int wp1 = uni(rw.base + min(token_of(p, row0 + 31), rw.nq - 1));
   const bool wave_rows = row0 < rw.nq * p.group;
 
   // One key tile: scores, softmax, O^T.  all: every row sees every key.
@@ -522,7 +530,12 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     TL::values(o, la, s, kt + TILEB, lane);
   };
 
-  const int t_lo = (int)((int64_t)ks.tiles * part / parts), t_hi = (int)((int64_t)ks.tiles * (part + 1) / parts);
+  int t_lo = 0, t_hi = ks.tiles;
+  if (parts > 1) {
+    const int each = (int)((unsigned)ks.tiles / (unsigned)parts), more = ks.tiles - each * parts;
+    t_lo = part * each + min(part, more);
+    t_hi = t_lo + each + (part < more ? 1 : 0);
+  }
   int pages = t_lo < t_hi ? tile_pages(t_lo) : -1;
   if (t_lo < t_hi) load_tile(t_lo, 0, pages);
   int next_pages = t_lo + 1 < t_hi ? tile_pages(t_lo + 1) : -1;
@@ -593,7 +606,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
   int own;
   const int before = uni(__builtin_amdgcn_readlane(parts_before<BN, PAGED>(p, d, b & ~63, lane, own), b & 63));
   const int row = qt * kBM + 32 * wave + lq;
-  const int tok = row / p.group;
+  const int tok = token_of(p, row);
   if (tok >= rows_of<PAGED>(p, b).nq) return;
   const int hq = hkv * p.group + (row - tok * p.group);
   const float* w = p.ws + ((size_t)before + hkv * parts * s.tiles + (s.tiles - 1 - qt)) * part_floats<D>() +
@@ -648,6 +661,10 @@ int64_t plan_slots(WinParams& p, int64_t keys, int d_k, int esize) {
   return !p.slots ? 0 : parts < 2 * slots + tiles ? parts : 2 * slots + tiles;
 }
 
+// Rows that token_of() divides exactly: the magic's excess, below group, times a row stays below 2^32.  (Rows of the
+// last tile count.)
+bool rows_ok(int64_t seq_q, int64_t group) { return (seq_q * group + kBM) * group < ((int64_t)1 << 32); }
+
 size_t part_bytes(int d_k) { return (d_k == 64 ? part_floats<64>() : part_floats<128>()) * sizeof(float); }
 
 template <typename T, int D>
@@ -655,10 +672,10 @@ int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) 
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
   if (tiles > (1 << 27)) return TL_ERR_UNSUPPORTED;
   const int64_t units = (int64_t)p.batch * p.n_kv;
-  p.q_step = 8;  // units * q_step is a multiple of 8
-  while (p.q_step > 1 && units % (16 / p.q_step) == 0) p.q_step /= 2;
-  p.n_lvl = (p.n_qt + p.q_step - 1) / p.q_step;
-  p.xcd_groups = (int)(units * p.q_step / 8);
+  p.q_shift = 3;  // units << q_shift is a multiple of 8
+  while (p.q_shift > 0 && units % (16 >> p.q_shift) == 0) --p.q_shift;
+  p.n_lvl = (p.n_qt + (1 << p.q_shift) - 1) >> p.q_shift;
+  p.xcd_groups = (int)((units << p.q_shift) / 8);
   const dim3 grid(p.slots > 0 ? (unsigned)((most_parts + 7) / 8 * 8) : (unsigned)(8 * p.xcd_groups * p.n_lvl));
   if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
@@ -692,7 +709,8 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
   p.v_sb = vs[0], p.v_sh = vs[1], p.v_ss = vs[2];
   p.o_sb = os[0], p.o_sh = os[1], p.o_ss = os[2];
   p.group = p.n_head / p.n_kv;
-  if ((int64_t)p.seq_q * p.group > (1 << 30)) return TL_ERR_UNSUPPORTED;
+  if (!rows_ok(p.seq_q, p.group)) return TL_ERR_UNSUPPORTED;
+  p.group_magic = (uint32_t)((((uint64_t)1 << 32) + p.group - 1) / p.group);
   p.n_qt = (p.seq_q * p.group + kBM - 1) / kBM;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.vec_out = ((uintptr_t)p.o % (4 * esize)) == 0 && os[0] % 4 == 0 && os[1] % 4 == 0 && os[2] % 4 == 0;
@@ -717,7 +735,7 @@ extern "C" {
 size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q, int most_keys, int d_k, int window,
                                  int sinks, int dtype) {
   if (batch < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || seq_q < 1 || seq_q > (1 << 29) || most_keys < 1 ||
-      window < 0 || sinks < 0 || (d_k != 64 && d_k != 128) || (int64_t)seq_q * (n_head / n_kv_head) > (1 << 30) ||
+      window < 0 || sinks < 0 || (d_k != 64 && d_k != 128) || !rows_ok(seq_q, n_head / n_kv_head) ||
       (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16))
     return 0;
   WinParams p{};
