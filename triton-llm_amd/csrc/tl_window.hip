@@ -415,29 +415,39 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     voff[i] = r * v_row + (((lane % NSL) ^ v_swz<T, D>(rt)) << 4);
   }
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)smem;
-  const int32_t* table = PAGED ? p.pm.table + (int64_t)b * p.pm.max_pages : nullptr;
-  // lane i < BN / 16: the page of the tile's block i, -1 where there is none
-  auto tile_pages = [&](int t) {
-    int id = -1;
+  // The pages of 64 / TB tiles from pages_t on, lane by lane: tile (pages_t + lane / TB)'s block lane % TB; gone: which of
+  // these there are not.  A load for each tile would be waited for with every LDS-DMA before it, which the compiler does
+  // not know of, and scalar loads with every LDS read: 4 x 500 rows on prefixes took 48.5 and 53.1 us, 45.4 so.
+  constexpr int TB = BN / kBlk;
+  int pages = 0, pages_t = 0;
+  uint64_t gone_lanes = 0;
+  int t_lo = 0, t_hi = ks.tiles;
+  if (parts > 1) {
+    const int each = (int)((unsigned)ks.tiles / (unsigned)parts), more = ks.tiles - each * parts;
+    t_lo = part * each + min(part, more);
+    t_hi = t_lo + each + (part < more ? 1 : 0);
+  }
+  auto look_up = [&](int t) __attribute__((always_inline)) {
     if constexpr (PAGED) {
-      const int e = (ks.key0(t) * BN + kBlk * lane) >> p.pm.shift;
-      if (lane < BN / kBlk && e < p.pm.max_pages) id = table[e];
-      if ((unsigned)id >= (unsigned)p.pm.n_pages) id = -1;
+      pages_t = t;
+      const int e = (ks.key0(min(t + lane / TB, t_hi - 1)) * BN + kBlk * (lane % TB)) >> p.pm.shift;
+      pages = e < p.pm.max_pages ? p.pm.table[(int64_t)b * p.pm.max_pages + e] : -1;
+      gone_lanes = __ballot((unsigned)pages >= (unsigned)p.pm.n_pages);
     }
-    return id;
   };
   // Rows past the last key, and rows of pages that are not there, read as zeros.
   const char* const kbase = (const char*)((const B*)p.k + (PAGED ? 0 : b * p.k_sb) + hkv * p.k_sh);
   const char* const vbase = (const char*)((const B*)p.v + (PAGED ? 0 : b * p.v_sb) + hkv * p.v_sh);
-  auto load_tile = [&](int t, int buf, int pages) __attribute__((always_inline)) {
+  auto load_tile = [&](int t, int buf) __attribute__((always_inline)) {
     const int pos0 = ks.key0(t) * BN + wave * WROWS;
     int rows = min(max(ks.end - pos0, 0), WROWS);
     int64_t ka, va;
     if constexpr (PAGED) {
-      const int id = __builtin_amdgcn_readlane(pages, (wave * WROWS) / kBlk);
+      const int id = __builtin_amdgcn_readlane(pages, (t - pages_t) * TB + (wave * WROWS) / kBlk);
       const int in = pos0 & ((1 << p.pm.shift) - 1);
-      if (id < 0) rows = 0;
-      const int64_t at = id < 0 ? 0 : id;
+      const bool page = (unsigned)id < (unsigned)p.pm.n_pages;
+      if (!page) rows = 0;
+      const int64_t at = page ? id : 0;
       ka = at * p.k_sb * T::size + (int64_t)in * k_row;
       va = at * p.v_sb * T::size + (int64_t)in * v_row;
     } else {
@@ -472,7 +482,10 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   // One key tile: scores, softmax, O^T.  all: every row sees every key.
   auto step = [&](int k0, const char* kt, uint32_t gone, bool all) __attribute__((always_inline)) {
     f32x16 s[NMB];
+    // matrix phases win over the other workgroup's softmax: 133 -> 130.4 us at 8192 tokens
+    __builtin_amdgcn_s_setprio(1);
     TL::scores(s, q, kt, lq, h);
+    __builtin_amdgcn_s_setprio(0);
     if (!all) {
       asm volatile("");  // a branch: as selects the tests would run for every tile
       // key k0 + kl + 4 h of this lane is seen if kl <= hi and (kl > lo or kl < sk)
@@ -527,34 +540,28 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
         s[mb][r] = fast_exp2(fmaf(s[mb][r], scale, -shift));
         if (!TL::kSumMfma) l += s[mb][r];
       }
+    __builtin_amdgcn_s_setprio(1);
     TL::values(o, la, s, kt + TILEB, lane);
+    __builtin_amdgcn_s_setprio(0);
   };
 
-  int t_lo = 0, t_hi = ks.tiles;
-  if (parts > 1) {
-    const int each = (int)((unsigned)ks.tiles / (unsigned)parts), more = ks.tiles - each * parts;
-    t_lo = part * each + min(part, more);
-    t_hi = t_lo + each + (part < more ? 1 : 0);
+  if (t_lo < t_hi) {
+    look_up(t_lo);
+    load_tile(t_lo, 0);
   }
-  int pages = t_lo < t_hi ? tile_pages(t_lo) : -1;
-  if (t_lo < t_hi) load_tile(t_lo, 0, pages);
-  int next_pages = t_lo + 1 < t_hi ? tile_pages(t_lo + 1) : -1;
   for (int t = t_lo; t < t_hi; ++t) {
     wait_vmcnt<0>();  // this wave's rows of tile t are in LDS
     lds_barrier();    // everybody's are, and tile t - 1 has been read
     const int buf = (t - t_lo) & 1;
-    const int these = pages;
+    const uint32_t gone = PAGED ? (uint32_t)(gone_lanes >> ((t - pages_t) * TB)) & ((1u << TB) - 1) : 0;
     if (t + 1 < t_hi) {
-      load_tile(t + 1, buf ^ 1, next_pages);
-      pages = next_pages;
-      if (t + 2 < t_hi) next_pages = tile_pages(t + 2);
+      if (PAGED && t + 1 - pages_t == 64 / TB) look_up(t + 1);
+      load_tile(t + 1, buf ^ 1);
     }
     const int k0 = ks.key0(t) * BN;
     // does any row of this wave see a key of the tile, and does every row see all of them
     const bool any = wave_rows && k0 <= wp1 && (p.window <= 0 || k0 + BN - 1 > wp0 - p.window || k0 < p.sinks);
     if (!any) continue;
-    uint32_t gone = 0;  // blocks that have no page
-    if constexpr (PAGED) gone = (uint32_t)__ballot(these < 0) & ((1u << (BN / kBlk)) - 1);
     const bool all = k0 + BN - 1 <= wp0 && k0 + BN <= ks.end && gone == 0 &&
                      (p.window <= 0 || k0 > wp1 - p.window || k0 + BN <= p.sinks);
     const char* kt = smem + buf * 2 * TILEB;
