@@ -16,7 +16,7 @@ import math
 import numpy as np
 
 from triton_llm import _lib, gpu
-from ._common import launch, scratch, vp
+from ._common import launch, scratch
 
 __all__ = ["beam_select", "max_select"]
 
@@ -73,6 +73,6 @@ def beam_select(logits_dev, scores_dev, n_select: int | None = None, out=None, w
     if batch == 0 or n_select == 0:
         return out
     ws = scratch(need, workspace, key="beam")
-    launch(gpu.runtime().tl_beam_select, vp(logits_dev), vp(scores_dev), batch, beams, vocab, vocab, n_select,
-           vp(out[0]), vp(out[1]), vp(out[2]), vp(ws), ws.nbytes, code, None, what="beam_select")
+    launch(gpu.runtime().tl_beam_select, logits_dev.ptr, scores_dev.ptr, batch, beams, vocab, vocab, n_select,
+           out[0].ptr, out[1].ptr, out[2].ptr, ws.ptr, ws.nbytes, code, None, what="beam_select")
     return out

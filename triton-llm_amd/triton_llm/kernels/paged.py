@@ -29,11 +29,12 @@ import ctypes
 import functools
 import math
 import operator
+import struct
 
 import numpy as np
 
 from triton_llm import _lib, gpu
-from ._common import default_scale, launch, same_dtype, scratch, vp
+from ._common import default_scale, launch, same_dtype, scratch
 
 MIN_PAGE, MAX_PAGE = 16, 1024
 
@@ -62,6 +63,23 @@ def _is_int32(t) -> bool:
     return t.dtype.char == "i"
 
 
+def _code(*tensors) -> int:
+    """Dtype code shared by all tensors; ValueError if they differ (same_dtype, without its pass over the
+    names where every tensor has the very same dtype object)."""
+    dt = tensors[0].dtype
+    for t in tensors:
+        if t.dtype is not dt:
+            return same_dtype(*tensors)
+    return _BF16 if dt is gpu.bfloat16 else gpu.dtype_code(dt)
+
+
+_BF16 = _lib.DTYPE_BF16
+
+
+def _ptr(t):
+    return None if t is None else t.ptr
+
+
 def _check_pool(k_shape, v_shape):
     if len(k_shape) != 4 or k_shape != v_shape:
         raise ValueError(f"k_pages/v_pages must be matching 4-D (n_pages, n_kv_head, page_size, d_k), "
@@ -85,6 +103,8 @@ def _check_table(table_shape, lens_shape, new_lens_shape, page_size, most):
 
 
 def _check_int32(page_table, cache_lens, new_lens=None):
+    if page_table.dtype.char == cache_lens.dtype.char == "i" and (new_lens is None or new_lens.dtype.char == "i"):
+        return
     for name, t in (("page_table", page_table), ("cache_lens", cache_lens), ("new_lens", new_lens)):
         if t is not None and not _is_int32(t):
             raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
@@ -172,14 +192,14 @@ def paged_kv_append(q_dev, k_new, v_new, k_pages, v_pages, page_table, cache_len
     if q_dev is None:
         if q_out is not None:
             raise ValueError("q_out is given without q_dev")
-        code = same_dtype(k_new, v_new, k_pages, v_pages)
+        code = _code(k_new, v_new, k_pages, v_pages)
     else:
         q_out = q_dev if q_out is None else _same_output(q_out, q_dev)
-        code = same_dtype(k_new, v_new, k_pages, v_pages, q_dev)
+        code = _code(k_new, v_new, k_pages, v_pages, q_dev)
     if cos_dev is not None and not cos_dev.dtype.char == sin_dev.dtype.char == "f":
         raise ValueError(f"cos/sin tables must be float32, got {cos_dev.dtype} and {sin_dev.dtype}")
-    launch(gpu.runtime().tl_paged_kv_append, vp(q_dev), vp(q_out), vp(k_new), vp(v_new), vp(k_pages), vp(v_pages),
-           vp(page_table), *pages, vp(cache_lens), vp(new_lens), vp(cos_dev), vp(sin_dev), *tables,
+    launch(gpu.runtime().tl_paged_kv_append, _ptr(q_dev), _ptr(q_out), k_new.ptr, v_new.ptr, k_pages.ptr,
+           v_pages.ptr, page_table.ptr, *pages, cache_lens.ptr, _ptr(new_lens), _ptr(cos_dev), _ptr(sin_dev), *tables,
            1 if interleaved else 0, *sizes, code, None, what="paged_kv_append")
     return q_out
 
@@ -230,14 +250,14 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
     _check_int32(page_table, cache_lens)
     pages, sizes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape, None,
                                    q_dev.shape, n_head, n_kv_head, window, sinks, False)
-    code = same_dtype(q_dev, k_pages, v_pages)
+    code = _code(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
     d_k = k_pages.shape[3]
     if sm_scale is None:
         sm_scale = default_scale(d_k)
     ws = scratch(_decode_workspace_bytes(n_head, n_kv_head, d_k), workspace, key="paged_decode")
-    launch(gpu.runtime().tl_paged_attention_decode, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), *pages,
-           vp(cache_lens), int(len_add), int(window), int(sinks), vp(out), vp(ws), ws.nbytes, *sizes, float(sm_scale), code, None,
+    launch(gpu.runtime().tl_paged_attention_decode, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
+           cache_lens.ptr, int(len_add), int(window), int(sinks), out.ptr, ws.ptr, ws.nbytes, *sizes, float(sm_scale), code, None,
            what="paged_attention_decode")
     return out
 
@@ -253,15 +273,18 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
     _check_int32(page_table, cache_lens, new_lens)
     pages, sizes, ws_bytes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
                                              _shape(new_lens), q_dev.shape, n_head, n_kv_head, window, sinks, True)
-    code = same_dtype(q_dev, k_pages, v_pages)
+    code = _code(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
     ws = scratch(ws_bytes[code], workspace, key="window")
     if sm_scale is None:
         sm_scale = default_scale(k_pages.shape[3])
-    launch(gpu.runtime().tl_paged_attention_prefill, vp(q_dev), vp(k_pages), vp(v_pages), vp(page_table), *pages,
-           vp(cache_lens), vp(new_lens), vp(out), vp(ws), ws.nbytes if ws is not None else 0, *sizes, float(sm_scale), int(window), int(sinks), code, None,
+    launch(gpu.runtime().tl_paged_attention_prefill, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
+           cache_lens.ptr, _ptr(new_lens), out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes, float(sm_scale), int(window), int(sinks), code, None,
            what="paged_attention_prefill")
     return out
+
+
+_get_shape, _get_dtype = operator.attrgetter("shape"), operator.attrgetter("dtype")
 
 
 def copy_kv_pages(caches, src, dst) -> None:
@@ -284,9 +307,10 @@ def copy_kv_pages(caches, src, dst) -> None:
         raise ValueError(f"pools must be 4-D (n_pages, n_kv_head, page_size, d_k), got {shape}")
     _check_page_size(shape[2])
     gpu.dtype_code(dtype)
-    for c in caches:
-        if c.shape != shape or (c.dtype is not dtype and gpu.dtype_name(c.dtype) != gpu.dtype_name(dtype)):
-            raise ValueError(f"pools differ: {shape} {gpu.dtype_name(dtype)} and {c.shape} {gpu.dtype_name(c.dtype)}")
+    if list(map(_get_shape, caches)).count(shape) != len(caches) or list(map(_get_dtype, caches)).count(dtype) != len(caches):
+        for c in caches:
+            if c.shape != shape or gpu.dtype_name(c.dtype) != gpu.dtype_name(dtype):
+                raise ValueError(f"pools differ: {shape} {gpu.dtype_name(dtype)} and {c.shape} {gpu.dtype_name(c.dtype)}")
     if min(src) < 0 or min(dst) < 0 or max(src) >= shape[0] or max(dst) >= shape[0]:
         raise ValueError(f"page numbers must be in [0, {shape[0]})")
     to = set(dst)
@@ -295,7 +319,7 @@ def copy_kv_pages(caches, src, dst) -> None:
     if not to.isdisjoint(src):
         raise ValueError("a page is source and destination")
     page_bytes = shape[1] * shape[2] * shape[3] * dtype.itemsize
-    bases = (ctypes.c_void_p * len(caches))(*[c.ptr.value for c in caches])
+    bases = (ctypes.c_void_p * len(caches)).from_buffer_copy(struct.pack(f"{len(caches)}Q", *[c.ptr.value or 0 for c in caches]))
     launch(gpu.runtime().tl_copy_pages, bases, len(caches), page_bytes, page_bytes, shape[0], (ctypes.c_int32 * n)(*src),
            (ctypes.c_int32 * n)(*dst), n, None, what="copy_kv_pages")
 
@@ -326,5 +350,5 @@ def write_i32(dst, index, value) -> None:
         raise ValueError("an index is given twice")
     if min(value) < -(1 << 31) or max(value) >= 1 << 31:
         raise ValueError("values must fit in int32")
-    launch(gpu.runtime().tl_write_i32, vp(dst), dst.size, (ctypes.c_int32 * n)(*index), (ctypes.c_int32 * n)(*value), n,
+    launch(gpu.runtime().tl_write_i32, dst.ptr, dst.size, (ctypes.c_int32 * n)(*index), (ctypes.c_int32 * n)(*value), n,
            None, what="write_i32")
