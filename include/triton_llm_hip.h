@@ -378,13 +378,15 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * {batch, head}, over L = min(cache_lens[b] + len_add, max_pages * page_size)
  * positions; with window > 0 it sees only the last `window` of them and the first
  * `sinks`.  A sequence that sees nothing gives zeros.  Hidden positions are not
- * read.  Two launches; the workspace (tl_paged_decode_workspace_bytes, 16-byte
- * aligned) holds partial results and needs no initialisation.  d_k 64 or 128,
- * rows aligned to d_k / 16 elements.
+ * read.  One launch, or two where a sequence's positions are shared by several
+ * workgroups: the workspace (tl_paged_decode_workspace_bytes, 16-byte aligned, given
+ * either way) holds their results and needs no initialisation; calls that overlap in time need
+ * one each.  d_k 64 or 128, rows aligned to d_k / 16 elements; batch <= 65535, and
+ * at most 2^31 - 1 blocks of 16 positions over batch, KV heads and pages.
  *
  * tl_paged_attention_prefill: n_new queries per sequence (new_lens[b] where it is
  * not NULL; rows behind them are left as they were), query i at position
- * cache_lens[b] + i, over the pages (their own positions appended before), with
+ * cache_lens[b] + i (lengths past 2^30 count as 2^30), over the pages (their own positions appended before), with
  * the same window.  q / o (batch, n_new, n_head, d_k) {batch, head, seq}.
  * tl_window_attention: the same over K / V (batch, n_kv_head, seq_k, d_k)
  * {batch, head, seq}, query i at position seq_k - seq_q + i.
@@ -394,14 +396,15 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * workspace (tl_window_workspace_bytes bytes, 16-byte aligned, most_keys = seq_k, or
  * max_pages * page_size; no initialisation) and are joined by a second launch;
  * given less (NULL: none) the call runs in one.  Either is deterministic.
+ * (n_new or seq_q) <= 2^28, seq_k <= 2^29, and times the square of n_head / n_kv_head below 2^32.
  * A NaN or infinity in a V row makes NaN of the rows that are computed in one
  * tile with it, seen or not, as a product with a zero weight does.
  *
  * tl_copy_pages: page host_dst[i] = page host_src[i], i < count, in every cache of
  * the list (page_bytes bytes at page_stride_bytes * page of each base, all three
- * multiples of 16).  The lists are host memory and travel with the launch: they may be
+ * multiples of 16, a page at most 2^30).  The lists are host memory and travel with the launch: they may be
  * released at once, and a captured graph keeps them.  A page that is a destination
- * twice, or a source and a destination, ends up with either content.
+ * twice, or a source and a destination, ends up with some of each content.
  * tl_write_i32: dst[host_index[i]] = host_value[i] on the device, by value likewise
  * (page table entries, lengths); an index twice: either value.
  * ------------------------------------------------------------------------- */

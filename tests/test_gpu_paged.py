@@ -211,6 +211,33 @@ def test_prefill_pages_that_are_not_there(dtype):
         P.check(f"prefill without pages {dtype} sequence {b}", got[b].transpose(1, 0, 2), want, tol)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 0), (30, 5), (1000, 2), ((1 << 31) - 1, 0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prefill_past_the_table(dtype, window, sinks):
+    """Queries behind the last page, some by more than the window: they see what there is."""
+    rng = np.random.default_rng(12)
+    Hq, Hkv, D, page, n_new, cap = 2, 1, 64, 16, 140, 112
+    lens = np.array([100, 200, 2 ** 31 - 1, 0, -2 ** 31], np.int32)
+    table = rng.permutation(30)[:7][None].repeat(5, 0).astype(np.int32)
+    kp, vp = P.values(rng, (30, Hkv, page, D), dtype), P.values(rng, (30, Hkv, page, D), dtype)
+    q = P.values(rng, (5, n_new, Hq, D), dtype)
+    out = paged_attention_prefill(P.dev(q, dtype), P.dev(kp, dtype), P.dev(vp, dtype), P.int32(table), P.int32(lens), Hq, Hkv,
+                                  window=window, sinks=sinks)
+    got = P.back(out, dtype)
+    k, there = op.gather(on.from_storage(kp, dtype), table[0], cap)
+    v, _ = op.gather(on.from_storage(vp, dtype), table[0], cap)
+    for b in (0, 1, 3):
+        want, tol = P.rows_want(q[b].transpose(1, 0, 2), k, v, lens[b] + np.arange(n_new), there, window, sinks, D ** -0.5, dtype)
+        P.check(f"prefill past the table {dtype} window {window} sequence {b}", got[b].transpose(1, 0, 2), want, tol)
+    assert (got[4] == 0).all()
+    if window == 30 and sinks == 0:
+        assert (got[2] == 0).all()
+    else:  # the window hides nothing or all but the sinks
+        far = np.full(n_new, cap if window in (0, (1 << 31) - 1) else cap + window)
+        want, tol = P.rows_want(q[2].transpose(1, 0, 2), k, v, far, there, window, sinks, D ** -0.5, dtype)
+        P.check(f"prefill far past the table {dtype} window {window}", got[2].transpose(1, 0, 2), want, tol)
+
+
 # ---- pools of more than 4 GiB ------------------------------------------------------------
 
 def test_pages_beyond_32_bit_offsets():

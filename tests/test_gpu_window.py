@@ -47,6 +47,12 @@ def test_scales(scale):
     run("float32", 1, 2, 1, 100, 100, 64, 0, 0, scale=scale)
 
 
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 3 << 29, (3 << 29) - 1, 1 << 30])
+def test_windows_beyond_every_key(window):
+    run("float32", 1, 2, 1, 90, 50, 64, window, 3)  # the first 40 rows stand before position 0
+    run("float16", 1, 2, 1, 50, 90, 128, window, 0)
+
+
 def test_long():
     run("bfloat16", 1, 1, 1, 4000, 4000, 128, 700, 4)
 

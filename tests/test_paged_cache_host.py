@@ -160,7 +160,7 @@ def test_window_gives_pages_back():
 
 @pytest.mark.parametrize("args,kw,msg", [
     ((2, 10, 3, 64), {}, "bad head counts"), ((0, 9, 3, 64), {}, "bad head counts"),
-    ((2, 9, 3, 64), {"n_pages": 0}, "must be positive"), ((2, 9, 3, 64), {"max_seq": 0}, "must be positive"),
+    ((2, 9, 3, 96), {}, "d_k in"), ((2, 9, 3, 64), {"n_pages": 0}, "must be positive"), ((2, 9, 3, 64), {"max_seq": 0}, "must be positive"),
     ((2, 9, 3, 64), {"window": -1}, "window and sinks"), ((2, 9, 3, 64), {"page_size": 24}, "power of 2")])
 def test_constructor_refuses(args, kw, msg):
     with pytest.raises(ValueError, match=msg):

@@ -232,6 +232,7 @@ def test_c_copy_and_write_refuse():
                 dict(pages=0), dict(pages=4), dict(src=ints(-1, 2)), dict(dst=ints(3, 9)), dict(src=None), dict(count=-1),
                 dict(caches=(ctypes.c_void_p * 2)(0x100000, 0x200008)), dict(caches=(ctypes.c_void_p * 2)(0x100000, None))):
         assert copy(**bad) == 1, bad
+    assert copy(page=(1 << 30) + 16, stride=1 << 31) == 801
     assert lib.tl_write_i32(None, 9, None, None, 0, None) == 0
     assert lib.tl_write_i32(None, 9, ints(1), ints(1), 1, None) == 1
     assert lib.tl_write_i32(PTR, 9, ints(9), ints(1), 1, None) == 1

@@ -1038,12 +1038,13 @@ int tl_copy_pages(void* const* caches, int n_caches, int64_t page_bytes, int64_t
                   const int32_t* host_src, const int32_t* host_dst, int count, void* stream) {
   if (n_caches == 0 || count == 0) return 0;
   if (!caches || !host_src || !host_dst || n_caches < 0 || count < 0 || n_pages < 1 || page_bytes < 16 ||
-      page_bytes % 16 || page_bytes > INT32_MAX || page_stride_bytes < page_bytes || page_stride_bytes % 16)
+      page_bytes % 16 || page_stride_bytes < page_bytes || page_stride_bytes % 16)
     return TL_ERR_INVALID;
   for (int c = 0; c < n_caches; ++c)
     if (!caches[c] || ((uintptr_t)caches[c] & 15)) return TL_ERR_INVALID;
   for (int i = 0; i < count; ++i)
     if (host_src[i] < 0 || host_src[i] >= n_pages || host_dst[i] < 0 || host_dst[i] >= n_pages) return TL_ERR_INVALID;
+  if (page_bytes > (1 << 30)) return TL_ERR_UNSUPPORTED;  // offsets in a page are 32-bit
   hipStream_t st = tl_resolve_stream(stream);
   CopyParams p;
   p.page_stride = page_stride_bytes;

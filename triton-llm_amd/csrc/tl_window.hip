@@ -29,6 +29,9 @@ constexpr int kThreads = 256;
 constexpr int kBM = 128;  // query rows of a workgroup
 constexpr int kMinShare = 4;  // key tiles of a part at least
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kMostRows = 1 << 28;     // query rows of a sequence
+constexpr int kWholeWindow = 3 << 29;  // positions lie in [-2^28, 2^30 + 2^28): a window this long hides nothing, and
+                                       // below it position - window fits in 32 bits
 
 struct WinParams {
   const void* q;
@@ -222,8 +225,8 @@ template <bool PAGED>
 __device__ __forceinline__ Rows rows_of(const WinParams& p, int b) {
   Rows r;
   if constexpr (PAGED) {
-    constexpr int kFar = 1 << 30;
-    r.base = min(max(p.lens[b], -kFar), kFar);
+    // rows before position -seq_q see nothing, as those there; lengths past 2^30 count as 2^30
+    r.base = min(max(p.lens[b], -p.seq_q), 1 << 30);
     r.nq = p.new_lens ? min(max(p.new_lens[b], 0), p.seq_q) : p.seq_q;
     r.end = min(r.base + r.nq, p.pm.max_pages << p.pm.shift);
   } else {
@@ -246,7 +249,7 @@ __device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int q
   const int p1 = min(r.base + min(token_of(p, qt * kBM + kBM - 1) + 1, r.nq), r.end) - 1;  // last key any row sees
   if (p1 < 0) return k;
   if (p.window > 0) {
-    k.t0 = max(p0 - p.window + 1, 0) / BN;
+    k.t0 = min(max(p0 - p.window + 1, 0) / BN, p1 / BN + 1);  // rows past the pages may see none of the window's
     k.ns = (min(p.sinks, p1 + 1) + BN - 1) / BN;
     if (k.t0 <= k.ns) k.ns = k.t0 = 0;
   }
@@ -491,7 +494,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
       // key k0 + kl + 4 h of this lane is seen if kl <= hi and (kl > lo or kl < sk)
       const int off = k0 + 4 * h;
       const int hi = min(pos, ks.end - 1) - off;
-      const int lo = p.window > 0 ? pos - p.window - off : -BN - 1;
+      const int lo = p.window > 0 ? pos - off - p.window : -BN - 1;
       const int sk = p.sinks - off;
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb)
@@ -701,7 +704,8 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
     return TL_ERR_INVALID;
   if (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16) return TL_ERR_INVALID;
   if (d_k != 64 && d_k != 128) return TL_ERR_UNSUPPORTED;
-  if (p.seq_q > (1 << 29) || p.seq_k > (1 << 29)) return TL_ERR_UNSUPPORTED;
+  if (p.seq_q > kMostRows || p.seq_k > (1 << 29)) return TL_ERR_UNSUPPORTED;
+  if (p.window >= kWholeWindow) p.window = 0;
   // rows are moved 16 bytes at a time, a block of 16 with 32-bit offsets
   const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
   const int64_t vec = 16 / esize;
@@ -741,7 +745,7 @@ extern "C" {
 
 size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q, int most_keys, int d_k, int window,
                                  int sinks, int dtype) {
-  if (batch < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || seq_q < 1 || seq_q > (1 << 29) || most_keys < 1 ||
+  if (batch < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || seq_q < 1 || seq_q > kMostRows || most_keys < 1 ||
       window < 0 || sinks < 0 || (d_k != 64 && d_k != 128) || !rows_ok(seq_q, n_head / n_kv_head) ||
       (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16))
     return 0;

@@ -238,6 +238,8 @@ class PagedKVCache:
                  max_seq: int, page_size: int = 16, window: int = 0, sinks: int = 0, dtype=np.float32):
         if n_layer <= 0 or n_kv_head <= 0 or n_head <= 0 or n_head % n_kv_head:
             raise ValueError(f"bad head counts: n_layer={n_layer} n_head={n_head} n_kv_head={n_kv_head}")
+        if d_k not in (64, 128):
+            raise ValueError(f"paged attention supports d_k in (64, 128), got {d_k}")
         self.tables = PageTables(n_pages, page_size, max_batch, max_seq, window, sinks)
         self.n_layer, self.n_head, self.n_kv_head, self.d_k = n_layer, n_head, n_kv_head, d_k
         self.window, self.sinks = window, sinks
