@@ -262,27 +262,36 @@ __device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int q
 // the device knows the lengths, so only it can make the parts about `slots`, equally long, without gaps between
 // them: with a grid by the longest lengths that there could be, workgroups without work stood among the
 // others, and 4 x 500 rows on prefixes of 2875 to 3835 (of at most 4608) took 47.8 us.
-struct Deal {
-  int share, total;
-  int n, incl;  // parts of lane's sequence, and of all up to it (of the first 64)
-};
 struct Seq {
+  Rows r;
   int tiles, keys;  // row tiles, key tiles of the last of them
-  __device__ __forceinline__ int parts(int share) const { return max(1, (keys + share - 1) / share); }
+  int parts, all;   // parts of a row tile, of all of them and every KV head
+  __device__ __forceinline__ void cut(const WinParams& p, int share) {
+    parts = max(1, (int)((unsigned)(keys + share - 1) / (unsigned)share));
+    all = tiles * parts * p.n_kv;
+  }
 };
 template <int BN, bool PAGED>
 __device__ __forceinline__ Seq seq_at(const WinParams& p, int b) {
-  if (b >= p.batch) return Seq{0, 0};
-  const Rows r = rows_of<PAGED>(p, b);
-  const int tiles = (r.nq * p.group + kBM - 1) / kBM;
-  return Seq{tiles, tiles ? min(keys_of<BN>(p, r, tiles - 1).tiles, 1 << 20) : 0};
+  Seq s{{0, 0, 0}, 0, 0, 0, 0};
+  if (b < p.batch) {
+    s.r = rows_of<PAGED>(p, b);
+    s.tiles = (s.r.nq * p.group + kBM - 1) / kBM;
+    if (s.tiles) s.keys = min(keys_of<BN>(p, s.r, s.tiles - 1).tiles, 1 << 20);
+  }
+  return s;
 }
+struct Deal {
+  int share, total;
+  Seq s;     // lane's sequence, of the first 64
+  int incl;  // parts of all up to it
+};
 template <int BN, bool PAGED>
 __device__ __forceinline__ Deal deal_of(const WinParams& p, int lane) {
   // the sums are over few row tiles (the host divides no others), of at most 2^20 key tiles
   Deal d;
-  const Seq s = seq_at<BN, PAGED>(p, lane);
-  int work = last_lane(wave_scan(s.tiles * s.keys)), tiles = last_lane(wave_scan(s.tiles));
+  d.s = seq_at<BN, PAGED>(p, lane);
+  int work = last_lane(wave_scan(d.s.tiles * d.s.keys)), tiles = last_lane(wave_scan(d.s.tiles));
   for (int b0 = 64; b0 < p.batch; b0 += 64) {
     const Seq t = seq_at<BN, PAGED>(p, b0 + lane);
     work += last_lane(wave_scan(t.tiles * t.keys));
@@ -292,27 +301,33 @@ __device__ __forceinline__ Deal deal_of(const WinParams& p, int lane) {
   const int aim = max(p.slots - tiles * p.n_kv, p.slots / 2);
   // rounded up past the 32-bit quotient's error
   d.share = max((int)((float)work * (float)p.n_kv * __builtin_amdgcn_rcpf((float)aim) * 1.00001f) + 1, kMinShare);
-  d.n = s.tiles * s.parts(d.share) * p.n_kv;
-  d.incl = wave_scan(d.n);
+  d.s.cut(p, d.share);
+  d.incl = wave_scan(d.s.all);
   d.total = last_lane(d.incl);
   for (int b0 = 64; b0 < p.batch; b0 += 64) {
-    const Seq t = seq_at<BN, PAGED>(p, b0 + lane);
-    d.total += last_lane(wave_scan(t.tiles * t.parts(d.share) * p.n_kv));
+    Seq t = seq_at<BN, PAGED>(p, b0 + lane);
+    t.cut(p, d.share);
+    d.total += last_lane(wave_scan(t.all));
   }
   return d;
 }
-// The parts before lane's sequence of the 64 from b0 on, and its own.
+// The 64 sequences from b0 on, lane by lane: s, and the parts of all up to it.
 template <int BN, bool PAGED>
-__device__ __forceinline__ int parts_before(const WinParams& p, const Deal& d, int b0, int lane, int& own) {
-  int n = d.n, incl = d.incl;
+__device__ __forceinline__ int parts_upto(const WinParams& p, const Deal& d, int b0, int lane, Seq& s) {
+  s = d.s;
+  int incl = d.incl;
   for (int b = 64; b <= b0; b += 64) {
     const int base = last_lane(incl);
-    const Seq t = seq_at<BN, PAGED>(p, b + lane);
-    n = t.tiles * t.parts(d.share) * p.n_kv;
-    incl = base + wave_scan(n);
+    s = seq_at<BN, PAGED>(p, b + lane);
+    s.cut(p, d.share);
+    incl = base + wave_scan(s.all);
   }
-  own = n;
-  return incl - n;
+  return incl;
+}
+// Lane li's sequence, on every lane.
+__device__ __forceinline__ Seq seq_of_lane(const Seq& s, int li) {
+  auto of = [&](int x) { return uni(__builtin_amdgcn_readlane(x, li)); };
+  return Seq{{of(s.r.base), of(s.r.nq), of(s.r.end)}, of(s.tiles), of(s.keys), of(s.parts), of(s.all)};
 }
 
 // Four neighbouring outputs, rounded to nearest even.
@@ -362,21 +377,25 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   // within an XCD the longest rows come first.  Divided: an XCD takes a contiguous range of the parts.
   const int xcd = blockIdx.x % 8, at = blockIdx.x / 8;
   int b, hkv, qt, part = 0, parts = 1, place = 0;
+  Rows rw;
   if (p.slots > 0) {
     const Deal d = deal_of<BN, PAGED>(p, lane);
     const int per = (d.total + 7) / 8;
     place = xcd * per + at;
     if (at >= per || place >= d.total) return;
-    int b0 = 0, own, before = parts_before<BN, PAGED>(p, d, 0, lane, own);
-    while (last_lane(before + own) <= place) {
+    Seq s;
+    int b0 = 0, incl = parts_upto<BN, PAGED>(p, d, 0, lane, s);
+    while (last_lane(incl) <= place) {
       b0 += 64;
-      before = parts_before<BN, PAGED>(p, d, b0, lane, own);
+      incl = parts_upto<BN, PAGED>(p, d, b0, lane, s);
     }
-    const int li = uni(__ffsll((unsigned long long)__ballot(before + own > place)) - 1);
+    const int li = uni(__ffsll((unsigned long long)__ballot(incl > place)) - 1);
     b = b0 + li;
-    const Seq s = seq_at<BN, PAGED>(p, b);
-    const int in = place - uni(__builtin_amdgcn_readlane(before, li));
-    parts = s.parts(d.share);
+    const int before = uni(__builtin_amdgcn_readlane(incl - s.all, li));
+    s = seq_of_lane(s, li);
+    rw = s.r;
+    const int in = place - before;
+    parts = s.parts;
     hkv = (int)((unsigned)in / (unsigned)(parts * s.tiles));
     const int r = in - hkv * parts * s.tiles;
     part = (int)((unsigned)r / (unsigned)s.tiles);
@@ -389,8 +408,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     if (qt >= p.n_qt || kvh >= p.batch * p.n_kv) return;
     b = (int)((unsigned)kvh / (unsigned)p.n_kv);
     hkv = kvh - b * p.n_kv;
+    rw = rows_of<PAGED>(p, b);
   }
-  const Rows rw = rows_of<PAGED>(p, b);
   const Keys ks = keys_of<BN>(p, rw, qt);
   if (qt * kBM >= rw.nq * p.group) return;
 
@@ -608,16 +627,16 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
   const int qt = tile - kvh * p.n_qt;
   const int b = kvh / p.n_kv;
   const int hkv = kvh - b * p.n_kv;
-  const Seq s = seq_at<BN, PAGED>(p, b);
-  if (qt >= s.tiles) return;
   const Deal d = deal_of<BN, PAGED>(p, lane);
-  const int parts = s.parts(d.share);
-  if (parts <= 1) return;
-  int own;
-  const int before = uni(__builtin_amdgcn_readlane(parts_before<BN, PAGED>(p, d, b & ~63, lane, own), b & 63));
+  Seq s;
+  const int incl = parts_upto<BN, PAGED>(p, d, b & ~63, lane, s);
+  const int before = uni(__builtin_amdgcn_readlane(incl - s.all, b & 63));
+  s = seq_of_lane(s, b & 63);
+  const int parts = s.parts;
+  if (qt >= s.tiles || parts <= 1) return;
   const int row = qt * kBM + 32 * wave + lq;
   const int tok = token_of(p, row);
-  if (tok >= rows_of<PAGED>(p, b).nq) return;
+  if (tok >= s.r.nq) return;
   const int hq = hkv * p.group + (row - tok * p.group);
   const float* w = p.ws + ((size_t)before + hkv * parts * s.tiles + (s.tiles - 1 - qt)) * part_floats<D>() +
                    (size_t)wave * (64 + 64 * (D / 2));
