@@ -13,7 +13,7 @@
 // beam_finish, a workgroup a batch item, has everything else from those.  The best score in a unit (a segment, or
 // a group where the segments are few) is base_j + its maximum, base_j = s_j - log-sum-exp.  The units are
 // dealt to 64 classes; the n-th largest of the classes' best (n <= 64) is a bound that n continuations reach,
-// so only units that reach it are read again, and their entries that reach it are the
+// so (the bound is that value cut to its upper word) only units that reach it are read again, and their entries that reach it are the
 // candidates: about n for scattered scores.  A candidate's rank is the number of better ones.  Where the
 // candidates are many (ties, rows in order) every wave walks its units in order instead and keeps its 64 best in
 // its lanes; those are the candidates then.  beam_finish is latency alone: dependent steps on one CU.
@@ -46,6 +46,7 @@ struct BeamParams {
   int batch, beams, vocab, select;
   int n_seg, n_grp;
   int unit, n_units;  // entries of a unit, units of a row
+  uint32_t unit_magic;  // u / n_units = mulhi(u, unit_magic) for every unit u (n_units > 1)
   float* gmax;    // [rows][n_grp]
   float* smax;    // [rows][n_seg]
   double* ssum;   // [rows][n_seg]
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   const int J = p.beams, n = p.select;
   __shared__ double s_base[kMaxBeams];
   __shared__ double s_best[kFT];
-  __shared__ double s_bound;
+  __shared__ uint32_t s_bound;
   __shared__ int s_n_list, s_n_cand;
   __shared__ int s_list[kMaxList];
   __shared__ double s_cv[kMaxCand];
@@ -194,21 +195,31 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   float um[kAtOnce];  // the first of this thread's units, on their way during the sums
 #pragma unroll
   for (int k = 0; k < kAtOnce; ++k) um[k] = tid + k * kFT < J * U ? umax[tid + k * kFT] : -INFINITY;
-  if (tid == 0) s_n_list = s_n_cand = 0;
+  if (tid == 0) s_n_list = s_n_cand = 0, s_bound = ~0u;
+  auto beam_of = [&](int u) { return U == 1 ? u : (int)__umulhi((uint32_t)u, p.unit_magic); };
   // base_j = s_j - log-sum-exp of the row; -inf where either has no value, and such a beam has no
   // continuations
   for (int j = wave; j < J; j += kFW) {
     const int64_t row = (int64_t)item * J + j;
     const float* sm = p.smax + row * p.n_seg;
     const double* ss = p.ssum + row * p.n_seg;
-    float m = -INFINITY;
-    for (int i = lane; i < p.n_seg; i += 64) m = fmaxf(m, sm[i]);
+    constexpr int K = kMaxVocab / kSeg / 64;
+    float sx[K], m = -INFINITY;
+    double part[K], s = 0.;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int i = lane + 64 * k;
+      sx[k] = i < p.n_seg ? sm[i] : -INFINITY;
+      part[k] = i < p.n_seg ? ss[i] : 0.;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) m = fmaxf(m, sx[k]);
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-    double s = 0.;
-    for (int i = lane; i < p.n_seg; i += 64) {
-      const double part = ss[i];
-      s += sm[i] == -INFINITY ? part : part * exp((double)sm[i] - (double)m);  // (a NaN's sum comes through)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (64 * k >= p.n_seg) break;
+      s += sx[k] == -INFINITY ? part[k] : part[k] * exp((double)sx[k] - (double)m);  // (a NaN's sum comes through)
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
@@ -223,25 +234,32 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   double best = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kAtOnce; ++k)
-    if (tid + k * kFT < J * U) best = fmax(best, s_base[(tid + k * kFT) / U] + (double)um[k]);
-  for (int u = tid + kAtOnce * kFT; u < J * U; u += kFT) best = fmax(best, s_base[u / U] + (double)umax[u]);
+    if (tid + k * kFT < J * U) best = fmax(best, s_base[beam_of(tid + k * kFT)] + (double)um[k]);
+  for (int u = tid + kAtOnce * kFT; u < J * U; u += kFT) best = fmax(best, s_base[beam_of(u)] + (double)umax[u]);
   s_best[tid] = best;
   __syncthreads();
   if (wave == 0) {
     double c = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kFW; ++w) c = fmax(c, s_best[w * 64 + lane]);
-    int rank = 0;  // of this class
-    for (int i = 0; i < 64; ++i) rank += better(lane_d(c, i), i, c, lane) ? 1 : 0;
-    if (rank == n - 1) s_bound = c;
+    // by the values' upper words, in an order of unsigned numbers: the bound may be lower than the n-th best
+    const uint32_t hi = (uint32_t)(__builtin_bit_cast(uint64_t, c) >> 32);
+    const uint32_t key = (int32_t)hi < 0 ? ~hi : hi | 0x80000000u;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane(key, i) > key ? 1 : 0;
+    if (above < n) atomicMin(&s_bound, key);
   }
   __syncthreads();
-  const double bound = s_bound;
+  // the lowest value of this upper word; -inf's has no lower one
+  const uint32_t key = s_bound, bhi = key & 0x80000000u ? key & 0x7FFFFFFFu : ~key;
+  const uint64_t blo = (int32_t)bhi < 0 && bhi != 0xFFF00000u ? 0xFFFFFFFFu : 0u;
+  const double bound = __builtin_bit_cast(double, (uint64_t)bhi << 32 | blo);
   auto reaches = [&](double v) { return v >= bound && v > -INFINITY; };
 
   if (reaches(best)) {
     auto list = [&](int u, float x) {
-      if (reaches(s_base[u / U] + (double)x)) {
+      if (reaches(s_base[beam_of(u)] + (double)x)) {
         const int at = atomicAdd(&s_n_list, 1);
         if (at < kMaxList) s_list[at] = u;
       }
@@ -255,7 +273,7 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   const int n_list = s_n_list;
   // this lane's entry 64 c + lane of unit u (of beam u / U)
   auto entry = [&](int u, int c, double& v, int& i) __attribute__((always_inline)) {
-    const int j = u / U, at = (u - j * U) * p.unit + c * 64 + lane;
+    const int j = beam_of(u), at = (u - j * U) * p.unit + c * 64 + lane;
     v = -INFINITY;
     i = INT_MAX;
     if (at < p.vocab) {
@@ -268,24 +286,36 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
     if (at < kMaxCand) s_cv[at] = v, s_ci[at] = i;
   };
   if (n_list <= kMaxList && p.unit == kSeg) {
-    // a wave a segment, read as beam_scan does
-    for (int w = wave; w < n_list; w += kFW) {
-      const int u = s_list[w], j = u / U, at = (u - j * U) * kSeg + lane * kVec;
-      const double base = s_base[j];
-      float x[kVecs][kVec];
+    // a wave two segments, read as beam_scan does
+    for (int w = wave; w < n_list; w += 2 * kFW) {
+      float x[2][kVecs][kVec];
+      int j[2], at[2];
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k)
-        load_vec<T>(x[k], (const B*)p.logits + ((int64_t)item * J + j) * p.row_stride, at + k * 64 * kVec, p.vocab);
+      for (int q = 0; q < 2; ++q) {
+        const int wq = w + q * kFW;
+        if (wq >= n_list) break;
+        const int u = s_list[wq];
+        j[q] = beam_of(u);
+        at[q] = (u - j[q] * U) * kSeg + lane * kVec;
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
-        float m = x[k][0];
+        for (int k = 0; k < kVecs; ++k)
+          load_vec<T>(x[q][k], (const B*)p.logits + ((int64_t)item * J + j[q]) * p.row_stride, at[q] + k * 64 * kVec, p.vocab);
+      }
 #pragma unroll
-        for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[k][e]);
-        if (!reaches(base + (double)m)) continue;
+      for (int q = 0; q < 2; ++q) {
+        if (w + q * kFW >= n_list) break;
+        const double base = s_base[j[q]];
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const double v = base + (double)x[k][e];
-          if (reaches(v)) push(v, j * p.vocab + at + k * 64 * kVec + e);
+        for (int k = 0; k < kVecs; ++k) {
+          float m = x[q][k][0];
+#pragma unroll
+          for (int e = 1; e < kVec; ++e) m = fmaxf(m, x[q][k][e]);
+          if (!reaches(base + (double)m)) continue;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) {
+            const double v = base + (double)x[q][k][e];
+            if (reaches(v)) push(v, j[q] * p.vocab + at[q] + k * 64 * kVec + e);
+          }
         }
       }
     }
@@ -305,7 +335,7 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
     __syncthreads();
     Cand kept{-INFINITY, INT_MAX};  // this wave's 64 best so far, best in lane 0
     for (int u = wave; u < J * U; u += kFW) {
-      const double uv = s_base[u / U] + (double)umax[u];
+      const double uv = s_base[beam_of(u)] + (double)umax[u];
       if (!(reaches(uv) && uv >= lane_d(kept.v, 63))) continue;
       for (int c = 0; c < p.unit / 64; ++c) {
         Cand x;
@@ -334,6 +364,7 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
     const double v = s_cv[c];
     const int i = s_ci[c];
     int rank = 0;
+#pragma unroll 8
     for (int k = 0; k < n_cand; ++k) rank += better(s_cv[k], s_ci[k], v, i) ? 1 : 0;
     if (rank < n) {
       p.out_scores[o + rank] = (float)v;
@@ -412,6 +443,8 @@ int tl_beam_select(const void* logits, const float* scores, int batch, int beams
   const bool segments = (int64_t)beams * p.n_seg >= kUnitsAPlace * select && (int64_t)beams * p.n_seg >= 64;
   p.unit = segments ? kSeg : kGrp;
   p.n_units = segments ? p.n_seg : p.n_grp;
+  // exact: at most 2^18 units in all, and n_units <= 2^12, so that the magic's excess times a unit stays below 2^32
+  p.unit_magic = (uint32_t)((((uint64_t)1 << 32) + p.n_units - 1) / p.n_units);
   ws_layout((int64_t)batch * beams, vocab, (char*)workspace, &p);
   p.out_scores = out_scores;
   p.out_parents = out_parents;
