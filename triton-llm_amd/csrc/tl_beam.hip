@@ -105,11 +105,49 @@ __device__ __forceinline__ double shfl_d(double x, int lane) {
   return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
 }
 
+// Reductions by DPP moves, a few cycles each where a move through LDS takes about a hundred, over 8 lanes or a wave: for
+// beam_finish, whose steps wait for each other (9.8 -> 9.4 us at 4 x 50257).  beam_scan has enough waves to cover
+// the moves through LDS, and the vector unit is what it has least of (16 x 8 x 128256: 20.2 us, with DPP 21.1).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  const int i = __float_as_int(x);
+  return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const int a = (int)u, b = (int)(u >> 32);
+  const uint32_t c = __builtin_amdgcn_update_dpp(a, a, CTRL, 0xF, 0xF, false);
+  const uint32_t d = __builtin_amdgcn_update_dpp(b, b, CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)c | ((uint64_t)d << 32));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;  // quad_perm, row_half_mirror, row_mirror
+__device__ __forceinline__ float max8(float x) {
+  x = fmaxf(x, dpp<kXor1>(x));
+  x = fmaxf(x, dpp<kXor2>(x));
+  return fmaxf(x, dpp<kMirror8>(x));
+}
+__device__ __forceinline__ float lane_f(float x, int i) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
+}
+__device__ __forceinline__ float wave_max_of8(float x) {  // of max8's results
+  x = fmaxf(x, dpp<kMirror16>(x));
+  return fmaxf(fmaxf(lane_f(x, 0), lane_f(x, 16)), fmaxf(lane_f(x, 32), lane_f(x, 48)));
+}
+
 // Lane i's value, i the same on every lane.
 __device__ __forceinline__ double lane_d(double x, int i) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x);
   const uint32_t a = __builtin_amdgcn_readlane((uint32_t)u, i), b = __builtin_amdgcn_readlane((uint32_t)(u >> 32), i);
   return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+  x += dpp<kXor1>(x);
+  x += dpp<kXor2>(x);
+  x += dpp<kMirror8>(x);
+  x += dpp<kMirror16>(x);
+  return (lane_d(x, 0) + lane_d(x, 16)) + (lane_d(x, 32) + lane_d(x, 48));
 }
 
 template <typename T>
@@ -214,15 +252,13 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) m = fmaxf(m, sx[k]);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
+    m = wave_max_of8(max8(m));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (64 * k >= p.n_seg) break;
       s += sx[k] == -INFINITY ? part[k] : part[k] * exp((double)sx[k] - (double)m);  // (a NaN's sum comes through)
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
+    s = wave_sum(s);
     if (lane == 0) {
       const double base = (double)p.scores[row] - ((double)m + log(s));
       s_base[j] = base > -INFINITY && base < INFINITY ? base : -INFINITY;
