@@ -12,7 +12,7 @@
 //   * the maximum of every group of 64 entries.
 // beam_finish, a workgroup a batch item, has everything else from those.  The best score in a unit (a segment, or
 // a group where the segments are few) is base_j + its maximum, base_j = s_j - log-sum-exp.  The units are
-// dealt to 64 classes; the n-th largest of the classes' best (n <= 64) is a bound that n continuations reach,
+// dealt to 64 or 256 classes; the n-th largest of the classes' best is a bound that n continuations reach,
 // so (the bound is that value cut to its upper word) only units that reach it are read again, and their entries that reach it are the
 // candidates: about n for scattered scores.  A candidate's rank is the number of better ones.  Where the
 // candidates are many (ties, rows in order) every wave walks its units in order instead and keeps its 64 best in
@@ -31,6 +31,8 @@ constexpr int kSeg = 64 * kVec * kVecs;  // entries of a segment, a wave's
 constexpr int kGrp = 64;                 // entries of a group: 8 lanes
 constexpr int kFT = 1024;                // threads of beam_finish
 constexpr int kFW = kFT / 64;
+constexpr int kClasses = 256;            // of units, where the places are more than
+constexpr int kFewPlaces = 16;
 constexpr int kMaxVocab = 262144;
 constexpr int kMaxBeams = 64;
 constexpr int kMaxSelect = 64;
@@ -223,6 +225,8 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   __shared__ double s_base[kMaxBeams];
   __shared__ double s_best[kFT];
   __shared__ uint32_t s_bound;
+  __shared__ __attribute__((aligned(16))) uint32_t s_key[kClasses];
+  __shared__ int s_above[kClasses];
   __shared__ int s_n_list, s_n_cand;
   __shared__ int s_list[kMaxList];
   __shared__ double s_cv[kMaxCand];
@@ -266,25 +270,49 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
   }
   __syncthreads();
 
-  // the bound: n-th best of the 64 classes' best
+  // the bound: n-th best of the classes' best
   double best = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kAtOnce; ++k)
     if (tid + k * kFT < J * U) best = fmax(best, s_base[beam_of(tid + k * kFT)] + (double)um[k]);
   for (int u = tid + kAtOnce * kFT; u < J * U; u += kFT) best = fmax(best, s_base[beam_of(u)] + (double)umax[u]);
   s_best[tid] = best;
-  __syncthreads();
-  if (wave == 0) {
-    double c = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kFW; ++w) c = fmax(c, s_best[w * 64 + lane]);
-    // by the values' upper words, in an order of unsigned numbers: the bound may be lower than the n-th best
+  // by the values' upper words, in an order of unsigned numbers: the bound may be lower than the n-th best
+  auto key_of = [](double c) {
     const uint32_t hi = (uint32_t)(__builtin_bit_cast(uint64_t, c) >> 32);
-    const uint32_t key = (int32_t)hi < 0 ? ~hi : hi | 0x80000000u;
+    return (int32_t)hi < 0 ? ~hi : hi | 0x80000000u;
+  };
+  if (n <= kFewPlaces) {
+    __syncthreads();
+    if (wave == 0) {
+      double c = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kFW; ++w) c = fmax(c, s_best[w * 64 + lane]);
+      const uint32_t key = key_of(c);
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane(key, i) > key ? 1 : 0;
+      if (above < n) atomicMin(&s_bound, key);
+    }
+  } else {
+    if (tid < kClasses) s_above[tid] = 0;
+    __syncthreads();
+    if (tid < kClasses) {
+      double c = s_best[tid];
+#pragma unroll
+      for (int k = kClasses; k < kFT; k += kClasses) c = fmax(c, s_best[tid + k]);
+      s_key[tid] = key_of(c);
+    }
+    __syncthreads();
+    // every thread a class against a part of the others
+    constexpr int kPart = kClasses * kClasses / kFT;
+    const uint32_t* others = s_key + tid / kClasses * kPart;
     int above = 0;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) above += (uint32_t)__builtin_amdgcn_readlane(key, i) > key ? 1 : 0;
-    if (above < n) atomicMin(&s_bound, key);
+    for (int i = 0; i < kPart; ++i) above += others[i] > s_key[tid % kClasses] ? 1 : 0;
+    atomicAdd(&s_above[tid % kClasses], above);
+    __syncthreads();
+    if (tid < kClasses && s_above[tid] < n) atomicMin(&s_bound, s_key[tid]);
   }
   __syncthreads();
   // the lowest value of this upper word; -inf's has no lower one
@@ -356,11 +384,17 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
       }
     }
   } else if (n_list <= kMaxList) {
-    for (int w = wave; w < n_list; w += kFW) {  // a wave a group
-      double v;
-      int i;
-      entry(s_list[w], 0, v, i);
-      if (reaches(v)) push(v, i);
+    for (int w = wave; w < n_list; w += kAtOnce * kFW) {  // a wave kAtOnce groups
+      double v[kAtOnce];
+      int i[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        v[k] = -INFINITY;
+        if (w + k * kFW < n_list) entry(s_list[w + k * kFW], 0, v[k], i[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k)
+        if (reaches(v[k])) push(v[k], i[k]);
     }
   }
   __syncthreads();
