@@ -9,13 +9,16 @@
 // sees no key gives zeros.  The reference has no windows and no pages; its causal attention
 // (attention_gqa.py:21-146) is window = 0.
 //
-// A workgroup is 4 waves of 32 query rows of one head.  It walks only the key tiles that any of
+// A workgroup is 4 waves of 32 query rows of one KV head, its query heads side by side (row r is token r / group).  It walks only the key tiles that any of
 // its 128 rows sees: the sinks' tiles, then those from the first row's window on to the last row's
 // position.  As in the causal prefill the products are transposed, S^T = K . Q^T and
 // O^T = V^T . P^T, on 32 x 32 MFMA blocks: lane l of the accumulator holds query row l % 32, so maximum and
 // rescale are a lane's own (one exchange between l and l ^ 32), and P^T goes from the accumulator's
 // registers straight into the second product.  K / V tiles come by LDS-DMA, the next one while this
 // one is used; V is read by transposing LDS reads.
+//
+// Bound by the matrix products and, at d_k 64, as much by exp and the conversions: 8192 tokens, window 1024, 24 / 8 heads
+// of 128, bf16: 131 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 43.4 us, 7.4 of them the join.
 #include "tl_paged.h"
 #include "tl_prefill.h"
 
@@ -678,13 +681,16 @@ int64_t most_tiles(int64_t keys, int window, int sinks, int group, int bn) {
 }
 
 // Whether the keys of the row tiles are divided, and by how many workgroups: where the row tiles alone would not fill
-// the device and a row tile can have several parts.  fp32 is bound by its matrix products, which one workgroup a CU
-// keeps busy; the 16-bit kernels take as many as fit.  Returns the most parts there can be (0: undivided).
+// the device and a row tile can have several parts (1 x 100 rows on 4000 keys, 15 / 5 heads, d_k 64, fp16: 22.7 us,
+// undivided 58.6; 1000 causal rows, 9 / 3 heads: 16.3 and 18.5).  The 16-bit kernels and fp32 at d_k 128 take as many
+// workgroups as fit (1 x 500 rows on 4000 keys, 24 / 8 heads, d_k 128: fp16 43.1 us, one a CU 51.6; fp32 at 300 rows on
+// 2000 keys 89 and 101); fp32 at d_k 64 is bound by its matrix products, which one workgroup a CU keeps busy (1023
+// rows, window 256: 27.8 us, with two 31.5).  Returns the most parts there can be (0: undivided).
 int64_t plan_slots(WinParams& p, int64_t keys, int d_k, int esize) {
   const int bn = esize == 2 ? 64 : 32;
   const int64_t most = most_tiles(keys, p.window, p.sinks, p.group, bn);
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
-  const int64_t slots = (int64_t)tl_device_cus() * (esize == 4 ? 1 : d_k == 64 ? 3 : 2);
+  const int64_t slots = (int64_t)tl_device_cus() * (d_k == 128 ? 2 : esize == 4 ? 1 : 3);
   p.slots = tiles >= slots || most < 2 * kMinShare ? 0 : (int)slots;
   const int64_t parts = tiles * ((most + kMinShare - 1) / kMinShare);
   return !p.slots ? 0 : parts < 2 * slots + tiles ? parts : 2 * slots + tiles;
