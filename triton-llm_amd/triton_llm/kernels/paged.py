@@ -29,7 +29,6 @@ import ctypes
 import functools
 import math
 import operator
-import struct
 
 import numpy as np
 
@@ -284,9 +283,6 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
     return out
 
 
-_get_shape, _get_dtype = operator.attrgetter("shape"), operator.attrgetter("dtype")
-
-
 def copy_kv_pages(caches, src, dst) -> None:
     """Page ``dst[i]`` = page ``src[i]`` in every pool of ``caches``.
 
@@ -307,10 +303,9 @@ def copy_kv_pages(caches, src, dst) -> None:
         raise ValueError(f"pools must be 4-D (n_pages, n_kv_head, page_size, d_k), got {shape}")
     _check_page_size(shape[2])
     gpu.dtype_code(dtype)
-    if list(map(_get_shape, caches)).count(shape) != len(caches) or list(map(_get_dtype, caches)).count(dtype) != len(caches):
-        for c in caches:
-            if c.shape != shape or gpu.dtype_name(c.dtype) != gpu.dtype_name(dtype):
-                raise ValueError(f"pools differ: {shape} {gpu.dtype_name(dtype)} and {c.shape} {gpu.dtype_name(c.dtype)}")
+    for c in caches:
+        if c.shape != shape or (c.dtype is not dtype and gpu.dtype_name(c.dtype) != gpu.dtype_name(dtype)):
+            raise ValueError(f"pools differ: {shape} {gpu.dtype_name(dtype)} and {c.shape} {gpu.dtype_name(c.dtype)}")
     if min(src) < 0 or min(dst) < 0 or max(src) >= shape[0] or max(dst) >= shape[0]:
         raise ValueError(f"page numbers must be in [0, {shape[0]})")
     to = set(dst)
@@ -319,7 +314,7 @@ def copy_kv_pages(caches, src, dst) -> None:
     if not to.isdisjoint(src):
         raise ValueError("a page is source and destination")
     page_bytes = shape[1] * shape[2] * shape[3] * dtype.itemsize
-    bases = (ctypes.c_void_p * len(caches)).from_buffer_copy(struct.pack(f"{len(caches)}Q", *[c.ptr.value or 0 for c in caches]))
+    bases = (ctypes.c_void_p * len(caches)).from_buffer_copy(b"".join([c.ptr for c in caches]))
     launch(gpu.runtime().tl_copy_pages, bases, len(caches), page_bytes, page_bytes, shape[0], (ctypes.c_int32 * n)(*src),
            (ctypes.c_int32 * n)(*dst), n, None, what="copy_kv_pages")
 
