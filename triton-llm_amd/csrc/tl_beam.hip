@@ -368,7 +368,8 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
         at[q] = (u - j[q] * U) * kSeg + lane * kVec;
 #pragma unroll
         for (int k = 0; k < kVecs; ++k)
-          load_vec<T>(x[q][k], (const B*)p.logits + ((int64_t)item * J + j[q]) * p.row_stride, at[q] + k * 64 * kVec, p.vocab);
+          load_vec<T>(x[q][k], (const B*)p.logits + ((int64_t)item * J + j[q]) * p.row_stride, at[q] + k * 64 * kVec,
+                      p.vocab);
       }
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -471,7 +472,8 @@ size_t ws_layout(int64_t rows, int vocab, char* base, BeamParams* p) {
 
 template <typename T>
 int launch_beam(const BeamParams& p, hipStream_t st) {
-  hipLaunchKernelGGL(beam_scan_kernel<T>, dim3((p.n_seg + kST / 64 - 1) / (kST / 64), p.batch * p.beams), dim3(kST), 0, st, p);
+  hipLaunchKernelGGL(beam_scan_kernel<T>, dim3((p.n_seg + kST / 64 - 1) / (kST / 64), p.batch * p.beams), dim3(kST), 0,
+                     st, p);
   const int e = tl_launch_status();
   if (e) return e;
   hipLaunchKernelGGL(beam_finish_kernel<T>, dim3(p.batch), dim3(kFT), 0, st, p);

@@ -166,7 +166,8 @@ int tl_fill_bytes(void* dst, unsigned char value, size_t nbytes, hipStream_t st)
 //                  persistent and equal-share schedules plan for (0: none),
 //                  so small problems take multi-round schedules;
 //   decode_shares  TRITON_LLM_HIP_DECODE_SHARES nonzero: small-cache decode
-//                  takes the equal-share path instead of pair mode;
+//                  (contiguous or paged) takes the equal-share path
+//                  instead of pair mode;
 //   prefill_w64    TRITON_LLM_HIP_PREFILL_W64 nonzero: 16-bit d_k 128
 //                  prefill runs flash_fwd_w64 (64 query rows per wave)
 //                  instead of flash_fwd_16, so tests and A/B timing can

@@ -356,7 +356,8 @@ __device__ __forceinline__ Layout layout_of(const DecodeParams& p, int lane) {
   if (y.padded) {
     y.incl = wave_scan(y.unit(y.n) * p.n_pairs);
     y.total = last_lane(y.incl);
-    for (int b0 = 64; b0 < p.batch; b0 += 64) y.total += last_lane(wave_scan(y.unit(blocks_at(p, b0 + lane)) * p.n_pairs));
+    for (int b0 = 64; b0 < p.batch; b0 += 64)
+      y.total += last_lane(wave_scan(y.unit(blocks_at(p, b0 + lane)) * p.n_pairs));
   }
   return y;
 }
@@ -809,13 +810,15 @@ template <typename T, int D, int G>
 int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
   const int64_t pair_bytes = most / ((int64_t)p.batch * p.n_pairs) * kBlk * 2 * D * T::size;
   if (pair_mode(p, pair_bytes)) {
-    hipLaunchKernelGGL((paged_decode_kernel<T, D, G, kPairWaves, kPairBlocks<T, D>, true>), dim3(p.batch * p.n_pairs), dim3(64 * kPairWaves), 0, st, p);
+    hipLaunchKernelGGL((paged_decode_kernel<T, D, G, kPairWaves, kPairBlocks<T, D>, true>), dim3(p.batch * p.n_pairs),
+                       dim3(64 * kPairWaves), 0, st, p);
     return tl_launch_status();
   }
   static int per_cu = 0;
   if (per_cu == 0) {
     int n = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_decode_kernel<T, D, G, kDecWaves, 1, false>, kDecThreads, 0) != hipSuccess ||
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_decode_kernel<T, D, G, kDecWaves, 1, false>,
+                                                     kDecThreads, 0) != hipSuccess ||
         n <= 0)
       n = 1;
     per_cu = n;

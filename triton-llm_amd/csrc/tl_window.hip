@@ -9,13 +9,13 @@
 // sees no key gives zeros.  The reference has no windows and no pages; its causal attention
 // (attention_gqa.py:21-146) is window = 0.
 //
-// A workgroup is 4 waves of 32 query rows of one KV head, its query heads side by side (row r is token r / group).  It walks only the key tiles that any of
-// its 128 rows sees: the sinks' tiles, then those from the first row's window on to the last row's
-// position.  As in the causal prefill the products are transposed, S^T = K . Q^T and
-// O^T = V^T . P^T, on 32 x 32 MFMA blocks: lane l of the accumulator holds query row l % 32, so maximum and
-// rescale are a lane's own (one exchange between l and l ^ 32), and P^T goes from the accumulator's
-// registers straight into the second product.  K / V tiles come by LDS-DMA, the next one while this
-// one is used; V is read by transposing LDS reads.
+// A workgroup is 4 waves of 32 query rows of one KV head, its query heads side by side (row r is token r /
+// group).  It walks only the key tiles that any of its 128 rows sees: the sinks' tiles, then those from the
+// first row's window on to the last row's position.  As in the causal prefill the products are transposed, S^T =
+// K . Q^T and O^T = V^T . P^T, on 32 x 32 MFMA blocks: lane l of the accumulator holds query row l % 32, so
+// maximum and rescale are a lane's own (one exchange between l and l ^ 32), and P^T goes from the accumulator's
+// registers straight into the second product.  K / V tiles come by LDS-DMA, the next one while this one is used;
+// V is read by transposing LDS reads.
 //
 // Bound by the matrix products and, at d_k 64, as much by exp and the conversions: 8192 tokens, window 1024, 24 / 8 heads
 // of 128, bf16: 131 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 43.4 us, 7.4 of them the join.
@@ -129,7 +129,8 @@ struct Tile16 {
   }
   // s holds the probabilities; they are rounded to the storage type here (at most half a step
   // each, as the causal prefill does), the sum l is of the unrounded ones.
-  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt, int lane) {
+  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt,
+                                                int lane) {
     typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
     constexpr int NG = 2 * NMB * NDB;
@@ -193,7 +194,8 @@ struct Tile32 {
       for (int i = 0; i < 4; ++i) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], q.f[4 * c + i], s[0], 0, 0, 0);
     }
   }
-  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt, int lane) {
+  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt,
+                                                int lane) {
     const int lq = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -426,7 +428,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   const bool there = tok < rw.nq;
   const int pos = rw.base + tok;
   typename TL::Q q;
-  TL::load_q(q, (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh + (int64_t)tok * p.q_ss), there && p.scale_log2 != 0.f,
+  TL::load_q(q, (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh + (int64_t)tok * p.q_ss),
+             there && p.scale_log2 != 0.f,
              h, p.scale_log2 < 0.f ? 0x80000000u : 0u);
   const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
 
@@ -722,8 +725,13 @@ int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) 
   return tl_launch_status();
 }
 
-int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t workspace_bytes, int d_k, const int64_t* qs, const int64_t* ks, const int64_t* vs,
-                 const int64_t* os, float sm_scale, int dtype, void* stream) {
+template <typename T>
+int launch_window_d(WinParams& p, bool paged, int d_k, int64_t most_parts, hipStream_t st) {
+  return d_k == 64 ? launch_window<T, 64>(p, paged, most_parts, st) : launch_window<T, 128>(p, paged, most_parts, st);
+}
+
+int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t workspace_bytes, int d_k,
+                 const int64_t* qs, const int64_t* ks, const int64_t* vs, const int64_t* os, float sm_scale, int dtype, void* stream) {
   if (!p.q || !p.k || !p.v || !p.o || !qs || !ks || !vs || !os || p.batch < 0 || p.n_head < 0 || p.n_kv < 1 ||
       p.n_head % p.n_kv || p.seq_q < 0 || p.window < 0 || p.sinks < 0)
     return TL_ERR_INVALID;
@@ -758,9 +766,9 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
   }
   hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
-    case TL_DTYPE_F32: return d_k == 64 ? launch_window<F32, 64>(p, paged, most_parts, st) : launch_window<F32, 128>(p, paged, most_parts, st);
-    case TL_DTYPE_F16: return d_k == 64 ? launch_window<F16, 64>(p, paged, most_parts, st) : launch_window<F16, 128>(p, paged, most_parts, st);
-    default: return d_k == 64 ? launch_window<BF16, 64>(p, paged, most_parts, st) : launch_window<BF16, 128>(p, paged, most_parts, st);
+    case TL_DTYPE_F32: return launch_window_d<F32>(p, paged, d_k, most_parts, st);
+    case TL_DTYPE_F16: return launch_window_d<F16>(p, paged, d_k, most_parts, st);
+    default: return launch_window_d<BF16>(p, paged, d_k, most_parts, st);
   }
 }
 
@@ -784,8 +792,8 @@ size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q
   return (size_t)plan_slots(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2) * part_bytes(d_k);
 }
 
-int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace, size_t workspace_bytes, int batch, int n_head, int n_kv_head,
-                        int seq_q, int seq_k, int d_k, const int64_t* q_strides, const int64_t* k_strides,
+int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace, size_t workspace_bytes,
+                        int batch, int n_head, int n_kv_head, int seq_q, int seq_k, int d_k, const int64_t* q_strides, const int64_t* k_strides,
                         const int64_t* v_strides, const int64_t* o_strides, float sm_scale, int window, int sinks,
                         int dtype, void* stream) {
   if (batch == 0 || n_head == 0 || seq_q == 0) return 0;
@@ -802,13 +810,14 @@ int tl_window_attention(const void* q, const void* k, const void* v, void* o, vo
   p.seq_k = seq_k;
   p.window = window;
   p.sinks = sinks;
-  return window_entry(p, false, seq_k, workspace, workspace_bytes, d_k, q_strides, k_strides, v_strides, o_strides, sm_scale, dtype, stream);
+  return window_entry(p, false, seq_k, workspace, workspace_bytes, d_k, q_strides, k_strides, v_strides, o_strides,
+                      sm_scale, dtype, stream);
 }
 
 int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
                                int max_pages, int n_pages, int page_size, const int32_t* cache_lens,
-                               const int32_t* new_lens, void* o, void* workspace, size_t workspace_bytes, int batch, int n_new, int n_head, int n_kv_head,
-                               int d_k, const int64_t* q_strides, const int64_t* k_page_strides,
+                               const int32_t* new_lens, void* o, void* workspace, size_t workspace_bytes, int batch,
+                               int n_new, int n_head, int n_kv_head, int d_k, const int64_t* q_strides, const int64_t* k_page_strides,
                                const int64_t* v_page_strides, const int64_t* o_strides, float sm_scale, int window,
                                int sinks, int dtype, void* stream) {
   if (batch == 0 || n_head == 0 || n_new == 0) return 0;
@@ -830,7 +839,8 @@ int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v
   p.seq_q = n_new;
   p.window = window;
   p.sinks = sinks;
-  return window_entry(p, true, (int64_t)max_pages << shift, workspace, workspace_bytes, d_k, q_strides, k_page_strides, v_page_strides, o_strides, sm_scale, dtype, stream);
+  return window_entry(p, true, (int64_t)max_pages << shift, workspace, workspace_bytes, d_k, q_strides, k_page_strides,
+                      v_page_strides, o_strides, sm_scale, dtype, stream);
 }
 
 }  // extern "C"

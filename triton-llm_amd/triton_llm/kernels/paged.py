@@ -256,8 +256,8 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
         sm_scale = default_scale(d_k)
     ws = scratch(_decode_workspace_bytes(n_head, n_kv_head, d_k), workspace, key="paged_decode")
     launch(gpu.runtime().tl_paged_attention_decode, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
-           cache_lens.ptr, int(len_add), int(window), int(sinks), out.ptr, ws.ptr, ws.nbytes, *sizes, float(sm_scale), code, None,
-           what="paged_attention_decode")
+           cache_lens.ptr, int(len_add), int(window), int(sinks), out.ptr, ws.ptr, ws.nbytes, *sizes, float(sm_scale),
+           code, None, what="paged_attention_decode")
     return out
 
 
@@ -278,8 +278,8 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
     if sm_scale is None:
         sm_scale = default_scale(k_pages.shape[3])
     launch(gpu.runtime().tl_paged_attention_prefill, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
-           cache_lens.ptr, _ptr(new_lens), out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes, float(sm_scale), int(window), int(sinks), code, None,
-           what="paged_attention_prefill")
+           cache_lens.ptr, _ptr(new_lens), out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes,
+           float(sm_scale), int(window), int(sinks), code, None, what="paged_attention_prefill")
     return out
 
 

@@ -39,9 +39,10 @@ def window_attention_strided(q, k, v, out, *, batch, n_head, n_kv_head, seq_q, s
         raise ValueError("seq_k must be >= 1")
     if sm_scale is None:
         sm_scale = default_scale(d_k)
-    ws = scratch(_workspace_bytes(batch, n_head, n_kv_head, seq_q, seq_k, d_k, window, sinks, code), workspace, key="window")
-    launch(gpu.runtime().tl_window_attention, vp(q), vp(k), vp(v), vp(out), vp(ws), ws.nbytes if ws is not None else 0, batch, n_head, n_kv_head, seq_q, seq_k,
-           d_k, _lib.strides(*q_strides), _lib.strides(*k_strides), _lib.strides(*v_strides),
+    ws = scratch(_workspace_bytes(batch, n_head, n_kv_head, seq_q, seq_k, d_k, window, sinks, code), workspace,
+                 key="window")
+    launch(gpu.runtime().tl_window_attention, vp(q), vp(k), vp(v), vp(out), vp(ws), ws.nbytes if ws is not None else 0,
+           batch, n_head, n_kv_head, seq_q, seq_k, d_k, _lib.strides(*q_strides), _lib.strides(*k_strides), _lib.strides(*v_strides),
            _lib.strides(*o_strides), float(sm_scale), int(window), int(sinks), code, None, what="window_attention")
     return out
 
