@@ -30,7 +30,8 @@ def run(logits, scores, n, dtype="float32"):
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("B,J,V,n", [(1, 4, 50257, 8), (3, 5, 1000, 10), (2, 1, 1, 1), (1, 2, 1, 4), (1, 1, 63, 64), (2, 3, 65, 7),
-                                     (1, 64, 300, 64), (5, 7, 2049, 14), (1, 8, 128256, 16), (40, 2, 500, 3)])
+                                     (1, 64, 300, 64), (5, 7, 2049, 14), (1, 8, 128256, 16), (40, 2, 500, 3),
+                                     (1, 8, 128256, 20), (2, 16, 20000, 64), (1, 2, 262144, 33)])
 def test_normal_logits(dtype, B, J, V, n):
     rng = np.random.default_rng(V)
     run(2.5 * rng.standard_normal((B * J, V)), -rng.uniform(3, 9, (B, J)), n, dtype)
@@ -39,6 +40,8 @@ def test_normal_logits(dtype, B, J, V, n):
 def test_ties_go_to_the_lowest_place():
     run(np.zeros((4, 5000)), np.zeros((1, 4)), 64)                       # everything equal
     run(np.zeros((4, 5000)), np.array([[-2, -1, -1, -3.0]]), 9)
+    run(np.zeros((8, 20000)), np.zeros((1, 8)), 12)
+    run(np.zeros((8, 20000)), np.zeros((1, 8)), 40)
     x = np.zeros((2, 9000))
     x[:, 4000:8000] = 5
     run(x, np.zeros((1, 2)), 40)
