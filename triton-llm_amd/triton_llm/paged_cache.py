@@ -54,6 +54,7 @@ class PageTables:
         self.lens = [0] * max_batch
         self.new = [0] * max_batch
         self.refs = [0] * n_pages
+        self._gone = [0] * max_batch  # columns before it are given back, the sinks' aside
         self._free = list(range(n_pages - 1, -1, -1))
         self.table_edits: dict[tuple[int, int], int] = {}
         self.copies: list[tuple[int, int]] = []
@@ -96,7 +97,7 @@ class PageTables:
         for slot, t in enumerate(self.tables):
             if t is None:
                 self.tables[slot] = []
-                self.lens[slot] = 0
+                self.lens[slot] = self._gone[slot] = 0
                 return slot
         raise ValueError(f"all {self.max_batch} slots are open")
 
@@ -128,16 +129,17 @@ class PageTables:
             raise ValueError("a slot is given twice")
         for s in slots + parents:
             self._check_slot(s)
-        taken = [(list(self.tables[p]), self.lens[p]) for p in parents]
-        for pages, _ in taken:
+        parents, slots = [p for s, p in zip(slots, parents) if s != p], [s for s, p in zip(slots, parents) if s != p]
+        taken = [(list(self.tables[p]), self.lens[p], self._gone[p]) for p in parents]
+        for pages, _, _ in taken:
             for page in pages:
                 if page >= 0:
                     self.refs[page] += 1
-        for s, (pages, n) in zip(slots, taken):
+        for s, (pages, n, gone) in zip(slots, taken):
             for page in self.tables[s]:
                 self._drop(page)
             self._set(s, pages)
-            self.lens[s] = n
+            self.lens[s], self._gone[s] = n, gone
 
     def begin(self, new) -> None:
         """Find room for ``new[slot]`` more tokens of every slot (0 for those that rest): new pages, and a copy of a
@@ -151,8 +153,8 @@ class PageTables:
             raise ValueError("a step needs at least one new token")
         ps = self.page_size
         need = 0
-        left = list(self.refs)  # references once the slots before have taken their copies
-        copied = []
+        left = {}  # references of pages once the slots before have taken their copies
+        copied = set()
         for slot, n in enumerate(new):
             if n < 0:
                 raise ValueError(f"new tokens must be >= 0, got {n}")
@@ -165,25 +167,27 @@ class PageTables:
             need += -(-(at + n) // ps) - len(self.tables[slot])
             if at % ps:
                 last = self.tables[slot][at // ps]
-                if left[last] > 1:
-                    left[last] -= 1
+                refs = left.get(last, self.refs[last])
+                if refs > 1:
+                    left[last] = refs - 1
                     need += 1
-                    copied.append(slot)
+                    copied.add(slot)
         if need > len(self._free):
             raise ValueError(f"{need} pages needed, {len(self._free)} free")
         for slot, n in enumerate(new):
             if n == 0:
                 continue
-            pages = list(self.tables[slot])
+            pages = self.tables[slot]
             at = self.lens[slot]
             if slot in copied:
                 page = self._take()
                 self.copies.append((pages[at // ps], page))
                 self._drop(pages[at // ps])
-                pages[at // ps] = page
+                pages[at // ps] = self.table_edits[slot, at // ps] = page
             while len(pages) * ps < at + n:
-                pages.append(self._take())
-            self._set(slot, pages)
+                page = self._take()
+                self.table_edits[slot, len(pages)] = page
+                pages.append(page)
         self.new = new
 
     def advance(self) -> None:
@@ -197,11 +201,11 @@ class PageTables:
             self.lens[slot] += n
             if self.window:
                 first = (self.lens[slot] - self.window + 1) // self.page_size  # pages before it are out of sight
-                pages = list(self.tables[slot])
-                for c in range(-(-self.sinks // self.page_size), min(first, len(pages))):
+                pages = self.tables[slot]
+                for c in range(max(self._gone[slot], -(-self.sinks // self.page_size)), min(first, len(pages))):
                     self._drop(pages[c])
-                    pages[c] = -1
-                self._set(slot, pages)
+                    pages[c] = self.table_edits[slot, c] = -1
+                    self._gone[slot] = c + 1
         self.new = [0] * self.max_batch
 
     def compact(self) -> int:
