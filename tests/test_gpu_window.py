@@ -36,7 +36,7 @@ def test_window(dtype, D, Sq, Sk, window, sinks):
     run(dtype, 1, 2, 1, Sq, Sk, D, window, sinks)
 
 
-@pytest.mark.parametrize("B,Hq,Hkv", [(2, 6, 2), (3, 5, 5), (1, 9, 3), (1, 8, 1)])
+@pytest.mark.parametrize("B,Hq,Hkv", [(2, 6, 2), (3, 5, 5), (1, 9, 3), (1, 8, 1), (1, 40, 1), (1, 160, 1)])
 def test_heads_and_batches(B, Hq, Hkv):
     run("bfloat16", B, Hq, Hkv, 200, 210, 64, 50, 3)
 

@@ -62,7 +62,7 @@ def _is_int32(t) -> bool:
     return t.dtype.char == "i"
 
 
-def _code(*tensors) -> int:
+def dtype_code_of(*tensors) -> int:
     """Dtype code shared by all tensors; ValueError if they differ (same_dtype, without its pass over the
     names where every tensor has the very same dtype object)."""
     dt = tensors[0].dtype
@@ -191,10 +191,10 @@ def paged_kv_append(q_dev, k_new, v_new, k_pages, v_pages, page_table, cache_len
     if q_dev is None:
         if q_out is not None:
             raise ValueError("q_out is given without q_dev")
-        code = _code(k_new, v_new, k_pages, v_pages)
+        code = dtype_code_of(k_new, v_new, k_pages, v_pages)
     else:
         q_out = q_dev if q_out is None else _same_output(q_out, q_dev)
-        code = _code(k_new, v_new, k_pages, v_pages, q_dev)
+        code = dtype_code_of(k_new, v_new, k_pages, v_pages, q_dev)
     if cos_dev is not None and not cos_dev.dtype.char == sin_dev.dtype.char == "f":
         raise ValueError(f"cos/sin tables must be float32, got {cos_dev.dtype} and {sin_dev.dtype}")
     launch(gpu.runtime().tl_paged_kv_append, _ptr(q_dev), _ptr(q_out), k_new.ptr, v_new.ptr, k_pages.ptr,
@@ -249,7 +249,7 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
     _check_int32(page_table, cache_lens)
     pages, sizes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape, None,
                                    q_dev.shape, n_head, n_kv_head, window, sinks, False)
-    code = _code(q_dev, k_pages, v_pages)
+    code = dtype_code_of(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
     d_k = k_pages.shape[3]
     if sm_scale is None:
@@ -272,7 +272,7 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
     _check_int32(page_table, cache_lens, new_lens)
     pages, sizes, ws_bytes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
                                              _shape(new_lens), q_dev.shape, n_head, n_kv_head, window, sinks, True)
-    code = _code(q_dev, k_pages, v_pages)
+    code = dtype_code_of(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
     ws = scratch(ws_bytes[code], workspace, key="window")
     if sm_scale is None:

@@ -257,6 +257,7 @@ class PagedKVCache:
         self._table = gpu.to_device(np.full(shape, -1, np.int32))
         # row 0: tokens before the step, row 1: the step's, row 2: tokens with the step's
         self._counts = gpu.zeros((3, max_batch), np.int32)
+        self._most_new = self._longest = 0  # the step's tokens of a slot at most, the longest sequence with them
         self._told = [0] * (3 * max_batch)  # what the device has in it
         self._lens, self._new, self._ends = (self._row(i) for i in range(3))
         self._decode_ws = paged_decode_workspace(max_batch, n_head, n_kv_head, max_seq, d_k)
@@ -323,12 +324,16 @@ class PagedKVCache:
 
     def begin(self, new) -> None:
         """Start a step with ``new[slot]`` tokens of every slot (0: the slot rests)."""
-        self.tables.begin(new)
+        t = self.tables
+        t.begin(new)
+        self._most_new = max(t.new)
+        self._longest = max(a + b for a, b in zip(t.lens, t.new) if b)
         self._publish()
 
     def advance(self) -> None:
         """End the step: its tokens are cached."""
         self.tables.advance()
+        self._most_new = 0
 
     def attention(self, layer: int, q_dev, k_dev, v_dev, cos_dev=None, sin_dev=None, sm_scale: float | None = None,
                   interleaved: bool = False, out=None):
@@ -341,17 +346,16 @@ class PagedKVCache:
         t = self.tables
         if not 0 <= layer < self.n_layer:
             raise ValueError(f"layer {layer} out of range [0, {self.n_layer})")
-        if not any(t.new):
+        if not self._most_new:
             raise ValueError("begin() starts a step")
         for name, x, heads in (("q", q_dev, self.n_head), ("k", k_dev, self.n_kv_head), ("v", v_dev, self.n_kv_head)):
             if len(x.shape) != 4 or x.shape[0] != t.max_batch or x.shape[2:] != (heads, self.d_k):
                 raise ValueError(f"{name} must be ({t.max_batch}, n_new, {heads}, {self.d_k}), got {x.shape}")
         n_new = q_dev.shape[1]
-        if n_new < max(t.new):
-            raise ValueError(f"q has {n_new} rows a slot, the step {max(t.new)} tokens")
-        longest = max(a + b for a, b in zip(t.lens, t.new) if b)
-        if cos_dev is not None and longest > cos_dev.shape[0]:
-            raise ValueError(f"{longest} positions exceed the cos/sin table size ({cos_dev.shape[0]})")
+        if n_new < self._most_new:
+            raise ValueError(f"q has {n_new} rows a slot, the step {self._most_new} tokens")
+        if cos_dev is not None and self._longest > cos_dev.shape[0]:
+            raise ValueError(f"{self._longest} positions exceed the cos/sin table size ({cos_dev.shape[0]})")
         pool = self.layers[layer]
         paged_kv_append(q_dev, k_dev, v_dev, pool["k"], pool["v"], self._table, self._lens, cos_dev, sin_dev,
                         new_lens=self._new, interleaved=interleaved)
