@@ -394,7 +394,8 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; o may not overlap q, k or v.
  * With few rows the keys are shared by several workgroups, whose results lie in the
  * workspace (tl_window_workspace_bytes bytes, 16-byte aligned, most_keys = seq_k, or
- * max_pages * page_size; no initialisation) and are joined by a second launch;
+ * max_pages * page_size; no initialisation; calls that overlap in time need one each)
+ * and are joined by the last of them or by a second launch;
  * given less (NULL: none) the call runs in one.  Either is deterministic.
  * (n_new or seq_q) <= 2^28, seq_k <= 2^29, and times the square of n_head / n_kv_head below 2^32.
  * A NaN or infinity in a V row makes NaN of the rows that are computed in one

@@ -103,3 +103,31 @@ def test_captured_calls_replay():
         g.replay()
         window_attention(*x, 50, 0)
         np.testing.assert_array_equal(gpu.to_host(out).view(np.uint16), want.view(np.uint16))
+
+
+@pytest.mark.parametrize("dtype,D,cus", [("float32", 64, 16), ("float16", 64, 8), ("bfloat16", 128, 10)])
+def test_few_parts_joined_without_a_second_launch(monkeypatch, dtype, D, cus):
+    """Row tiles of two or three parts: from a workspace that holds anything, eager and replayed with other calls on the
+    same workspace between, always the same bits."""
+    P.H.set_override(monkeypatch, "TRITON_LLM_HIP_MAX_CUS", cus)
+    rng = np.random.default_rng(11)
+    B, Hq, Hkv, Sq, Sk = 1, 4, 2, 200, 600
+    q, k, v = (P.values(rng, s, dtype) for s in [(B, Hq, Sq, D), (B, Hkv, Sk, D), (B, Hkv, Sk, D)])
+    x = [P.dev(t, dtype) for t in (q, k, v)]
+    y = [P.dev(P.values(rng, s, dtype), dtype) for s in [(B, Hq, 150, D), (B, Hkv, 700, D), (B, Hkv, 700, D)]]
+    ws = gpu.to_device(np.full(1 << 24, 0xFF, np.uint8))
+    first = P.back(window_attention(*x, 0, workspace=ws), dtype)
+    want, tol = P.rows_want(q[0], on.from_storage(k[0], dtype), on.from_storage(v[0], dtype), Sk - Sq + np.arange(Sq), True, 0, 0,
+                            D ** -0.5, dtype)
+    P.check(f"few parts {dtype} d{D}", first[0], want, tol)
+    out = P.dev(np.zeros(q.shape, q.dtype), dtype)
+    gpu.synchronize()
+    with gpu.capture() as g:
+        window_attention(*x, 0, out=out, workspace=ws)
+    for i in range(4):
+        out.from_numpy(np.full(q.shape, on.nan_storage(dtype), q.dtype))
+        if i % 2:
+            window_attention(*y, 0, workspace=ws)
+        g.replay()
+        np.testing.assert_array_equal(P.back(out, dtype), first)
+        np.testing.assert_array_equal(P.back(window_attention(*x, 0, workspace=ws), dtype), first)

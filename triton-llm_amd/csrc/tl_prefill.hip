@@ -1553,25 +1553,6 @@ static size_t plan_flash_16(FlashParams& p, int D, bool causal, size_t split_roo
   return bytes;
 }
 
-// This call's arrival tag: a per-process random base plus a call count, so a
-// word left in a reused workspace by an earlier call (or holding unrelated
-// data) is not mistaken for it.  Never 0, the value a merge leaves behind.
-static uint64_t next_split_token() {
-  static const uint64_t base = [] {
-    uint64_t b = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull ^
-                 (uint64_t)(uintptr_t)&b;
-    try {  // no exception may leave the C ABI
-      std::random_device rd;
-      b ^= ((uint64_t)rd() << 32) ^ (uint64_t)rd();
-    } catch (...) {
-    }
-    return b;
-  }();
-  static std::atomic<uint64_t> count{0};
-  const uint64_t t = base + 2 * (count.fetch_add(1, std::memory_order_relaxed) + 1);
-  return t ? t : 1;
-}
-
 // V rows that flash_fwd_16 can read in place: a tile's reads are bounded by its
 // row count times the row stride, with 32-bit byte offsets.
 bool v_rows_ok(const FlashParams& p, int d_k) {
@@ -1624,7 +1605,7 @@ int launch_flash_16(FlashParams& p, void* ws, size_t ws_bytes, bool causal, hipS
   p.split_token = 0;
   if (plan_flash_16(p, D, causal, w64 ? 0 : room)) {
     p.split_ws = (char*)ws + align256(vt_need);
-    p.split_token = next_split_token();
+    p.split_token = tl_arrival_tag();
   }
   if constexpr (D != 64) {
     if (!vnat) {
@@ -1695,6 +1676,25 @@ bool mfma_shape_ok(const FlashParams& p, int d_k, int dtype) {
 }
 
 }  // namespace
+
+// This call's arrival tag: a per-process random base plus a call count, so a
+// word left in a reused workspace by an earlier call (or holding unrelated
+// data) is not mistaken for it.  Never 0, the value a merge leaves behind.
+uint64_t tl_arrival_tag() {
+  static const uint64_t base = [] {
+    uint64_t b = (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() * 0x9e3779b97f4a7c15ull ^
+                 (uint64_t)(uintptr_t)&b;
+    try {  // no exception may leave the C ABI
+      std::random_device rd;
+      b ^= ((uint64_t)rd() << 32) ^ (uint64_t)rd();
+    } catch (...) {
+    }
+    return b;
+  }();
+  static std::atomic<uint64_t> count{0};
+  const uint64_t t = base + 2 * (count.fetch_add(1, std::memory_order_relaxed) + 1);
+  return t ? t : 1;
+}
 
 extern "C" {
 

@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBM = 128;  // query rows of a workgroup
 constexpr int kMinShare = 4;  // key tiles of a part at least
+constexpr int kWaveParts = 4;  // parts of a row tile that the waves join themselves
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kMostRows = 1 << 28;     // query rows of a sequence
 constexpr int kWholeWindow = 3 << 29;  // positions lie in [-2^28, 2^30 + 2^28): a window this long hides nothing, and
@@ -50,6 +51,8 @@ struct WinParams {
   int slots;           // workgroups that the keys are shared by; 0: a row tile's keys are not divided
   int q_shift, n_lvl, xcd_groups;  // how workgroups are dealt (window_fwd_kernel)
   int vec_out;         // o's rows take 4 elements at once
+  uint64_t tag;        // this call's, where the waves join the parts; 0: window_join_kernel does
+  uint64_t* words;     // [part][wave]: the tag where the part's results are there
   float* ws;           // partial results by part (slots > 0)
   int64_t q_sb, q_sh, q_ss;
   int64_t k_sb, k_sh, k_ss;
@@ -381,7 +384,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   // Undivided: these are cut into every 2^q_shift-th row tile, so that a multiple of 8 groups is dealt to the XCDs;
   // within an XCD the longest rows come first.  Divided: an XCD takes a contiguous range of the parts.
   const int xcd = blockIdx.x % 8, at = blockIdx.x / 8;
-  int b, hkv, qt, part = 0, parts = 1, place = 0;
+  int b, hkv, qt, part = 0, parts = 1, place = 0, stride = 0;  // stride: places from part to part
   Rows rw;
   if (p.slots > 0) {
     const Deal d = deal_of<BN, PAGED>(p, lane);
@@ -401,6 +404,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     rw = s.r;
     const int in = place - before;
     parts = s.parts;
+    stride = s.tiles;
     hkv = (int)((unsigned)in / (unsigned)(parts * s.tiles));
     const int r = in - hkv * parts * s.tiles;
     part = (int)((unsigned)r / (unsigned)s.tiles);
@@ -597,19 +601,70 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   }
 
   l = TL::kSumMfma ? la[0] : tlp::sum_xor32(l);
+  // Divided keys: a wave leaves its part's results.  Where a row tile has few parts (p.tag: see window_entry) it waits for
+  // its stores and then leaves the call's tag.  A wave that
+  // finds the tags of all parts there (the last one does; several may, and write the same) adds them up in the
+  // parts' order and takes the tags away, for a graph's next replay.  Nothing waits for another workgroup.  Stores,
+  // tags and loads are device-coherent (sc1), which orders them across XCDs without write-backs of a cache.
   if (parts > 1) {
-    float* w = p.ws + (size_t)place * part_floats<D>() + (size_t)wave * (64 + 64 * (D / 2));
-    if (h == 0) {
-      w[2 * lq] = m;
-      w[2 * lq + 1] = l;
-    }
+    if (!wave_rows) return;
+    constexpr int kSc1 = 16;
+    constexpr uint32_t kWaveBytes = (64 + 64 * (D / 2)) * 4;
+    auto part_rsrc = [&](int k) {
+      return __builtin_amdgcn_make_buffer_rsrc((char*)(p.ws + (size_t)k * part_floats<D>()) + wave * kWaveBytes, (short)0,
+                                               (int)kWaveBytes, kBufRsrcWord3);
+    };
+    const auto mine = part_rsrc(place);
+    const int o_at = 256 + 16 * lane, ml_at = 8 * lq;
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
-        *(f32x4*)(w + 64 + (4 * db + a) * 256 + 4 * lane) =
-            f32x4{o[db][4 * a], o[db][4 * a + 1], o[db][4 * a + 2], o[db][4 * a + 3]};
-    return;
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 x = {o[db][4 * a], o[db][4 * a + 1], o[db][4 * a + 2], o[db][4 * a + 3]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), mine, o_at, (4 * db + a) * 1024, kSc1);
+      }
+    if (h == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, mine, ml_at, 0, kSc1);
+    if (!p.tag) return;
+    wait_vmcnt<0>();
+    const int first = place - part * stride;
+    auto word = [&](int k) { return p.words + 4 * (size_t)(first + k * stride) + wave; };
+    if (lane == 0) __hip_atomic_store(word(part), p.tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    wait_vmcnt<0>();
+    bool all = true;
+    for (int k0 = 0; k0 < parts; k0 += 64) {
+      uint64_t x = p.tag;
+      if (k0 + lane < parts) x = __hip_atomic_load(word(k0 + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      all = all && __all(x == p.tag);
+    }
+    if (!all) return;
+    asm volatile("" ::: "memory");
+    float top = -INFINITY;
+    for (int k = 0; k < parts; ++k)
+      top = fmaxf(top, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(part_rsrc(first + k * stride), ml_at, 0, kSc1)));
+    const float shift = top == -INFINITY ? 0.f : top;
+    l = 0.f;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    for (int k = 0; k < parts; ++k) {
+      const auto rs = part_rsrc(first + k * stride);
+      const u32x2 ml = __builtin_amdgcn_raw_buffer_load_b64(rs, ml_at, 0, kSc1);
+      u32x4 x[NDB][4];
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) x[db][a] = __builtin_amdgcn_raw_buffer_load_b128(rs, o_at, (4 * db + a) * 1024, kSc1);
+      const float f = fast_exp2(__uint_as_float(ml.x) - shift);
+      l = fmaf(__uint_as_float(ml.y), f, l);
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[db][4 * a + e] = fmaf(__uint_as_float(x[db][a][e]), f, o[db][4 * a + e]);
+    }
+    for (int k = lane; k < parts; k += 64) __hip_atomic_store(word(k), (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!there) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -622,7 +677,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
                 o[db][4 * a + 3] * inv, p.vec_out);
 }
 
-// Joins the parts of a row tile: the same lanes that wrote them.
+// Joins the parts of a row tile where the waves do not: the same lanes that wrote them.
 template <typename T, int D, bool PAGED>
 __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
   using B = typename T::bits;
@@ -703,6 +758,8 @@ int64_t plan_slots(WinParams& p, int64_t keys, int d_k, int esize) {
 // last tile count.)
 bool rows_ok(int64_t seq_q, int64_t group) { return (seq_q * group + kBM) * group < ((int64_t)1 << 32); }
 
+// Workspace of so many parts: their tags, then their results.
+size_t words_bytes(int64_t parts) { return ((size_t)parts * 4 * sizeof(uint64_t) + 255) & ~(size_t)255; }
 size_t part_bytes(int d_k) { return (d_k == 64 ? part_floats<64>() : part_floats<128>()) * sizeof(float); }
 
 template <typename T, int D>
@@ -717,8 +774,8 @@ int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) 
   const dim3 grid(p.slots > 0 ? (unsigned)((most_parts + 7) / 8 * 8) : (unsigned)(8 * p.xcd_groups * p.n_lvl));
   if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
-  int e = tl_launch_status();
-  if (e || p.slots == 0) return e;
+  const int e = tl_launch_status();
+  if (e || p.slots == 0 || p.tag) return e;
   const dim3 join((unsigned)tiles, D / 32);
   if (paged) hipLaunchKernelGGL((window_join_kernel<T, D, true>), join, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_join_kernel<T, D, false>), join, dim3(kThreads), 0, st, p);
@@ -761,8 +818,15 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
   const int64_t most_parts = plan_slots(p, keys, d_k, esize);
   if (p.slots > 0) {
     // without room for the parts the keys stay undivided
-    if (!workspace || workspace_bytes < (size_t)most_parts * part_bytes(d_k) || ((uintptr_t)workspace & 15)) p.slots = 0;
-    p.ws = (float*)workspace;
+    if (!workspace || workspace_bytes < words_bytes(most_parts) + (size_t)most_parts * part_bytes(d_k) || ((uintptr_t)workspace & 15)) p.slots = 0;
+    // Few parts are joined by the wave that ends last, without a second launch; many would be added up one after the
+    // other by one wave.  us with this rule's first side / second: 1023 rows, window 256, fp32 (2 parts) 25.0 / 27.9,
+    // 4 x 500 rows on prefixes (3 parts) 40.4 / 43.0; 500 rows on 4000 keys, d_k 128 (5 parts) 43.6 / 41.9, 100 rows (21
+    // parts) 39.9 / 28.8.
+    const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
+    p.tag = p.slots <= kWaveParts * tiles ? tl_arrival_tag() : 0;
+    p.words = (uint64_t*)workspace;
+    p.ws = (float*)((char*)workspace + words_bytes(most_parts));
   }
   hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
@@ -789,7 +853,8 @@ size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q
   p.n_qt = (seq_q * p.group + kBM - 1) / kBM;
   p.window = window;
   p.sinks = sinks;
-  return (size_t)plan_slots(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2) * part_bytes(d_k);
+  const int64_t parts = plan_slots(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2);
+  return parts ? words_bytes(parts) + (size_t)parts * part_bytes(d_k) : 0;
 }
 
 int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace, size_t workspace_bytes,
