@@ -18,7 +18,7 @@
 // V is read by transposing LDS reads.
 //
 // Bound by the matrix products and, at d_k 64, as much by exp and the conversions: 8192 tokens, window 1024, 24 / 8 heads
-// of 128, bf16: 131 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 43.4 us, 7.4 of them the join.
+// of 128, bf16: 131 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 40.9 to 43.5 us by device.
 #include "tl_paged.h"
 #include "tl_prefill.h"
 
@@ -739,11 +739,11 @@ int64_t most_tiles(int64_t keys, int window, int sinks, int group, int bn) {
 }
 
 // Whether the keys of the row tiles are divided, and by how many workgroups: where the row tiles alone would not fill
-// the device and a row tile can have several parts (1 x 100 rows on 4000 keys, 15 / 5 heads, d_k 64, fp16: 22.7 us,
-// undivided 58.6; 1000 causal rows, 9 / 3 heads: 16.3 and 18.5).  The 16-bit kernels and fp32 at d_k 128 take as many
-// workgroups as fit (1 x 500 rows on 4000 keys, 24 / 8 heads, d_k 128: fp16 43.1 us, one a CU 51.6; fp32 at 300 rows on
-// 2000 keys 89 and 101); fp32 at d_k 64 is bound by its matrix products, which one workgroup a CU keeps busy (1023
-// rows, window 256: 27.8 us, with two 31.5).  Returns the most parts there can be (0: undivided).
+// the device and a row tile can have several parts (1 x 100 rows on 4000 keys, 15 / 5 heads, d_k 64, fp16: 22.0 us,
+// undivided 58; 1000 causal rows, 9 / 3 heads: 14.4 and 18.5).  The 16-bit kernels and fp32 at d_k 128 take as many
+// workgroups as fit (1 x 500 rows on 4000 keys, 24 / 8 heads, d_k 128: fp16 39.6 us, one a CU 47; fp32 at 300 rows on
+// 2000 keys 86 and 98); fp32 at d_k 64 is bound by its matrix products, which one workgroup a CU keeps busy (1023
+// rows, window 256: 25.0 us, with two 30.1).  Returns the most parts there can be (0: undivided).
 int64_t plan_slots(WinParams& p, int64_t keys, int d_k, int esize) {
   const int bn = esize == 2 ? 64 : 32;
   const int64_t most = most_tiles(keys, p.window, p.sinks, p.group, bn);
@@ -820,9 +820,9 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
     // without room for the parts the keys stay undivided
     if (!workspace || workspace_bytes < words_bytes(most_parts) + (size_t)most_parts * part_bytes(d_k) || ((uintptr_t)workspace & 15)) p.slots = 0;
     // Few parts are joined by the wave that ends last, without a second launch; many would be added up one after the
-    // other by one wave.  us with this rule's first side / second: 1023 rows, window 256, fp32 (2 parts) 25.0 / 27.9,
-    // 4 x 500 rows on prefixes (3 parts) 40.4 / 43.0; 500 rows on 4000 keys, d_k 128 (5 parts) 43.6 / 41.9, 100 rows (21
-    // parts) 39.9 / 28.8.
+    // other by one wave.  us joined by the waves / by a second launch: 1023 rows, window 256, fp32 (2 parts) 25.0 / 26.2,
+    // 4 x 500 rows on prefixes (3 parts) 43.5 / 44.8; 500 rows on 4000 keys, d_k 128 (5 parts) 43.7 / 39.6, 100 rows (21
+    // parts) 40.7 / 27.6.
     const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
     p.tag = p.slots <= kWaveParts * tiles ? tl_arrival_tag() : 0;
     p.words = (uint64_t*)workspace;
