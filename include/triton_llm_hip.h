@@ -378,9 +378,9 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * {batch, head}, over L = min(cache_lens[b] + len_add, max_pages * page_size)
  * positions; with window > 0 it sees only the last `window` of them and the first
  * `sinks`.  A sequence that sees nothing gives zeros.  Hidden positions are not
- * read.  One launch, or two where a sequence's positions are shared by several
- * workgroups: the workspace (tl_paged_decode_workspace_bytes, 16-byte aligned, given
- * either way) holds their results and needs no initialisation; calls that overlap in time need
+ * read.  Where several workgroups share a sequence's positions the workspace
+ * (tl_paged_decode_workspace_bytes, 16-byte aligned, given either way) holds their
+ * results and needs no initialisation; calls that overlap in time need
  * one each.  d_k 64 or 128, rows aligned to d_k / 16 elements; batch <= 65535, and
  * at most 2^31 - 1 blocks of 16 positions over batch, KV heads and pages.
  *

@@ -371,3 +371,40 @@ def test_prefill_divided_keys(monkeypatch, dtype, D, batch, cus):
             v, _ = op.gather(on.from_storage(vp, dtype), table[b], n + m)
             want, tol = P.rows_want(q[b, :m].transpose(1, 0, 2), k, v, n + np.arange(m), there, window, sinks, D ** -0.5, dtype)
             P.check(f"divided {dtype} sequence {b} {n}+{m} window {window}", got[b, :m].transpose(1, 0, 2), want, tol)
+
+
+@pytest.mark.parametrize("dtype,D,lens", [("float32", 64, [700]), ("bfloat16", 128, [1500, 3, 900, 0]),
+                                          ("float16", 64, [40] * 70 + [2000])])
+def test_shared_positions_replay(monkeypatch, dtype, D, lens):
+    """Sequences shared by workgroups: from a workspace that holds anything, eager and replayed with other calls on the same
+    workspace between, always the same bits."""
+    P.H.set_override(monkeypatch, "TRITON_LLM_HIP_DECODE_SHARES", 1)
+    rng = np.random.default_rng(21)
+    Hq, Hkv, page = 6, 2, 16
+    lens = np.array(lens, np.int32)
+    max_pages = 2048 // page
+    n_pages = int(sum(-(-int(n) // page) for n in lens)) + 1
+    table = P.shuffled_table(rng, lens, page, max_pages, n_pages)
+    kp, vp = (P.dev(P.values(rng, (n_pages, Hkv, page, D), dtype), dtype) for _ in range(2))
+    q = P.dev(P.values(rng, (len(lens), Hq, D), dtype), dtype)
+    t_d, l_d, short = P.int32(table), P.int32(lens), P.int32(np.minimum(lens, 333))
+    ws = gpu.to_device(np.full(1 << 26, 0xFF, np.uint8))
+
+    def call(n, **kw):
+        return paged_attention_decode(q, kp, vp, t_d, n, Hq, Hkv, workspace=ws, **kw)
+
+    first = P.back(call(l_d), dtype)
+    plain = P.back(paged_attention_decode(q, kp, vp, t_d, l_d, Hq, Hkv), dtype)
+    np.testing.assert_array_equal(plain, first)
+    assert np.isfinite(first).all()
+    out = P.dev(np.zeros(q.shape, on.storage_dtype(dtype)), dtype)
+    gpu.synchronize()
+    with gpu.capture() as g:
+        call(l_d, out=out)
+    for i in range(4):
+        out.from_numpy(np.full(q.shape, on.nan_storage(dtype), on.storage_dtype(dtype)))
+        if i % 2:
+            call(short)
+        g.replay()
+        np.testing.assert_array_equal(P.back(out, dtype), first)
+        np.testing.assert_array_equal(P.back(call(l_d), dtype), first)

@@ -188,7 +188,9 @@ def test_c_decode_refuses():
                 dict(q=ctypes.c_void_p(0x100004)), dict(ks=_lib.strides(512, -64, 64))):
         assert c_decode(**bad) == 801, bad
     ws = _lib.load().tl_paged_decode_workspace_bytes
-    assert ws(24, 8, 128) == 2048 * 2 * 3 * (2 + 128) * 4 and ws(16, 1, 64) == 2048 * 2 * 8 * (2 + 64) * 4
+    tags = 2048 * 2 * 8
+    assert ws(24, 8, 128) == tags + 2048 * 2 * 3 * (2 + 128) * 4
+    assert ws(16, 1, 64) == tags + 2048 * 2 * 8 * (2 + 64) * 4
     assert ws(0, 1, 64) == ws(5, 2, 64) == ws(4, 2, 0) == 0
 
 

@@ -159,6 +159,9 @@ static inline bool tl_overlap(const void* a, size_t na, const void* b, size_t nb
 // HIP graph as a kernel node).
 int tl_fill_bytes(void* dst, unsigned char value, size_t nbytes, hipStream_t st);
 
+// A tag of this call's own (never 0), for words in a workspace that say that results are there (tl_prefill.hip).
+uint64_t tl_arrival_tag();
+
 // Test-only overrides.  tl_init reads them from the environment on every
 // call (so a test re-reads them by calling tl_init again); launches read only
 // these fields, never the environment.

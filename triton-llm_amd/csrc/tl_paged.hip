@@ -1,5 +1,5 @@
 // The paged KV cache: what writes it (paged_append), reads it for one new token a
-// sequence (paged_decode, paged_combine) and copies its pages (copy_pages).
+// sequence (paged_decode) and copies its pages (copy_pages).
 //
 // The reference keeps one contiguous cache per sequence on the host
 // (smollm2_triton/model.py:190-225) and has no pages; positions, RoPE and attention
@@ -257,12 +257,12 @@ int launch_append(const AppendParams& p, int mode, hipStream_t st) {
 // 8 of its query heads, and cut into equal shares, a workgroup each, whatever the lengths.
 // A share may end inside a pair and go on in the next; each piece is a segment.  A pair inside one
 // share is finished there; else each segment leaves (m, l, acc) in the workspace, and
-// paged_combine joins them.  A share has at most one segment of a pair that began before it
+// the last of them joins them.  A share has at most one segment of a pair that began before it
 // (slot 0) and one of a pair that goes on after it (slot 1), so the workspace is two
 // slots a workgroup, whatever batch and length are.
 //
-// Bound by the reading of K and V: 64 sequences of 4096 to 16383 positions, 24 / 8 heads of 128, bf16, 2.9 GB: 438 us
-// and 4.6 for the join, 6.6 TB/s; shorter calls by the latency of a few dependent loads.
+// Bound by the reading of K and V: 64 sequences of 4096 to 16383 positions, 24 / 8 heads of 128, bf16, 2.9 GB: 444 us,
+// 6.5 TB/s; shorter calls by the latency of a few dependent loads.
 // ---------------------------------------------------------------------------------
 constexpr int kDecThreads = 256;
 constexpr int kDecWaves = kDecThreads / 64;
@@ -282,6 +282,8 @@ struct DecodeParams {
   const void* v;
   const int32_t* lens;
   PageMap pm;
+  uint64_t tag;     // this call's
+  uint64_t* words;  // [share][2]: the tag where that segment's results are there
   float* ws_ml;   // [share][2][heads_per_pair][2]
   float* ws_acc;  // [share][2][heads_per_pair][D]
   void* o;
@@ -451,6 +453,89 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_rsrc(const char* base, u
   return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)a, (short)0, (int)bytes, kBufRsrcWord3);
 }
 
+// Stores and loads past an XCD's L2 (sc1), which order partial results across XCDs without a write-back of a cache.
+__device__ __forceinline__ void put(float* at, float x) {
+  __hip_atomic_store(at, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get(const float* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// After a segment of a pair that several shares have: once its stores are done the workgroup leaves the call's tag, and
+// where it finds those of all segments (the last one does; several may, and write the same) it joins them, a wave a head,
+// and takes the tags away, for a graph's next replay.  Nothing waits for another workgroup.  (With a
+// second launch for the joins, 3.6 us, one sequence of 100 positions, 9 / 3 heads, fp32, took 9.0 us for 8.15, and 64 long
+// ones 442.5 for 445.)  Lane s holds segment s's (m, l);
+// accumulators are read eight segments at a time.
+template <typename T, int D, int G, int NW>
+__device__ __forceinline__ void join_segments(const DecodeParams& p, int b, int hq0, int n_g, int first,
+                                              int parts, int wave, int lane, int& s_all) {
+  constexpr int NJ = D / 64, R = 8;
+  using B = typename T::bits;
+  auto at_slot = [&](int s) { return (first + s) * 2 + (s == 0 ? 1 : 0); };
+  wait_vmcnt<0>();
+  __syncthreads();
+  if (wave == 0) {
+    if (lane == 0)
+      __hip_atomic_store(p.words + at_slot((int)blockIdx.x - first), p.tag, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    wait_vmcnt<0>();
+    bool all = true;
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+      uint64_t x = p.tag;
+      if (s0 + lane < parts) x = __hip_atomic_load(p.words + at_slot(s0 + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      all = all && __all(x == p.tag);
+    }
+    if (lane == 0) s_all = all ? 1 : 0;
+  }
+  __syncthreads();
+  if (!s_all) return;
+  asm volatile("" ::: "memory");
+  for (int g = wave; g < n_g; g += NW) {
+    auto at = [&](int s) { return at_slot(s) * G + g; };
+    auto load = [&](int s0, float (&r)[R][NJ]) {
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) r[k][j] = s0 + k < parts ? get(p.ws_acc + (int64_t)at(s0 + k) * D + lane + 64 * j) : 0.f;
+    };
+    float r[R][NJ];
+    load(0, r);
+    auto ml = [&](int s) { return make_float2(get(p.ws_ml + 2 * at(s)), get(p.ws_ml + 2 * at(s) + 1)); };
+    const float2 e0 = lane < parts ? ml(lane) : make_float2(-INFINITY, 0.f);
+    float mx = e0.x;
+    for (int s = lane + 64; s < parts; s += 64) mx = fmaxf(mx, get(p.ws_ml + 2 * at(s)));
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float ls = 0.f, wl = 0.f, a[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) a[j] = 0.f;
+    for (int s0 = 0; s0 < parts; s0 += R) {
+      if ((s0 & 63) == 0) {
+        const int s = s0 + lane;
+        const float2 e = s0 == 0 ? e0 : s < parts ? ml(s) : make_float2(-INFINITY, 0.f);
+        wl = s < parts ? fast_exp2(e.x - base) : 0.f;
+        ls += e.y * wl;
+      }
+      if (s0 > 0) load(s0, r);
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wl), (s0 + k) & 63));
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) a[j] = fmaf(r[k][j], w, a[j]);
+      }
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) ls += __shfl_xor(ls, off);
+    B* o = (B*)p.o + b * p.o_sb + (int64_t)(hq0 + g) * p.o_sh;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = from_f32<T>(ls == 0.f ? 0.f : a[j] / ls);
+  }
+  if (wave == 0)
+    for (int s = lane; s < parts; s += 64)
+      __hip_atomic_store(p.words + at_slot(s), (uint64_t)0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // 16 lanes read a row, a wave 4 rows a load and a block in 4 loads of K and 4 of V; wave w takes blocks
 // w, w + NW, ... of the segment, NB of them at a time.  PAIR: a workgroup takes a whole pair (see pair_mode).
 // (8 lanes with 16-byte loads for rows of 128 bytes were slower: 32 sequences, 15 / 5 heads, d_k 64, 1000 positions
@@ -468,13 +553,16 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
   const int n_chunks = p.n_pairs / p.n_kv;
   __shared__ float s_m[NW][G], s_l[NW][G];
   __shared__ float s_acc[NW][G][D];
+  __shared__ int s_all;
   const uint32_t k_lane = rowg * p.k_row_bytes + sub * (EPL * T::size);
   const uint32_t v_lane = rowg * p.v_row_bytes + sub * (EPL * T::size);
 
   // Blocks [v0, v1) of the Seen blocks of pair `pair` of sequence b; r0 of share blocks of the workgroup's
   // share are done before.
-  auto segment = [&](const int b, const Seen& sn, const int pair, const int v0, const int v1, const bool whole,
-                     const int slot, const int done, const int share) {
+  auto segment = [&](const int b, const Seen& sn, const int pair, const int v0, const int v1, const int first,
+                     const int parts, const int done, const int share) {
+    const bool whole = parts == 1;
+    const int slot = v0 == 0 ? 1 : 0;
     const int hkv = pair / n_chunks;
     const int hq0 = hkv * p.group + (pair - hkv * n_chunks) * G;
     const int n_g = min(G, hkv * p.group + p.group - hq0);
@@ -664,122 +752,55 @@ __global__ __launch_bounds__(64 * NW) void paged_decode_kernel(DecodeParams p) {
         ((B*)p.o)[b * p.o_sb + (int64_t)(hq0 + g) * p.o_sh + d] = from_f32<T>(ls == 0.f ? 0.f : a / ls);
       } else {
         const int64_t at = ((int64_t)blockIdx.x * 2 + slot) * G + g;
-        p.ws_acc[at * D + d] = a;
+        put(p.ws_acc + at * D + d, a);
         if (d == 0) {
-          p.ws_ml[at * 2] = mx;
-          p.ws_ml[at * 2 + 1] = ls;
+          put(p.ws_ml + at * 2, mx);
+          put(p.ws_ml + at * 2 + 1, ls);
         }
       }
+    }
+    if constexpr (!PAIR) {
+      if (!whole) join_segments<T, D, G, NW>(p, b, hq0, n_g, first, parts, wave, lane, s_all);
     }
   };
 
   if constexpr (PAIR) {
     const int b = (int)blockIdx.x / p.n_pairs;
     const Seen sn = seen_of(p, b);
-    segment(b, sn, (int)blockIdx.x - b * p.n_pairs, 0, sn.n, true, 0, 0, 0);
+    segment(b, sn, (int)blockIdx.x - b * p.n_pairs, 0, sn.n, 0, 1, 0, 0);
   } else {
     const Layout lay = layout_of(p, lane);
+    const int64_t begin = (int64_t)blockIdx.x * lay.share;
     if (lay.padded) {
       // one segment a workgroup: part blockIdx.x - first of its pair
       const int w = (int)blockIdx.x;
-      if (w >= lay.total) return;
-      const Owner own = owner_of(p, lay, w, lane);
-      const Seen sn = seen_of(p, own.b);
-      const int parts = (sn.n + lay.share - 1) / lay.share;
-      const int pair = (w - own.first) / parts;
-      const int part = (w - own.first) - pair * parts;
-      const int v0 = part * lay.share, v1 = min(v0 + lay.share, sn.n);
-      segment(own.b, sn, pair, v0, v1, parts == 1, part == 0 ? 1 : 0, 0, v1 - v0);
-      return;
+      if (w < lay.total) {
+        const Owner own = owner_of(p, lay, w, lane);
+        const Seen sn = seen_of(p, own.b);
+        const int parts = (sn.n + lay.share - 1) / lay.share;
+        const int pair = (w - own.first) / parts;
+        const int first = own.first + pair * parts, v0 = (w - first) * lay.share, v1 = min(v0 + lay.share, sn.n);
+        segment(own.b, sn, pair, v0, v1, first, parts, 0, v1 - v0);
+      }
+    } else if (begin < lay.total) {
+      const int r0 = (int)begin, r1 = (int)min((int64_t)lay.total, begin + lay.share);
+      for (int r = r0; r < r1;) {
+        const Owner own = owner_of(p, lay, r, lane);
+        const Seen sn = seen_of(p, own.b);
+        const int pair = (r - own.first) / sn.n;
+        const int pair0 = own.first + pair * sn.n;
+        const int v0 = r - pair0, v1 = min(r1 - pair0, sn.n);
+        const int first = pair0 / lay.share, parts = (pair0 + sn.n - 1) / lay.share - first + 1;
+        segment(own.b, sn, pair, v0, v1, first, parts, r - r0, r1 - r0);
+        r = pair0 + v1;
+      }
     }
-    const int64_t first = (int64_t)blockIdx.x * lay.share;
-    if (first >= lay.total) return;
-    const int r0 = (int)first, r1 = (int)min((int64_t)lay.total, first + lay.share);
-    for (int r = r0; r < r1;) {
-      const Owner own = owner_of(p, lay, r, lane);
-      const Seen sn = seen_of(p, own.b);
-      const int pair = (r - own.first) / sn.n;
-      const int pair0 = own.first + pair * sn.n;
-      const int v0 = r - pair0, v1 = min(r1 - pair0, sn.n);
-      segment(own.b, sn, pair, v0, v1, v0 == 0 && v1 == sn.n, v0 == 0 ? 1 : 0, r - r0, r1 - r0);
-      r = pair0 + v1;
+    // sequences that see nothing
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+      if (seen_of(p, b).n > 0) continue;
+      for (int i = threadIdx.x; i < p.n_head * D; i += 64 * NW) ((B*)p.o)[b * p.o_sb + (int64_t)(i / D) * p.o_sh + i % D] = 0;
     }
   }
-}
-
-// One wave a (sequence, query head): join the shares of its pair.  A pair inside one share
-// is finished already; a sequence that sees nothing gets zeros here.  All latency: lane s holds share s's
-// (m, l), accumulators are read eight shares at a time.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void paged_combine_kernel(DecodeParams p) {
-  constexpr int NJ = D / 64, R = 8;
-  using B = typename T::bits;
-  const int hq = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
-  B* o = (B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh;
-  const Seen sn = seen_of(p, b);
-  if (sn.n == 0) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = 0;
-    return;
-  }
-  const Layout lay = layout_of(p, lane);
-  const int hkv = hq / p.group, in = hq - hkv * p.group;
-  const int pair = hkv * (p.n_pairs / p.n_kv) + in / p.heads_per_pair;
-  const int g = in % p.heads_per_pair;
-  int parts, first;
-  if (lay.padded) {
-    parts = (sn.n + lay.share - 1) / lay.share;
-    if (parts == 1) return;
-    first = first_of(p, lay, b, lane) + pair * parts;
-  } else {
-    const int pair0 = first_of(p, lay, b, lane) + pair * sn.n;
-    first = pair0 / lay.share;
-    parts = (pair0 + sn.n - 1) / lay.share - first + 1;
-    if (parts == 1) return;
-  }
-  auto at = [&](int s) { return ((first + s) * 2 + (s == 0 ? 1 : 0)) * p.heads_per_pair + g; };
-  auto load = [&](int s0, float (&r)[R][NJ]) {
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) r[k][j] = s0 + k < parts ? p.ws_acc[(int64_t)at(s0 + k) * D + lane + 64 * j] : 0.f;
-  };
-  float r[R][NJ];
-  load(0, r);
-  const float2* ml = (const float2*)p.ws_ml;
-  const float2 e0 = lane < parts ? ml[at(lane)] : make_float2(-INFINITY, 0.f);
-  float mx = e0.x;
-  for (int s = lane + 64; s < parts; s += 64) mx = fmaxf(mx, ml[at(s)].x);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float ls = 0.f, wl = 0.f, a[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) a[j] = 0.f;
-  for (int s0 = 0; s0 < parts; s0 += R) {
-    if ((s0 & 63) == 0) {
-      const int s = s0 + lane;
-      const float2 e = s0 == 0 ? e0 : s < parts ? ml[at(s)] : make_float2(-INFINITY, 0.f);
-      wl = s < parts ? fast_exp2(e.x - base) : 0.f;
-      ls += e.y * wl;
-    }
-    float rn[R][NJ];
-    if (s0 + R < parts) load(s0 + R, rn);
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wl), (s0 + k) & 63));
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) a[j] = fmaf(r[k][j], w, a[j]);
-    }
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) r[k][j] = rn[k][j];
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) ls += __shfl_xor(ls, off);
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) o[lane + 64 * j] = from_f32<T>(ls == 0.f ? 0.f : a[j] / ls);
 }
 
 // Blocks that one sequence's query can see at most.
@@ -794,12 +815,13 @@ int64_t most_blocks(int64_t cap, int window, int sinks) {
 
 int heads_per_pair(int n_head, int n_kv) { return n_head / n_kv < 8 ? n_head / n_kv : 8; }
 
+constexpr size_t kWordsBytes = (size_t)kMaxShares * 2 * sizeof(uint64_t);
 size_t ws_ml_bytes(int hpp) { return (size_t)kMaxShares * 2 * hpp * 2 * sizeof(float); }
 
 // A workgroup for each pair, which finishes it: no partial results, one launch.  Taken where the longest pair
 // there can be (pair_bytes of K and V) is short: one CU streams it.  us a call as pairs / as shares, 250 KB a pair,
-// 16 bits: 5 pairs 13.2 / 9.6, 40 pairs 13.5 / 12.3, 64 (d_k 128) 12.9 / 14.2, 96 (MHA) 10.5 / 13.7, 160 15.2 / 17.7; 350 KB: 32
-// 15.1 / 12.9, 128 16.4 / 17.8, 24 (fp32) 12.5 / 11.4; 126 KB: 320 13.9 / 17.8; 50 KB: 8 7.0 / 10.0, 128 7.7 / 10.8.
+// 16 bits: 5 pairs 13.2 / 9.0, 40 pairs 13.5 / 12.0, 64 (d_k 128) 12.3 / 13.5, 96 (MHA) 10.8 / 13.4, 160 14.3 / 17.6;
+// 350 KB: 32 15.1 / 12.3, 128 16.1 / 17.0, 24 (fp32) 12.5 / 10.7; 126 KB: 320 13.8 / 16.2; 50 KB: 8 7.1 / 9.2, 128 7.8 / 9.7.
 bool pair_mode(const DecodeParams& p, int64_t pair_bytes) {
   const int64_t pairs = (int64_t)p.batch * p.n_pairs;
   return !tl_overrides.decode_shares && pair_bytes <= kPairMaxBytes && pair_bytes * pairs <= kPairMaxAll &&
@@ -830,10 +852,8 @@ int launch_decode_g(DecodeParams& p, int64_t most, hipStream_t st) {
   const int64_t pairs = (int64_t)p.batch * p.n_pairs;
   const int64_t full = (most + kMinShare - 1) / kMinShare + pairs;
   p.n_shares = (int)(shares < full ? shares : full);
+  p.tag = tl_arrival_tag();
   hipLaunchKernelGGL((paged_decode_kernel<T, D, G, kDecWaves, 1, false>), dim3(p.n_shares), dim3(kDecThreads), 0, st, p);
-  const int e = tl_launch_status();
-  if (e) return e;
-  hipLaunchKernelGGL((paged_combine_kernel<T, D>), dim3(p.n_head, p.batch), dim3(64), 0, st, p);
   return tl_launch_status();
 }
 
@@ -978,7 +998,7 @@ int tl_paged_kv_append(const void* q, void* q_out, const void* k_new, const void
 size_t tl_paged_decode_workspace_bytes(int n_head, int n_kv_head, int d_k) {
   if (n_head <= 0 || n_kv_head <= 0 || n_head % n_kv_head || d_k <= 0) return 0;
   const int hpp = heads_per_pair(n_head, n_kv_head);
-  return ws_ml_bytes(hpp) + (size_t)kMaxShares * 2 * hpp * d_k * sizeof(float);
+  return kWordsBytes + ws_ml_bytes(hpp) + (size_t)kMaxShares * 2 * hpp * d_k * sizeof(float);
 }
 
 int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
@@ -996,7 +1016,7 @@ int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_
   const int64_t cap = (int64_t)max_pages << (shift < 0 ? 0 : shift);
   if (shift < 0 || cap > INT32_MAX) return TL_ERR_INVALID;
   if (d_k != 64 && d_k != 128) return TL_ERR_UNSUPPORTED;
-  if (batch > 65535) return TL_ERR_UNSUPPORTED;  // the combine's grid
+  if (batch > 65535) return TL_ERR_UNSUPPORTED;
   if (workspace_bytes < tl_paged_decode_workspace_bytes(n_head, n_kv_head, d_k)) return TL_ERR_INVALID;
   // a lane reads d_k / 16 elements of a row in 8- or 16-byte words, a block of 16 rows with 32-bit offsets
   const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
@@ -1023,8 +1043,9 @@ int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_
   p.group = n_head / n_kv_head;
   p.heads_per_pair = heads_per_pair(n_head, n_kv_head);
   p.n_pairs = n_kv_head * ((p.group + p.heads_per_pair - 1) / p.heads_per_pair);
-  p.ws_ml = (float*)workspace;
-  p.ws_acc = (float*)((char*)workspace + ws_ml_bytes(p.heads_per_pair));
+  p.words = (uint64_t*)workspace;
+  p.ws_ml = (float*)((char*)workspace + kWordsBytes);
+  p.ws_acc = (float*)((char*)workspace + kWordsBytes + ws_ml_bytes(p.heads_per_pair));
   p.q_sb = q_strides[0], p.q_sh = q_strides[1];
   p.o_sb = o_strides[0], p.o_sh = o_strides[1];
   p.k_sp = k_page_strides[0], p.k_sh = k_page_strides[1];

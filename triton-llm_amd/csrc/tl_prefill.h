@@ -133,5 +133,3 @@ __host__ __device__ inline int sched_rank(const FlashParams& p, int j, int r) {
 int launch_flash_w64(FlashParams& p, int dtype, bool causal, hipStream_t st);
 
 }  // namespace tlp
-
-uint64_t tl_arrival_tag();
