@@ -32,7 +32,6 @@ constexpr int kThreads = 256;
 constexpr int kBM = 128;  // query rows of a workgroup
 constexpr int kMinShare = 4;  // key tiles of a part at least
 constexpr int kWaveParts = 4;  // parts of a row tile that the waves join themselves
-constexpr float kRescaleLog2 = 8.f;
 constexpr int kMostRows = 1 << 28;     // query rows of a sequence
 constexpr int kWholeWindow = 3 << 29;  // positions lie in [-2^28, 2^30 + 2^28): a window this long hides nothing, and
                                        // below it position - window fits in 32 bits
@@ -109,6 +108,12 @@ struct Tile16 {
   // The sum of a row's weights.  At d_k 64 the vector unit is the limit and the matrix unit half idle: there it is one
   // more MFMA per 16 keys, ones . P^T, of the rounded weights (4 x 500 rows on prefixes, fp16: 51.4 -> 47.8 us).
   static constexpr bool kSumMfma = D == 64;
+  // Weights are rounded to the storage type for the second product.  A weight is 2^kLift times exp2 of its score's
+  // distance to the running maximum, and that lags behind the largest score by kRescale at most.  bf16 has fp32's exponents:
+  // half a step each.  fp16 ends at 2^16 and is subnormal below 2^-14: lifted by 2^11 a weight is at most 2^15, has half a
+  // step down to 2^-25 of the row's largest, and below that an error of 2^-36 of it at most.
+  static constexpr float kLift = T::code == TL_DTYPE_F16 ? 11.f : 0.f;
+  static constexpr float kRescale = T::code == TL_DTYPE_F16 ? 4.f : 8.f;
   static __device__ __forceinline__ void scores(f32x16 (&s)[NMB], const Q& q, const char* kt, int lq, int h) {
     constexpr int NG = NMB * NKS;
     const char* row = kt + lq * ROWB;
@@ -130,8 +135,9 @@ struct Tile16 {
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // s holds the probabilities; they are rounded to the storage type here (at most half a step
-  // each, as the causal prefill does), the sum l is of the unrounded ones.
+  // s holds the weights; they are rounded to the storage type here (see kLift).  The sum of a row's weights is
+  // of the rounded ones in la (kSumMfma) and of the unrounded ones in l otherwise, in fp32 either way: a weight's rounding
+  // then counts in numerator and denominator, or in the numerator alone, half a step of the output at most in both.
   static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt,
                                                 int lane) {
     typedef short v4s __attribute__((ext_vector_type(4)));
@@ -175,6 +181,7 @@ template <int D>
 struct Tile32 {
   static constexpr int ROWB = D * 4, NDB = D / 32, NMB = 1;
   static constexpr bool kSumMfma = false;
+  static constexpr float kLift = 0.f, kRescale = 8.f;
   struct Q {
     float f[D / 2];  // features h D / 2 .. of the row
   };
@@ -549,8 +556,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
       for (int r = 0; r < 16; r += 2)
         mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, s[mb][r]), s[mb][r + 1]);
     mx = tlp::max_xor32(mx) * scale;
-    // the maximum moves only when a score passes it by 2^8 (it only bounds the exponents)
-    if (__any(mx > m + kRescaleLog2)) {
+    // the maximum moves only when a score passes it by kRescale (it only bounds the exponents)
+    if (__any(mx > m + TL::kRescale)) {
       const float mn = fmaxf(m, mx);
       const float a = fast_exp2(m - (mn == -INFINITY ? 0.f : mn));
       m = mn;
@@ -564,7 +571,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= a;
     }
-    const float shift = m == -INFINITY ? 0.f : m;
+    const float shift = m == -INFINITY ? 0.f : m - TL::kLift;
 #pragma unroll
     for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
