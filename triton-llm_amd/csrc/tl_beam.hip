@@ -4,11 +4,10 @@
 // the sampler that replaces its _sample (smollm2_triton/model.py:566-584).
 //
 // Scores are ordered in 64 bits: neighbours of different beams may differ by less than a 32-bit step of
-// their size.  x - max and exp are 32-bit (the argument of exp2 carried in two words, so that its
-// rounding does not grow with the distance from the maximum), their sum 64.
+// their size.  exp, its sums and the logarithm are 64-bit too (see exp_below).
 //
-// Bytes: every logit is read once, by beam_scan, a wave a segment of 1024 entries of a row (16 x 8 x 128256 bf16, 33 MB:
-// 10.4 us, 3.2 TB/s; with segments of 2048 and 4096 entries a call took 3 and 9 us more), which leaves
+// Every logit is read once, by beam_scan, a wave a segment of 1024 entries of a row, bound by the 64-bit operations of exp
+// (16 x 8 x 128256 bf16, 33 MB: 15.8 us, 2.1 TB/s; with a 32-bit exp 10.4; with segments of 2048 and 4096 entries a call took 3 and 9 us more), which leaves
 //   * the segment's maximum and its sum of exp against it;
 //   * the maximum of every group of 64 entries.
 // beam_finish, a workgroup a batch item, has everything else from those.  The best score in a unit (a segment, or
@@ -68,16 +67,29 @@ typedef uint32_t words32 __attribute__((ext_vector_type(4), aligned(4)));
 
 size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 
-// exp(x - m) for x <= m; 0 where it is under the smallest 32-bit number, NaN for NaN (the IEEE maximum
-// passes it on).
-__device__ __forceinline__ float exp_below(float x, float m) {
-  constexpr float kL = 1.44269504f, kLlo = 1.92596303e-8f;  // log2 e in two words
-  const float d = __builtin_elementwise_maximum(x - m, -126.f);
-  const float hi = d * kL;
-  const float lo = fmaf(d, kLlo, fmaf(d, kL, -hi));
-  const float e = fast_exp2(hi);
-  return fmaf(e * 0.693147181f, lo, e);
+// exp(x - m) for x <= m, to 2^-45 of it (any finite number for NaN).  In 64 bits throughout: continuations of different
+// beams are ordered by their rows' log-sum-exp, and an error that all entries of a flat floor share does not average
+// out (in 32 bits it reached 5e-7).  d log2 e = n + f with whole n and |f| <= 1/2; 2^f by its interpolation of degree 9 at the
+// Chebyshev points; n goes into the exponent.  Below e^-700 it is e^-700, which no sum with a 1 in it notices.
+// 64-bit products take no longer than 32-bit ones here; their number is what counts (degree 11 and a clamp that keeps
+// NaN: 16 x 8 x 128256 27.3 us a call, so 24.9).
+__device__ __forceinline__ double exp_below(float x, double m) {
+  constexpr double kL = 1.4426950408889634;
+  constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: added, a number's whole part stands in its low bits
+  constexpr double c[] = {1.0000000000000135,     6.9314718055994617e-01, 2.4022650695640341e-01, 5.5504108664651670e-02,
+                          9.6181291939343126e-03, 1.3333558200794592e-03, 1.5403433751251010e-04, 1.5252672924850737e-05,
+                          1.3259645244887111e-06, 1.0205905413765595e-07};
+  const double d = fmax((double)x - m, -700.);
+  const double t = fma(d, kL, kRound);
+  const double f = fma(d, kL, kRound - t);
+  double e = c[9];
+#pragma unroll
+  for (int k = 8; k >= 0; --k) e = fma(e, f, c[k]);
+  return __builtin_ldexp(e, (int)__builtin_bit_cast(uint64_t, t));
 }
+
+// The IEEE maximum: NaN where either is.
+__device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // kVec neighbouring entries of a row from i on, -inf behind its end.
 template <typename T>
@@ -168,30 +180,27 @@ __global__ __launch_bounds__(kST) void beam_scan_kernel(BeamParams p) {
   const int i0 = seg * kSeg + lane * kVec;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) load_vec<T>(v[k], x, i0 + k * 64 * kVec, p.vocab);
+  // NaN anywhere makes the segment's maximum NaN, by which the row's log-sum-exp is one too
   float m = -INFINITY;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
     float g = v[k][0];
 #pragma unroll
-    for (int e = 1; e < kVec; ++e) g = fmaxf(g, v[k][e]);
+    for (int e = 1; e < kVec; ++e) g = max_or_nan(g, v[k][e]);
 #pragma unroll
-    for (int off = 1; off < 8; off <<= 1) g = fmaxf(g, __shfl_xor(g, off));
+    for (int off = 1; off < 8; off <<= 1) g = max_or_nan(g, __shfl_xor(g, off));
     const int i = i0 + k * 64 * kVec;
     if ((lane & 7) == 0 && i < p.vocab) p.gmax[(int64_t)row * p.n_grp + i / kGrp] = g;
-    m = fmaxf(m, g);
+    m = max_or_nan(m, g);
   }
 #pragma unroll
-  for (int off = 8; off < 64; off <<= 1) m = fmaxf(m, __shfl_xor(m, off));
-  // a segment of -inf alone has no mass; NaN in it comes through the maximum as -inf
-  const float base = m == -INFINITY ? 0.f : m;
+  for (int off = 8; off < 64; off <<= 1) m = max_or_nan(m, __shfl_xor(m, off));
+  const double base = m == -INFINITY ? 0. : (double)m;  // a segment of -inf alone has no mass
   double s = 0.;
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    float e = 0.f;
+  for (int k = 0; k < kVecs; ++k)
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) e += exp_below(v[k][i], base);
-    s += e;
-  }
+    for (int i = 0; i < kVec; ++i) s += exp_below(v[k][i], base);
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
   if (lane == 0) {
@@ -265,7 +274,7 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (64 * k >= p.n_seg) break;
-      s += sx[k] == -INFINITY ? part[k] : part[k] * exp((double)sx[k] - (double)m);  // (a NaN's sum comes through)
+      s += sx[k] == -INFINITY ? part[k] : part[k] * exp((double)sx[k] - (double)m);  // NaN for NaN and +inf
     }
     s = wave_sum(s);
     if (lane == 0) {
