@@ -30,12 +30,6 @@ static inline int page_shift(int page_size) {
   return __builtin_ctz((unsigned)page_size);
 }
 
-// Which keys a query at position `pos` sees: j <= pos, and behind a window (> 0) of them
-// only the last `window` and the first `sinks` of the sequence.
-__host__ __device__ __forceinline__ bool key_seen(int j, int pos, int window, int sinks) {
-  return j <= pos && (window <= 0 || j > pos - window || j < sinks);
-}
-
 // Values equal on every lane, moved to scalar registers.
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uni(int64_t x) {
