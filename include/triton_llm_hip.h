@@ -381,7 +381,8 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * read.  Where several workgroups share a sequence's positions the workspace
  * (tl_paged_decode_workspace_bytes, 16-byte aligned, given either way) holds their
  * results and needs no initialisation; calls that overlap in time need
- * one each.  d_k 64 or 128, rows aligned to d_k / 16 elements; batch <= 65535, and
+ * one each.  o may be q (the same layout and address), and overlaps none of q, k, v
+ * otherwise.  d_k 64 or 128, rows aligned to d_k / 16 elements; batch <= 65535, and
  * at most 2^31 - 1 blocks of 16 positions over batch, KV heads and pages.
  *
  * tl_paged_attention_prefill: n_new queries per sequence (new_lens[b] where it is
@@ -391,7 +392,8 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * tl_window_attention: the same over K / V (batch, n_kv_head, seq_k, d_k)
  * {batch, head, seq}, query i at position seq_k - seq_q + i.
  * Both: window = 0 is plain causal attention; a row that sees no key gives zeros;
- * d_k 64 or 128, rows of q, k and v 16-byte aligned; o may not overlap q, k or v.
+ * d_k 64 or 128, rows of q, k and v 16-byte aligned; o may not overlap q, k or v
+ * (refused; rows side by side in one buffer do not overlap).
  * With few rows the keys are shared by several workgroups, whose results lie in the
  * workspace (tl_window_workspace_bytes bytes, 16-byte aligned, most_keys = seq_k, or
  * max_pages * page_size; no initialisation; calls that overlap in time need one each)

@@ -11,6 +11,7 @@
 
 #include "tl_common.h"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace tlpg {
@@ -28,6 +29,50 @@ struct PageMap {
 static inline int page_shift(int page_size) {
   if (page_size < kMinPage || page_size > kMaxPage || (page_size & (page_size - 1))) return -1;
   return __builtin_ctz((unsigned)page_size);
+}
+
+// A tensor of rows of `row` bytes at base + i0 s0 + i1 s1 + i2 s2, i_k < n[k], strides s[k] in bytes.
+struct Rows3 {
+  const void* base;
+  int64_t n[3], s[3], row;
+  Rows3 upward() const {  // the same rows from the lowest on
+    Rows3 t = *this;
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0) t.base = (const char*)t.base + (n[i] - 1) * s[i], t.s[i] = -s[i];
+    return t;
+  }
+  // bytes from the first to behind the last of what the dims of strides below m span
+  int64_t span(int64_t m) const {
+    int64_t e = row;
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < m) e += (n[i] - 1) * s[i];
+    return e;
+  }
+};
+
+// Whether two such tensors may share a byte.  Not if their spans do not meet, nor if they lie side by side in the rows of one
+// buffer: all strides from some size on are multiples of m, and what the smaller ones span is apart modulo m.
+static inline bool rows_overlap(const Rows3& x, const Rows3& y) {
+  const Rows3 a = x.upward(), b = y.upward();
+  if (!tl_overlap(a.base, (size_t)a.span(INT64_MAX), b.base, (size_t)b.span(INT64_MAX))) return false;
+  for (const Rows3* t : {&a, &b})
+    for (int i = 0; i < 3; ++i) {
+      const int64_t least = t->s[i];
+      if (t->n[i] < 2 || least < 1) continue;
+      int64_t m = 0;
+      for (const Rows3* u : {&a, &b})
+        for (int k = 0; k < 3; ++k)
+          if (u->n[k] > 1 && u->s[k] >= least)
+            for (int64_t d = u->s[k]; d;) {  // m = gcd(m, d)
+              const int64_t r = m % d;
+              m = d;
+              d = r;
+            }
+      const int64_t ea = a.span(least), eb = b.span(least);
+      const int64_t from_a = (int64_t)(((uintptr_t)b.base % m + m - (uintptr_t)a.base % m) % m);  // a's start to b's
+      if (ea <= from_a && eb <= m - from_a) return false;
+    }
+  return true;
 }
 
 // Values equal on every lane, moved to scalar registers.

@@ -1027,6 +1027,16 @@ int tl_paged_attention_decode(const void* q, const void* k_pages, const void* v_
     if (s < 0 || s % slice) return TL_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages) % (uintptr_t)(slice * esize)) return TL_ERR_UNSUPPORTED;
   if (k_page_strides[2] > (1 << 24) || v_page_strides[2] > (1 << 24)) return TL_ERR_UNSUPPORTED;
+  // o may be q, as every head's q is read before its o is written
+  auto rows = [&](const void* at, int64_t n0, int64_t n1, int64_t n2, int64_t s0, int64_t s1, int64_t s2) {
+    return Rows3{at, {n0, n1, n2}, {s0 * esize, s1 * esize, s2 * esize}, (int64_t)d_k * esize};
+  };
+  const Rows3 out = rows(o, batch, n_head, 1, o_strides[0], o_strides[1], 0);
+  const bool is_q = o == q && o_strides[0] == q_strides[0] && o_strides[1] == q_strides[1];
+  auto pool = [&](const void* at, const int64_t* s) { return rows(at, n_pages, n_kv_head, page_size, s[0], s[1], s[2]); };
+  if ((!is_q && rows_overlap(out, rows(q, batch, n_head, 1, q_strides[0], q_strides[1], 0))) ||
+      rows_overlap(out, pool(k_pages, k_page_strides)) || rows_overlap(out, pool(v_pages, v_page_strides)))
+    return TL_ERR_INVALID;
   DecodeParams p{};
   p.q = q;
   p.k = k_pages;

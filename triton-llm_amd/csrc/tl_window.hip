@@ -816,6 +816,16 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
   p.k_sb = ks[0], p.k_sh = ks[1], p.k_ss = ks[2];
   p.v_sb = vs[0], p.v_sh = vs[1], p.v_ss = vs[2];
   p.o_sb = os[0], p.o_sh = os[1], p.o_ss = os[2];
+  // a workgroup writes o while others still read q, k and v
+  const int64_t row = (int64_t)d_k * esize;
+  auto rows = [&](const void* at, int64_t n0, int64_t n1, int64_t n2, const int64_t* s) {
+    return Rows3{at, {n0, n1, n2}, {s[0] * esize, s[1] * esize, s[2] * esize}, row};
+  };
+  const int64_t n0 = paged ? p.pm.n_pages : p.batch, n2 = paged ? (int64_t)1 << p.pm.shift : p.seq_k;
+  const Rows3 out = rows(p.o, p.batch, p.n_head, p.seq_q, os);
+  if (rows_overlap(out, rows(p.q, p.batch, p.n_head, p.seq_q, qs)) || rows_overlap(out, rows(p.k, n0, p.n_kv, n2, ks)) ||
+      rows_overlap(out, rows(p.v, n0, p.n_kv, n2, vs)))
+    return TL_ERR_INVALID;
   p.group = p.n_head / p.n_kv;
   if (!rows_ok(p.seq_q, p.group)) return TL_ERR_UNSUPPORTED;
   p.group_magic = (uint32_t)((((uint64_t)1 << 32) + p.group - 1) / p.group);
