@@ -30,6 +30,7 @@ ziliangpeng/triton-llm: ``DeviceTensor`` :184-227, ``allocate`` :230,
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import os
 import threading
@@ -82,6 +83,24 @@ def _detect_backend() -> str:
     return "hip"
 
 
+_device_plans: list = []
+
+
+def plan_cache(maxsize: int):
+    """An ``lru_cache`` for answers of the library that depend on the device and its overrides (workspace
+    sizes): emptied when either is read again."""
+    def keep(fn):
+        cached = functools.lru_cache(maxsize=maxsize)(fn)
+        _device_plans.append(cached)
+        return cached
+    return keep
+
+
+def _forget_plans():
+    for p in _device_plans:
+        p.cache_clear()
+
+
 _initialized = False
 _backend = None
 _rt = None
@@ -103,6 +122,7 @@ def _initialize():
         )
     device = int(os.environ.get("TRITON_LLM_DEVICE", "0"))
     check_error(lib.tl_init(device))
+    _forget_plans()
     _rt = lib
     _initialized = True
 
@@ -114,6 +134,7 @@ def reload_overrides():
     TRITON_LLM_HIP_PREFILL_NO_SPLIT), which it reads
     in tl_init, never per launch.  Does nothing before the first GPU use."""
     if _initialized:
+        _forget_plans()
         check_error(_rt.tl_init(int(os.environ.get("TRITON_LLM_DEVICE", "0"))))
 
 

@@ -211,7 +211,7 @@ def paged_decode_workspace(batch: int, n_head: int, n_kv_head: int, max_ctx: int
     return gpu.allocate((gpu.runtime().tl_paged_decode_workspace_bytes(n_head, n_kv_head, d_k),), np.uint8)
 
 
-@functools.lru_cache(maxsize=1024)
+@gpu.plan_cache(1024)
 def _attention_plan(pool, v_pool, table, lens, new_lens, q, n_head, n_kv_head, window, sinks, prefill):
     """Strides and sizes of an attention call by its shapes."""
     n_pages, n_kv, page_size, d_k = _check_pool(pool, v_pool)

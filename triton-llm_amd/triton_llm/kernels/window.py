@@ -19,7 +19,7 @@ from ._common import contiguous_strides, default_scale, launch, scratch
 from .paged import check_window, dtype_code_of
 
 
-@functools.lru_cache(maxsize=1024)
+@gpu.plan_cache(1024)
 def _strided_plan(batch, n_head, n_kv_head, seq_q, seq_k, d_k, q_strides, k_strides, v_strides, o_strides, window, sinks):
     """The C entry's sizes and strides in their order, and its workspace's bytes by dtype code."""
     if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head:
