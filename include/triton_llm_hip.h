@@ -389,14 +389,18 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * not NULL; rows behind them are left as they were), query i at position
  * cache_lens[b] + i (lengths past 2^30 count as 2^30), over the pages (their own positions appended before), with
  * the same window.  q / o (batch, n_new, n_head, d_k) {batch, head, seq}.
+ * tl_paged_attention_prefill_counted: the same where the host has new_lens's values too, host_new_lens (batch; read
+ * before the call returns; NULL: as without).  How the work is shared then goes by the rows there are, else as if
+ * every sequence had n_new.  Where new_lens holds more than host_new_lens, rows may be left as they were; a captured
+ * call does not use it, as its replays may come with other values.
  * tl_window_attention: the same over K / V (batch, n_kv_head, seq_k, d_k)
  * {batch, head, seq}, query i at position seq_k - seq_q + i.
  * Both: window = 0 is plain causal attention; a row that sees no key gives zeros;
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; o may not overlap q, k or v
  * (refused; rows side by side in one buffer do not overlap).
  * With few rows the keys are shared by several workgroups, whose results lie in the
- * workspace (tl_window_workspace_bytes bytes, 16-byte aligned, most_keys = seq_k, or
- * max_pages * page_size; no initialisation; calls that overlap in time need one each)
+ * workspace (tl_window_workspace_bytes bytes, or with host_new_lens
+ * tl_paged_prefill_workspace_bytes, 16-byte aligned, most_keys = seq_k, or max_pages * page_size; no initialisation; calls that overlap in time need one each)
  * and are joined by the last of them or by a second launch;
  * given less (NULL: none) the call runs in one.  Either is deterministic.
  * (n_new or seq_q) <= 2^28, seq_k <= 2^29, and times the square of n_head / n_kv_head below 2^32.
@@ -440,6 +444,17 @@ int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v
                                const int64_t* q_strides, const int64_t* k_page_strides,
                                const int64_t* v_page_strides, const int64_t* o_strides,
                                float sm_scale, int window, int sinks, int dtype, void* stream);
+int tl_paged_attention_prefill_counted(const void* q, const void* k_pages, const void* v_pages,
+                                       const int32_t* page_table, int max_pages, int n_pages,
+                                       int page_size, const int32_t* cache_lens, const int32_t* new_lens,
+                                       const int32_t* host_new_lens, void* o, void* workspace,
+                                       size_t workspace_bytes, int batch, int n_new, int n_head,
+                                       int n_kv_head, int d_k, const int64_t* q_strides,
+                                       const int64_t* k_page_strides, const int64_t* v_page_strides,
+                                       const int64_t* o_strides, float sm_scale, int window, int sinks,
+                                       int dtype, void* stream);
+size_t tl_paged_prefill_workspace_bytes(const int32_t* host_new_lens, int batch, int n_head, int n_kv_head, int n_new,
+                                        int most_keys, int d_k, int window, int sinks, int dtype);
 size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q, int most_keys,
                                  int d_k, int window, int sinks, int dtype);
 int tl_window_attention(const void* q, const void* k, const void* v, void* o, void* workspace,

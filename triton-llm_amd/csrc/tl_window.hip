@@ -48,6 +48,8 @@ struct WinParams {
   uint32_t group_magic;  // row / group = mulhi(row, group_magic) for the rows there are (group > 1)
   int window, sinks;
   int slots;           // workgroups that the keys are shared by; 0: a row tile's keys are not divided
+  int room;            // parts that there may be (slots > 0): the workspace holds as many, the grid has as many workgroups
+  int key_cap;         // key tiles of a row tile count as this many at most, so that their sum fits in 32 bits
   int q_shift, n_lvl, xcd_groups;  // how workgroups are dealt (window_fwd_kernel)
   int vec_out;         // o's rows take 4 elements at once
   uint64_t tag;        // this call's, where the waves join the parts; 0: window_join_kernel does
@@ -292,7 +294,7 @@ __device__ __forceinline__ Seq seq_at(const WinParams& p, int b) {
   if (b < p.batch) {
     s.r = rows_of<PAGED>(p, b);
     s.tiles = (s.r.nq * p.group + kBM - 1) / kBM;
-    if (s.tiles) s.keys = min(keys_of<BN>(p, s.r, s.tiles - 1).tiles, 1 << 20);
+    if (s.tiles) s.keys = min(keys_of<BN>(p, s.r, s.tiles - 1).tiles, p.key_cap);
   }
   return s;
 }
@@ -303,7 +305,6 @@ struct Deal {
 };
 template <int BN, bool PAGED>
 __device__ __forceinline__ Deal deal_of(const WinParams& p, int lane) {
-  // the sums are over few row tiles (the host divides no others), of at most 2^20 key tiles
   Deal d;
   d.s = seq_at<BN, PAGED>(p, lane);
   int work = last_lane(wave_scan(d.s.tiles * d.s.keys)), tiles = last_lane(wave_scan(d.s.tiles));
@@ -316,13 +317,24 @@ __device__ __forceinline__ Deal deal_of(const WinParams& p, int lane) {
   const int aim = max(p.slots - tiles * p.n_kv, p.slots / 2);
   // rounded up past the 32-bit quotient's error
   d.share = max((int)((float)work * (float)p.n_kv * __builtin_amdgcn_rcpf((float)aim) * 1.00001f) + 1, kMinShare);
-  d.s.cut(p, d.share);
-  d.incl = wave_scan(d.s.all);
-  d.total = last_lane(d.incl);
-  for (int b0 = 64; b0 < p.batch; b0 += 64) {
-    Seq t = seq_at<BN, PAGED>(p, b0 + lane);
-    t.cut(p, d.share);
-    d.total += last_lane(wave_scan(t.all));
+  constexpr int kWhole = 1 << 30;
+  while (true) {
+    int longest = d.s.keys;
+    d.s.cut(p, d.share);
+    d.incl = wave_scan(d.s.all);
+    d.total = last_lane(d.incl);
+    for (int b0 = 64; b0 < p.batch; b0 += 64) {
+      Seq t = seq_at<BN, PAGED>(p, b0 + lane);
+      longest = max(longest, t.keys);
+      t.cut(p, d.share);
+      d.total += last_lane(wave_scan(t.all));
+    }
+    // Row tiles stay whole where their parts would take two rounds of the workgroups and two parts be as long as
+    // the longest (sequences of 2 x share - 1 tiles and fewer beside short ones: 31 tokens on 4000 keys beside a prompt of 100,
+    // 24 / 8 heads of 128, 99 us, cut in two 126), and where there is no room for the parts: more rows than the host said.
+    if (d.share == kWhole || (d.total <= p.slots && d.total <= p.room)) break;
+    if (d.total <= p.room && __any(longest > 2 * d.share)) break;
+    d.share = kWhole;
   }
   return d;
 }
@@ -695,6 +707,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
   const int qt = tile - kvh * p.n_qt;
   const int b = kvh / p.n_kv;
   const int hkv = kvh - b * p.n_kv;
+  if (qt * kBM >= rows_of<PAGED>(p, b).nq * p.group) return;
   const Deal d = deal_of<BN, PAGED>(p, lane);
   Seq s;
   const int incl = parts_upto<BN, PAGED>(p, d, b & ~63, lane, s);
@@ -751,14 +764,27 @@ int64_t most_tiles(int64_t keys, int window, int sinks, int group, int bn) {
 // workgroups as fit (1 x 500 rows on 4000 keys, 24 / 8 heads, d_k 128: fp16 39.6 us, one a CU 47; fp32 at 300 rows on
 // 2000 keys 86 and 98); fp32 at d_k 64 is bound by its matrix products, which one workgroup a CU keeps busy (1023
 // rows, window 256: 25.0 us, with two 30.1).  Returns the most parts there can be (0: undivided).
-int64_t plan_slots(WinParams& p, int64_t keys, int d_k, int esize) {
+int64_t plan_slots(WinParams& p, int64_t tiles, int64_t keys, int d_k, int esize) {
   const int bn = esize == 2 ? 64 : 32;
   const int64_t most = most_tiles(keys, p.window, p.sinks, p.group, bn);
-  const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
   const int64_t slots = (int64_t)tl_device_cus() * (d_k == 128 ? 2 : esize == 4 ? 1 : 3);
-  p.slots = tiles >= slots || most < 2 * kMinShare ? 0 : (int)slots;
+  p.slots = tiles < 1 || tiles >= slots || most < 2 * kMinShare ? 0 : (int)slots;
   const int64_t parts = tiles * ((most + kMinShare - 1) / kMinShare);
   return !p.slots ? 0 : parts < 2 * slots + tiles ? parts : 2 * slots + tiles;
+}
+
+// The call's row tiles: by the rows that the sequences have where the host knows them (counts), else as if all had seq_q.  A
+// padded batch planned by seq_q is taken for one with many row tiles, and its keys stay whole: one sequence of 500 rows on 4000
+// keys among 8 slots, 24 / 8 heads of 128, 41.1 us by its rows, 108 by seq_q (alone 39.5); beside seven tokens on 16000 keys
+// 94 and 320.
+int64_t row_tiles(const WinParams& p, const int32_t* counts) {
+  if (!counts) return (int64_t)p.batch * p.n_kv * p.n_qt;
+  int64_t n = 0;
+  for (int b = 0; b < p.batch; ++b) {
+    const int64_t rows = counts[b] < 0 ? 0 : counts[b] < p.seq_q ? counts[b] : p.seq_q;
+    n += (rows * p.group + kBM - 1) / kBM;
+  }
+  return n * p.n_kv;
 }
 
 // Rows that token_of() divides exactly: the magic's excess, below group, times a row stays below 2^32.  (Rows of the
@@ -770,7 +796,7 @@ size_t words_bytes(int64_t parts) { return ((size_t)parts * 4 * sizeof(uint64_t)
 size_t part_bytes(int d_k) { return (d_k == 64 ? part_floats<64>() : part_floats<128>()) * sizeof(float); }
 
 template <typename T, int D>
-int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) {
+int launch_window(WinParams& p, bool paged, hipStream_t st) {
   const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
   if (tiles > (1 << 27)) return TL_ERR_UNSUPPORTED;
   const int64_t units = (int64_t)p.batch * p.n_kv;
@@ -778,7 +804,7 @@ int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) 
   while (p.q_shift > 0 && units % (16 >> p.q_shift) == 0) --p.q_shift;
   p.n_lvl = (p.n_qt + (1 << p.q_shift) - 1) >> p.q_shift;
   p.xcd_groups = (int)((units << p.q_shift) / 8);
-  const dim3 grid(p.slots > 0 ? (unsigned)((most_parts + 7) / 8 * 8) : (unsigned)(8 * p.xcd_groups * p.n_lvl));
+  const dim3 grid(p.slots > 0 ? (unsigned)((p.room + 7) / 8 * 8) : (unsigned)(8 * p.xcd_groups * p.n_lvl));
   if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
   else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
   const int e = tl_launch_status();
@@ -790,11 +816,11 @@ int launch_window(WinParams& p, bool paged, int64_t most_parts, hipStream_t st) 
 }
 
 template <typename T>
-int launch_window_d(WinParams& p, bool paged, int d_k, int64_t most_parts, hipStream_t st) {
-  return d_k == 64 ? launch_window<T, 64>(p, paged, most_parts, st) : launch_window<T, 128>(p, paged, most_parts, st);
+int launch_window_d(WinParams& p, bool paged, int d_k, hipStream_t st) {
+  return d_k == 64 ? launch_window<T, 64>(p, paged, st) : launch_window<T, 128>(p, paged, st);
 }
 
-int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t workspace_bytes, int d_k,
+int window_entry(WinParams& p, bool paged, int64_t keys, const int32_t* counts, void* workspace, size_t workspace_bytes, int d_k,
                  const int64_t* qs, const int64_t* ks, const int64_t* vs, const int64_t* os, float sm_scale, int dtype, void* stream) {
   if (!p.q || !p.k || !p.v || !p.o || !qs || !ks || !vs || !os || p.batch < 0 || p.n_head < 0 || p.n_kv < 1 ||
       p.n_head % p.n_kv || p.seq_q < 0 || p.window < 0 || p.sinks < 0)
@@ -832,24 +858,31 @@ int window_entry(WinParams& p, bool paged, int64_t keys, void* workspace, size_t
   p.n_qt = (p.seq_q * p.group + kBM - 1) / kBM;
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.vec_out = ((uintptr_t)p.o % (4 * esize)) == 0 && os[0] % 4 == 0 && os[1] % 4 == 0 && os[2] % 4 == 0;
-  const int64_t most_parts = plan_slots(p, keys, d_k, esize);
+  hipStream_t st = tl_resolve_stream(stream);
+  if (counts) {  // a graph's replays may come with other counts
+    hipStreamCaptureStatus c;
+    if (hipStreamIsCapturing(st, &c) != hipSuccess || c != hipStreamCaptureStatusNone) counts = nullptr;
+  }
+  const int64_t tiles = row_tiles(p, counts);
+  const int64_t most_parts = plan_slots(p, tiles, keys, d_k, esize);
   if (p.slots > 0) {
+    p.room = (int)most_parts;
+    const int64_t cap = INT32_MAX / ((int64_t)p.batch * p.n_qt);
+    p.key_cap = (int)(cap < (1 << 20) ? cap : 1 << 20);
     // without room for the parts the keys stay undivided
     if (!workspace || workspace_bytes < words_bytes(most_parts) + (size_t)most_parts * part_bytes(d_k) || ((uintptr_t)workspace & 15)) p.slots = 0;
     // Few parts are joined by the wave that ends last, without a second launch; many would be added up one after the
     // other by one wave.  us joined by the waves / by a second launch: 1023 rows, window 256, fp32 (2 parts) 25.0 / 26.2,
     // 4 x 500 rows on prefixes (3 parts) 43.5 / 44.8; 500 rows on 4000 keys, d_k 128 (5 parts) 43.7 / 39.6, 100 rows (21
     // parts) 40.7 / 27.6.
-    const int64_t tiles = (int64_t)p.batch * p.n_kv * p.n_qt;
     p.tag = p.slots <= kWaveParts * tiles ? tl_arrival_tag() : 0;
     p.words = (uint64_t*)workspace;
     p.ws = (float*)((char*)workspace + words_bytes(most_parts));
   }
-  hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
-    case TL_DTYPE_F32: return launch_window_d<F32>(p, paged, d_k, most_parts, st);
-    case TL_DTYPE_F16: return launch_window_d<F16>(p, paged, d_k, most_parts, st);
-    default: return launch_window_d<BF16>(p, paged, d_k, most_parts, st);
+    case TL_DTYPE_F32: return launch_window_d<F32>(p, paged, d_k, st);
+    case TL_DTYPE_F16: return launch_window_d<F16>(p, paged, d_k, st);
+    default: return launch_window_d<BF16>(p, paged, d_k, st);
   }
 }
 
@@ -859,6 +892,11 @@ extern "C" {
 
 size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q, int most_keys, int d_k, int window,
                                  int sinks, int dtype) {
+  return tl_paged_prefill_workspace_bytes(nullptr, batch, n_head, n_kv_head, seq_q, most_keys, d_k, window, sinks, dtype);
+}
+
+size_t tl_paged_prefill_workspace_bytes(const int32_t* host_new_lens, int batch, int n_head, int n_kv_head, int seq_q,
+                                        int most_keys, int d_k, int window, int sinks, int dtype) {
   if (batch < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || seq_q < 1 || seq_q > kMostRows || most_keys < 1 ||
       window < 0 || sinks < 0 || (d_k != 64 && d_k != 128) || !rows_ok(seq_q, n_head / n_kv_head) ||
       (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16))
@@ -867,10 +905,11 @@ size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q
   p.batch = batch;
   p.n_kv = n_kv_head;
   p.group = n_head / n_kv_head;
+  p.seq_q = seq_q;
   p.n_qt = (seq_q * p.group + kBM - 1) / kBM;
   p.window = window;
   p.sinks = sinks;
-  const int64_t parts = plan_slots(p, most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2);
+  const int64_t parts = plan_slots(p, row_tiles(p, host_new_lens), most_keys, d_k, dtype == TL_DTYPE_F32 ? 4 : 2);
   return parts ? words_bytes(parts) + (size_t)parts * part_bytes(d_k) : 0;
 }
 
@@ -892,7 +931,7 @@ int tl_window_attention(const void* q, const void* k, const void* v, void* o, vo
   p.seq_k = seq_k;
   p.window = window;
   p.sinks = sinks;
-  return window_entry(p, false, seq_k, workspace, workspace_bytes, d_k, q_strides, k_strides, v_strides, o_strides,
+  return window_entry(p, false, seq_k, nullptr, workspace, workspace_bytes, d_k, q_strides, k_strides, v_strides, o_strides,
                       sm_scale, dtype, stream);
 }
 
@@ -902,7 +941,21 @@ int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v
                                int n_new, int n_head, int n_kv_head, int d_k, const int64_t* q_strides, const int64_t* k_page_strides,
                                const int64_t* v_page_strides, const int64_t* o_strides, float sm_scale, int window,
                                int sinks, int dtype, void* stream) {
+  return tl_paged_attention_prefill_counted(q, k_pages, v_pages, page_table, max_pages, n_pages, page_size, cache_lens,
+                                            new_lens, nullptr, o, workspace, workspace_bytes, batch, n_new, n_head, n_kv_head,
+                                            d_k, q_strides, k_page_strides, v_page_strides, o_strides, sm_scale, window,
+                                            sinks, dtype, stream);
+}
+
+int tl_paged_attention_prefill_counted(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                                       int max_pages, int n_pages, int page_size, const int32_t* cache_lens,
+                                       const int32_t* new_lens, const int32_t* host_new_lens, void* o, void* workspace,
+                                       size_t workspace_bytes, int batch, int n_new, int n_head, int n_kv_head, int d_k,
+                                       const int64_t* q_strides, const int64_t* k_page_strides,
+                                       const int64_t* v_page_strides, const int64_t* o_strides, float sm_scale, int window,
+                                       int sinks, int dtype, void* stream) {
   if (batch == 0 || n_head == 0 || n_new == 0) return 0;
+  if (host_new_lens && !new_lens) return TL_ERR_INVALID;
   const int shift = page_shift(page_size);
   if (!page_table || !cache_lens || max_pages < 1 || n_pages < 1 || shift < 0 ||
       ((int64_t)max_pages << shift) > (1 << 30))
@@ -921,7 +974,7 @@ int tl_paged_attention_prefill(const void* q, const void* k_pages, const void* v
   p.seq_q = n_new;
   p.window = window;
   p.sinks = sinks;
-  return window_entry(p, true, (int64_t)max_pages << shift, workspace, workspace_bytes, d_k, q_strides, k_page_strides,
+  return window_entry(p, true, (int64_t)max_pages << shift, host_new_lens, workspace, workspace_bytes, d_k, q_strides, k_page_strides,
                       v_page_strides, o_strides, sm_scale, dtype, stream);
 }
 

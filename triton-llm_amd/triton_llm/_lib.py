@@ -131,6 +131,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _c_int, _c_int, _c_int, _c_int, _c_int,
          _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
     ),
+    "tl_paged_attention_prefill_counted": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _i32p, _vp, _vp, _c_size,
+         _c_int, _c_int, _c_int, _c_int, _c_int,
+         _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
+    ),
+    "tl_paged_prefill_workspace_bytes": (
+        _c_size, [_i32p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "tl_window_workspace_bytes": (
         _c_size, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "tl_window_attention": (

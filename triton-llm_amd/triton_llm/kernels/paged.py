@@ -263,24 +263,46 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
 
 def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_head: int, n_kv_head: int,
                             new_lens=None, sm_scale: float | None = None, window: int = 0, sinks: int = 0, out=None,
-                            workspace=None):
+                            workspace=None, host_new_lens=None):
     """Queries ``(batch, n_new, n_head, d_k)`` at positions ``cache_lens[b] + i`` over the pages.
 
     The new tokens' own k and v are appended before.  ``new_lens`` as in :func:`paged_kv_append`: rows
-    behind a sequence's tokens are left as they were.
+    behind a sequence's tokens are left as they were.  ``host_new_lens``: the same numbers on the host, where the program has
+    them (a sequence of int or a ctypes array): how the work is shared goes by them, and by n_new for every sequence
+    otherwise, which is slow where few of a batch's sequences have many tokens.  They may not be less than
+    ``new_lens``'s (rows would be left as they were); a captured call goes without them.
     """
     _check_int32(page_table, cache_lens, new_lens)
     pages, sizes, ws_bytes = _attention_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape,
                                              _shape(new_lens), q_dev.shape, n_head, n_kv_head, window, sinks, True)
     code = dtype_code_of(q_dev, k_pages, v_pages)
     out = _same_output(out, q_dev)
-    ws = scratch(ws_bytes[code], workspace, key="window")
+    need = ws_bytes[code]
+    if host_new_lens is not None:
+        if new_lens is None:
+            raise ValueError("host_new_lens is given without new_lens")
+        host_new_lens = _host_counts(host_new_lens, sizes[0])
+        need = max(need, _lib.load().tl_paged_prefill_workspace_bytes(
+            host_new_lens, sizes[0], n_head, n_kv_head, sizes[1], pages[0] * pages[2], sizes[4], window, sinks, code))
+    ws = scratch(need, workspace, key="window")
     if sm_scale is None:
         sm_scale = default_scale(k_pages.shape[3])
-    launch(gpu.runtime().tl_paged_attention_prefill, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
-           cache_lens.ptr, _ptr(new_lens), out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes,
+    launch(gpu.runtime().tl_paged_attention_prefill_counted, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
+           cache_lens.ptr, _ptr(new_lens), host_new_lens, out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes,
            float(sm_scale), int(window), int(sinks), code, None, what="paged_attention_prefill")
     return out
+
+
+def _host_counts(counts, batch: int):
+    """An int32 ctypes array of a batch's counts."""
+    if not isinstance(counts, ctypes.Array):
+        counts = _numbers(counts)
+        if counts and not (min(counts) >= -(1 << 31) and max(counts) < 1 << 31):
+            raise ValueError("host_new_lens must fit in int32")
+        counts = (ctypes.c_int32 * len(counts))(*counts)
+    if len(counts) != batch or counts._type_ is not ctypes.c_int32:
+        raise ValueError(f"host_new_lens must hold {batch} int32 numbers, got {len(counts)}")
+    return counts
 
 
 def copy_kv_pages(caches, src, dst) -> None:

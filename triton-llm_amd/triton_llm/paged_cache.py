@@ -257,6 +257,7 @@ class PagedKVCache:
         self._table = gpu.to_device(np.full(shape, -1, np.int32))
         # row 0: tokens before the step, row 1: the step's, row 2: tokens with the step's
         self._counts = gpu.zeros((3, max_batch), np.int32)
+        self._host_new = (ctypes.c_int32 * max_batch)()
         self._most_new = self._longest = 0  # the step's tokens of a slot at most, the longest sequence with them
         self._told = [0] * (3 * max_batch)  # what the device has in it
         self._lens, self._new, self._ends = (self._row(i) for i in range(3))
@@ -327,6 +328,7 @@ class PagedKVCache:
         t = self.tables
         t.begin(new)
         self._most_new = max(t.new)
+        self._host_new[:] = t.new  # in place: a recorded call finds the step's counts there
         self._longest = max(a + b for a, b in zip(t.lens, t.new) if b)
         self._publish()
 
@@ -366,4 +368,4 @@ class PagedKVCache:
                                           out=out, workspace=self._decode_ws)
         return paged_attention_prefill(q_dev, pool["k"], pool["v"], self._table, self._lens, self.n_head,
                                        self.n_kv_head, new_lens=self._new, sm_scale=sm_scale, window=self.window,
-                                       sinks=self.sinks, out=out)
+                                       sinks=self.sinks, out=out, host_new_lens=self._host_new)
