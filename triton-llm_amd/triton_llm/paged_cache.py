@@ -255,7 +255,7 @@ class PagedKVCache:
         self._pools = [layer[n] for layer in self.layers for n in "kv"]
         shape = (max_batch, self.tables.max_pages)
         self._table = gpu.to_device(np.full(shape, -1, np.int32))
-        # row 0: tokens before the step, row 1: the step's, row 2: tokens with the step's
+        # row 0: tokens before the step, row 1: the step's, row 2: tokens with the step's (0 for a slot that rests)
         self._counts = gpu.zeros((3, max_batch), np.int32)
         self._host_new = (ctypes.c_int32 * max_batch)()
         self._most_new = self._longest = 0  # the step's tokens of a slot at most, the longest sequence with them
@@ -292,7 +292,7 @@ class PagedKVCache:
         self._copy(copies[start:])
         if edits:
             write_i32(self._table, [s * t.max_pages + c for s, c in edits], list(edits.values()))
-        now = t.lens + t.new + [a + b for a, b in zip(t.lens, t.new)]
+        now = t.lens + t.new + [a + b if b else 0 for a, b in zip(t.lens, t.new)]
         changed = [i for i, n in enumerate(now) if n != self._told[i]]
         write_i32(self._counts, changed, [now[i] for i in changed])
         self._told = now
@@ -343,7 +343,7 @@ class PagedKVCache:
         n_kv_head, d_k)`` in the cache's dtype, n_new at least the step's largest count; a slot's tokens are the first
         of its rows.  q is rotated in place.  cos/sin as in ``paged_kv_append``, of at least as many rows as the
         longest sequence has tokens.  Returns the attention output, like q; the rows that are no tokens
-        hold nothing of meaning.
+        hold nothing of meaning.  A slot that rests costs nothing: its pages are not read.
         """
         t = self.tables
         if not 0 <= layer < self.n_layer:
@@ -362,7 +362,6 @@ class PagedKVCache:
         paged_kv_append(q_dev, k_dev, v_dev, pool["k"], pool["v"], self._table, self._lens, cos_dev, sin_dev,
                         new_lens=self._new, interleaved=interleaved)
         if n_new == 1:
-            # a resting slot's row runs over its cached tokens: the batch's kernels have no gaps
             return paged_attention_decode(q_dev, pool["k"], pool["v"], self._table, self._ends, self.n_head,
                                           self.n_kv_head, sm_scale=sm_scale, window=self.window, sinks=self.sinks,
                                           out=out, workspace=self._decode_ws)
