@@ -32,6 +32,19 @@ from triton_llm.kernels.paged import (allocate_kv_pages, copy_kv_pages, paged_at
 __all__ = ["PageTables", "PagedKVCache"]
 
 
+def _differing(a: list[int], b: list[int]) -> list[int]:
+    """Where two lists of pages differ, places that one has alone among them.  What they share is compared 32 pages at a time:
+    beams have most of theirs in common."""
+    out, n = [], min(len(a), len(b))
+    for lo in range(0, n, 32):
+        hi = min(lo + 32, n)
+        x, y = a[lo:hi], b[lo:hi]
+        if x != y:
+            out.extend(lo + i for i, (p, q) in enumerate(zip(x, y)) if p != q)
+    out.extend(range(n, max(len(a), len(b))))
+    return out
+
+
 class PageTables:
     """Which pages every slot's sequence has, and which are free.  Host only.
 
@@ -85,10 +98,8 @@ class PageTables:
     def _set(self, slot: int, pages: list[int] | None) -> None:
         """The slot's pages become `pages`, whose references are the caller's."""
         old, new = self.tables[slot] or [], pages or []
-        for c in range(max(len(old), len(new))):
-            a, b = old[c] if c < len(old) else -1, new[c] if c < len(new) else -1
-            if a != b:
-                self.table_edits[slot, c] = b
+        for c in _differing(old, new):
+            self.table_edits[slot, c] = new[c] if c < len(new) else -1
         self.tables[slot] = pages
 
     def open(self) -> int:
@@ -130,15 +141,22 @@ class PageTables:
         for s in slots + parents:
             self._check_slot(s)
         parents, slots = [p for s, p in zip(slots, parents) if s != p], [s for s, p in zip(slots, parents) if s != p]
-        taken = [(list(self.tables[p]), self.lens[p], self._gone[p]) for p in parents]
-        for pages, _, _ in taken:
-            for page in pages:
-                if page >= 0:
-                    self.refs[page] += 1
-        for s, (pages, n, gone) in zip(slots, taken):
-            for page in self.tables[s]:
-                self._drop(page)
-            self._set(s, pages)
+        # pages that a slot and its parent have in the same place keep their references
+        taken = []
+        for s, p in zip(slots, parents):
+            old, pages = self.tables[s], list(self.tables[p])
+            places = _differing(old, pages)
+            for c in places:
+                if c < len(pages) and pages[c] >= 0:
+                    self.refs[pages[c]] += 1
+            taken.append((pages, places, self.lens[p], self._gone[p]))
+        for s, (pages, places, n, gone) in zip(slots, taken):
+            old = self.tables[s]
+            for c in places:
+                if c < len(old):
+                    self._drop(old[c])
+                self.table_edits[s, c] = pages[c] if c < len(pages) else -1
+            self.tables[s] = pages
             self.lens[s], self._gone[s] = n, gone
 
     def begin(self, new) -> None:
