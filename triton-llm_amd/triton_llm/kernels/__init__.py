@@ -36,10 +36,11 @@ from .paged import (
     paged_attention_prefill,
     paged_decode_workspace,
     paged_kv_append,
+    paged_prefill_workspace_bytes,
     write_i32,
 )
-from .window import window_attention, window_attention_strided
-from .beam import beam_select
+from .window import window_attention, window_attention_strided, window_workspace_bytes
+from .beam import beam_select, beam_workspace_bytes
 
 __all__ = [
     "attention",
@@ -67,9 +68,12 @@ __all__ = [
     "paged_attention_decode",
     "paged_decode_workspace",
     "paged_attention_prefill",
+    "paged_prefill_workspace_bytes",
     "copy_kv_pages",
     "write_i32",
     "window_attention",
     "window_attention_strided",
+    "window_workspace_bytes",
     "beam_select",
+    "beam_workspace_bytes",
 ]

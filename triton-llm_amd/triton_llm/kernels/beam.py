@@ -18,12 +18,17 @@ import numpy as np
 from triton_llm import _lib, gpu
 from ._common import launch, scratch
 
-__all__ = ["beam_select", "max_select"]
+__all__ = ["beam_select", "beam_workspace_bytes", "max_select"]
 
 
 def max_select() -> int:
     """Most continuations a call selects per batch item."""
     return int(_lib.load().tl_beam_max_select())
+
+
+def beam_workspace_bytes(batch: int, beams: int, vocab: int) -> int:
+    """Bytes of a ``workspace`` for :func:`beam_select` (0: the sizes are not supported)."""
+    return int(_lib.load().tl_beam_select_workspace_bytes(batch, beams, vocab))
 
 
 @functools.lru_cache(maxsize=256)

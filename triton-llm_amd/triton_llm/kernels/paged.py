@@ -112,7 +112,7 @@ def _check_int32(page_table, cache_lens, new_lens=None):
 def _check_heads(n_head, n_kv_head, n_kv, d_k):
     if n_kv != n_kv_head:
         raise ValueError(f"pool has {n_kv} KV heads, n_kv_head={n_kv_head}")
-    if n_head <= 0 or n_head % n_kv_head:
+    if n_head <= 0 or n_kv_head <= 0 or n_head % n_kv_head:
         raise ValueError(f"n_head ({n_head}) must be a positive multiple of n_kv_head ({n_kv_head})")
     if d_k not in (64, 128):
         raise ValueError(f"paged attention supports d_k in (64, 128), got {d_k}")
@@ -261,6 +261,18 @@ def paged_attention_decode(q_dev, k_pages, v_pages, page_table, cache_lens, n_he
     return out
 
 
+def paged_prefill_workspace_bytes(batch: int, n_head: int, n_kv_head: int, n_new: int, max_ctx: int, d_k: int, dtype,
+                                  window: int = 0, sinks: int = 0, host_new_lens=None) -> int:
+    """Bytes of a ``workspace`` for :func:`paged_attention_prefill` (0: none is used), max_ctx the positions that a table
+    holds.  With ``host_new_lens`` for that call with these counts."""
+    _check_heads(n_head, n_kv_head, n_kv_head, d_k)
+    check_window(window, sinks)
+    need = _lib.load().tl_paged_prefill_workspace_bytes
+    dims = (batch, n_head, n_kv_head, n_new, max_ctx, d_k, window, sinks, gpu.dtype_code(dtype))
+    most = need(None, *dims)
+    return most if host_new_lens is None else max(most, need(_host_counts(host_new_lens, batch), *dims))
+
+
 def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_head: int, n_kv_head: int,
                             new_lens=None, sm_scale: float | None = None, window: int = 0, sinks: int = 0, out=None,
                             workspace=None, host_new_lens=None):
@@ -282,6 +294,7 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
         if new_lens is None:
             raise ValueError("host_new_lens is given without new_lens")
         host_new_lens = _host_counts(host_new_lens, sizes[0])
+        # the plan without the counts has its room too: a captured call goes by that
         need = max(need, _lib.load().tl_paged_prefill_workspace_bytes(
             host_new_lens, sizes[0], n_head, n_kv_head, sizes[1], pages[0] * pages[2], sizes[4], window, sinks, code))
     ws = scratch(need, workspace, key="window")

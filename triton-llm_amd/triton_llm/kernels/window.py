@@ -34,6 +34,14 @@ def _strided_plan(batch, n_head, n_kv_head, seq_q, seq_k, d_k, q_strides, k_stri
     return sizes, ws
 
 
+def window_workspace_bytes(batch: int, n_head: int, n_kv_head: int, seq_q: int, seq_k: int, d_k: int, dtype, window: int = 0,
+                           sinks: int = 0) -> int:
+    """Bytes of a ``workspace`` for a call with these sizes (0: none is used)."""
+    check_window(window, sinks)
+    return _lib.load().tl_window_workspace_bytes(batch, n_head, n_kv_head, seq_q, seq_k, d_k, window, sinks,
+                                                 gpu.dtype_code(dtype))
+
+
 def window_attention_strided(q, k, v, out, *, batch, n_head, n_kv_head, seq_q, seq_k, d_k, q_strides, k_strides,
                              v_strides, o_strides, window, sinks=0, sm_scale=None, workspace=None):
     """The kernel on raw layouts given by {batch, head, seq} element strides."""
