@@ -38,7 +38,7 @@ from ._common import default_scale, launch, same_dtype, scratch
 MIN_PAGE, MAX_PAGE = 16, 1024
 
 
-def _check_page_size(page_size: int) -> None:
+def check_page_size(page_size: int) -> None:
     if not (MIN_PAGE <= page_size <= MAX_PAGE and page_size & (page_size - 1) == 0):
         raise ValueError(f"page_size must be a power of 2 in [{MIN_PAGE}, {MAX_PAGE}], got {page_size}")
 
@@ -47,7 +47,7 @@ def allocate_kv_pages(n_pages: int, n_kv_head: int, page_size: int, d_k: int, dt
     """(k_pages, v_pages), each ``(n_pages, n_kv_head, page_size, d_k)`` on the GPU."""
     if n_pages <= 0 or n_kv_head <= 0 or d_k <= 0:
         raise ValueError(f"pool dims must be positive, got n_pages={n_pages} n_kv_head={n_kv_head} d_k={d_k}")
-    _check_page_size(page_size)
+    check_page_size(page_size)
     gpu.dtype_code(dtype)
     alloc = gpu.zeros if zero else gpu.allocate
     shape = (n_pages, n_kv_head, page_size, d_k)
@@ -85,7 +85,7 @@ def _check_pool(k_shape, v_shape):
                          f"got {k_shape} and {v_shape}")
     if min(k_shape) <= 0:
         raise ValueError(f"pool dims must be positive, got {k_shape}")
-    _check_page_size(k_shape[2])
+    check_page_size(k_shape[2])
     return k_shape
 
 
@@ -336,7 +336,7 @@ def copy_kv_pages(caches, src, dst) -> None:
     shape, dtype = caches[0].shape, caches[0].dtype
     if len(shape) != 4 or min(shape) <= 0:
         raise ValueError(f"pools must be 4-D (n_pages, n_kv_head, page_size, d_k), got {shape}")
-    _check_page_size(shape[2])
+    check_page_size(shape[2])
     gpu.dtype_code(dtype)
     for c in caches:
         if c.shape != shape or (c.dtype is not dtype and gpu.dtype_name(c.dtype) != gpu.dtype_name(dtype)):

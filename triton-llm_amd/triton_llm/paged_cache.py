@@ -26,8 +26,9 @@ import ctypes
 import numpy as np
 
 from triton_llm import gpu
-from triton_llm.kernels.paged import (allocate_kv_pages, copy_kv_pages, paged_attention_decode,
-                                      paged_attention_prefill, paged_decode_workspace, paged_kv_append, write_i32)
+from triton_llm.kernels.paged import (allocate_kv_pages, check_page_size, check_window, copy_kv_pages,
+                                      paged_attention_decode, paged_attention_prefill, paged_decode_workspace,
+                                      paged_kv_append, write_i32)
 
 __all__ = ["PageTables", "PagedKVCache"]
 
@@ -57,8 +58,13 @@ class PageTables:
     def __init__(self, n_pages: int, page_size: int, max_batch: int, max_seq: int, window: int = 0, sinks: int = 0):
         if n_pages <= 0 or max_batch <= 0 or max_seq <= 0:
             raise ValueError(f"n_pages, max_batch and max_seq must be positive, got {n_pages}, {max_batch}, {max_seq}")
-        if window < 0 or sinks < 0:
-            raise ValueError(f"window and sinks must be >= 0, got {window} and {sinks}")
+        # what a step's append and attention would refuse
+        check_page_size(page_size)
+        check_window(window, sinks)
+        if max_batch > 65535:
+            raise ValueError(f"max_batch must be at most 65535, got {max_batch}")
+        if -(-max_seq // page_size) * page_size > 1 << 30:
+            raise ValueError(f"max_seq must be at most 2^30, got {max_seq}")
         self.n_pages, self.page_size = n_pages, page_size
         self.max_batch, self.max_seq = max_batch, max_seq
         self.window, self.sinks = window, sinks
@@ -263,6 +269,13 @@ class PagedKVCache:
         if d_k not in (64, 128):
             raise ValueError(f"paged attention supports d_k in (64, 128), got {d_k}")
         self.tables = PageTables(n_pages, page_size, max_batch, max_seq, window, sinks)
+        blocks = self.tables.max_pages * page_size // 16
+        if window:
+            blocks = min(blocks, window // 16 + 2 + -(-sinks // 16))
+        pairs = n_kv_head * -(-n_head // n_kv_head // 8)
+        if max_batch * pairs * blocks >= 1 << 31:
+            raise ValueError(f"{max_batch} sequences of {max_seq} tokens and {n_kv_head} KV heads are more than one-token "
+                             f"attention counts (2^31 - 1 blocks of 16 positions a KV head and 8 of its query heads)")
         self.n_layer, self.n_head, self.n_kv_head, self.d_k = n_layer, n_head, n_kv_head, d_k
         self.window, self.sinks = window, sinks
         self.dtype = dtype
