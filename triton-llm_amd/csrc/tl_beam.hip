@@ -7,7 +7,8 @@
 // their size.  exp, its sums and the logarithm are 64-bit too (see exp_below).
 //
 // Every logit is read once, by beam_scan, a wave a segment of 1024 entries of a row, bound by the 64-bit operations of exp
-// (16 x 8 x 128256 bf16, 33 MB: 15.8 us, 2.1 TB/s; with a 32-bit exp 10.4; with segments of 2048 and 4096 entries a call took 3 and 9 us more), which leaves
+// (16 x 8 x 128256 bf16, 33 MB: 14.6 us, 2.3 TB/s; with a 32-bit exp 10.4; with segments of 2048 entries a call takes 2 us
+// more, with 512 up to 3 more where the places are many), which leaves
 //   * the segment's maximum and its sum of exp against it;
 //   * the maximum of every group of 64 entries.
 // beam_finish, a workgroup a batch item, has everything else from those.  The best score in a unit (a segment, or
@@ -32,9 +33,9 @@ constexpr int kSeg = 64 * kVec * kVecs;  // entries of a segment, a wave's
 constexpr int kGrp = 64;                 // entries of a group: 8 lanes
 constexpr int kFT = 1024;                // threads of beam_finish
 constexpr int kFW = kFT / 64;
-// Up to kFewPlaces places 64 classes, ranked by one wave (4 x 50257 for 8: 9.7 us, with 256 classes 10.3); beyond them
-// 256, ranked by all waves, as of 64 classes too many units reach the bound (4 of 4 x 50257 for 64: 18.5 us, with 64
-// classes 52; 16 of 2 x 32000 for 32: 13.0 and 14.3).
+// Up to kFewPlaces places 64 classes, ranked by one wave (4 x 50257 for 8: 9.5 us, with 256 classes 10.1); beyond them
+// 256, ranked by all waves, as of 64 classes too many units reach the bound (4 of 4 x 50257 for 64: 18.7 us, with 64
+// classes 57; 16 of 2 x 32000 for 32: 13.0 and 14.6).
 constexpr int kFewPlaces = 16;
 constexpr int kClasses = 256;
 constexpr int kMaxVocab = 262144;
@@ -72,7 +73,7 @@ size_t align256(size_t b) { return (b + 255) & ~size_t(255); }
 // out (in 32 bits it reached 5e-7).  d log2 e = n + f with whole n and |f| <= 1/2; 2^f by its interpolation of degree 9 at the
 // Chebyshev points; n goes into the exponent.  Below e^-700 it is e^-700, which no sum with a 1 in it notices.
 // 64-bit products take no longer than 32-bit ones here; their number is what counts (degree 11 and a clamp that keeps
-// NaN: 16 x 8 x 128256 27.3 us a call, so 24.9).
+// NaN: 16 x 8 x 128256 27.3 us a call, so 24.1).
 __device__ __forceinline__ double exp_below(float x, double m) {
   constexpr double kL = 1.4426950408889634;
   constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: added, a number's whole part stands in its low bits
@@ -124,9 +125,8 @@ __device__ __forceinline__ double shfl_d(double x, int lane) {
   return __builtin_bit_cast(double, (uint64_t)a | ((uint64_t)b << 32));
 }
 
-// Reductions by DPP moves, a few cycles each where a move through LDS takes about a hundred, over 8 lanes or a wave: for
-// beam_finish, whose steps wait for each other (9.8 -> 9.4 us at 4 x 50257).  beam_scan has enough waves to cover
-// the moves through LDS, and the vector unit is what it has least of (16 x 8 x 128256: 20.2 us, with DPP 21.1).
+// Reductions by DPP moves, a few cycles each where a move through LDS takes about a hundred, over 8 lanes or a wave (16 x 8 x
+// 128256 24.9 -> 24.1 us, 4 x 50257 9.6 -> 9.5 for beam_scan's; 9.8 -> 9.4 before for beam_finish's).
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   const int i = __float_as_int(x);
@@ -142,16 +142,16 @@ __device__ __forceinline__ double dpp(double x) {
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;  // quad_perm, row_half_mirror, row_mirror
 __device__ __forceinline__ float max8(float x) {
-  x = fmaxf(x, dpp<kXor1>(x));
-  x = fmaxf(x, dpp<kXor2>(x));
-  return fmaxf(x, dpp<kMirror8>(x));
+  x = max_or_nan(x, dpp<kXor1>(x));
+  x = max_or_nan(x, dpp<kXor2>(x));
+  return max_or_nan(x, dpp<kMirror8>(x));
 }
 __device__ __forceinline__ float lane_f(float x, int i) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
 }
 __device__ __forceinline__ float wave_max_of8(float x) {  // of max8's results
-  x = fmaxf(x, dpp<kMirror16>(x));
-  return fmaxf(fmaxf(lane_f(x, 0), lane_f(x, 16)), fmaxf(lane_f(x, 32), lane_f(x, 48)));
+  x = max_or_nan(x, dpp<kMirror16>(x));
+  return max_or_nan(max_or_nan(lane_f(x, 0), lane_f(x, 16)), max_or_nan(lane_f(x, 32), lane_f(x, 48)));
 }
 
 // Lane i's value, i the same on every lane.
@@ -187,22 +187,19 @@ __global__ __launch_bounds__(kST) void beam_scan_kernel(BeamParams p) {
     float g = v[k][0];
 #pragma unroll
     for (int e = 1; e < kVec; ++e) g = max_or_nan(g, v[k][e]);
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1) g = max_or_nan(g, __shfl_xor(g, off));
+    g = max8(g);
     const int i = i0 + k * 64 * kVec;
     if ((lane & 7) == 0 && i < p.vocab) p.gmax[(int64_t)row * p.n_grp + i / kGrp] = g;
     m = max_or_nan(m, g);
   }
-#pragma unroll
-  for (int off = 8; off < 64; off <<= 1) m = max_or_nan(m, __shfl_xor(m, off));
+  m = wave_max_of8(m);
   const double base = m == -INFINITY ? 0. : (double)m;  // a segment of -inf alone has no mass
   double s = 0.;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k)
 #pragma unroll
     for (int i = 0; i < kVec; ++i) s += exp_below(v[k][i], base);
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) s += shfl_xor_d(s, off);
+  s = wave_sum(s);
   if (lane == 0) {
     p.smax[(int64_t)row * p.n_seg + seg] = m;
     p.ssum[(int64_t)row * p.n_seg + seg] = s;
@@ -269,7 +266,7 @@ __global__ __launch_bounds__(kFT) void beam_finish_kernel(BeamParams p) {
       part[k] = i < p.n_seg ? ss[i] : 0.;
     }
 #pragma unroll
-    for (int k = 0; k < K; ++k) m = fmaxf(m, sx[k]);
+    for (int k = 0; k < K; ++k) m = max_or_nan(m, sx[k]);
     m = wave_max_of8(max8(m));
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -526,8 +523,8 @@ int tl_beam_select(const void* logits, const float* scores, int batch, int beams
   p.n_seg = n_segments(vocab);
   p.n_grp = n_groups(vocab);
   // Segments where they are several for each place, so that few of them reach the bound, and no class is empty.  us a
-  // call with segments / with groups: 16 x 8 x 128256 for 16 21.2 / 28.3, 4 x 50257 for 8 9.7 / 10.3; 1 x 50257 for 4
-  // 8.9 / 8.3, 16 of 2 x 32000 for 32 19.1 / 13.0.
+  // call with segments / with groups: 16 x 8 x 128256 for 16 24.1 / 30.3, 4 x 50257 for 8 9.5 / 9.8; 1 x 50257 for 4
+  // 8.5 / 8.3, 16 of 2 x 32000 for 32 34.0 / 13.0.
   const bool segments = (int64_t)beams * p.n_seg >= kUnitsAPlace * select && (int64_t)beams * p.n_seg >= 64;
   p.unit = segments ? kSeg : kGrp;
   p.n_units = segments ? p.n_seg : p.n_grp;
