@@ -18,7 +18,7 @@
 // V is read by transposing LDS reads.
 //
 // Bound by the matrix products and, at d_k 64, as much by exp and the conversions: 8192 tokens, window 1024, 24 / 8 heads
-// of 128, bf16: 131 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 40.9 to 43.5 us by device.
+// of 128, bf16: 126 to 137 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 40.7 to 43 us, by device.
 #include "tl_paged.h"
 #include "tl_prefill.h"
 
@@ -278,7 +278,8 @@ __device__ __forceinline__ Keys keys_of(const WinParams& p, const Rows& r, int q
 // `share` key tiles a part, and its parts, by (KV head, part, row tile), stand behind those of the sequences before it.  Only
 // the device knows the lengths, so only it can make the parts about `slots`, equally long, without gaps between
 // them: with a grid by the longest lengths that there could be, workgroups without work stood among the
-// others, and 4 x 500 rows on prefixes of 2875 to 3835 (of at most 4608) took 47.8 us.
+// others, and 4 x 500 rows on prefixes of 2875 to 3835 (of at most 4608) took 47.8 us.  Lengths are walked 64 at a time by every
+// workgroup; 2 rows of each of 8, 64 and 150 sequences, 131072 keys in all, 15 / 5 heads of 64, bf16, take 42, 33 and 35 us.
 struct Seq {
   Rows r;
   int tiles, keys;  // row tiles, key tiles of the last of them
