@@ -405,7 +405,7 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * given less (NULL: none) the call runs in one.  Either is deterministic.
  * (n_new or seq_q) <= 2^28, seq_k <= 2^29, and times the square of n_head / n_kv_head below 2^32.
  * With 16-bit types a row's weights are rounded to the type for the product with V, as the causal prefill's
- * are: half a step each (fp16: down to 2^-25 of the row's largest, below it at most 2^-36 of that); the maximum, both
+ * are: half a step each (fp16: down to 2^-23 of the row's largest, below it at most 2^-34 of that); the maximum, both
  * sums and o are held in 32 bits.  tl_paged_attention_decode rounds no weights.
  * A NaN or infinity in a V row makes NaN of the rows that are computed in one
  * tile with it, seen or not, as a product with a zero weight does.
