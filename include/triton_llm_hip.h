@@ -392,7 +392,7 @@ int tl_sample_row(const void* logits, int vocab, float temperature, int top_k, d
  * tl_paged_attention_prefill_counted: the same where the host has new_lens's values too, host_new_lens (batch; read
  * before the call returns; NULL: as without).  How the work is shared then goes by the rows there are, else as if
  * every sequence had n_new.  Where new_lens holds more than host_new_lens, rows may be left as they were; a captured
- * call does not use it, as its replays may come with other values.
+ * call does not use it, as its replays may come with other values (its workspace is tl_window_workspace_bytes's).
  * tl_window_attention: the same over K / V (batch, n_kv_head, seq_k, d_k)
  * {batch, head, seq}, query i at position seq_k - seq_q + i.
  * Both: window = 0 is plain causal attention; a row that sees no key gives zeros;

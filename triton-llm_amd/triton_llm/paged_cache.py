@@ -58,13 +58,10 @@ class PageTables:
     def __init__(self, n_pages: int, page_size: int, max_batch: int, max_seq: int, window: int = 0, sinks: int = 0):
         if n_pages <= 0 or max_batch <= 0 or max_seq <= 0:
             raise ValueError(f"n_pages, max_batch and max_seq must be positive, got {n_pages}, {max_batch}, {max_seq}")
-        # what a step's append and attention would refuse
-        check_page_size(page_size)
-        check_window(window, sinks)
-        if max_batch > 65535:
-            raise ValueError(f"max_batch must be at most 65535, got {max_batch}")
-        if -(-max_seq // page_size) * page_size > 1 << 30:
-            raise ValueError(f"max_seq must be at most 2^30, got {max_seq}")
+        if page_size <= 0:
+            raise ValueError(f"page_size must be positive, got {page_size}")
+        if window < 0 or sinks < 0:
+            raise ValueError(f"window and sinks must be >= 0, got {window} and {sinks}")
         self.n_pages, self.page_size = n_pages, page_size
         self.max_batch, self.max_seq = max_batch, max_seq
         self.window, self.sinks = window, sinks
@@ -268,7 +265,14 @@ class PagedKVCache:
             raise ValueError(f"bad head counts: n_layer={n_layer} n_head={n_head} n_kv_head={n_kv_head}")
         if d_k not in (64, 128):
             raise ValueError(f"paged attention supports d_k in (64, 128), got {d_k}")
+        # what a step's append and attention would refuse
+        check_page_size(page_size)
+        check_window(window, sinks)
+        if max_batch > 65535:
+            raise ValueError(f"max_batch must be at most 65535, got {max_batch}")
         self.tables = PageTables(n_pages, page_size, max_batch, max_seq, window, sinks)
+        if self.tables.max_pages * page_size > 1 << 30:
+            raise ValueError(f"max_seq must be at most 2^30, got {max_seq}")
         blocks = self.tables.max_pages * page_size // 16
         if window:
             blocks = min(blocks, window // 16 + 2 + -(-sinks // 16))
