@@ -473,7 +473,7 @@ int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
  * smollm2_triton/model.py:566-584).  logits (batch * beams, vocab) with
  * row_stride >= vocab, scores (batch, beams) fp32: of every batch item's
  * beams * vocab continuations, scored scores[b][j] + log softmax(logits[b, j])[v] (ordered
- * in 64 bits, written in 32), the `select` best, best first, ties to the lowest
+ * in 64 bits, the softmax's logarithm to 2^-44, written in 32), the `select` best, best first, ties to the lowest
  * j * vocab + v: score, parent beam j and token v, each (batch, select).
  * A logit of -inf is no continuation; nor is any of a beam whose score is not
  * finite or whose logits hold NaN, +inf or only -inf.  Where fewer are left the rest get

@@ -61,7 +61,8 @@ def beam_select(logits_dev, scores_dev, n_select: int | None = None, out=None, w
 
     logits_dev: ``(batch * beams, vocab)`` or ``(batch, beams, vocab)`` in a compute
     dtype; scores_dev: ``(batch, beams)`` float32.  n_select: default ``2 * beams`` (room for
-    beams that end).  Scores are ordered in 64 bits; ties go to the lowest
+    beams that end).  Scores are ordered in 64 bits (the softmax's logarithm
+    to 2^-44); ties go to the lowest
     ``beam * vocab + token``.  A beam whose score is not finite, or whose logits hold NaN,
     +inf or nothing but -inf, has no continuations, and a logit of -inf is none;
     where fewer are left the rest are ``(-inf, -1, -1)``.  No synchronisation.
