@@ -469,6 +469,112 @@ int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
                  const int32_t* host_value, int count, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * A paged cache whose tables the GPU keeps, and packed batches.  No counterpart in the
+ * reference (one sequence a cache, smollm2_triton/model.py:190-225).
+ * Pools, page_size and page tables as for tl_paged_kv_append.  The pages that no sequence has
+ * are a stack, free_pages[0 .. counts[0]) of n_pages entries, the last one taken first;
+ * counts is two numbers on the device.  A packed batch's rows are the sequences' new tokens one
+ * behind the other, in the order of the sequences: sequence b's are rows starts[b] .. starts[b + 1] - 1.
+ * Lengths, counts and tables are read and written on the device: nothing synchronises, and a captured
+ * call's replays go by what is there then.
+ *
+ * tl_release_pages: the pages of sequences with ended[b] != 0 go back: those that columns keep[b] (NULL: 0) ..
+ * ceil(lens[b] / page_size) - 1 name, entries outside [0, n_pages) left out, by sequence and column
+ * behind the stack's last.  counts_out: pages on the stack then, and how many had no room on it (0 unless a page is
+ * given back twice).  lens_out[b] is 0 for an ended sequence, else lens[b].  The table is not
+ * changed.  counts_out may be counts, lens_out may be lens; otherwise no output overlaps an input or another.
+ *
+ * tl_assign_pages: new_lens[b] (< 0 counts as 0) more tokens for each sequence of lens[b].  Sequences are granted pages in
+ * their order: b is granted if what it and those before it need is on the stack (or it needs none), its tokens fit in its row of
+ * the table and its rows below max_tokens; sequences without room need nothing, so later ones may be granted.  A granted sequence's
+ * new pages are written to its row of the table.  For row t < max_tokens of the packed batch slots[t] = page * page_size + row in
+ * page and positions[t] its position, or -1 and -1 for rows of sequences not granted and behind the last; a page number
+ * outside [0, n_pages) on the stack gives slot -1 and table entry -1.  starts (batch + 1):
+ * the first row of each sequence, at most max_tokens; ends[b]: lens[b] and what was granted.  counts_out: pages
+ * left on the stack, and how many sequences with new tokens were not granted.  counts_out may be counts; otherwise no
+ * output overlaps an input or another.
+ * Both: workspace of tl_pages_workspace_bytes, 16-byte aligned, no initialisation; calls that overlap in time
+ * need one each.  batch <= 65535, n_pages * page_size and max_pages * page_size below 2^31.
+ *
+ * tl_paged_kv_append_slots: tl_paged_kv_append for packed rows.  Token t goes to row slots[t] % page_size of page slots[t] /
+ * page_size, with the rotary positions of positions[t] (may be NULL without tables).  A token whose slot is outside
+ * [0, n_pages * page_size), or whose position is outside [0, rope_rows), writes nothing, its q_out row included.  A slot
+ * twice: some of each token's row.  Strides: q, q_out, k_new, v_new {token, head}.  q_out is q (the same layout) or overlaps
+ * nothing; the pools overlap no input.
+ *
+ * tl_paged_attention_packed: tl_paged_attention_prefill_counted for packed rows: query i of sequence b is row starts[b] + i of
+ * q / o (n_rows, n_head, d_k) {row, head}, at position cache_lens[b] + i.  max_new: the most rows of a
+ * sequence; those behind are left as they were, as are rows of no sequence.  Workspace: tl_paged_packed_workspace_bytes (with n_rows
+ * = 0 what tl_paged_prefill_workspace_bytes gives).  host_new_lens as there, and with the same promise.
+ * ------------------------------------------------------------------------- */
+size_t tl_pages_workspace_bytes(int batch);
+int tl_release_pages(const int32_t* page_table, int max_pages, int page_size, const int32_t* lens,
+                     const int32_t* ended, const int32_t* keep, int batch, int32_t* free_pages,
+                     int n_pages, const int32_t* counts, int32_t* counts_out, int32_t* lens_out,
+                     void* workspace, size_t workspace_bytes, void* stream);
+int tl_assign_pages(const int32_t* lens, const int32_t* new_lens, int batch, int32_t* page_table,
+                    int max_pages, int page_size, const int32_t* free_pages, int n_pages,
+                    const int32_t* counts, int32_t* counts_out, int max_tokens, int32_t* slots,
+                    int32_t* positions, int32_t* starts, int32_t* ends, void* workspace,
+                    size_t workspace_bytes, void* stream);
+int tl_paged_kv_append_slots(const void* q, void* q_out, const void* k_new, const void* v_new,
+                             void* k_pages, void* v_pages, int n_pages, int page_size,
+                             const int32_t* slots, const int32_t* positions, const float* cos_table,
+                             const float* sin_table, int rope_rows, int rotary, int interleaved,
+                             int n_tokens, int n_head, int n_kv_head, int d_k,
+                             const int64_t* q_strides, const int64_t* q_out_strides,
+                             const int64_t* k_new_strides, const int64_t* v_new_strides,
+                             const int64_t* k_page_strides, const int64_t* v_page_strides, int dtype,
+                             void* stream);
+size_t tl_paged_packed_workspace_bytes(const int32_t* host_new_lens, int n_rows, int batch, int n_head,
+                                       int n_kv_head, int max_new, int most_keys, int d_k, int window,
+                                       int sinks, int dtype);
+int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_pages,
+                              const int32_t* page_table, int max_pages, int n_pages, int page_size,
+                              const int32_t* cache_lens, const int32_t* starts,
+                              const int32_t* host_new_lens, void* o, void* workspace,
+                              size_t workspace_bytes, int batch, int n_rows, int max_new, int n_head,
+                              int n_kv_head, int d_k, const int64_t* q_strides,
+                              const int64_t* k_page_strides, const int64_t* v_page_strides,
+                              const int64_t* o_strides, float sm_scale, int window, int sinks, int dtype,
+                              void* stream);
+
+/* ---------------------------------------------------------------------------
+ * One new token a sequence where groups of sequences begin with the same pages: what a group
+ * shares is read once for all of it.  No counterpart in the reference.  Results are those of
+ * tl_paged_attention_decode without a window, to rounding.
+ * Group g is the sequences members[group_starts[g]] .. members[group_starts[g + 1] - 1]; members has
+ * batch entries, those outside [0, batch) name no sequence.  Sequence b sees L = cache_lens[b] + len_add positions (at
+ * least 0, at most max_pages * page_size); its first shared_lens[g] ones lie in the same pages for every sequence of the group
+ * (any number of them, whole pages or not).  The caller promises that: only the first sequence's entries of the
+ * table are read.  A sequence with L < shared_lens[g], or the only one of its group, is taken as one that shares nothing.  One
+ * that is in no group keeps its row of o; one that sees nothing gets zeros.  Named twice in one group it is computed twice.
+ *
+ * tl_shared_plan puts together who reads what, on the device, into `plan` (tl_shared_plan_bytes, 16-byte aligned): for all
+ * layers of a step, as long as the lengths, groups and table stay.  tl_paged_attention_shared is one layer's attention by
+ * it; q / o (batch, n_head, d_k) {batch, head}.  A plan of other sizes (batch, groups, heads, table, d_k or element size) is not followed:
+ * o is left as it was.  The workspace (tl_shared_workspace_bytes, 16-byte aligned) needs no initialisation; calls that overlap
+ * in time need one each.  o overlaps none of q and the pools.
+ * d_k 64 or 128, rows of q, k and v 16-byte aligned; batch and n_groups <= 65535, n_head / n_kv_head <= 128, max_pages *
+ * page_size <= 2^30.  Hidden positions are not read, but for V rows of pages before the first own one in its block of 16.
+ * With 16-bit types weights are rounded to the type for the product with V, as for tl_paged_attention_prefill.
+ * Deterministic.
+ * ------------------------------------------------------------------------- */
+size_t tl_shared_plan_bytes(int batch, int n_groups, int n_head, int n_kv_head, int d_k);
+size_t tl_shared_workspace_bytes(int batch, int n_groups, int n_head, int n_kv_head, int d_k);
+int tl_shared_plan(const int32_t* cache_lens, int len_add, const int32_t* members,
+                   const int32_t* group_starts, const int32_t* shared_lens, int batch, int n_groups,
+                   int n_head, int n_kv_head, int d_k, int max_pages, int page_size, int dtype, void* plan,
+                   size_t plan_bytes, void* stream);
+int tl_paged_attention_shared(const void* q, const void* k_pages, const void* v_pages,
+                              const int32_t* page_table, int max_pages, int n_pages, int page_size,
+                              const void* plan, size_t plan_bytes, int n_groups, void* o, void* workspace,
+                              size_t workspace_bytes, int batch, int n_head, int n_kv_head, int d_k,
+                              const int64_t* q_strides, const int64_t* k_page_strides,
+                              const int64_t* v_page_strides, const int64_t* o_strides, float sm_scale,
+                              int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Beam search's selection.  No counterpart in the reference (it samples:
  * smollm2_triton/model.py:566-584).  logits (batch * beams, vocab) with
  * row_stride >= vocab, scores (batch, beams) fp32: of every batch item's

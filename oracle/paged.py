@@ -95,6 +95,63 @@ def append(q, k_new, v_new, k_pages, v_pages, table, lens, cos=None, sin=None, n
     return qo, kp, vp
 
 
+def release(table, lens, ended, free, counts, page: int, keep=None):
+    """(free_pages, counts, lens) after the ended sequences' pages went back."""
+    free, lens = free.copy(), np.array(lens, np.int64)
+    n = free.size
+    at, lost = min(max(int(counts[0]), 0), n), 0
+    out = lens.copy()
+    for b in range(len(lens)):
+        if not ended[b]:
+            continue
+        held = -(-max(int(lens[b]), 0) // page)
+        for c in range(max(int(keep[b]), 0) if keep is not None else 0, min(held, table.shape[1])):
+            e = int(table[b, c])
+            if not 0 <= e < n:
+                continue
+            if at < n:
+                free[at] = e
+                at += 1
+            else:
+                lost += 1
+        out[b] = 0
+    return free, [at, lost], out
+
+
+def assign(lens, new_lens, table, free, counts, page: int, max_tokens: int):
+    """(table, slots, positions, starts, ends, counts) of a step's new tokens."""
+    table, B = table.copy(), len(lens)
+    slots, positions = np.full(max_tokens, -1, np.int64), np.full(max_tokens, -1, np.int64)
+    starts, ends = np.zeros(B + 1, np.int64), np.array(lens, np.int64)
+    n = free.size
+    top = min(max(int(counts[0]), 0), n)
+    left, short, denied, row = top, False, 0, 0
+    for b in range(B):
+        at, m = int(lens[b]), max(int(new_lens[b]), 0)
+        starts[b] = min(row, max_tokens)
+        row += m
+        need = -(-(at + m) // page) - -(-at // page)
+        if at < 0 or at + m > table.shape[1] * page or row > max_tokens:
+            denied += m > 0
+            continue
+        if need and (short or need > left):
+            short = True  # what those behind it need comes after what it needs
+            denied += 1
+            continue
+        for i in range(need):
+            e = int(free[left - 1 - i])
+            table[b, -(-at // page) + i] = e if 0 <= e < n else -1
+        left -= need
+        ends[b] = at + m
+        for i in range(m):
+            t, pos = row - m + i, at + i
+            e = int(table[b, pos // page])
+            positions[t] = pos
+            slots[t] = e * page + pos % page if 0 <= e < n else -1
+    starts[B] = min(row, max_tokens)
+    return table, slots, positions, starts, ends, [left, denied]
+
+
 def beam_select(logits, scores, n: int):
     """logits (batch, beams, vocab), scores (batch, beams): (scores, parents, tokens), (batch, n) each."""
     B, J, V = logits.shape

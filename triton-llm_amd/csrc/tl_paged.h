@@ -99,4 +99,29 @@ __device__ __forceinline__ int wave_scan(int x) {
 
 __device__ __forceinline__ int last_lane(int x) { return uni(__builtin_amdgcn_readlane(x, 63)); }
 
+// Of a workgroup of kScanWaves waves: the sum over its threads up to and with each, and of all.  Every thread takes part.
+constexpr int kScanWaves = 16;
+struct Scan {
+  int64_t incl, total;
+};
+__device__ __forceinline__ Scan block_scan(int64_t x, int64_t (&sums)[kScanWaves]) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  __syncthreads();  // the sums of the scan before have been read
+  if (lane == 63) sums[wave] = x;
+  __syncthreads();
+  int64_t s = sums[lane & (kScanWaves - 1)];
+#pragma unroll
+  for (int off = 1; off < kScanWaves; off <<= 1) {
+    const int64_t y = __shfl_up(s, off);
+    if ((lane & (kScanWaves - 1)) >= off) s += y;
+  }
+  const int64_t before = __shfl(s, wave ? wave - 1 : 0);
+  return Scan{x + (wave ? before : 0), __shfl(s, kScanWaves - 1)};
+}
+
 }  // namespace tlpg

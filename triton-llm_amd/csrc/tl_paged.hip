@@ -15,7 +15,8 @@ using namespace tlpg;
 namespace {
 
 // ---------------------------------------------------------------------------------
-// Append: rotary positions on q and k, k and v into the pages.
+// Append: rotary positions on q and k, k and v into the pages.  A padded batch's token s of sequence b has position lens[b] + s
+// and finds its page in the table; a packed one's (SLOTS) comes with its position and its slot, page * page_size + row.
 //
 //   half         (x_i, x_{i + r/2}) -> (x_i c - x_{i + r/2} s, x_{i + r/2} c + x_i s)
 //   interleaved  (x_{2i}, x_{2i+1}) likewise;   i < r / 2, r rotated features of d_k
@@ -36,6 +37,8 @@ struct AppendParams {
   PageMap pm;
   const int32_t* lens;
   const int32_t* new_lens;  // NULL: n_new for every sequence
+  const int32_t* slots;      // SLOTS: by token (batch 1), and positions (NULL without rotary positions)
+  const int32_t* positions;
   const float* cos_t;
   const float* sin_t;
   int rope_rows, rot_half;
@@ -48,22 +51,31 @@ struct AppendParams {
   int64_t vp_sp, vp_sh, vp_sr;
 };
 
-// Where token s of sequence b goes; false: it is not written (see the header).
-__device__ __forceinline__ bool token_place(const AppendParams& p, int b, int s, bool rope, int& pos, int& page) {
-  if (p.new_lens && s >= p.new_lens[b]) return false;
-  const int64_t at = (int64_t)p.lens[b] + s;
-  if (at < 0 || (at >> p.pm.shift) >= p.pm.max_pages || (rope && at >= p.rope_rows)) return false;
-  pos = (int)at;
-  page = p.pm.table[(int64_t)b * p.pm.max_pages + (pos >> p.pm.shift)];
+// Where token s of sequence b goes (row: in its page); false: it is not written (see the header).
+template <bool SLOTS>
+__device__ __forceinline__ bool token_place(const AppendParams& p, int b, int s, bool rope, int& pos, int& page, int& row) {
+  if constexpr (SLOTS) {
+    const int slot = p.slots[s];
+    pos = rope ? p.positions[s] : 0;
+    page = slot >> p.pm.shift;
+    row = slot & ((1 << p.pm.shift) - 1);
+    if (rope && (unsigned)pos >= (unsigned)p.rope_rows) return false;
+  } else {
+    if (p.new_lens && s >= p.new_lens[b]) return false;
+    const int64_t at = (int64_t)p.lens[b] + s;
+    if (at < 0 || (at >> p.pm.shift) >= p.pm.max_pages || (rope && at >= p.rope_rows)) return false;
+    pos = (int)at;
+    page = p.pm.table[(int64_t)b * p.pm.max_pages + (pos >> p.pm.shift)];
+    row = pos & ((1 << p.pm.shift) - 1);
+  }
   return (unsigned)page < (unsigned)p.pm.n_pages;
 }
 
 // Row r of token (b, s) -- its n_head q rows, then n_kv k rows, then n_kv v rows -- as
 // source and destination addresses.
 template <typename B>
-__device__ __forceinline__ void token_row(const AppendParams& p, int b, int s, int pos, int page, int r, const B*& src,
+__device__ __forceinline__ void token_row(const AppendParams& p, int b, int s, int row, int page, int r, const B*& src,
                                           B*& dst) {
-  const int row = pos & ((1 << p.pm.shift) - 1);
   if (r < p.n_head) {
     src = (const B*)p.q + b * p.q_sb + s * p.q_ss + r * p.q_sh;
     dst = (B*)p.qo + b * p.qo_sb + s * p.qo_ss + r * p.qo_sh;
@@ -79,7 +91,7 @@ __device__ __forceinline__ void token_row(const AppendParams& p, int b, int s, i
 }
 
 // One element pair a thread: any even d_k, any strides.
-template <typename T, int MODE>
+template <typename T, int MODE, bool SLOTS>
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   using B = typename T::bits;
   const int pairs = p.d_k / 2, rows = p.n_head + 2 * p.n_kv;
@@ -90,11 +102,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
   const int r = (int)(t % rows);
   const int64_t tok = t / rows;
   const int b = (int)(tok / p.n_new), s = (int)(tok % p.n_new);
-  int pos, page;
-  if (!token_place(p, b, s, MODE != kNoRope, pos, page)) return;
+  int pos, page, row;
+  if (!token_place<SLOTS>(p, b, s, MODE != kNoRope, pos, page, row)) return;
   const B* src;
   B* dst;
-  token_row(p, b, s, pos, page, r, src, dst);
+  token_row(p, b, s, row, page, r, src, dst);
   int x = 2 * i, y = 2 * i + 1;
   if (MODE == kHalf && i < p.rot_half) x = i, y = i + p.rot_half;
   const B sx = src[x], sy = src[y];
@@ -115,7 +127,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // and in the other layouts two neighbours (an interleaved chunk is turned in itself).  A thread takes
 // rows g, g + R, ... of its token and loads its angles once for all of them.  8 prompts of up to 1999 tokens, 15 / 5 heads
 // of 64, fp16, 72 MB: 18.4 us, 3.9 TB/s; by pairs of elements (paged_append_kernel) 51 us.
-template <typename T, int MODE>
+template <typename T, int MODE, bool SLOTS>
 __global__ __launch_bounds__(256) void paged_append_vec_kernel(AppendParams p, int R) {
   using B = typename T::bits;
   constexpr int VEC = 16 / T::size;
@@ -128,8 +140,8 @@ __global__ __launch_bounds__(256) void paged_append_vec_kernel(AppendParams p, i
   const int rest = (int)(tid - tok * per_tok);
   const int g = rest / per_row, j = rest - g * per_row;
   const int b = (int)(tok / p.n_new), s = (int)(tok - (int64_t)b * p.n_new);
-  int pos, page;
-  if (!token_place(p, b, s, MODE != kNoRope, pos, page)) return;
+  int pos, page, row;
+  if (!token_place<SLOTS>(p, b, s, MODE != kNoRope, pos, page, row)) return;
 
   const int turned = MODE == kHalf ? p.rot_half / VEC : 0;  // pairs of chunks that turn into each other
   const bool across = MODE == kHalf && j < turned;
@@ -172,7 +184,7 @@ __global__ __launch_bounds__(256) void paged_append_vec_kernel(AppendParams p, i
     for (int u = 0; u < UNROLL; ++u) {
       if (r + u * R < rows) {
         const B* src;
-        token_row(p, b, s, pos, page, r + u * R, src, out[u]);
+        token_row(p, b, s, row, page, r + u * R, src, out[u]);
         wa[u] = *(const u32x4*)(src + ca * VEC);
         wb[u] = *(const u32x4*)(src + cb * VEC);
       }
@@ -219,7 +231,7 @@ bool append_vec_ok(const AppendParams& p, int mode) {
   return !(((uintptr_t)p.q | (uintptr_t)p.qo | (uintptr_t)p.kn | (uintptr_t)p.vn | (uintptr_t)p.kp | (uintptr_t)p.vp) & 15);
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool SLOTS>
 int launch_append_mode(const AppendParams& p, hipStream_t st) {
   const int rows = p.n_head + 2 * p.n_kv;
   if (append_vec_ok<T>(p, MODE)) {
@@ -230,20 +242,20 @@ int launch_append_mode(const AppendParams& p, hipStream_t st) {
     groups = groups < 1 ? 1 : groups > rows ? rows : groups;
     const int64_t blocks = (lanes * groups + 255) / 256;
     if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((paged_append_vec_kernel<T, MODE>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)groups);
+    hipLaunchKernelGGL((paged_append_vec_kernel<T, MODE, SLOTS>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)groups);
     return tl_launch_status();
   }
   const int64_t blocks = ((int64_t)p.batch * p.n_new * rows * (p.d_k / 2) + 255) / 256;
   if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((paged_append_kernel<T, MODE>), dim3((unsigned)blocks), dim3(256), 0, st, p);
+  hipLaunchKernelGGL((paged_append_kernel<T, MODE, SLOTS>), dim3((unsigned)blocks), dim3(256), 0, st, p);
   return tl_launch_status();
 }
 
-template <typename T>
+template <typename T, bool SLOTS>
 int launch_append(const AppendParams& p, int mode, hipStream_t st) {
-  return mode == kHalf          ? launch_append_mode<T, kHalf>(p, st)
-         : mode == kInterleaved ? launch_append_mode<T, kInterleaved>(p, st)
-                                : launch_append_mode<T, kNoRope>(p, st);
+  return mode == kHalf          ? launch_append_mode<T, kHalf, SLOTS>(p, st)
+         : mode == kInterleaved ? launch_append_mode<T, kInterleaved, SLOTS>(p, st)
+                                : launch_append_mode<T, kNoRope, SLOTS>(p, st);
 }
 
 // ---------------------------------------------------------------------------------
@@ -991,9 +1003,76 @@ int tl_paged_kv_append(const void* q, void* q_out, const void* k_new, const void
   const int mode = !cos_table ? kNoRope : interleaved ? kInterleaved : kHalf;
   hipStream_t st = tl_resolve_stream(stream);
   switch (dtype) {
-    case TL_DTYPE_F32: return launch_append<F32>(p, mode, st);
-    case TL_DTYPE_F16: return launch_append<F16>(p, mode, st);
-    default: return launch_append<BF16>(p, mode, st);
+    case TL_DTYPE_F32: return launch_append<F32, false>(p, mode, st);
+    case TL_DTYPE_F16: return launch_append<F16, false>(p, mode, st);
+    default: return launch_append<BF16, false>(p, mode, st);
+  }
+}
+
+int tl_paged_kv_append_slots(const void* q, void* q_out, const void* k_new, const void* v_new, void* k_pages, void* v_pages,
+                             int n_pages, int page_size, const int32_t* slots, const int32_t* positions,
+                             const float* cos_table, const float* sin_table, int rope_rows, int rotary, int interleaved,
+                             int n_tokens, int n_head, int n_kv_head, int d_k, const int64_t* q_strides,
+                             const int64_t* q_out_strides, const int64_t* k_new_strides, const int64_t* v_new_strides,
+                             const int64_t* k_page_strides, const int64_t* v_page_strides, int dtype, void* stream) {
+  if (n_tokens == 0) return 0;
+  if (!k_new || !v_new || !k_pages || !v_pages || !slots || n_tokens < 0 || n_head < 0 || n_kv_head < 1 || d_k < 2 ||
+      (d_k & 1) || n_pages < 1 || !k_new_strides || !v_new_strides || !k_page_strides || !v_page_strides ||
+      !known_dtype(dtype))
+    return TL_ERR_INVALID;
+  const int shift = page_shift(page_size);
+  if (shift < 0 || ((int64_t)n_pages << shift) > INT32_MAX) return TL_ERR_INVALID;
+  if ((cos_table == nullptr) != (sin_table == nullptr)) return TL_ERR_INVALID;
+  if (cos_table && (!positions || rope_rows < 0 || rotary < 2 || (rotary & 1) || rotary > d_k)) return TL_ERR_INVALID;
+  const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
+  auto rows = [&](const void* at, int64_t heads, const int64_t* s) {
+    return Rows3{at, {n_tokens, heads, 1}, {s[0] * esize, s[1] * esize, 0}, (int64_t)d_k * esize};
+  };
+  auto pool = [&](const void* at, const int64_t* s) {
+    return Rows3{at, {n_pages, n_kv_head, page_size}, {s[0] * esize, s[1] * esize, s[2] * esize}, (int64_t)d_k * esize};
+  };
+  const Rows3 kp = pool(k_pages, k_page_strides), vp = pool(v_pages, v_page_strides);
+  const Rows3 kn = rows(k_new, n_kv_head, k_new_strides), vn = rows(v_new, n_kv_head, v_new_strides);
+  if (rows_overlap(kp, kn) || rows_overlap(kp, vn) || rows_overlap(vp, kn) || rows_overlap(vp, vn)) return TL_ERR_INVALID;
+  AppendParams p{};
+  if (q && n_head > 0) {
+    if (!q_out || !q_strides || !q_out_strides) return TL_ERR_INVALID;
+    const Rows3 from = rows(q, n_head, q_strides), to = rows(q_out, n_head, q_out_strides);
+    const bool same = q == q_out && q_strides[0] == q_out_strides[0] && q_strides[1] == q_out_strides[1];
+    if ((!same && rows_overlap(from, to)) || rows_overlap(to, kn) || rows_overlap(to, vn) || rows_overlap(to, kp) ||
+        rows_overlap(to, vp) || rows_overlap(from, kp) || rows_overlap(from, vp))
+      return TL_ERR_INVALID;
+    p.n_head = cos_table || q != q_out ? n_head : 0;  // nothing to do in place without positions
+    p.q = q;
+    p.qo = q_out;
+    p.q_ss = q_strides[0], p.q_sh = q_strides[1];
+    p.qo_ss = q_out_strides[0], p.qo_sh = q_out_strides[1];
+  }
+  p.kn = k_new;
+  p.vn = v_new;
+  p.kp = k_pages;
+  p.vp = v_pages;
+  p.pm = PageMap{nullptr, 0, n_pages, shift};
+  p.slots = slots;
+  p.positions = positions;
+  p.cos_t = cos_table;
+  p.sin_t = sin_table;
+  p.rope_rows = rope_rows;
+  p.rot_half = cos_table ? rotary / 2 : 0;
+  p.batch = 1;
+  p.n_new = n_tokens;
+  p.n_kv = n_kv_head;
+  p.d_k = d_k;
+  p.kn_ss = k_new_strides[0], p.kn_sh = k_new_strides[1];
+  p.vn_ss = v_new_strides[0], p.vn_sh = v_new_strides[1];
+  p.kp_sp = k_page_strides[0], p.kp_sh = k_page_strides[1], p.kp_sr = k_page_strides[2];
+  p.vp_sp = v_page_strides[0], p.vp_sh = v_page_strides[1], p.vp_sr = v_page_strides[2];
+  const int mode = !cos_table ? kNoRope : interleaved ? kInterleaved : kHalf;
+  hipStream_t st = tl_resolve_stream(stream);
+  switch (dtype) {
+    case TL_DTYPE_F32: return launch_append<F32, true>(p, mode, st);
+    case TL_DTYPE_F16: return launch_append<F16, true>(p, mode, st);
+    default: return launch_append<BF16, true>(p, mode, st);
   }
 }
 

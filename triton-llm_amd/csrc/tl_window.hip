@@ -19,11 +19,12 @@
 //
 // Bound by the matrix products and, at d_k 64, as much by exp and the conversions: 8192 tokens, window 1024, 24 / 8 heads
 // of 128, bf16: 126 to 137 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 40.7 to 43 us, by device.
+#include "tl_attn_tile.h"
 #include "tl_paged.h"
-#include "tl_prefill.h"
 
 #include <math.h>
 
+using namespace tlat;
 using namespace tlpg;
 
 namespace {
@@ -44,6 +45,8 @@ struct WinParams {
   PageMap pm;  // pages: k / v strides are {page, head, row}; else {batch, head, row}
   const int32_t* lens;
   const int32_t* new_lens;
+  const int32_t* starts;  // packed rows: sequence b's are q's rows starts[b] .. starts[b + 1] - 1 (q_sb = o_sb = 0), else NULL
+  int packed_rows;        // rows of q
   int batch, n_head, n_kv, group, seq_q, seq_k, n_qt;
   uint32_t group_magic;  // row / group = mulhi(row, group_magic) for the rows there are (group > 1)
   int window, sinks;
@@ -62,191 +65,29 @@ struct WinParams {
   float scale_log2;
 };
 
-// Keys of a tile.  fp32 rows are twice as long: half as many keys in the same LDS.
-template <typename T>
-constexpr int tile_keys() { return T::size == 2 ? 64 : 32; }
-
-// Slot of 16-byte chunk c of LDS row r is c ^ swz(r).  K: the 32 rows of an operand read take the same
-// chunk.  V: a transposing read takes 4 consecutive rows (see tl_prefill.hip); fp32 V
-// is read 32 consecutive words at a time and needs none.
-template <typename T, int D>
-__device__ __forceinline__ int k_swz(int r) {
-  if constexpr (T::size == 2) return tlp::lds_swz<D>(r);
-  else return r & 15;
-}
-template <typename T, int D>
-__device__ __forceinline__ int v_swz(int r) {
-  if constexpr (T::size == 4) return 0;
-  else return D == 64 ? 2 * ((r >> 1) & 1) : 4 * (r & 3);
-}
-
-// The matrix products of one 32-row block, by storage type.
-template <typename T, int D>
-struct Tile;
-
-template <typename T, int D>
-struct Tile16 {
-  using M = Mfma<T>;
-  using frag = typename M::frag;
-  static constexpr int ROWB = D * 2, NKS = D / 16, NDB = D / 32, NMB = 2;
-  struct Q {
-    frag f[NKS];
-  };
-  // sign: flips of the values' sign bits
-  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int h, uint32_t sign) {
-    sign |= sign >> 16;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      u32x4 x = u32x4{0u, 0u, 0u, 0u};
-      if (there) x = *(const u32x4*)(row + 32 * ks + 16 * h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] ^= sign;
-      q.f[ks] = __builtin_bit_cast(frag, x);
-    }
-  }
-  // Operands are read kAhead MFMAs ahead; the barriers keep the compiler from reading them all at
-  // once, which their registers do not allow at d_k 128.
-  static constexpr int kAhead = 4;
-  // The sum of a row's weights.  At d_k 64 the vector unit is the limit and the matrix unit half idle: there it is one
-  // more MFMA per 16 keys, ones . P^T, of the rounded weights (4 x 500 rows on prefixes, fp16: 51.4 -> 47.8 us).
-  static constexpr bool kSumMfma = D == 64;
-  // Weights are rounded to the storage type for the second product: an error of the size of the output's own rounding (a second
-  // word a weight takes it away, and 169 us for 134 at 8192 bf16 rows, 53 for 41 at 4 x 500 fp16 ones).  A weight is 2^kLift times exp2 of its score's
-  // distance to the running maximum, and that lags behind the largest score by kRescale at most.  bf16 has fp32's exponents:
-  // half a step each.  fp16 ends at 2^16 and is subnormal below 2^-14: lifted by 2^9 a weight is at most 2^15, has half a
-  // step down to 2^-23 of the row's largest, and below that an error of 2^-34 of it at most.  (A lift of 2^11 leaves 2^4 for
-  // the lag: 6000 rows, window 1024, 15 / 5 heads of 64, scores of deviation 6, 47.5 us for 45.5; of deviation 1 43 with either.)
-  static constexpr float kLift = T::code == TL_DTYPE_F16 ? 9.f : 0.f;
-  static constexpr float kRescale = T::code == TL_DTYPE_F16 ? 6.f : 8.f;
-  static __device__ __forceinline__ void scores(f32x16 (&s)[NMB], const Q& q, const char* kt, int lq, int h) {
-    constexpr int NG = NMB * NKS;
-    const char* row = kt + lq * ROWB;
-    const int sw = (h ^ k_swz<T, D>(lq)) << 4;
-    u32x4 f[NG];
-    auto fetch = [&](int g) __attribute__((always_inline)) {
-      f[g] = *(const u32x4*)(row + 32 * (g % NMB) * ROWB + (sw ^ ((g / NMB) << 5)));
-    };
-#pragma unroll
-    for (int g = 0; g < kAhead; ++g) fetch(g);
-#pragma unroll
-    for (int mb = 0; mb < NMB; ++mb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[mb][r] = 0.f;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      if (g + kAhead < NG) fetch(g + kAhead);
-      s[g % NMB] = M::mma(__builtin_bit_cast(frag, f[g]), q.f[g / NMB], s[g % NMB]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  // s holds the weights; they are rounded to the storage type here (see kLift).  The sum of a row's weights is
-  // of the rounded ones in la (kSumMfma) and of the unrounded ones in l otherwise, in fp32 either way: a weight's rounding
-  // then counts in numerator and denominator, or in the numerator alone, half a step of the output at most in both.
-  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt,
-                                                int lane) {
-    typedef short v4s __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) v4s lds_v4s;
-    constexpr int NG = 2 * NMB * NDB;
-    const int g16 = lane >> 4, e = (lane >> 2) & 3, c = lane & 3;
-    const auto* lds = (const __attribute__((address_space(3))) char*)vt + (4 * (g16 >> 1) + e) * ROWB + 8 * (c & 1);
-    const int sw = ((2 * (g16 & 1) + (c >> 1)) ^ v_swz<T, D>(e)) << 4;
-    u32x4 f[NG];
-    u32x4 pw[2 * NMB];
-    auto fetch = [&](int g) __attribute__((always_inline)) {
-      const auto* at = lds + 16 * (g / NDB) * ROWB + (sw ^ ((g % NDB) << 6));
-      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)at));
-      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(at + 8 * ROWB)));
-      f[g] = u32x4{a.x, a.y, b.x, b.y};
-    };
-#pragma unroll
-    for (int g = 0; g < kAhead; ++g) fetch(g);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int tt = g / NDB, db = g % NDB;
-      if (db == 0) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x[2] = {s[tt >> 1][8 * (tt & 1) + 2 * j], s[tt >> 1][8 * (tt & 1) + 2 * j + 1]};
-          pw[tt][j] = pack2<T>(x);
-        }
-      }
-      if (g + kAhead < NG) fetch(g + kAhead);
-      o[db] = M::mma(__builtin_bit_cast(frag, f[g]), __builtin_bit_cast(frag, pw[tt]), o[db]);
-      if (kSumMfma && db == 0) {
-        const frag ones = __builtin_bit_cast(frag, u32x4{T::one_pair, T::one_pair, T::one_pair, T::one_pair});
-        la = M::mma(ones, __builtin_bit_cast(frag, pw[tt]), la);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-};
-
-template <int D>
-struct Tile32 {
-  static constexpr int ROWB = D * 4, NDB = D / 32, NMB = 1;
-  static constexpr bool kSumMfma = false;
-  static constexpr float kLift = 0.f, kRescale = 8.f;
-  struct Q {
-    float f[D / 2];  // features h D / 2 .. of the row
-  };
-  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int h, uint32_t sign) {
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      u32x4 x = u32x4{0u, 0u, 0u, 0u};
-      if (there) x = *(const u32x4*)(row + h * (D * 2) + 16 * c);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q.f[4 * c + i] = __uint_as_float(x[i] ^ sign);
-    }
-  }
-  static __device__ __forceinline__ void scores(f32x16 (&s)[NMB], const Q& q, const char* kt, int lq, int h) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[0][r] = 0.f;
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) {
-      const f32x4 a = *(const f32x4*)(kt + lq * ROWB + (((h * (D / 8) + c) ^ k_swz<F32, D>(lq)) << 4));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], q.f[4 * c + i], s[0], 0, 0, 0);
-    }
-  }
-  static __device__ __forceinline__ void values(f32x16 (&o)[NDB], f32x16& la, const f32x16 (&s)[NMB], const char* vt,
-                                                int lane) {
-    const int lq = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int key = 8 * (r >> 2) + 4 * h + (r & 3);
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const float a = *(const float*)(vt + key * ROWB + (32 * db + lq) * 4);
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[0][r], o[db], 0, 0, 0);
-      }
-    }
-  }
-};
-
-template <int D>
-struct Tile<BF16, D> : Tile16<BF16, D> {};
-template <int D>
-struct Tile<F16, D> : Tile16<F16, D> {};
-template <int D>
-struct Tile<F32, D> : Tile32<D> {};
-
 // The token of a row.  Integer divisions are long dependent chains, and what runs before a short call's first
 // load counts: this one is a multiplication.
 __device__ __forceinline__ int token_of(const WinParams& p, int row) {
   return p.group == 1 ? row : (int)__umulhi((uint32_t)row, p.group_magic);
 }
 
-// Where a sequence's query rows stand: token i at position base + i, nq tokens, no key from `end` on.
+// Where a sequence's query rows stand: token i at position base + i and in row first + i of q, nq tokens, no key from `end` on.
 struct Rows {
-  int base, nq, end;
+  int base, nq, end, first;
 };
 template <bool PAGED>
 __device__ __forceinline__ Rows rows_of(const WinParams& p, int b) {
   Rows r;
+  r.first = 0;
   if constexpr (PAGED) {
     // rows before position -seq_q see nothing, as those there; lengths past 2^30 count as 2^30
     r.base = min(max(p.lens[b], -p.seq_q), 1 << 30);
-    r.nq = p.new_lens ? min(max(p.new_lens[b], 0), p.seq_q) : p.seq_q;
+    if (p.starts) {
+      r.first = min(max(p.starts[b], 0), p.packed_rows);
+      r.nq = min(max(min(p.starts[b + 1], p.packed_rows) - r.first, 0), p.seq_q);
+    } else {
+      r.nq = p.new_lens ? min(max(p.new_lens[b], 0), p.seq_q) : p.seq_q;
+    }
     r.end = min(r.base + r.nq, p.pm.max_pages << p.pm.shift);
   } else {
     r.base = p.seq_k - p.seq_q;
@@ -293,7 +134,7 @@ struct Seq {
 };
 template <int BN, bool PAGED>
 __device__ __forceinline__ Seq seq_at(const WinParams& p, int b) {
-  Seq s{{0, 0, 0}, 0, 0, 0, 0};
+  Seq s{{0, 0, 0, 0}, 0, 0, 0, 0};
   if (b < p.batch) {
     s.r = rows_of<PAGED>(p, b);
     s.tiles = (s.r.nq * p.group + kBM - 1) / kBM;
@@ -357,27 +198,7 @@ __device__ __forceinline__ int parts_upto(const WinParams& p, const Deal& d, int
 // Lane li's sequence, on every lane.
 __device__ __forceinline__ Seq seq_of_lane(const Seq& s, int li) {
   auto of = [&](int x) { return uni(__builtin_amdgcn_readlane(x, li)); };
-  return Seq{{of(s.r.base), of(s.r.nq), of(s.r.end)}, of(s.tiles), of(s.keys), of(s.parts), of(s.all)};
-}
-
-// Four neighbouring outputs, rounded to nearest even.
-template <typename T>
-__device__ __forceinline__ void store4(typename T::bits* d, float a, float b, float c, float e, int vec) {
-  if constexpr (T::size == 4) {
-    if (vec) {
-      *(f32x4*)d = f32x4{a, b, c, e};
-    } else {
-      d[0] = __float_as_uint(a), d[1] = __float_as_uint(b), d[2] = __float_as_uint(c), d[3] = __float_as_uint(e);
-    }
-  } else {
-    const float x[2] = {a, b}, y[2] = {c, e};
-    const uint32_t lo = pack2<T>(x), hi = pack2<T>(y);
-    if (vec) {
-      *(u32x2*)d = u32x2{lo, hi};
-    } else {
-      d[0] = (uint16_t)lo, d[1] = (uint16_t)(lo >> 16), d[2] = (uint16_t)hi, d[3] = (uint16_t)(hi >> 16);
-    }
-  }
+  return Seq{{of(s.r.base), of(s.r.nq), of(s.r.end), of(s.r.first)}, of(s.tiles), of(s.keys), of(s.parts), of(s.all)};
 }
 
 // A part's results: 32 rows a wave, each wave's m and l (by row) and then its O^T, the registers as
@@ -454,7 +275,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   const bool there = tok < rw.nq;
   const int pos = rw.base + tok;
   typename TL::Q q;
-  TL::load_q(q, (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh + (int64_t)tok * p.q_ss),
+  TL::load_q(q, (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh + (int64_t)(rw.first + tok) * p.q_ss),
              there && p.scale_log2 != 0.f,
              h, p.scale_log2 < 0.f ? 0x80000000u : 0u);
   const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
@@ -690,7 +511,7 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   }
   if (!there) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)tok * p.o_ss;
+  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)(rw.first + tok) * p.o_ss;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
@@ -745,7 +566,7 @@ __global__ __launch_bounds__(kThreads) void window_join_kernel(WinParams p) {
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)tok * p.o_ss;
+  B* out = (B*)p.o + b * p.o_sb + hq * p.o_sh + (int64_t)(s.r.first + tok) * p.o_ss;
 #pragma unroll
   for (int a = 0; a < 4; ++a)
     store4<T>(out + 32 * db + 8 * a + 4 * h, o[a][0] * inv, o[a][1] * inv, o[a][2] * inv, o[a][3] * inv, p.vec_out);
@@ -780,8 +601,12 @@ int64_t plan_slots(WinParams& p, int64_t tiles, int64_t keys, int d_k, int esize
 // padded batch planned by seq_q is taken for one with many row tiles, and its keys stay whole: one sequence of 500 rows on 4000
 // keys among 8 slots, 24 / 8 heads of 128, 41.1 us by its rows, 108 by seq_q (alone 39.5); beside seven tokens on 16000 keys
 // 94 and 320.
+// Packed rows are so many in all, whatever the lengths.
 int64_t row_tiles(const WinParams& p, const int32_t* counts) {
-  if (!counts) return (int64_t)p.batch * p.n_kv * p.n_qt;
+  if (!counts) {
+    const int64_t all = (int64_t)p.batch * p.n_qt, packed = p.batch + (int64_t)p.packed_rows * p.group / kBM;
+    return (p.packed_rows && packed < all ? packed : all) * p.n_kv;
+  }
   int64_t n = 0;
   for (int b = 0; b < p.batch; ++b) {
     const int64_t rows = counts[b] < 0 ? 0 : counts[b] < p.seq_q ? counts[b] : p.seq_q;
@@ -851,8 +676,9 @@ int window_entry(WinParams& p, bool paged, int64_t keys, const int32_t* counts, 
     return Rows3{at, {n0, n1, n2}, {s[0] * esize, s[1] * esize, s[2] * esize}, row};
   };
   const int64_t n0 = paged ? p.pm.n_pages : p.batch, n2 = paged ? (int64_t)1 << p.pm.shift : p.seq_k;
-  const Rows3 out = rows(p.o, p.batch, p.n_head, p.seq_q, os);
-  if (rows_overlap(out, rows(p.q, p.batch, p.n_head, p.seq_q, qs)) || rows_overlap(out, rows(p.k, n0, p.n_kv, n2, ks)) ||
+  const int64_t q0 = p.starts ? 1 : p.batch, q2 = p.starts ? p.packed_rows : p.seq_q;
+  const Rows3 out = rows(p.o, q0, p.n_head, q2, os);
+  if (rows_overlap(out, rows(p.q, q0, p.n_head, q2, qs)) || rows_overlap(out, rows(p.k, n0, p.n_kv, n2, ks)) ||
       rows_overlap(out, rows(p.v, n0, p.n_kv, n2, vs)))
     return TL_ERR_INVALID;
   p.group = p.n_head / p.n_kv;
@@ -900,6 +726,14 @@ size_t tl_window_workspace_bytes(int batch, int n_head, int n_kv_head, int seq_q
 
 size_t tl_paged_prefill_workspace_bytes(const int32_t* host_new_lens, int batch, int n_head, int n_kv_head, int seq_q,
                                         int most_keys, int d_k, int window, int sinks, int dtype) {
+  return tl_paged_packed_workspace_bytes(host_new_lens, 0, batch, n_head, n_kv_head, seq_q, most_keys, d_k, window, sinks,
+                                         dtype);
+}
+
+size_t tl_paged_packed_workspace_bytes(const int32_t* host_new_lens, int n_rows, int batch, int n_head, int n_kv_head,
+                                       int seq_q, int most_keys, int d_k, int window, int sinks, int dtype) {
+  if (n_rows < 0) return 0;
+  if (n_rows > 0 && seq_q > n_rows) seq_q = n_rows;
   if (batch < 1 || n_head < 1 || n_kv_head < 1 || n_head % n_kv_head || seq_q < 1 || seq_q > kMostRows || most_keys < 1 ||
       window < 0 || sinks < 0 || (d_k != 64 && d_k != 128) || !rows_ok(seq_q, n_head / n_kv_head) ||
       (dtype != TL_DTYPE_F32 && dtype != TL_DTYPE_F16 && dtype != TL_DTYPE_BF16))
@@ -908,6 +742,7 @@ size_t tl_paged_prefill_workspace_bytes(const int32_t* host_new_lens, int batch,
   p.batch = batch;
   p.n_kv = n_kv_head;
   p.group = n_head / n_kv_head;
+  p.packed_rows = n_rows;
   p.seq_q = seq_q;
   p.n_qt = (seq_q * p.group + kBM - 1) / kBM;
   p.window = window;
@@ -979,6 +814,37 @@ int tl_paged_attention_prefill_counted(const void* q, const void* k_pages, const
   p.sinks = sinks;
   return window_entry(p, true, (int64_t)max_pages << shift, host_new_lens, workspace, workspace_bytes, d_k, q_strides, k_page_strides,
                       v_page_strides, o_strides, sm_scale, dtype, stream);
+}
+
+int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, int max_pages,
+                              int n_pages, int page_size, const int32_t* cache_lens, const int32_t* starts,
+                              const int32_t* host_new_lens, void* o, void* workspace, size_t workspace_bytes, int batch,
+                              int n_rows, int max_new, int n_head, int n_kv_head, int d_k, const int64_t* q_strides,
+                              const int64_t* k_page_strides, const int64_t* v_page_strides, const int64_t* o_strides,
+                              float sm_scale, int window, int sinks, int dtype, void* stream) {
+  if (batch == 0 || n_head == 0 || n_rows == 0 || max_new == 0) return 0;
+  const int shift = page_shift(page_size);
+  if (!page_table || !cache_lens || !starts || n_rows < 0 || max_pages < 1 || n_pages < 1 || shift < 0 ||
+      ((int64_t)max_pages << shift) > (1 << 30) || !q_strides || !o_strides)
+    return TL_ERR_INVALID;
+  WinParams p{};
+  p.q = q;
+  p.k = k_pages;
+  p.v = v_pages;
+  p.o = o;
+  p.pm = PageMap{page_table, max_pages, n_pages, shift};
+  p.lens = cache_lens;
+  p.starts = starts;
+  p.packed_rows = n_rows;
+  p.batch = batch;
+  p.n_head = n_head;
+  p.n_kv = n_kv_head;
+  p.seq_q = max_new < n_rows ? max_new : n_rows;
+  p.window = window;
+  p.sinks = sinks;
+  const int64_t qs[] = {0, q_strides[1], q_strides[0]}, os[] = {0, o_strides[1], o_strides[0]};
+  return window_entry(p, true, (int64_t)max_pages << shift, host_new_lens, workspace, workspace_bytes, d_k, qs,
+                      k_page_strides, v_page_strides, os, sm_scale, dtype, stream);
 }
 
 }  // extern "C"

@@ -149,6 +149,35 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tl_copy_pages": (
         _c_int, [ctypes.POINTER(_vp), _c_int, _c_i64, _c_i64, _c_int, _i32p, _i32p, _c_int, _vp]),
     "tl_write_i32": (_c_int, [_vp, _c_i64, _i32p, _i32p, _c_int, _vp]),
+    "tl_pages_workspace_bytes": (_c_size, [_c_int]),
+    "tl_release_pages": (
+        _c_int, [_vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_size, _vp]),
+    "tl_assign_pages": (
+        _c_int,
+        [_vp, _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),
+    "tl_paged_kv_append_slots": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_int, _c_int, _i64p, _i64p, _i64p, _i64p, _i64p, _i64p, _c_int, _vp],
+    ),
+    "tl_paged_packed_workspace_bytes": (
+        _c_size, [_i32p, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "tl_paged_attention_packed": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _i32p, _vp, _vp, _c_size,
+         _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _c_int, _c_int, _vp],
+    ),
+    "tl_shared_plan_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "tl_shared_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "tl_shared_plan": (
+        _c_int,
+        [_vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_size, _vp]),
+    "tl_paged_attention_shared": (
+        _c_int,
+        [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_size, _c_int, _vp, _vp, _c_size,
+         _c_int, _c_int, _c_int, _c_int, _i64p, _i64p, _i64p, _i64p, _c_float, _c_int, _vp],
+    ),
     "tl_beam_max_select": (_c_int, []),
     "tl_beam_select_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
     "tl_beam_select": (

@@ -8,7 +8,8 @@ layers: the projection ``gemm``, ``rms_norm`` (plus the fused
 ``add_rms_norm``), ``swiglu`` and ``add``, and on-device next-token
 ``sample`` / ``sample_rows`` (the models' ``_sample``).  Serving many sequences
 adds the cache in pages (append, attention, page copies), attention through a
-sliding window, and beam search's selection.  The reference's gelu,
+sliding window, attention that reads a shared prefix once, page tables that the GPU keeps with packed
+batches, and beam search's selection.  The reference's gelu,
 layer_norm, softmax and embedding kernels (GPT-2 and host-side pieces) are
 outside this library's scope.
 """
@@ -33,13 +34,17 @@ from .paged import (
     allocate_kv_pages,
     copy_kv_pages,
     paged_attention_decode,
+    paged_attention_packed,
     paged_attention_prefill,
     paged_decode_workspace,
     paged_kv_append,
+    paged_kv_append_slots,
     paged_prefill_workspace_bytes,
     write_i32,
 )
 from .window import window_attention, window_attention_strided, window_workspace_bytes
+from .pages import assign_kv_pages, pages_workspace_bytes, release_kv_pages
+from .shared import SharedPlan, paged_attention_shared, plan_shared_attention, shared_workspace_bytes
 from .beam import beam_select, beam_workspace_bytes
 
 __all__ = [
@@ -74,6 +79,15 @@ __all__ = [
     "window_attention",
     "window_attention_strided",
     "window_workspace_bytes",
+    "paged_kv_append_slots",
+    "paged_attention_packed",
+    "assign_kv_pages",
+    "release_kv_pages",
+    "pages_workspace_bytes",
+    "SharedPlan",
+    "plan_shared_attention",
+    "paged_attention_shared",
+    "shared_workspace_bytes",
     "beam_select",
     "beam_workspace_bytes",
 ]

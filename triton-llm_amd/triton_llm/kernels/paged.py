@@ -13,7 +13,10 @@ sequences of any length share one pool, and a common prefix is held once:
 * :func:`paged_attention_prefill` -- many new tokens per sequence over their
   pages, a prefix that is there already among them;
 * :func:`copy_kv_pages` -- pages copied in every layer at once, for forks and
-  compaction.
+  compaction;
+* :func:`paged_kv_append_slots`, :func:`paged_attention_packed` -- the append and the attention of packed
+  batches, whose sequences' tokens stand one behind the other without padding
+  (:mod:`~triton_llm.kernels.pages` makes their slots).
 
 ``page_size`` is a power of two from 16 to 1024.  A table entry outside
 ``[0, n_pages)`` (-1, by convention) names no page: its positions are not written,
@@ -203,6 +206,70 @@ def paged_kv_append(q_dev, k_new, v_new, k_pages, v_pages, page_table, cache_len
     return q_out
 
 
+@functools.lru_cache(maxsize=1024)
+def _slots_plan(pool, v_pool, slots, positions, k, v, q, cos, sin):
+    """Strides and sizes of a packed append by its shapes."""
+    n_pages, n_kv, page_size, d_k = _check_pool(pool, v_pool)
+    if n_pages * page_size >= 1 << 31:
+        raise ValueError(f"{n_pages} pages of {page_size} exceed 2^31 - 1 slots")
+    if len(k) != 3 or k[1:] != (n_kv, d_k):
+        raise ValueError(f"k_new shape {k} is not (tokens, n_kv_head={n_kv}, d_k={d_k})")
+    if v != k:
+        raise ValueError(f"v_new shape {v} != k_new shape {k}")
+    n = k[0]
+    for name, shape in (("slots", slots), ("positions", positions)):
+        if shape is not None and shape != (n,):
+            raise ValueError(f"{name} must be int32 of shape ({n},), got {shape}")
+    if d_k % 2:
+        raise ValueError(f"d_k must be even, got {d_k}")
+    n_head = 0
+    if q is not None:
+        if len(q) != 3 or q[0] != n or q[2] != d_k:
+            raise ValueError(f"q shape {q} does not match k_new {k}")
+        n_head = q[1]
+        if n_head <= 0 or n_head % n_kv:
+            raise ValueError(f"n_head ({n_head}) must be a positive multiple of n_kv_head ({n_kv})")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos_dev and sin_dev must both be given or both be None")
+    if cos is not None and (cos != sin or len(cos) != 2 or not 1 <= cos[1] <= d_k // 2):
+        raise ValueError(f"cos/sin tables must be float32 (rows, r // 2) with r <= {d_k}, got {cos} and {sin}")
+    if cos is not None and positions is None:
+        raise ValueError("cos/sin tables are given without positions")
+    rows, rotary = (0, 0) if cos is None else (cos[0], 2 * cos[1])
+    q_str, kv_str = _lib.strides(n_head * d_k, d_k), _lib.strides(n_kv * d_k, d_k)
+    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
+    return (n_pages, page_size), (rows, rotary), (n, n_head, n_kv, d_k, q_str, q_str, kv_str, kv_str, p_str, p_str)
+
+
+def paged_kv_append_slots(q_dev, k_new, v_new, k_pages, v_pages, slots, positions=None, cos_dev=None, sin_dev=None,
+                          q_out=None, interleaved: bool = False):
+    """:func:`paged_kv_append` for packed rows: token t's k and v go to row ``slots[t] % page_size`` of page
+    ``slots[t] // page_size``, q and k turned to ``positions[t]``.
+
+    q_dev: ``(tokens, n_head, d_k)`` or None; k_new / v_new: ``(tokens, n_kv_head, d_k)``; slots and positions: int32
+    ``(tokens,)``, as :func:`~triton_llm.kernels.assign_kv_pages` gives them (positions None: without cos/sin only).  A token with a slot
+    outside the pool (-1) or a position outside cos/sin is skipped, q row and all.  No slot may be given twice.
+    """
+    for name, t in (("slots", slots), ("positions", positions)):
+        if t is not None and not _is_int32(t):
+            raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
+    pages, tables, sizes = _slots_plan(k_pages.shape, v_pages.shape, slots.shape, _shape(positions), k_new.shape, v_new.shape,
+                                       _shape(q_dev), _shape(cos_dev), _shape(sin_dev))
+    if q_dev is None:
+        if q_out is not None:
+            raise ValueError("q_out is given without q_dev")
+        code = dtype_code_of(k_new, v_new, k_pages, v_pages)
+    else:
+        q_out = q_dev if q_out is None else _same_output(q_out, q_dev)
+        code = dtype_code_of(k_new, v_new, k_pages, v_pages, q_dev)
+    if cos_dev is not None and not cos_dev.dtype.char == sin_dev.dtype.char == "f":
+        raise ValueError(f"cos/sin tables must be float32, got {cos_dev.dtype} and {sin_dev.dtype}")
+    launch(gpu.runtime().tl_paged_kv_append_slots, _ptr(q_dev), _ptr(q_out), k_new.ptr, v_new.ptr, k_pages.ptr, v_pages.ptr,
+           *pages, slots.ptr, _ptr(positions), _ptr(cos_dev), _ptr(sin_dev), *tables, 1 if interleaved else 0, *sizes, code,
+           None, what="paged_kv_append_slots")
+    return q_out
+
+
 def paged_decode_workspace(batch: int, n_head: int, n_kv_head: int, max_ctx: int, d_k: int):
     """A workspace of :func:`paged_attention_decode`, reusable by consecutive calls on the
     library stream (calls that overlap in time need one each).  Its size goes by the heads alone."""
@@ -303,6 +370,57 @@ def paged_attention_prefill(q_dev, k_pages, v_pages, page_table, cache_lens, n_h
     launch(gpu.runtime().tl_paged_attention_prefill_counted, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
            cache_lens.ptr, _ptr(new_lens), host_new_lens, out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes,
            float(sm_scale), int(window), int(sinks), code, None, what="paged_attention_prefill")
+    return out
+
+
+@gpu.plan_cache(1024)
+def _packed_plan(pool, v_pool, table, lens, starts, q, n_head, n_kv_head, max_new, window, sinks):
+    """Strides and sizes of packed attention by its shapes."""
+    n_pages, n_kv, page_size, d_k = _check_pool(pool, v_pool)
+    batch, max_pages = _check_table(table, lens, None, page_size, 1 << 30)
+    _check_heads(n_head, n_kv_head, n_kv, d_k)
+    check_window(window, sinks)
+    if starts != (batch + 1,):
+        raise ValueError(f"starts must be int32 of shape ({batch + 1},), got {starts}")
+    if len(q) != 3 or q[1:] != (n_head, d_k):
+        raise ValueError(f"q shape {q} is not (rows, n_head={n_head}, d_k={d_k})")
+    if max_new < 0:
+        raise ValueError(f"max_new must be >= 0, got {max_new}")
+    p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
+    q_str = _lib.strides(n_head * d_k, d_k)
+    ws = [_lib.load().tl_paged_packed_workspace_bytes(None, q[0], batch, n_head, n_kv_head, max_new, max_pages * page_size,
+                                                      d_k, window, sinks, code) for code in range(3)]  # by dtype code
+    return (max_pages, n_pages, page_size), (batch, q[0], max_new, n_head, n_kv_head, d_k, q_str, p_str, p_str, q_str), ws
+
+
+def paged_attention_packed(q_dev, k_pages, v_pages, page_table, cache_lens, starts, n_head: int, n_kv_head: int,
+                           max_new: int, sm_scale: float | None = None, window: int = 0, sinks: int = 0, out=None,
+                           workspace=None, host_new_lens=None):
+    """:func:`paged_attention_prefill` for packed rows: query i of sequence b is row ``starts[b] + i`` of q ``(rows, n_head,
+    d_k)``, at position ``cache_lens[b] + i``.
+
+    ``starts``: int32 ``(batch + 1,)`` on the device.  ``max_new``: the most rows that a sequence may have; rows behind them,
+    and rows of no sequence, are left as they were.  ``host_new_lens`` as there: the sequences' rows, where the host has them.
+    """
+    _check_int32(page_table, cache_lens, starts)
+    pages, sizes, ws_bytes = _packed_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape, starts.shape,
+                                          q_dev.shape, n_head, n_kv_head, max_new, window, sinks)
+    code = dtype_code_of(q_dev, k_pages, v_pages)
+    out = _same_output(out, q_dev)
+    if sizes[1] == 0 or max_new == 0:
+        return out
+    need = ws_bytes[code]
+    if host_new_lens is not None:
+        host_new_lens = _host_counts(host_new_lens, sizes[0])
+        # the plan without the counts has its room too: a captured call goes by that
+        need = max(need, _lib.load().tl_paged_packed_workspace_bytes(
+            host_new_lens, sizes[1], sizes[0], n_head, n_kv_head, max_new, pages[0] * pages[2], sizes[5], window, sinks, code))
+    ws = scratch(need, workspace, key="window")
+    if sm_scale is None:
+        sm_scale = default_scale(k_pages.shape[3])
+    launch(gpu.runtime().tl_paged_attention_packed, q_dev.ptr, k_pages.ptr, v_pages.ptr, page_table.ptr, *pages,
+           cache_lens.ptr, starts.ptr, host_new_lens, out.ptr, _ptr(ws), ws.nbytes if ws is not None else 0, *sizes,
+           float(sm_scale), int(window), int(sinks), code, None, what="paged_attention_packed")
     return out
 
 
