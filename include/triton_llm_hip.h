@@ -548,16 +548,18 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * least 0, at most max_pages * page_size); its first shared_lens[g] ones lie in the same pages for every sequence of the group
  * (any number of them, whole pages or not).  The caller promises that: only the first sequence's entries of the
  * table are read.  A sequence with L < shared_lens[g], or the only one of its group, is taken as one that shares nothing.  One
- * that is in no group keeps its row of o; one that sees nothing gets zeros.  Named twice in one group it is computed twice.
+ * that is in no group keeps its row of o; one that sees nothing gets zeros.  One that is named twice counts where it
+ * is named last.
  *
  * tl_shared_plan puts together who reads what, on the device, into `plan` (tl_shared_plan_bytes, 16-byte aligned): for all
  * layers of a step, as long as the lengths, groups and table stay.  tl_paged_attention_shared is one layer's attention by
  * it; q / o (batch, n_head, d_k) {batch, head}.  A plan of other sizes (batch, groups, heads, table, d_k or element size) is not followed:
  * o is left as it was.  The workspace (tl_shared_workspace_bytes, 16-byte aligned) needs no initialisation; calls that overlap
- * in time need one each.  o overlaps none of q and the pools.
+ * in time need one each.  o may be q (the same layout and address), and overlaps none of q and the pools otherwise.
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; batch and n_groups <= 65535, n_head / n_kv_head <= 128, max_pages *
- * page_size <= 2^30.  Hidden positions are not read, but for V rows of pages before the first own one in its block of 16.
- * With 16-bit types weights are rounded to the type for the product with V, as for tl_paged_attention_prefill.
+ * page_size <= 2^30, and at most 2^31 - 1 blocks of 16 positions over batch, KV heads and pages.  Hidden positions are not read.
+ * With 16-bit types the weights of shared keys are rounded to the type for the product with V, as for
+ * tl_paged_attention_prefill; those of a sequence's own keys are not.
  * Deterministic.
  * ------------------------------------------------------------------------- */
 size_t tl_shared_plan_bytes(int batch, int n_groups, int n_head, int n_kv_head, int d_k);

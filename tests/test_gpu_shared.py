@@ -176,8 +176,24 @@ def test_lengths_past_the_table():
 
 
 def test_a_sequence_named_twice():
-    c = Case("bfloat16", 4, 2, 64, 16, [96, 130, 50], [([0, 1, 1], 32)])
+    """It counts where it is named last."""
+    c = Case("bfloat16", 4, 2, 64, 16, [96, 130, 50, 70], [([0, 3, 1, 1], 32)])
     c.run()
+    c = Case("bfloat16", 4, 2, 64, 16, [96, 130, 50, 200], [([0, 1, 3], 64), ([3], 16)], blind=False)
+    c.run()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_output_over_the_queries(dtype):
+    c = Case(dtype, 6, 2, 64, 16, [700, 290, 257, 5000], [([3, 1, 0, 2], 256)], blind=False)
+    want = c.run()
+    members, starts, shared = c.lists()
+    q, table = P.dev(c.q, dtype), P.int32(c.table)
+    plan = plan_shared_attention(table, P.int32(c.lens), P.int32(members), P.int32(starts), P.int32(shared), 6, 2, 64, 16,
+                                 P.H.GPU_DTYPES[dtype])
+    out = paged_attention_shared(q, P.dev(c.kp, dtype), P.dev(c.vp, dtype), table, plan, 6, 2, out=q)
+    assert out is q
+    np.testing.assert_array_equal(P.back(q, dtype), want)
 
 
 def test_starts_that_go_back():

@@ -263,12 +263,12 @@ def test_c_shared_refuses():
     assert c_shared(batch=0) == c_shared(heads=(0, 2)) == 0
     for bad in (dict(q=NULL), dict(table=NULL), dict(plan=NULL), dict(o=NULL), dict(ws=NULL), dict(ws=odd), dict(plan=odd),
                 dict(batch=-1), dict(groups=0), dict(heads=(5, 2)), dict(max_pages=0), dict(n_pages=0), dict(page=12),
-                dict(max_pages=1 << 27), dict(dtype=BAD), dict(plan_bytes=64), dict(ws_bytes=64), dict(qs=None), dict(o=at(0)),
-                dict(o=at(16)), dict(o=at(32))):
+                dict(max_pages=1 << 27), dict(dtype=BAD), dict(plan_bytes=64), dict(ws_bytes=64), dict(qs=None), dict(o=at(0), os=_lib.strides(512, 128)),
+                dict(o=ctypes.c_void_p(at(0).value + 128)), dict(o=at(16)), dict(o=at(32))):
         assert c_shared(**bad) == 1, bad
     for bad in (dict(batch=65536), dict(groups=65536), dict(heads=(129, 1)), dict(d_k=96), dict(q=odd),
                 dict(qs=_lib.strides(512, 68)), dict(ks=_lib.strides(512, 64, 60)), dict(ks=_lib.strides(512, -64, 64)),
-                dict(ks=_lib.strides(512, 64, 1 << 25)), dict(os=_lib.strides(-512, 64))):
+                dict(ks=_lib.strides(512, 64, 1 << 25)), dict(os=_lib.strides(-512, 64)), dict(batch=40, max_pages=1 << 26)):
         assert c_shared(**bad) == 801, bad
     need = _lib.load().tl_shared_plan_bytes
     assert need(0, 1, 4, 2, 64) == need(3, 0, 4, 2, 64) == need(3, 1, 5, 2, 64) == need(3, 1, 4, 2, 32) == 0

@@ -10,10 +10,10 @@
 //
 // A sequence shorter than S_g, or the only one of its group, is taken as one that shares nothing.
 //
-// Two steps.  The plan (plan_kernel, one workgroup), from the lengths, which only the device knows: which sequences share,
-// and the list of items, each a tile of up to 128 query rows of one KV head and a range of keys, all of about the same length.
-// It holds for every layer of a model's step.  Then each layer's attention: a workgroup an item (shared_kernel) and, where a
-// row's keys are in several items, their join (shared_join_kernel).
+// A step has one plan (plan_one_kernel, one workgroup), from the lengths, which only the device knows: which sequences share, and a
+// list of items, each a tile of up to 128 query rows of one KV head and a range of keys, a group's or a sequence's own.  It holds for
+// every layer.  A layer's attention: a workgroup an item (shared_kernel) and, where a row's keys are in several items, their join
+// (shared_join_kernel).
 #include "tl_attn_tile.h"
 #include "tl_paged.h"
 
@@ -27,20 +27,20 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBM = 128;  // query rows of an item at most
 constexpr int kMostBatch = 65535;
-constexpr int kMinTiles = 4;  // key tiles of an item at least
+constexpr int kMinTiles = 2;  // key tiles of an item at least, if there are more
 constexpr int kScanThreads = 64 * kScanWaves;
 
-// Rows row0 .. of a block of R: row r is query head hkv * group + r % group of the i0 + r / group-th sequence that shares (i0
-// < 0: of sequence b), over positions [lo, hi) of sequence b's pages.  lo is a multiple of 16 but for the first own ones.
+// Rows row0 .. of R: row r is query head hkv * group + r % group of the i0 + r / group-th sequence that shares (i0 < 0: of sequence
+// b), over positions [lo, hi) of sequence b's pages.  lo is a multiple of 16 but for a sequence's first own ones.
 struct Item {
   int b, hkv, lo, hi;
-  int i0, row0, R, out;  // out: where the rows' results go in the workspace, -1: to o, as they are all there is
+  int i0, row0, R, out;  // out: the first row's place in the workspace, -1: the rows go to o, as these are all their keys
 };
 // Where the results of a sequence's heads are: of head hkv * group + g, the shared keys' at p_base + (hkv * p_parts + k) * R +
 // r0 + g and its own ones' at s_base + (hkv * s_parts + k) * group + g.
 struct Join {
-  int b, R, p_base, p_parts;
-  int r0, s_base, s_parts, done;  // done: an item has written o itself, or there is nothing to write
+  int R, p_base, p_parts, r0;
+  int s_base, s_parts, done, spare;  // done: there is nothing to join
 };
 struct Group {
   int shared, i0, R, tiles;
@@ -49,19 +49,22 @@ struct Group {
 
 // The plan's layout, from sizes that host and device know.
 struct PlanDims {
-  int batch, n_groups, n_kv, group, slots;
+  int batch, n_groups, n_kv, group;
+  int slots;  // workgroups that the device holds at once, about
+  // A unit is a KV head and a row tile of a group, or a KV head of a sequence.  The key tiles of all are at most slots * share, and of
+  // a unit's parts of `share` one is not full.
   __host__ __device__ int64_t max_items() const {
     const int64_t tiles = (int64_t)batch * group / kBM + (batch / 2 < n_groups ? batch / 2 : n_groups);
     return slots + n_kv * (batch + tiles);
   }
-  // rows of partial results: parts are at most 1 + tiles / share, and sum tiles / share at most slots
-  __host__ __device__ int64_t max_rows() const { return (int64_t)slots * (kBM + group) + 2ll * n_kv * group * batch; }
-  __host__ __device__ int64_t items_at() const { return 64; }
-  __host__ __device__ int64_t joins_at() const { return items_at() + max_items() * (int64_t)sizeof(Item); }
-  __host__ __device__ int64_t groups_at() const { return joins_at() + batch * (int64_t)sizeof(Join); }
+  __host__ __device__ int64_t max_rows() const { return (int64_t)slots * kBM + 2ll * n_kv * group * batch; }
+  __host__ __device__ int64_t joins_at() const { return 64; }
+  __host__ __device__ int64_t items_at() const { return joins_at() + batch * (int64_t)sizeof(Join); }
+  __host__ __device__ int64_t groups_at() const { return items_at() + max_items() * (int64_t)sizeof(Item); }
   __host__ __device__ int64_t before_at() const { return groups_at() + n_groups * (int64_t)sizeof(Group); }
   __host__ __device__ int64_t order_at() const { return before_at() + 4 * ((int64_t)batch + 1); }
-  __host__ __device__ int64_t bytes() const { return (order_at() + 4 * (int64_t)batch + 255) & ~(int64_t)255; }
+  __host__ __device__ int64_t named_at() const { return order_at() + 4 * (int64_t)batch; }
+  __host__ __device__ int64_t bytes() const { return (named_at() + 4 * (int64_t)batch + 255) & ~(int64_t)255; }
   // A word that a plan of other sizes does not begin with.
   __host__ __device__ uint32_t check(int cap, int esize, int d_k) const {
     uint32_t h = 0x9E3779B9u;
@@ -71,7 +74,7 @@ struct PlanDims {
 };
 struct Head {
   uint32_t check;
-  int n_items, n_joins;
+  int n_items;
 };
 
 struct PlanParams {
@@ -85,7 +88,158 @@ struct PlanParams {
   uint32_t check;
 };
 
-__global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
+// Key tiles from lo to hi, the first of them at lo's block of 16.
+__device__ __forceinline__ int tiles_of(int lo, int hi, int bn) {
+  return lo < hi ? (hi - (lo & ~(kBlk - 1)) + bn - 1) / bn : 0;
+}
+// Key tiles of an item at most: as many as `slots` workgroups have each if all end together.
+__device__ __forceinline__ int share_of(int64_t work, int slots) {
+  return (int)min(max((work + slots - 1) / slots, (int64_t)kMinTiles), (int64_t)1 << 30);
+}
+// The items of a sequence's own positions lo .. len - 1, t tiles in `parts` parts: at, at + 1, ..; base: their rows' place, -1: o.
+__device__ __forceinline__ void own_items(const PlanParams& p, Item* at, int b, int lo, int len, int t, int parts, int base) {
+  const int lo16 = lo & ~(kBlk - 1);
+  const int each = parts ? t / parts : 0, more = parts ? t - each * parts : 0;
+  for (int h = 0; h < p.d.n_kv; ++h) {
+    int t0 = 0;
+    for (int k = 0; k < parts; ++k) {
+      const int t1 = t0 + each + (k < more ? 1 : 0);
+      *at++ = Item{b, h, t0 ? lo16 + t0 * p.bn : lo, min(len, lo16 + t1 * p.bn), -1, 0, p.d.group,
+                   base < 0 ? -1 : base + (h * parts + k) * p.d.group};
+      t0 = t1;
+    }
+  }
+}
+// Item e of those of shared positions.  Workgroups are dealt to the 8 XCDs in turn: the row tiles of one range of keys stand 8
+// apart.
+__device__ __forceinline__ Item group_item(const PlanParams& p, const Group* groups, const int* order, int e) {
+  int lo = 0, hi = p.d.n_groups;  // the last group that begins at or before e, those without items passed over
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (groups[mid].item <= e) lo = mid;
+    else hi = mid;
+  }
+  const Group g = groups[lo];
+  const int rt = (g.R + kBM - 1) / kBM, ranges = p.d.n_kv * g.parts, in = e - g.item;
+  const int whole = ranges / 8 * 8 * rt;
+  int tile, range;
+  if (in < whole) {
+    const int r = in / 8, q = r / rt;
+    range = q * 8 + in % 8;
+    tile = r - q * rt;
+  } else {
+    const int some = ranges % 8;
+    tile = (in - whole) / some;
+    range = ranges - some + (in - whole) - tile * some;
+  }
+  const int h = range / g.parts, k = range - h * g.parts;
+  const int each = g.tiles / g.parts, more = g.tiles - each * g.parts;
+  const int t0 = k * each + min(k, more), t1 = t0 + each + (k < more ? 1 : 0);
+  return Item{order[g.i0], h, t0 * p.bn, min(g.shared, t1 * p.bn), g.i0, tile * kBM, g.R, g.row + range * g.R + tile * kBM};
+}
+
+constexpr int kOneBatch = 1024;  // sequences and groups that the plan of one pass holds: a thread each
+
+// Up to 1024 sequences and groups, a thread each of either: what the threads need of one another is in LDS.
+__global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
+  __shared__ int s_start[kOneBatch + 1], s_shared[kOneBatch], s_before[kOneBatch + 1], s_order[kOneBatch], s_named[kOneBatch];
+  __shared__ Group s_group[kOneBatch];
+  __shared__ int s_sums[4][kScanWaves];
+  const PlanDims& d = p.d;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = tid < d.batch ? p.members[tid] : -1;
+  s_named[tid] = -1;
+  if (tid < d.n_groups) {
+    s_start[tid] = min(max(p.starts[tid], 0), d.batch);
+    s_shared[tid] = min(max(p.shared[tid], 0), p.cap);
+  }
+  if (tid == 0) s_start[d.n_groups] = min(max(p.starts[d.n_groups], 0), d.batch);
+  const int64_t n = (unsigned)b < (unsigned)d.batch ? (int64_t)p.lens[b] + p.len_add : 0;
+  const int len = (int)(n < 0 ? 0 : n > p.cap ? p.cap : n);
+  // Sums over the threads up to and with each, four at once, and of all.
+  auto scan4 = [&](int (&x)[4], int (&total)[4]) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = wave_scan(x[i]);
+      if (lane == 63) s_sums[i][wave] = x[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int s = wave_scan(lane < kScanWaves ? s_sums[i][lane] : 0);
+      total[i] = last_lane(s);
+      if (wave) x[i] += uni(__builtin_amdgcn_readlane(s, wave - 1));
+    }
+  };
+  __syncthreads();
+  // this thread's sequence: its group, and whether it shares if the group does
+  int g = 0;
+  bool listed = (unsigned)b < (unsigned)d.batch && tid >= s_start[0] && tid < s_start[d.n_groups];
+  if (listed) atomicMax(&s_named[b], tid);
+  for (int hi = d.n_groups; hi - g > 1;) {
+    const int mid = (g + hi) >> 1;
+    if (s_start[mid] <= tid) g = mid;
+    else hi = mid;
+  }
+  const int shared = s_shared[g];
+  __syncthreads();
+  listed = listed && s_named[b] == tid;  // a sequence named twice is its last place's
+  const bool in = listed && shared > 0 && len >= shared;
+  int x[4] = {in ? 1 : 0, 0, 0, 0}, total[4];
+  scan4(x, total);
+  if (tid < d.batch) s_before[tid] = x[0] - (in ? 1 : 0);
+  if (tid == 0) s_before[d.batch] = total[0];
+  if (in) {
+    s_order[x[0] - 1] = b;
+    ((int*)(p.plan + d.order_at()))[x[0] - 1] = b;
+  }
+  __syncthreads();
+  auto sharing = [&](int i) { return s_before[max(s_start[i + 1], s_start[i])] - s_before[s_start[i]]; };
+  Group gr{};
+  if (tid < d.n_groups && sharing(tid) >= 2)
+    gr = Group{s_shared[tid], s_before[s_start[tid]], sharing(tid) * d.group, tiles_of(0, s_shared[tid], p.bn), 0, 0, 0, 0};
+  const int row_tiles = (gr.R + kBM - 1) / kBM;
+  const int peers = sharing(g), place = s_before[tid < d.batch ? tid : 0] - s_before[s_start[g]];
+  bool shares = in && peers >= 2 && place >= 0 && place < peers;
+  // work in 64 bits: the tiles' upper and lower halves
+  auto own_tiles = [&] { return listed ? tiles_of(shares ? shared : 0, len, p.bn) : 0; };
+  const int64_t both = (int64_t)row_tiles * gr.tiles + own_tiles();
+  x[0] = (int)(both & 0xFFFF), x[1] = (int)(both >> 16), x[2] = gr.R / d.group, x[3] = 0;
+  scan4(x, total);
+  if (total[2] > d.batch) {  // starts that go back: groups overlap, and nobody shares
+    shares = false;
+    gr = Group{};
+    x[0] = own_tiles() & 0xFFFF, x[1] = own_tiles() >> 16, x[2] = x[3] = 0;
+    scan4(x, total);
+  }
+  const int share = share_of((((int64_t)total[1] << 16) + total[0]) * d.n_kv, d.slots);
+  gr.parts = gr.R ? (gr.tiles + share - 1) / share : 0;
+  const int t = own_tiles(), parts = (t + share - 1) / share;
+  const bool direct = !shares && parts == 1;
+  const int gi = d.n_kv * gr.parts * ((gr.R + kBM - 1) / kBM), gn = d.n_kv * gr.parts * gr.R;
+  const int oi = d.n_kv * parts, on = direct ? 0 : oi * d.group;
+  x[0] = gi, x[1] = gn, x[2] = oi, x[3] = on;
+  scan4(x, total);
+  gr.item = x[0] - gi;
+  gr.row = x[1] - gn;
+  if (tid < d.n_groups) s_group[tid] = gr;
+  __syncthreads();
+  Item* const items = (Item*)(p.plan + d.items_at());
+  Join* const joins = (Join*)(p.plan + d.joins_at());
+  for (int e = tid; e < total[0]; e += kScanThreads) items[e] = group_item(p, s_group, s_order, e);
+  if (tid < d.batch && s_named[tid] < 0) joins[tid] = Join{0, 0, 0, 0, 0, 0, 1, 0};
+  if (listed) {
+    const int base = total[1] + x[3] - on;
+    const Group& of = s_group[g];
+    joins[b] = shares ? Join{of.R, of.row, of.parts, place * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
+    own_items(p, items + total[0] + x[2] - oi, b, shares ? shared : 0, len, t, parts, direct ? -1 : base);
+  }
+  if (tid == 0) *(Head*)p.plan = Head{p.check, total[0] + total[2]};
+}
+
+// Any number of them, 1024 at a time, with what the threads need of one another in the plan itself.
+__global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
   __shared__ int64_t sums[kScanWaves];
   const PlanDims& d = p.d;
   Item* const items = (Item*)(p.plan + d.items_at());
@@ -93,6 +247,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
   Group* const groups = (Group*)(p.plan + d.groups_at());
   int* const before = (int*)(p.plan + d.before_at());  // sequences that share before the i-th of the list
   int* const order = (int*)(p.plan + d.order_at());    // the sequences that share
+  int* const named = (int*)(p.plan + d.named_at());    // the last place of the list that names a sequence, -1: none
   const int tid = threadIdx.x;
   auto start_of = [&](int g) { return min(max(p.starts[g], 0), d.batch); };
   // The i-th of the list: its sequence (-1: none) and group, tokens, positions that it shares if the group does.
@@ -110,7 +265,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
     }
     m.g = lo;
     const int b = p.members[i];
-    if ((unsigned)b >= (unsigned)d.batch) return m;
+    if ((unsigned)b >= (unsigned)d.batch || named[b] != i) return m;
     m.b = b;
     const int64_t len = (int64_t)p.lens[b] + p.len_add;
     m.len = (int)(len < 0 ? 0 : len > p.cap ? p.cap : len);
@@ -118,8 +273,16 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
     m.shared = m.len >= sh ? sh : 0;
     return m;
   };
-  auto tiles_of = [&](int lo, int hi) { return lo < hi ? (hi - (lo & ~(kBlk - 1)) + p.bn - 1) / p.bn : 0; };
 
+  for (int b = tid; b < d.batch; b += kScanThreads) named[b] = -1;
+  __syncthreads();
+  for (int i = tid; i < d.batch; i += kScanThreads) {
+    const int b = p.members[i];
+    if (i >= start_of(0) && i < start_of(d.n_groups) && (unsigned)b < (unsigned)d.batch) atomicMax(&named[b], i);
+  }
+  __syncthreads();
+  for (int b = tid; b < d.batch; b += kScanThreads)
+    if (named[b] < 0) joins[b] = Join{0, 0, 0, 0, 0, 0, 1, 0};
   // who shares
   int64_t n = 0;
   for (int i0 = 0; i0 < d.batch; i0 += kScanThreads) {
@@ -133,11 +296,11 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
   }
   if (tid == 0) before[d.batch] = (int)n;
   __syncthreads();
-  // the groups' and the sequences' units: one for each KV head and row tile
-  int64_t work = 0, units = 0, rows = 0;
+  // the groups' key tiles, and where their items and results begin
+  int64_t work = 0, rows = 0;
   for (int g0 = 0; g0 < d.n_groups; g0 += kScanThreads) {
     const int g = g0 + tid;
-    int64_t w = 0, u = 0;
+    int64_t w = 0;
     Group x{};
     if (g < d.n_groups) {
       const int s = start_of(g), e = max(start_of(g + 1), s);
@@ -146,19 +309,17 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
       if (in >= 2) {
         x.shared = min(max(p.shared[g], 0), p.cap);
         x.R = in * d.group;
-        x.tiles = tiles_of(0, x.shared);
-        u = (x.R + kBM - 1) / kBM;
-        w = u * x.tiles;
+        x.tiles = tiles_of(0, x.shared, p.bn);
+        w = (int64_t)((x.R + kBM - 1) / kBM) * x.tiles;
       }
       groups[g] = x;
     }
     work += block_scan(w, sums).total;
-    units += block_scan(u, sums).total;
     rows += block_scan(x.R, sums).total;
   }
   if (rows > (int64_t)d.batch * d.group) {  // starts that go back: groups overlap, and nobody shares
     for (int g = tid; g < d.n_groups; g += kScanThreads) groups[g].R = groups[g].tiles = 0;
-    work = units = 0;
+    work = 0;
   }
   __syncthreads();
   // place of a sequence among its group's that share, -1: it shares nothing
@@ -169,17 +330,9 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
   };
   for (int i0 = 0; i0 < d.batch; i0 += kScanThreads) {
     const Member m = member(i0 + tid);
-    int t = 0;
-    if (m.b >= 0) t = tiles_of(place(m, i0 + tid) >= 0 ? m.shared : 0, m.len);
-    work += block_scan(t, sums).total;
-    units += block_scan(t > 0 ? 1 : 0, sums).total;
+    work += block_scan(m.b >= 0 ? tiles_of(place(m, i0 + tid) >= 0 ? m.shared : 0, m.len, p.bn) : 0, sums).total;
   }
-  work *= d.n_kv;
-  units *= d.n_kv;
-  // Key tiles of an item: items are about `slots`, and each unit's last one is short.
-  const int64_t aim = max((int64_t)d.slots - units, (int64_t)d.slots / 2);
-  const int64_t share = max((work + aim - 1) / aim, (int64_t)kMinTiles);
-  // where the groups' items and results begin
+  const int share = share_of(work * d.n_kv, d.slots);
   int64_t item = 0, row = 0;
   for (int g0 = 0; g0 < d.n_groups; g0 += kScanThreads) {
     const int g = g0 + tid;
@@ -201,69 +354,36 @@ __global__ __launch_bounds__(kScanThreads) void plan_kernel(PlanParams p) {
     row += sr.total;
   }
   __syncthreads();
-  const int p_items = (int)item;
-  // the sequences' own items, and where their results are
+  const int group_items = (int)item;
   for (int i0 = 0; i0 < d.batch; i0 += kScanThreads) {
-    const int i = i0 + tid;
-    const Member m = member(i);
-    const int j = m.b >= 0 ? place(m, i) : -1;
-    const int lo = j >= 0 ? m.shared : 0;
-    const int t = m.b >= 0 ? tiles_of(lo, m.len) : 0;
-    const int parts = (int)((t + share - 1) / share);
+    const Member m = member(i0 + tid);
+    const int j = m.b >= 0 ? place(m, i0 + tid) : -1;
+    const int lo = j >= 0 ? m.shared : 0, t = m.b >= 0 ? tiles_of(lo, m.len, p.bn) : 0, parts = (t + share - 1) / share;
     const bool direct = j < 0 && parts == 1;
-    const Scan si = block_scan((int64_t)d.n_kv * parts, sums);
-    const int64_t nr = direct ? 0 : (int64_t)d.n_kv * parts * d.group;
-    const Scan sr = block_scan(nr, sums);
-    const int base = (int)(row + sr.incl - nr);
-    if (i < d.batch) {
-      Join x{m.b, 0, 0, 0, 0, base, parts, direct || m.b < 0 ? 1 : 0};
-      if (j >= 0) {
-        const Group& g = groups[m.g];
-        x.R = g.R, x.p_base = g.row, x.p_parts = g.parts, x.r0 = j * d.group;
-      }
-      joins[i] = x;
-      Item* at = items + item + si.incl - (int64_t)d.n_kv * parts;
-      const int lo16 = lo & ~(kBlk - 1);
-      for (int h = 0; h < d.n_kv; ++h) {
-        int t0 = 0;
-        for (int k = 0; k < parts; ++k) {
-          const int t1 = t0 + t / parts + (k < t % parts ? 1 : 0);
-          *at++ = Item{m.b, h, t0 ? lo16 + t0 * p.bn : lo, min(m.len, lo16 + t1 * p.bn), -1, 0, d.group,
-                       direct ? -1 : base + (h * parts + k) * d.group};
-          t0 = t1;
-        }
-      }
+    const int oi = d.n_kv * parts, on = direct ? 0 : oi * d.group;
+    const Scan si = block_scan(oi, sums), sn = block_scan(on, sums);
+    if (m.b >= 0) {
+      const int base = (int)(row + sn.incl - on);
+      const Group& of = groups[m.g];
+      joins[m.b] = j >= 0 ? Join{of.R, of.row, of.parts, j * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
+      own_items(p, items + item + si.incl - oi, m.b, lo, m.len, t, parts, direct ? -1 : base);
     }
     item += si.total;
-    row += sr.total;
+    row += sn.total;
   }
-  // The groups' items.  Workgroups are dealt to the 8 XCDs in turn: the row tiles of one range of keys stand 8 apart.
-  for (int e = tid; e < p_items; e += kScanThreads) {
-    int lo = 0, hi = d.n_groups;  // the last group that begins at or before e, those without items passed over
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (groups[mid].item <= e) lo = mid;
-      else hi = mid;
-    }
-    const Group g = groups[lo];
-    const int rt = (g.R + kBM - 1) / kBM, ranges = d.n_kv * g.parts, in = e - g.item;
-    const int whole = ranges / 8 * 8 * rt;
-    int tile, range;
-    if (in < whole) {
-      range = in / (8 * rt) * 8 + in % 8;
-      tile = in / 8 % rt;
-    } else {
-      const int some = ranges % 8;
-      range = ranges - some + (in - whole) % some;
-      tile = (in - whole) / some;
-    }
-    const int h = range / g.parts, k = range - h * g.parts;
-    const int each = g.tiles / g.parts, more = g.tiles % g.parts;
-    const int t0 = k * each + min(k, more), t1 = t0 + each + (k < more ? 1 : 0);
-    items[e] = Item{order[g.i0], h, t0 * p.bn, min(g.shared, t1 * p.bn), g.i0, tile * kBM, g.R,
-                    g.row + range * g.R + tile * kBM};
-  }
-  if (tid == 0) *(Head*)p.plan = Head{p.check, (int)item, d.batch};
+  for (int e = tid; e < group_items; e += kScanThreads) items[e] = group_item(p, groups, order, e);
+  if (tid == 0) *(Head*)p.plan = Head{p.check, (int)item};
+}
+
+__device__ __forceinline__ float max_xor16(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_xor16(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 struct SharedParams {
@@ -285,9 +405,325 @@ struct SharedParams {
   float scale_log2;
 };
 
-// 4 waves of 32 rows; key tiles by LDS-DMA, the next one while this one is used.  Every row sees every key of the item.
+// The 16 x 16 matrix products of 16 keys with 16 query rows: scores S^T = K . Q^T, a lane then holding query row lane % 16 and
+// keys 4 (lane / 16) .. + 3, which is how O^T = V^T . P^T takes the weights.
 template <typename T, int D>
-__global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
+struct Narrow;
+
+template <typename T, int D>
+struct Narrow16 {
+  static constexpr int ROWB = D * 2;
+  struct Q {
+    u32x4 f[D / 32];
+  };
+  static __device__ __forceinline__ int kswz(int r) { return k_swz<T, D>(r); }
+  static __device__ __forceinline__ int vswz(int r) { return v_swz<T, D>(r & 3); }
+  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int g, uint32_t sign) {
+    sign |= sign >> 16;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) {
+      u32x4 x = u32x4{0u, 0u, 0u, 0u};
+      if (there) x = *(const u32x4*)(row + 64 * ks + 16 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] ^= sign;
+      q.f[ks] = x;
+    }
+  }
+  template <int NRB>
+  static __device__ __forceinline__ void scores(f32x4 (&s)[NRB], const Q (&q)[NRB], const char* kt, int lr, int g) {
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) s[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) {
+      const u32x4 a = *(const u32x4*)(kt + lr * ROWB + (((4 * ks + g) ^ kswz(lr)) << 4));
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb) {
+        if constexpr (T::code == TL_DTYPE_BF16)
+          s[rb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, q[rb].f[ks]), s[rb], 0, 0, 0);
+        else
+          s[rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, q[rb].f[ks]), s[rb], 0, 0, 0);
+      }
+    }
+  }
+  template <int NRB>
+  static __device__ __forceinline__ void values(f32x4 (&o)[NRB][D / 16], const f32x4 (&w)[NRB], const char* vt, int lane) {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s lds_v4s;
+    const int g = lane >> 4, e = (lane >> 2) & 3, c = lane & 3;
+    u32x2 pw[NRB];
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+      const float x[2] = {w[rb][0], w[rb][1]}, y[2] = {w[rb][2], w[rb][3]};
+      pw[rb] = u32x2{pack2<T>(x), pack2<T>(y)};
+    }
+    const auto* row = (const __attribute__((address_space(3))) char*)vt + (4 * g + e) * ROWB + 8 * (c & 1);
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) {
+      const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(row + (((2 * db + (c >> 1)) ^ vswz(e)) << 4)));
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb) {
+        if constexpr (T::code == TL_DTYPE_BF16)
+          o[rb][db] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, __builtin_bit_cast(v4s, pw[rb]), o[rb][db], 0, 0, 0);
+        else
+          o[rb][db] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, pw[rb]), o[rb][db], 0, 0, 0);
+      }
+    }
+  }
+};
+
+template <int D>
+struct Narrow32 {
+  static constexpr int ROWB = D * 4;
+  struct Q {
+    float f[D / 4];  // features g D / 4 .. of the row
+  };
+  static __device__ __forceinline__ int kswz(int r) { return r & 15; }
+  static __device__ __forceinline__ int vswz(int r) { return 4 * ((r >> 2) & 3); }
+  static __device__ __forceinline__ void load_q(Q& q, const char* row, bool there, int g, uint32_t sign) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      u32x4 x = u32x4{0u, 0u, 0u, 0u};
+      if (there) x = *(const u32x4*)(row + g * D + 16 * c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q.f[4 * c + i] = __uint_as_float(x[i] ^ sign);
+    }
+  }
+  template <int NRB>
+  static __device__ __forceinline__ void scores(f32x4 (&s)[NRB], const Q (&q)[NRB], const char* kt, int lr, int g) {
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) s[rb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      const f32x4 a = *(const f32x4*)(kt + lr * ROWB + (((g * (D / 16) + c) ^ kswz(lr)) << 4));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int rb = 0; rb < NRB; ++rb) s[rb] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], q[rb].f[4 * c + i], s[rb], 0, 0, 0);
+    }
+  }
+  template <int NRB>
+  static __device__ __forceinline__ void values(f32x4 (&o)[NRB][D / 16], const f32x4 (&w)[NRB], const char* vt, int lane) {
+    const int g = lane >> 4, lr = lane & 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) {
+        const float a = *(const float*)(vt + (4 * g + i) * ROWB + (((4 * db + (lr >> 2)) ^ vswz(4 * g)) << 4) + 4 * (lr & 3));
+#pragma unroll
+        for (int rb = 0; rb < NRB; ++rb) o[rb][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, w[rb][i], o[rb][db], 0, 0, 0);
+      }
+  }
+};
+
+template <int D>
+struct Narrow<BF16, D> : Narrow16<BF16, D> {};
+template <int D>
+struct Narrow<F16, D> : Narrow16<F16, D> {};
+template <int D>
+struct Narrow<F32, D> : Narrow32<D> {};
+
+// LDS of a workgroup: two key tiles of the wide form, and for the narrow one as many blocks of 16 keys a wave as keep two workgroups
+// (three at d_k 64 in 16 bits) on a CU.
+template <typename T, int D>
+constexpr int lds_bytes() { return D * T::size == 128 ? 48 << 10 : 64 << 10; }
+
+// Few rows, 16 NRB: every wave by itself takes blocks of 16 keys, w, w + 4, .., its own ring of them coming by LDS-DMA without a
+// barrier; the waves' states are joined at the end.
+template <typename T, int D, int NRB>
+__device__ __forceinline__ void narrow_item(const SharedParams& p, const Item& it, char* smem, float2 (&s_ml)[4][32]) {
+  using N = Narrow<T, D>;
+  using B = typename T::bits;
+  constexpr int ROWB = D * T::size, BLKB = kBlk * ROWB;
+  constexpr int NSL = ROWB / 16, RPR = 1024 / ROWB, NDMA = BLKB / 1024;
+  constexpr int NB = lds_bytes<T, D>() / (8 * BLKB);  // blocks in a wave's ring
+  static_assert(NB >= 1 && NB <= 3 && RPR >= 1, "the waits below");
+  const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6);
+  const int lr = lane & 15, g = lane >> 4;
+  const int b0 = it.lo >> kBlkShift;
+  const int blocks = ((it.hi + kBlk - 1) >> kBlkShift) - b0;
+  const int mine = (blocks - wave + 3) >> 2;  // this wave's
+  const int32_t* table = p.pm.table + (int64_t)it.b * p.pm.max_pages;
+  const int shift = p.pm.shift - kBlkShift;
+  // lane i: the page of this wave's block pages_t + i
+  int pages = 0;
+  auto look_up = [&](int t) __attribute__((always_inline)) {
+    const int e = (b0 + wave + 4 * min(t + lane, max(mine - 1, 0))) >> shift;
+    pages = e < p.pm.max_pages ? table[e] : -1;
+  };
+  look_up(0);
+  typename N::Q q[NRB];
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const int row = it.row0 + 16 * rb + lr;
+    const bool there = row < it.R;
+    const int seq = p.d.group == 1 ? row : (int)__umulhi((uint32_t)row, p.group_magic);
+    const int hq = there ? it.hkv * p.d.group + (row - seq * p.d.group) : 0;
+    const int b = !there || it.i0 < 0 ? it.b : ((const int*)(p.plan + p.d.order_at()))[it.i0 + seq];
+    N::load_q(q[rb], (const char*)((const B*)p.q + b * p.q_sb + hq * p.q_sh), there && p.scale_log2 != 0.f, g,
+              p.scale_log2 < 0.f ? 0x80000000u : 0u);
+  }
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+
+  const uint32_t k_row = (uint32_t)(p.k_sr * T::size), v_row = (uint32_t)(p.v_sr * T::size);
+  uint32_t koff[NDMA], voff[NDMA];
+#pragma unroll
+  for (int i = 0; i < NDMA; ++i) {
+    const int r = i * RPR + lane / NSL;
+    koff[i] = r * k_row + (((lane % NSL) ^ N::kswz(r)) << 4);
+    voff[i] = r * v_row + (((lane % NSL) ^ N::vswz(r)) << 4);
+  }
+  char* const ring = smem + wave * NB * 2 * BLKB;
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) char*)ring;
+  const char* const kbase = (const char*)((const B*)p.k + it.hkv * p.k_sh);
+  const char* const vbase = (const char*)((const B*)p.v + it.hkv * p.v_sh);
+  uint32_t gone = 0;  // places of the ring whose page is not there
+  // Rows past the last key, and rows of pages that are not there, read as zeros.
+  auto load = [&](int t) __attribute__((always_inline)) {
+    const int pos = (b0 + wave + 4 * t) << kBlkShift;
+    const int id = __builtin_amdgcn_readlane(pages, t & 63);
+    const bool page = (unsigned)id < (unsigned)p.pm.n_pages;
+    const int rows = page ? min(it.hi - pos, kBlk) : 0;
+    const int64_t at = page ? id : 0;
+    const int in = pos & ((1 << p.pm.shift) - 1);
+    const i32x4 rk = uniform_rsrc(kbase + at * p.k_sp * T::size + (int64_t)in * k_row, rows ? (rows - 1) * k_row + ROWB : 0);
+    const i32x4 rv = uniform_rsrc(vbase + at * p.v_sp * T::size + (int64_t)in * v_row, rows ? (rows - 1) * v_row + ROWB : 0);
+    const int place = t % NB;
+    gone = (gone & ~(1u << place)) | ((page ? 0u : 1u) << place);
+    const uint32_t la = lds0 + place * 2 * BLKB;
+    // a sequence's own keys are read once in the launch: they need not stay in the caches
+    if (it.i0 < 0) {
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) lds_dma16_nt(rk, koff[i], la + i * 1024);
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) lds_dma16_nt(rv, voff[i], la + BLKB + i * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) lds_dma16(rk, koff[i], la + i * 1024);
+#pragma unroll
+      for (int i = 0; i < NDMA; ++i) lds_dma16(rv, voff[i], la + BLKB + i * 1024);
+    }
+  };
+
+  f32x4 o[NRB][D / 16];
+  float m[NRB], l[NRB];
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    m[rb] = -INFINITY;
+    l[rb] = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) o[rb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int t = 0; t < NB; ++t)
+    if (t < mine) load(t);
+  for (int t = 0; t < mine; ++t) {
+    // blocks t + 1 .. are on their way
+    const int later = min(NB - 1, mine - 1 - t);
+    if (later >= 2) wait_vmcnt<NB >= 3 ? 4 * NDMA : 0>();
+    else if (later == 1) wait_vmcnt<NB >= 2 ? 2 * NDMA : 0>();
+    else wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    const char* kt = ring + (t % NB) * 2 * BLKB;
+    f32x4 s[NRB];
+    N::template scores<NRB>(s, q, kt, lr, g);
+    const int pos = (b0 + wave + 4 * t) << kBlkShift;
+    const bool hidden = (gone >> (t % NB)) & 1;
+    if (hidden || pos < it.lo || pos + kBlk > it.hi) {
+      asm volatile("");  // a branch: as selects the tests would run for every block
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = pos + 4 * g + i;
+        const bool seen = !hidden && at >= it.lo && at < it.hi;
+#pragma unroll
+        for (int rb = 0; rb < NRB; ++rb) s[rb][i] = seen ? s[rb][i] : -INFINITY;
+      }
+    }
+    float mx[NRB];
+    bool grow = false;
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+      mx[rb] = __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[rb][0], s[rb][1]),
+                                             __builtin_elementwise_maximum(s[rb][2], s[rb][3]));
+      mx[rb] = tlp::max_xor32(max_xor16(mx[rb])) * scale;
+      grow |= mx[rb] > m[rb] + Tile<T, D>::kRescale;
+    }
+    // the maximum moves only when a score passes it by kRescale (it only bounds the exponents)
+    if (__any(grow)) {
+#pragma unroll
+      for (int rb = 0; rb < NRB; ++rb) {
+        const float mn = fmaxf(m[rb], mx[rb]);
+        const float a = fast_exp2(m[rb] - (mn == -INFINITY ? 0.f : mn));
+        m[rb] = mn;
+        l[rb] *= a;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) o[rb][db] *= a;
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < NRB; ++rb) {
+      const float sh = m[rb] == -INFINITY ? 0.f : m[rb] - Tile<T, D>::kLift;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[rb][i] = fast_exp2(fmaf(s[rb][i], scale, -sh));
+        l[rb] += s[rb][i];
+      }
+    }
+    N::template values<NRB>(o, s, kt + BLKB, lane);
+    if (t + NB < mine) {
+      if (((t + NB) & 63) == 0) look_up(t + NB);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the block's place has been read
+      load(t + NB);
+    }
+  }
+
+  // the waves' states, through LDS: chunk c of row r's accumulators lies in place c ^ (r & 15)
+  constexpr int ROWS = 16 * NRB, CH = D / 4;
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) l[rb] = tlp::sum_xor32(sum_xor16(l[rb]));
+  __syncthreads();  // every wave is done with its ring
+  f32x4* const acc = (f32x4*)smem;
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const int r = 16 * rb + lr;
+    if (g == 0) s_ml[wave][r] = make_float2(m[rb] - Tile<T, D>::kLift, l[rb]);
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) acc[(wave * ROWS + r) * CH + ((4 * db + g) ^ (r & 15))] = o[rb][db];
+  }
+  __syncthreads();
+  const int rows = min(it.R - it.row0, ROWS);
+  for (int i = threadIdx.x; i < rows * CH; i += kThreads) {
+    const int r = i / CH, c = i - r * CH;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][r].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    f32x4 a = {0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 e = s_ml[w][r];
+      const float f = fast_exp2(e.x - base);
+      sum = fmaf(e.y, f, sum);
+      const f32x4 x = acc[(w * ROWS + r) * CH + (c ^ (r & 15))];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[k] = fmaf(x[k], f, a[k]);
+    }
+    if (it.out < 0) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      B* out = (B*)p.o + it.b * p.o_sb + (int64_t)(it.hkv * p.d.group + r) * p.o_sh + 4 * c;
+      store4<T>(out, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv, p.vec_out);
+    } else {
+      const int64_t at = it.out + r;
+      if (c == 0) p.ml[at] = make_float2(top, sum);
+      *(f32x4*)(p.acc + at * D + 4 * c) = a;
+    }
+  }
+}
+
+// More rows: 4 waves of 32.  Key tiles by LDS-DMA, the next one while this one is used.
+template <typename T, int D>
+__device__ __forceinline__ void wide_item(const SharedParams& p, const Item& it, char* smem) {
   using TL = Tile<T, D>;
   using B = typename T::bits;
   constexpr int BN = tile_keys<T>();
@@ -300,11 +736,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
   constexpr int NDB = TL::NDB, NMB = TL::NMB;
   constexpr int TB = BN / kBlk;  // blocks of a tile
   static_assert(WROWS <= kBlk && kBlk % WROWS == 0 && NDMA >= 1, "a wave's rows lie in one block");
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TILEB];  // (K, V) twice
-
-  const Head head = *(const Head*)p.plan;
-  if (head.check != p.check || (int)blockIdx.x >= head.n_items) return;
-  const Item it = ((const Item*)(p.plan + p.d.items_at()))[blockIdx.x];
   const int* order = (const int*)(p.plan + p.d.order_at());
 
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6);
@@ -455,13 +886,27 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
     return;
   }
   const int64_t at = it.out + 32 * wave + lq;
-  if (h == 0) p.ml[at] = make_float2(m, l);
+  if (h == 0) p.ml[at] = make_float2(m - TL::kLift, l);
   float* out = p.acc + at * D;
 #pragma unroll
   for (int db = 0; db < NDB; ++db)
 #pragma unroll
     for (int a = 0; a < 4; ++a)
       *(f32x4*)(out + 32 * db + 8 * a + 4 * h) = f32x4{o[db][4 * a], o[db][4 * a + 1], o[db][4 * a + 2], o[db][4 * a + 3]};
+}
+
+// A workgroup an item, by its rows.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(1024))) char smem[lds_bytes<T, D>()];
+  __shared__ float2 s_ml[4][32];
+  const Head head = *(const Head*)p.plan;
+  const Item it = ((const Item*)(p.plan + p.d.items_at()))[blockIdx.x];  // the grid is no larger than the room for them
+  if (head.check != p.check || (int)blockIdx.x >= head.n_items) return;
+  const int rows = it.R - it.row0;
+  if (rows <= 16) narrow_item<T, D, 1>(p, it, smem, s_ml);
+  else if (rows <= 32) narrow_item<T, D, 2>(p, it, smem, s_ml);
+  else wide_item<T, D>(p, it, smem);
 }
 
 // A wave a query head of a sequence: the states of its items, shared ones first.
@@ -471,11 +916,11 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   constexpr int NJ = D / 64, U = 8;
   const int lane = threadIdx.x & 63;
   const int64_t unit = (int64_t)blockIdx.x * (kThreads / 64) + uni((int)threadIdx.x >> 6);
-  const int i = (int)(unit / p.n_head), hq = (int)(unit - (int64_t)i * p.n_head);
+  const int b = (int)(unit / p.n_head), hq = (int)(unit - (int64_t)b * p.n_head);
+  if (b >= p.d.batch) return;
   const Head head = *(const Head*)p.plan;
-  if (head.check != p.check || i >= head.n_joins) return;
-  const Join x = ((const Join*)(p.plan + p.d.joins_at()))[i];
-  if (x.done) return;
+  const Join x = ((const Join*)(p.plan + p.d.joins_at()))[b];
+  if (head.check != p.check || x.done) return;
   const int hkv = hq / p.d.group, g = hq - hkv * p.d.group;
   const int parts = x.p_parts + x.s_parts;
   auto row_of = [&](int k) {
@@ -513,7 +958,7 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) l += __shfl_xor(l, off);
-  B* o = (B*)p.o + x.b * p.o_sb + (int64_t)hq * p.o_sh;
+  B* o = (B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh;
 #pragma unroll
   for (int j = 0; j < NJ; ++j) o[NJ * lane + j] = from_f32<T>(l == 0.f ? 0.f : a[j] / l);
 }
@@ -583,7 +1028,9 @@ int tl_shared_plan(const int32_t* cache_lens, int len_add, const int32_t* member
   const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
   p.bn = esize == 4 ? tile_keys<F32>() : tile_keys<BF16>();
   p.check = p.d.check(p.cap, esize, d_k);
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kScanThreads), 0, tl_resolve_stream(stream), p);
+  hipStream_t st = tl_resolve_stream(stream);
+  if (batch <= kOneBatch && n_groups <= kOneBatch) hipLaunchKernelGGL(plan_one_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
+  else hipLaunchKernelGGL(plan_many_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
   return tl_launch_status();
 }
 

@@ -58,7 +58,7 @@ def plan_shared_attention(page_table, cache_lens, members, group_starts, shared_
 
     page_table: int32 ``(batch, max_pages)``; cache_lens and members: int32 ``(batch,)``; group_starts: int32 ``(n_groups + 1,)``;
     shared_lens: int32 ``(n_groups,)``, all on the device.  Sequence b sees ``cache_lens[b] + len_add`` positions.  A member outside ``[0,
-    batch)`` is none; a sequence in no group is not computed.  One that is shorter than ``shared_lens[g]``, or the only one
+    batch)`` is none; a sequence in no group is not computed, one that is named twice counts where it is named last.  One that is shorter than ``shared_lens[g]``, or the only one
     of its group, shares nothing.  The plan holds for every layer, for as long as lengths, groups and table stay.  ``plan``: an
     earlier plan, which is written over if its sizes fit (it may be in use by calls issued before).
     """
@@ -96,9 +96,9 @@ def paged_attention_shared(q_dev, k_pages, v_pages, page_table, plan: SharedPlan
                            sm_scale: float | None = None, out=None, workspace=None):
     """One query per sequence, ``(batch, n_head, d_k)``, over its pages, by a plan of the step.
 
-    Results are those of ``paged_attention_decode`` without a window, to rounding (16-bit weights are rounded to the type, as in
+    Results are those of ``paged_attention_decode`` without a window, to rounding (in 16 bits the weights of shared keys are rounded to the type, as in
     ``paged_attention_prefill``).  A sequence that sees nothing gives zeros; the rows of sequences in no group are left
-    as they were.  ``out`` overlaps no input.
+    as they were.  ``out`` may be ``q_dev``.
     """
     if not _is_int32(page_table):
         raise ValueError(f"page_table must be int32, got {gpu.dtype_name(page_table.dtype)} {page_table.shape}")
