@@ -144,11 +144,12 @@ constexpr int kOneBatch = 1024;  // sequences and groups that the plan of one pa
 __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
   __shared__ int s_start[kOneBatch + 1], s_shared[kOneBatch], s_before[kOneBatch + 1], s_order[kOneBatch], s_named[kOneBatch];
   __shared__ Group s_group[kOneBatch];
-  __shared__ int s_sums[4][kScanWaves];
+  __shared__ int s_sums[4][kScanWaves], s_bucket[64];
   const PlanDims& d = p.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = tid < d.batch ? p.members[tid] : -1;
   s_named[tid] = -1;
+  if (tid < 64) s_bucket[tid] = 0;
   if (tid < d.n_groups) {
     s_start[tid] = min(max(p.starts[tid], 0), d.batch);
     s_shared[tid] = min(max(p.shared[tid], 0), p.cap);
@@ -224,7 +225,17 @@ __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
   gr.item = x[0] - gi;
   gr.row = x[1] - gn;
   if (tid < d.n_groups) s_group[tid] = gr;
+  // The longest own items first, by 64ths of a share: a launch of more items than workgroups ends with short ones (64 sequences of 1
+  // to 500 own positions, 24 / 8 heads of 128, bf16: 27.9 -> 22.6 us).  Among equals whoever comes first.
+  const int bucket = parts ? 63 - min(63, (int)((int64_t)(t / parts) * 64 / share)) : 0;
+  if (oi) atomicAdd(&s_bucket[bucket], oi);
   __syncthreads();
+  if (wave == 0) {
+    const int n = s_bucket[lane];
+    s_bucket[lane] = wave_scan(n) - n;
+  }
+  __syncthreads();
+  const int own_at = oi ? atomicAdd(&s_bucket[bucket], oi) : 0;
   Item* const items = (Item*)(p.plan + d.items_at());
   Join* const joins = (Join*)(p.plan + d.joins_at());
   for (int e = tid; e < total[0]; e += kScanThreads) items[e] = group_item(p, s_group, s_order, e);
@@ -233,7 +244,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
     const int base = total[1] + x[3] - on;
     const Group& of = s_group[g];
     joins[b] = shares ? Join{of.R, of.row, of.parts, place * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
-    own_items(p, items + total[0] + x[2] - oi, b, shares ? shared : 0, len, t, parts, direct ? -1 : base);
+    own_items(p, items + total[0] + own_at, b, shares ? shared : 0, len, t, parts, direct ? -1 : base);
   }
   if (tid == 0) *(Head*)p.plan = Head{p.check, total[0] + total[2]};
 }
