@@ -493,8 +493,8 @@ int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
  * the first row of each sequence, at most max_tokens; ends[b]: lens[b] and what was granted.  counts_out: pages
  * left on the stack, and how many sequences with new tokens were not granted.  counts_out may be counts; otherwise no
  * output overlaps an input or another.
- * Both: workspace of tl_pages_workspace_bytes, 16-byte aligned, no initialisation; calls that overlap in time
- * need one each.  batch <= 65535, n_pages * page_size and max_pages * page_size below 2^31.
+ * Its workspace (tl_pages_workspace_bytes, 16-byte aligned) needs no initialisation; calls that overlap in time need one
+ * each.  Both: batch <= 65535, n_pages * page_size and max_pages * page_size below 2^31.
  *
  * tl_paged_kv_append_slots: tl_paged_kv_append for packed rows.  Token t goes to row slots[t] % page_size of page slots[t] /
  * page_size, with the rotary positions of positions[t] (may be NULL without tables).  A token whose slot is outside
@@ -511,7 +511,7 @@ size_t tl_pages_workspace_bytes(int batch);
 int tl_release_pages(const int32_t* page_table, int max_pages, int page_size, const int32_t* lens,
                      const int32_t* ended, const int32_t* keep, int batch, int32_t* free_pages,
                      int n_pages, const int32_t* counts, int32_t* counts_out, int32_t* lens_out,
-                     void* workspace, size_t workspace_bytes, void* stream);
+                     void* stream);
 int tl_assign_pages(const int32_t* lens, const int32_t* new_lens, int batch, int32_t* page_table,
                     int max_pages, int page_size, const int32_t* free_pages, int n_pages,
                     const int32_t* counts, int32_t* counts_out, int max_tokens, int32_t* slots,
@@ -555,9 +555,9 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * layers of a step, as long as the lengths, groups and table stay.  tl_paged_attention_shared is one layer's attention by
  * it; q / o (batch, n_head, d_k) {batch, head}.  A plan of other sizes (batch, groups, heads, table, d_k or element size) is not followed:
  * o is left as it was.  The workspace (tl_shared_workspace_bytes, 16-byte aligned) needs no initialisation; calls that overlap
- * in time need one each.  o may be q (the same layout and address), and overlaps none of q and the pools otherwise.
+ * in time need one each.  o overlaps none of q and the pools.
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; batch and n_groups <= 65535, n_head / n_kv_head <= 128, max_pages *
- * page_size <= 2^30, and at most 2^31 - 1 blocks of 16 positions over batch, KV heads and pages.  Hidden positions are not read.
+ * page_size <= 2^30.  Hidden positions are not read.
  * With 16-bit types the weights of shared keys are rounded to the type for the product with V, as for
  * tl_paged_attention_prefill; those of a sequence's own keys are not.
  * Deterministic.

@@ -169,9 +169,9 @@ def at(i):
 
 
 def c_release(table=at(0), max_pages=7, page=16, lens=at(1), ended=at(2), keep=at(3), batch=3, free=at(4), n_pages=9, counts=at(5),
-              counts_out=at(6), lens_out=at(7), ws=at(8), ws_bytes=1 << 20):
+              counts_out=at(6), lens_out=at(7)):
     return _lib.load().tl_release_pages(table, max_pages, page, lens, ended, keep, batch, free, n_pages, counts, counts_out,
-                                        lens_out, ws, ws_bytes, None)
+                                        lens_out, None)
 
 
 def c_assign(lens=at(0), new=at(1), batch=3, table=at(2), max_pages=7, page=16, free=at(3), n_pages=9, counts=at(4),
@@ -183,9 +183,8 @@ def c_assign(lens=at(0), new=at(1), batch=3, table=at(2), max_pages=7, page=16, 
 def test_c_pages_refuse():
     odd = ctypes.c_void_p(0x10000008)
     for bad in (dict(table=NULL), dict(lens=NULL), dict(ended=NULL), dict(free=NULL), dict(counts=NULL), dict(counts_out=NULL),
-                dict(lens_out=NULL), dict(ws=NULL), dict(ws=odd), dict(ws_bytes=16), dict(batch=0), dict(max_pages=0),
-                dict(n_pages=0), dict(page=12), dict(lens_out=at(2)), dict(lens_out=ctypes.c_void_p(at(1).value + 4)),
-                dict(counts_out=ctypes.c_void_p(at(5).value + 4)), dict(free=at(0)), dict(counts_out=at(7)), dict(ws=at(4))):
+                dict(lens_out=NULL), dict(batch=0), dict(max_pages=0), dict(n_pages=0), dict(page=12), dict(lens_out=at(2)), dict(lens_out=ctypes.c_void_p(at(1).value + 4)),
+                dict(counts_out=ctypes.c_void_p(at(5).value + 4)), dict(free=at(0)), dict(counts_out=at(7))):
         assert c_release(**bad) == 1, bad
     for bad in (dict(lens=NULL), dict(new=NULL), dict(table=NULL), dict(free=NULL), dict(counts=NULL), dict(counts_out=NULL),
                 dict(slots=NULL), dict(positions=NULL), dict(starts=NULL), dict(ends=NULL), dict(ws=NULL), dict(ws=odd),
@@ -193,8 +192,8 @@ def test_c_pages_refuse():
                 dict(ends=at(0)), dict(starts=at(9)), dict(slots=at(7)), dict(table=at(3)),
                 dict(counts_out=ctypes.c_void_p(at(4).value + 4))):
         assert c_assign(**bad) == 1, bad
-    for fn in (c_release, c_assign):
-        assert fn(batch=65536, ws_bytes=1 << 30) == 801 and fn(max_pages=1 << 27, batch=1) == 801
+    assert c_release(batch=65536) == c_release(max_pages=1 << 27, batch=1) == 801
+    assert c_assign(batch=65536, ws_bytes=1 << 30) == c_assign(max_pages=1 << 27, batch=1) == 801
     assert c_assign(n_pages=1 << 27) == 801
 
 
@@ -263,12 +262,12 @@ def test_c_shared_refuses():
     assert c_shared(batch=0) == c_shared(heads=(0, 2)) == 0
     for bad in (dict(q=NULL), dict(table=NULL), dict(plan=NULL), dict(o=NULL), dict(ws=NULL), dict(ws=odd), dict(plan=odd),
                 dict(batch=-1), dict(groups=0), dict(heads=(5, 2)), dict(max_pages=0), dict(n_pages=0), dict(page=12),
-                dict(max_pages=1 << 27), dict(dtype=BAD), dict(plan_bytes=64), dict(ws_bytes=64), dict(qs=None), dict(o=at(0), os=_lib.strides(512, 128)),
+                dict(max_pages=1 << 27), dict(dtype=BAD), dict(plan_bytes=64), dict(ws_bytes=64), dict(qs=None), dict(o=at(0)), dict(o=at(0), os=_lib.strides(512, 128)),
                 dict(o=ctypes.c_void_p(at(0).value + 128)), dict(o=at(16)), dict(o=at(32))):
         assert c_shared(**bad) == 1, bad
     for bad in (dict(batch=65536), dict(groups=65536), dict(heads=(129, 1)), dict(d_k=96), dict(q=odd),
                 dict(qs=_lib.strides(512, 68)), dict(ks=_lib.strides(512, 64, 60)), dict(ks=_lib.strides(512, -64, 64)),
-                dict(ks=_lib.strides(512, 64, 1 << 25)), dict(os=_lib.strides(-512, 64)), dict(batch=40, max_pages=1 << 26)):
+                dict(ks=_lib.strides(512, 64, 1 << 25)), dict(os=_lib.strides(-512, 64))):
         assert c_shared(**bad) == 801, bad
     need = _lib.load().tl_shared_plan_bytes
     assert need(0, 1, 4, 2, 64) == need(3, 0, 4, 2, 64) == need(3, 1, 5, 2, 64) == need(3, 1, 4, 2, 32) == 0

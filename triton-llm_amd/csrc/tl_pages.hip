@@ -21,7 +21,6 @@ constexpr int kWaves = kScanWaves;
 constexpr int kMostBatch = 65535;
 constexpr int kOneBatch = 1024;     // sequences that one workgroup holds in LDS
 constexpr int kOneTokens = 8192;    // rows that one workgroup writes
-constexpr int kOneEntries = 32768;  // table entries that one workgroup looks through
 constexpr int kFillThreads = 256;
 constexpr int kSearchLds = 4096;    // sequences that the rows' workgroups search in LDS
 
@@ -43,23 +42,33 @@ struct AssignParams {
 
 __device__ __forceinline__ int64_t pages_of(int64_t n, int shift) { return (n + (1 << shift) - 1) >> shift; }
 
-// Grants, sequence by sequence, 1024 at a time; put(b, start, first, len) is called for each of them.
+// Grants, sequence by sequence, 1024 at a time; put(b, start, first, len) is called for each of them.  Sums can pass 32 bits: they are
+// of the upper and the lower halves of numbers that are cut off above what can be granted.
+struct GrantLds {
+  int sums[2][kWaves];
+  int taken, denied;
+};
 template <typename Put>
-__device__ __forceinline__ int grant(const AssignParams& p, int64_t (&sums)[kWaves], Put put) {
+__device__ __forceinline__ int grant(const AssignParams& p, GrantLds& lds, Put put) {
   const int avail = min(max(p.counts[0], 0), p.n_pages);
   const int64_t cap = (int64_t)p.max_pages << p.shift;
-  int64_t tokens = 0, needed = 0, taken = 0, denied = 0;
+  if (threadIdx.x == 0) lds.taken = lds.denied = 0;
+  int64_t tokens = 0, needed = 0;
   for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
     const int b = b0 + (int)threadIdx.x;
     const int64_t len = b < p.batch ? p.lens[b] : 0;
-    const int64_t add = b < p.batch ? max(p.new_lens[b], 0) : 0;
-    const Scan t = block_scan(add, sums);
-    const int64_t end = tokens + t.incl;
+    const int add = b < p.batch ? max(p.new_lens[b], 0) : 0;
+    int x[2] = {add & 0xFFFF, add >> 16}, total[2];
+    block_scan(x, total, lds.sums);
+    const int64_t end = tokens + ((int64_t)x[1] << 16) + x[0];
     const bool fine = len >= 0 && len + add <= cap && end <= p.tokens;
-    const int64_t need = fine ? pages_of(len + add, p.shift) - pages_of(len, p.shift) : 0;
-    const Scan n = block_scan(need, sums);
-    const int64_t upto = needed + n.incl;
+    const int need = fine ? (int)(pages_of(len + add, p.shift) - pages_of(len, p.shift)) : 0;
+    tokens += ((int64_t)total[1] << 16) + total[0];
+    x[0] = need & 0xFFFF, x[1] = need >> 16;
+    block_scan(x, total, lds.sums);
+    const int64_t upto = needed + ((int64_t)x[1] << 16) + x[0];
     const bool granted = fine && (need == 0 || upto <= avail);
+    needed += ((int64_t)total[1] << 16) + total[0];
     if (b < p.batch) {
       const int64_t start = end - add;
       const int s = (int)(start < p.tokens ? start : p.tokens);
@@ -68,17 +77,16 @@ __device__ __forceinline__ int grant(const AssignParams& p, int64_t (&sums)[kWav
       p.ends[b] = (int)(granted ? len + add : len);
       if (b == p.batch - 1) p.starts[p.batch] = (int)(end < p.tokens ? end : p.tokens);
       put(b, s, f, (int)len);
+      // granted needs are the first ones: their sum is the largest granted N_b
+      if (granted && need) atomicMax(&lds.taken, (int)upto);
+      if (!granted && add) atomicAdd(&lds.denied, 1);
     }
-    // granted needs are the first ones: their sum is the largest granted N_b
-    taken += block_scan(granted ? need : 0, sums).total;
-    denied += block_scan(!granted && add > 0 ? 1 : 0, sums).total;
-    tokens += t.total;
-    needed += n.total;
   }
-  // every thread has read counts, which counts_out may be, before the scans' barriers
+  __syncthreads();
+  // every thread has read counts, which counts_out may be
   if (threadIdx.x == 0) {
-    p.counts_out[0] = avail - (int)taken;
-    p.counts_out[1] = (int)denied;
+    p.counts_out[0] = avail - lds.taken;
+    p.counts_out[1] = lds.denied;
   }
   return avail;
 }
@@ -111,23 +119,22 @@ __device__ __forceinline__ void place_row(const AssignParams& p, int t, int avai
 
 // Few sequences and rows: one workgroup, one launch.
 __global__ __launch_bounds__(kThreads) void assign_one_kernel(AssignParams p) {
-  __shared__ int64_t sums[kWaves];
+  __shared__ GrantLds lds;
   __shared__ int s_start[kOneBatch + 1], s_first[kOneBatch], s_len[kOneBatch];
-  const int avail = grant(p, sums, [&](int b, int start, int first, int len) {
+  const int avail = grant(p, lds, [&](int b, int start, int first, int len) {
     s_start[b] = start;
     s_first[b] = first;
     s_len[b] = len;
     if (b == p.batch - 1) s_start[p.batch] = p.starts[p.batch];
   });
-  __syncthreads();
   for (int t = threadIdx.x; t < p.tokens; t += kThreads)
     place_row(p, t, avail, [&](int b) { return s_start[b]; }, [&](int b) { return s_first[b]; },
               [&](int b) { return s_len[b]; });
 }
 
 __global__ __launch_bounds__(kThreads) void assign_grant_kernel(AssignParams p) {
-  __shared__ int64_t sums[kWaves];
-  const int avail = grant(p, sums, [&](int b, int, int first, int) { p.first[b] = first; });
+  __shared__ GrantLds lds;
+  const int avail = grant(p, lds, [&](int b, int, int first, int) { p.first[b] = first; });
   if (threadIdx.x == 0) *p.base = avail;
 }
 
@@ -155,99 +162,94 @@ struct ReleaseParams {
   const int32_t* counts;
   int32_t* counts_out;
   int32_t* lens_out;
-  int32_t* found;  // workspace, by sequence: entries that name a page
-  int32_t* base;
   int batch, max_pages, n_pages, shift;
 };
 
-// Columns [lo, hi) of sequence b that are given back.
-struct Span {
-  int lo, hi;
-};
-__device__ __forceinline__ Span span_of(const ReleaseParams& p, int b) {
-  if (p.ended[b] == 0) return Span{0, 0};
-  const int64_t held = pages_of(max(p.lens[b], 0), p.shift);
-  return Span{p.keep ? max(p.keep[b], 0) : 0, (int)(held < p.max_pages ? held : p.max_pages)};
-}
+// One workgroup.  The columns that are given back are cut into pieces of 64, (sequence, column), and a wave takes kPieces of them at
+// a time: what names a page is counted by a ballot, the waves' counts meet in LDS, and every wave finds its places by a scan of all of
+// them.  The next pieces are on their way meanwhile.
+constexpr int kPieces = 4;
+constexpr int kRound = kPieces * kWaves;  // pieces of a round: as many as a wave has lanes
+static_assert(kRound == 64, "a wave scans a round's counts");
+constexpr int kMap = 1024;  // pieces whose sequences are known at a time
 
-// Entries of a sequence that name a page, a wave at a time; see(page, how many before it) for each.
-template <typename See>
-__device__ __forceinline__ int walk(const ReleaseParams& p, int b, const Span& s, See see) {
-  const int lane = threadIdx.x & 63;
-  const int32_t* row = p.table + (int64_t)b * p.max_pages;
-  int n = 0;
-  for (int c0 = s.lo; c0 < s.hi; c0 += 256) {
-    int page[4];
+__global__ __launch_bounds__(kThreads) void release_kernel(ReleaseParams p) {
+  __shared__ int sums[1][kWaves];
+  __shared__ int s_piece[kThreads + 1], s_lo[kThreads], s_hi[kThreads];  // by sequence: its first piece, its columns
+  __shared__ int s_seq[kMap];                                            // by piece: its sequence
+  __shared__ int s_count[2][kRound];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  int64_t at = min(max(p.counts[0], 0), p.n_pages);
+  for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+    const int b = b0 + tid;
+    int lo = 0, hi = 0;
+    if (b < p.batch) {
+      const int len = p.lens[b];
+      const bool ended = p.ended[b] != 0;
+      const int keep = p.keep ? p.keep[b] : 0;
+      if (ended) {
+        const int64_t held = pages_of(max(len, 0), p.shift);
+        lo = max(keep, 0);
+        hi = (int)(held < p.max_pages ? held : p.max_pages);
+      }
+      p.lens_out[b] = ended ? 0 : len;
+    }
+    const int pieces = lo < hi ? (hi - lo + 63) >> 6 : 0;
+    int x[1] = {pieces}, total[1];
+    block_scan(x, total, sums);
+    const int first = x[0] - pieces;
+    s_piece[tid] = first;
+    s_lo[tid] = lo;
+    s_hi[tid] = hi;
+    for (int m0 = 0; m0 < total[0]; m0 += kMap) {
+      __syncthreads();  // the map of the pieces before has been read
+      for (int i = max(first, m0); i < min(first + pieces, m0 + kMap); ++i) s_seq[i - m0] = tid;
+      __syncthreads();
+      const int n = min(total[0] - m0, kMap);
+      // this wave's pieces of round r
+      auto load = [&](int r, int (&page)[kPieces]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) page[u] = c0 + 64 * u + lane < s.hi ? row[c0 + 64 * u + lane] : -1;
+        for (int k = 0; k < kPieces; ++k) {
+          const int i = r * kRound + wave * kPieces + k;
+          page[k] = -1;
+          if (i < n) {
+            const int s = s_seq[i];
+            const int c = s_lo[s] + 64 * (m0 + i - s_piece[s]) + lane;
+            if (c < s_hi[s]) page[k] = p.table[(int64_t)(b0 + s) * p.max_pages + c];
+          }
+        }
+      };
+      const int rounds = (n + kRound - 1) / kRound;
+      int page[kPieces];
+      load(0, page);
+      for (int r = 0; r < rounds; ++r) {
+        uint64_t is[kPieces];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const bool is = (unsigned)page[u] < (unsigned)p.n_pages;
-      const uint64_t all = __ballot(is);
-      if (is) see(page[u], n + __popcll(all & (((uint64_t)1 << lane) - 1)));
-      n += __popcll(all);
+        for (int k = 0; k < kPieces; ++k) {
+          is[k] = __ballot((unsigned)page[k] < (unsigned)p.n_pages);
+          if (lane == k) s_count[r & 1][wave * kPieces + k] = __popcll(is[k]);
+        }
+        int next[kPieces];
+        if (r + 1 < rounds) load(r + 1, next);
+        __syncthreads();
+        const int c = s_count[r & 1][lane], upto = wave_scan(c);
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) {
+          const int64_t to = at + __builtin_amdgcn_readlane(upto - c, wave * kPieces + k) +
+                             __popcll(is[k] & (((uint64_t)1 << lane) - 1));
+          if (((is[k] >> lane) & 1) && to < p.n_pages) p.free_pages[to] = page[k];
+        }
+        at += last_lane(upto);
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) page[k] = r + 1 < rounds ? next[k] : -1;
+      }
     }
   }
-  return n;
-}
-
-__device__ __forceinline__ void put_back(const ReleaseParams& p, int64_t at, int page) {
-  if (at < p.n_pages) p.free_pages[at] = page;
-}
-__device__ __forceinline__ void put_counts(const ReleaseParams& p, int base, int64_t found) {
-  const int64_t n = base + found;
-  p.counts_out[0] = (int)(n < p.n_pages ? n : p.n_pages);
-  p.counts_out[1] = (int)(n < p.n_pages ? 0 : n - p.n_pages);
-}
-
-// Few table entries: one workgroup, a wave a sequence, one launch.
-__global__ __launch_bounds__(kThreads) void release_one_kernel(ReleaseParams p) {
-  __shared__ int64_t sums[kWaves];
-  __shared__ int s_found[kOneBatch];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int base = min(max(p.counts[0], 0), p.n_pages);
-  for (int b = wave; b < p.batch; b += kWaves) {
-    const int n = walk(p, b, span_of(p, b), [](int, int) {});
-    if (lane == 0) s_found[b] = n;
+  // every thread has read counts, which counts_out may be, before a barrier above
+  if (tid == 0) {
+    p.counts_out[0] = (int)(at < p.n_pages ? at : p.n_pages);
+    p.counts_out[1] = (int)(at < p.n_pages ? 0 : at - p.n_pages);
   }
-  __syncthreads();
-  const int mine = (int)threadIdx.x < p.batch ? s_found[threadIdx.x] : 0;
-  const Scan s = block_scan(mine, sums);
-  if ((int)threadIdx.x < p.batch) s_found[threadIdx.x] = (int)(s.incl - mine);
-  if (threadIdx.x == 0) put_counts(p, base, s.total);
-  __syncthreads();
-  for (int b = wave; b < p.batch; b += kWaves) {
-    const int64_t at = (int64_t)base + s_found[b];
-    walk(p, b, span_of(p, b), [&](int page, int i) { put_back(p, at + i, page); });
-    const int len = p.lens[b];
-    if (lane == 0) p.lens_out[b] = p.ended[b] ? 0 : len;
-  }
-}
-
-__global__ __launch_bounds__(256) void release_count_kernel(ReleaseParams p) {
-  const int b = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.base = min(max(p.counts[0], 0), p.n_pages);
-  if (b >= p.batch) return;
-  const int n = walk(p, b, span_of(p, b), [](int, int) {});
-  if ((threadIdx.x & 63) == 0) p.found[b] = n;
-}
-
-__global__ __launch_bounds__(256) void release_put_kernel(ReleaseParams p) {
-  const int b = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (b >= p.batch) return;
-  const Span s = span_of(p, b);
-  const bool last = b == p.batch - 1;
-  if (s.lo < s.hi || last) {
-    int64_t before = 0;
-    for (int i = lane; i < b; i += 64) before += p.found[i];
-#pragma unroll
-    for (int off = 32; off; off >>= 1) before += __shfl_xor(before, off);
-    const int base = *p.base;
-    walk(p, b, s, [&](int page, int i) { put_back(p, base + before + i, page); });
-    if (last && lane == 0) put_counts(p, base, before + p.found[b]);
-  }
-  const int len = p.lens[b];
-  if (lane == 0) p.lens_out[b] = p.ended[b] ? 0 : len;
 }
 
 bool apart(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -264,19 +266,18 @@ size_t tl_pages_workspace_bytes(int batch) {
 
 int tl_release_pages(const int32_t* page_table, int max_pages, int page_size, const int32_t* lens, const int32_t* ended,
                      const int32_t* keep, int batch, int32_t* free_pages, int n_pages, const int32_t* counts,
-                     int32_t* counts_out, int32_t* lens_out, void* workspace, size_t workspace_bytes, void* stream) {
+                     int32_t* counts_out, int32_t* lens_out, void* stream) {
   const int shift = page_shift(page_size);
-  if (!page_table || !lens || !ended || !free_pages || !counts || !counts_out || !lens_out || !workspace || batch < 1 ||
-      max_pages < 1 || n_pages < 1 || shift < 0 || ((uintptr_t)workspace & 15))
+  if (!page_table || !lens || !ended || !free_pages || !counts || !counts_out || !lens_out || batch < 1 || max_pages < 1 ||
+      n_pages < 1 || shift < 0)
     return TL_ERR_INVALID;
   if (batch > kMostBatch || ((int64_t)max_pages << shift) > INT32_MAX) return TL_ERR_UNSUPPORTED;
-  if (workspace_bytes < tl_pages_workspace_bytes(batch)) return TL_ERR_INVALID;
   const struct {
     const void* at;
     int64_t n;
   } in[] = {{page_table, (int64_t)batch * max_pages}, {ended, batch}, {keep, batch}, {lens, batch}, {counts, 2}},
-    out[] = {{free_pages, n_pages}, {lens_out, batch}, {counts_out, 2}, {workspace, batch + 4}};
-  for (int o = 0; o < 4; ++o) {
+    out[] = {{free_pages, n_pages}, {lens_out, batch}, {counts_out, 2}};
+  for (int o = 0; o < 3; ++o) {
     for (int i = 0; i < 5; ++i)
       if (!(o == 1 && i == 3 && lens_out == lens) && !(o == 2 && i == 4 && counts_out == counts) &&
           !apart(in[i].at, in[i].n, out[o].at, out[o].n))
@@ -284,18 +285,8 @@ int tl_release_pages(const int32_t* page_table, int max_pages, int page_size, co
     for (int i = 0; i < o; ++i)
       if (!apart(out[i].at, out[i].n, out[o].at, out[o].n)) return TL_ERR_INVALID;
   }
-  ReleaseParams p{page_table, lens, ended, keep, free_pages, counts, counts_out, lens_out,
-                  (int32_t*)workspace + 4, (int32_t*)workspace, batch, max_pages, n_pages, shift};
-  hipStream_t st = tl_resolve_stream(stream);
-  if (batch <= kOneBatch && (int64_t)batch * max_pages <= kOneEntries) {
-    hipLaunchKernelGGL(release_one_kernel, dim3(1), dim3(kThreads), 0, st, p);
-    return tl_launch_status();
-  }
-  const dim3 grid((batch + 3) / 4);
-  hipLaunchKernelGGL(release_count_kernel, grid, dim3(256), 0, st, p);
-  const int e = tl_launch_status();
-  if (e) return e;
-  hipLaunchKernelGGL(release_put_kernel, grid, dim3(256), 0, st, p);
+  ReleaseParams p{page_table, lens, ended, keep, free_pages, counts, counts_out, lens_out, batch, max_pages, n_pages, shift};
+  hipLaunchKernelGGL(release_kernel, dim3(1), dim3(kThreads), 0, tl_resolve_stream(stream), p);
   return tl_launch_status();
 }
 

@@ -157,22 +157,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
   if (tid == 0) s_start[d.n_groups] = min(max(p.starts[d.n_groups], 0), d.batch);
   const int64_t n = (unsigned)b < (unsigned)d.batch ? (int64_t)p.lens[b] + p.len_add : 0;
   const int len = (int)(n < 0 ? 0 : n > p.cap ? p.cap : n);
-  // Sums over the threads up to and with each, four at once, and of all.
-  auto scan4 = [&](int (&x)[4], int (&total)[4]) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = wave_scan(x[i]);
-      if (lane == 63) s_sums[i][wave] = x[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int s = wave_scan(lane < kScanWaves ? s_sums[i][lane] : 0);
-      total[i] = last_lane(s);
-      if (wave) x[i] += uni(__builtin_amdgcn_readlane(s, wave - 1));
-    }
-  };
+  auto scan4 = [&](int (&x)[4], int (&total)[4]) { block_scan(x, total, s_sums); };
   __syncthreads();
   // this thread's sequence: its group, and whether it shares if the group does
   int g = 0;

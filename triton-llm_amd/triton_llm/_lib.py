@@ -151,7 +151,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tl_write_i32": (_c_int, [_vp, _c_i64, _i32p, _i32p, _c_int, _vp]),
     "tl_pages_workspace_bytes": (_c_size, [_c_int]),
     "tl_release_pages": (
-        _c_int, [_vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp, _c_size, _vp]),
+        _c_int, [_vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _vp, _c_int, _vp, _vp, _vp, _vp]),
     "tl_assign_pages": (
         _c_int,
         [_vp, _vp, _c_int, _vp, _c_int, _c_int, _vp, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _vp, _vp, _c_size, _vp]),

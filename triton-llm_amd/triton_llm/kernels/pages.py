@@ -32,7 +32,7 @@ __all__ = ["assign_kv_pages", "release_kv_pages", "pages_workspace_bytes"]
 
 
 def pages_workspace_bytes(batch: int) -> int:
-    """Bytes of a ``workspace`` for :func:`assign_kv_pages` and :func:`release_kv_pages` (0: such a batch is not supported)."""
+    """Bytes of a ``workspace`` for :func:`assign_kv_pages` (0: such a batch is not supported)."""
     return int(_lib.load().tl_pages_workspace_bytes(batch))
 
 
@@ -69,8 +69,7 @@ def _shape(t):
     return None if t is None else t.shape
 
 
-def release_kv_pages(page_table, lens, ended, free_pages, counts, page_size: int, keep=None, lens_out=None, counts_out=None,
-                     workspace=None):
+def release_kv_pages(page_table, lens, ended, free_pages, counts, page_size: int, keep=None, lens_out=None, counts_out=None):
     """Give the pages of sequences with ``ended[b] != 0`` back; returns ``(lens_out, counts_out)``.
 
     They are those of columns ``keep[b]`` (int32 ``(batch,)``: leading pages that others have too; None: 0) up to
@@ -86,11 +85,10 @@ def release_kv_pages(page_table, lens, ended, free_pages, counts, page_size: int
     batch = page_table.shape[0] if page_table.shape else 0
     vectors = (("lens", batch, lens.shape), ("ended", batch, ended.shape), ("keep", batch, _shape(keep)),
                ("lens_out", batch, lens_out.shape))
-    batch, max_pages, n_pages, need = _plan(page_table.shape, free_pages.shape, page_size, vectors,
-                                            (counts.shape, counts_out.shape))
-    ws = scratch(need, workspace, key="pages")
+    batch, max_pages, n_pages, _ = _plan(page_table.shape, free_pages.shape, page_size, vectors,
+                                         (counts.shape, counts_out.shape))
     launch(gpu.runtime().tl_release_pages, page_table.ptr, max_pages, page_size, lens.ptr, ended.ptr, _ptr(keep), batch,
-           free_pages.ptr, n_pages, counts.ptr, counts_out.ptr, lens_out.ptr, ws.ptr, ws.nbytes, None,
+           free_pages.ptr, n_pages, counts.ptr, counts_out.ptr, lens_out.ptr, None,
            what="release_kv_pages")
     return lens_out, counts_out
 

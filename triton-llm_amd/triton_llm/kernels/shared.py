@@ -98,7 +98,7 @@ def paged_attention_shared(q_dev, k_pages, v_pages, page_table, plan: SharedPlan
 
     Results are those of ``paged_attention_decode`` without a window, to rounding (in 16 bits the weights of shared keys are rounded to the type, as in
     ``paged_attention_prefill``).  A sequence that sees nothing gives zeros; the rows of sequences in no group are left
-    as they were.  ``out`` may be ``q_dev``.
+    as they were.  ``out`` overlaps no input.
     """
     if not _is_int32(page_table):
         raise ValueError(f"page_table must be int32, got {gpu.dtype_name(page_table.dtype)} {page_table.shape}")
