@@ -250,11 +250,13 @@ def paged_kv_append_slots(q_dev, k_new, v_new, k_pages, v_pages, slots, position
     ``(tokens,)``, as :func:`~triton_llm.kernels.assign_kv_pages` gives them (positions None: without cos/sin only).  A token with a slot
     outside the pool (-1) or a position outside cos/sin is skipped, q row and all.  No slot may be given twice.
     """
-    for name, t in (("slots", slots), ("positions", positions)):
-        if t is not None and not _is_int32(t):
-            raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
-    pages, tables, sizes = _slots_plan(k_pages.shape, v_pages.shape, slots.shape, _shape(positions), k_new.shape, v_new.shape,
-                                       _shape(q_dev), _shape(cos_dev), _shape(sin_dev))
+    if slots.dtype.char != "i" or (positions is not None and positions.dtype.char != "i"):
+        for name, t in (("slots", slots), ("positions", positions)):
+            if t is not None and not _is_int32(t):
+                raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
+    pages, tables, sizes = _slots_plan(k_pages.shape, v_pages.shape, slots.shape, None if positions is None else positions.shape,
+                                       k_new.shape, v_new.shape, None if q_dev is None else q_dev.shape,
+                                       None if cos_dev is None else cos_dev.shape, None if sin_dev is None else sin_dev.shape)
     if q_dev is None:
         if q_out is not None:
             raise ValueError("q_out is given without q_dev")

@@ -36,37 +36,52 @@ def pages_workspace_bytes(batch: int) -> int:
     return int(_lib.load().tl_pages_workspace_bytes(batch))
 
 
+# What a call's shapes allow is found once for each combination of them, as in paged.py; types are looked at in every call.
+
 def _check_int32(**tensors) -> None:
     for name, t in tensors.items():
         if t is not None and not _is_int32(t):
             raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
 
 
-@functools.lru_cache(maxsize=256)
-def _plan(table, free, page_size, vectors, counts):
-    """(batch, max_pages, n_pages, workspace bytes) by shapes; vectors: those of a number for each sequence, by name."""
+def _check_pages(table, free, page_size, counts, counts_out):
     if len(table) != 2 or min(table) < 1:
         raise ValueError(f"page_table must be int32 (batch, max_pages), got {table}")
     check_page_size(page_size)
     if len(free) != 1 or free[0] < 1:
         raise ValueError(f"free_pages must be int32 (n_pages,), got {free}")
-    for name, n, shape in vectors:
-        if shape is not None and shape != (n,):
-            raise ValueError(f"{name} must be int32 of shape ({n},), got {shape}")
-    for shape in counts:
+    for shape in (counts, counts_out):
         if shape != (2,):
             raise ValueError(f"counts must be int32 of shape (2,), got {shape}")
-    batch, max_pages = table
-    if max(free[0], max_pages) * page_size >= 1 << 31:
-        raise ValueError(f"{max(free[0], max_pages)} pages of {page_size} exceed 2^31 - 1 positions")
-    need = pages_workspace_bytes(batch)
+    if max(free[0], table[1]) * page_size >= 1 << 31:
+        raise ValueError(f"{max(free[0], table[1])} pages of {page_size} exceed 2^31 - 1 positions")
+    need = pages_workspace_bytes(table[0])
     if need == 0:
-        raise ValueError(f"a batch of {batch} is not supported (at most 65535)")
-    return batch, max_pages, free[0], need
+        raise ValueError(f"a batch of {table[0]} is not supported (at most 65535)")
+    return need
 
 
-def _shape(t):
-    return None if t is None else t.shape
+def _check_vectors(**vectors) -> None:
+    for name, (shape, n) in vectors.items():
+        if shape is not None and shape != (n,):
+            raise ValueError(f"{name} must be int32 of shape ({n},), got {shape}")
+
+
+@functools.lru_cache(maxsize=256)
+def _release_plan(table, free, page_size, counts, counts_out, lens, ended, keep, lens_out):
+    _check_pages(table, free, page_size, counts, counts_out)
+    n = table[0]
+    _check_vectors(lens=(lens, n), ended=(ended, n), keep=(keep, n), lens_out=(lens_out, n))
+    return n, table[1], free[0]
+
+
+@functools.lru_cache(maxsize=256)
+def _assign_plan(table, free, page_size, counts, counts_out, cache_lens, new_lens, max_tokens, slots, positions, starts, ends):
+    need = _check_pages(table, free, page_size, counts, counts_out)
+    n = table[0]
+    _check_vectors(cache_lens=(cache_lens, n), new_lens=(new_lens, n), slots=(slots, max_tokens), positions=(positions, max_tokens),
+                   starts=(starts, n + 1), ends=(ends, n))
+    return n, table[1], free[0], need
 
 
 def release_kv_pages(page_table, lens, ended, free_pages, counts, page_size: int, keep=None, lens_out=None, counts_out=None):
@@ -78,18 +93,18 @@ def release_kv_pages(page_table, lens, ended, free_pages, counts, page_size: int
     ``counts_out`` (default: ``counts`` itself) the pages on the list and how many had no room on it (none, unless a page is given back twice).
     The table stays as it is.
     """
-    lens_out = lens if lens_out is None else lens_out
-    counts_out = counts if counts_out is None else counts_out
-    _check_int32(page_table=page_table, lens=lens, ended=ended, free_pages=free_pages, counts=counts, keep=keep,
-                 lens_out=lens_out, counts_out=counts_out)
-    batch = page_table.shape[0] if page_table.shape else 0
-    vectors = (("lens", batch, lens.shape), ("ended", batch, ended.shape), ("keep", batch, _shape(keep)),
-               ("lens_out", batch, lens_out.shape))
-    batch, max_pages, n_pages, _ = _plan(page_table.shape, free_pages.shape, page_size, vectors,
-                                         (counts.shape, counts_out.shape))
+    if lens_out is None:
+        lens_out = lens
+    if counts_out is None:
+        counts_out = counts
+    if not (page_table.dtype.char == lens.dtype.char == ended.dtype.char == free_pages.dtype.char == counts.dtype.char
+            == lens_out.dtype.char == counts_out.dtype.char == "i" and (keep is None or keep.dtype.char == "i")):
+        _check_int32(page_table=page_table, lens=lens, ended=ended, free_pages=free_pages, counts=counts, keep=keep,
+                     lens_out=lens_out, counts_out=counts_out)
+    batch, max_pages, n_pages = _release_plan(page_table.shape, free_pages.shape, page_size, counts.shape, counts_out.shape,
+                                              lens.shape, ended.shape, None if keep is None else keep.shape, lens_out.shape)
     launch(gpu.runtime().tl_release_pages, page_table.ptr, max_pages, page_size, lens.ptr, ended.ptr, _ptr(keep), batch,
-           free_pages.ptr, n_pages, counts.ptr, counts_out.ptr, lens_out.ptr, None,
-           what="release_kv_pages")
+           free_pages.ptr, n_pages, counts.ptr, counts_out.ptr, lens_out.ptr, None, what="release_kv_pages")
     return lens_out, counts_out
 
 
@@ -105,21 +120,23 @@ def assign_kv_pages(cache_lens, new_lens, page_table, free_pages, counts, page_s
     pages left, and the sequences with new tokens that were not granted.  ``out``: the four tensors, which
     overlap no input.
     """
-    counts_out = counts if counts_out is None else counts_out
+    if counts_out is None:
+        counts_out = counts
     if not 0 <= max_tokens < 1 << 31:
         raise ValueError(f"max_tokens must be >= 0 and fit in int32, got {max_tokens}")
-    batch = page_table.shape[0] if page_table.shape else 0
     if out is None:
+        batch = page_table.shape[0] if page_table.shape else 0
         out = tuple(gpu.allocate((n,), np.int32) for n in (max_tokens, max_tokens, batch + 1, batch))
     elif len(out) != 4:
         raise ValueError(f"out must be (slots, positions, starts, ends), got {len(out)} tensors")
     slots, positions, starts, ends = out
-    _check_int32(cache_lens=cache_lens, new_lens=new_lens, page_table=page_table, free_pages=free_pages, counts=counts,
-                 slots=slots, positions=positions, starts=starts, ends=ends, counts_out=counts_out)
-    vectors = (("cache_lens", batch, cache_lens.shape), ("new_lens", batch, new_lens.shape), ("slots", max_tokens, slots.shape),
-               ("positions", max_tokens, positions.shape), ("starts", batch + 1, starts.shape), ("ends", batch, ends.shape))
-    batch, max_pages, n_pages, need = _plan(page_table.shape, free_pages.shape, page_size, vectors,
-                                            (counts.shape, counts_out.shape))
+    if not (cache_lens.dtype.char == new_lens.dtype.char == page_table.dtype.char == free_pages.dtype.char == counts.dtype.char
+            == counts_out.dtype.char == slots.dtype.char == positions.dtype.char == starts.dtype.char == ends.dtype.char == "i"):
+        _check_int32(cache_lens=cache_lens, new_lens=new_lens, page_table=page_table, free_pages=free_pages, counts=counts,
+                     slots=slots, positions=positions, starts=starts, ends=ends, counts_out=counts_out)
+    batch, max_pages, n_pages, need = _assign_plan(page_table.shape, free_pages.shape, page_size, counts.shape, counts_out.shape,
+                                                   cache_lens.shape, new_lens.shape, max_tokens, slots.shape, positions.shape,
+                                                   starts.shape, ends.shape)
     ws = scratch(need, workspace, key="pages")
     launch(gpu.runtime().tl_assign_pages, cache_lens.ptr, new_lens.ptr, batch, page_table.ptr, max_pages, page_size,
            free_pages.ptr, n_pages, counts.ptr, counts_out.ptr, max_tokens, slots.ptr, positions.ptr, starts.ptr, ends.ptr,

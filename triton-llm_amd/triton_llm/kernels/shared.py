@@ -14,7 +14,7 @@ import numpy as np
 
 from triton_llm import _lib, gpu
 from ._common import default_scale, launch, scratch
-from .paged import _check_heads, _check_pool, _check_table, _is_int32, _same_output, check_page_size, dtype_code_of
+from .paged import _BF16, _check_heads, _check_pool, _check_table, _is_int32, _same_output, check_page_size, dtype_code_of
 
 __all__ = ["SharedPlan", "plan_shared_attention", "paged_attention_shared", "shared_workspace_bytes"]
 
@@ -62,12 +62,14 @@ def plan_shared_attention(page_table, cache_lens, members, group_starts, shared_
     of its group, shares nothing.  The plan holds for every layer, for as long as lengths, groups and table stay.  ``plan``: an
     earlier plan, which is written over if its sizes fit (it may be in use by calls issued before).
     """
-    for name, t in (("page_table", page_table), ("cache_lens", cache_lens), ("members", members),
-                    ("group_starts", group_starts), ("shared_lens", shared_lens)):
-        if not _is_int32(t):
-            raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
+    if not (page_table.dtype.char == cache_lens.dtype.char == members.dtype.char == group_starts.dtype.char
+            == shared_lens.dtype.char == "i"):
+        for name, t in (("page_table", page_table), ("cache_lens", cache_lens), ("members", members),
+                        ("group_starts", group_starts), ("shared_lens", shared_lens)):
+            if not _is_int32(t):
+                raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
     sizes, need = _plan_sizes(page_table.shape, cache_lens.shape, members.shape, group_starts.shape, shared_lens.shape, n_head,
-                              n_kv_head, d_k, page_size, gpu.dtype_code(dtype))
+                              n_kv_head, d_k, page_size, _BF16 if dtype is gpu.bfloat16 else gpu.dtype_code(dtype))
     if plan is None or plan.sizes != sizes or plan.buffer.nbytes < need:
         plan = SharedPlan(sizes, need)
     launch(gpu.runtime().tl_shared_plan, cache_lens.ptr, int(len_add), members.ptr, group_starts.ptr, shared_lens.ptr, sizes[0],
