@@ -105,6 +105,41 @@ def test_packed(dtype, D, page, window, sinks, counts):
 def test_packed_groups_and_single_tokens(Hq, Hkv):
     run_packed("bfloat16", Hq, Hkv, 64, 16, [0, 99, 3, 1000, 0, 17], [1] * 6, 0, 0)
     run_packed("float32", Hq, Hkv, 64, 16, [0, 99, 3, 1000, 0, 17], [1, 1, 30, 1, 2, 1], 0, 0)
+    run_packed("float16", Hq, Hkv, 128, 32, [0, 99, 3, 1000, -2, 17, 500], [1, 1, 30, 2, 3, 1, 6], 70, 20)
+    run_packed("float32", Hq, Hkv, 128, 64, [0, 99, 3, 1000, -2, 17, 500], [1, 1, 3, 2, 3, 1, 6], 1, 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+def test_packed_few_rows_every_length(dtype, D):
+    """Row tiles of up to 32 rows: blocks, rings and page look-ups that end everywhere; divided keys and whole ones."""
+    lens = [0, 14, 15, 16, 31, 48, 63, 64, 65, 127, 129, 191, 255, 300, 1100]
+    run_packed(dtype, 4, 2, D, 16, lens, [1] * len(lens), 0, 0)
+    run_packed(dtype, 8, 1, D, 16, lens, [1, 2, 3, 4] * 3 + [4, 1, 2], 0, 0)
+    run_packed(dtype, 3, 1, D, 64, [9000, 5], [1, 2], 0, 0)
+    run_packed(dtype, 3, 1, D, 16, [9000, 5], [5, 1], 3000, 100)
+
+
+def test_packed_pages_that_are_not_there():
+    rng = np.random.default_rng(9)
+    Hq, Hkv, D, page = 4, 2, 64, 16
+    lens, new = np.array([60, 200, 30], np.int32), np.array([1, 3, 40], np.int32)
+    total = lens + new
+    for dtype in DTYPES:
+        table = P.shuffled_table(rng, total, page, 14, 40)
+        table[0, 1], table[1, 5], table[1, 12], table[2, 0], table[2, 3] = -1, 40, 2 ** 31 - 1, -5, -1
+        keep = [np.arange(14 * page) < t for t in total]
+        kp, vp = (P.pool_with(rng, table, keep, (40, Hkv, page, D), dtype) for _ in range(2))
+        starts = np.concatenate([[0], np.cumsum(new)])
+        q = P.values(rng, (int(starts[-1]), Hq, D), dtype)
+        got = P.back(paged_attention_packed(P.dev(q, dtype), P.dev(kp, dtype), P.dev(vp, dtype), P.int32(table), P.int32(lens),
+                                            P.int32(starts), Hq, Hkv, 40), dtype)
+        for b in range(3):
+            at = slice(starts[b], starts[b + 1])
+            k, there = op.gather(on.from_storage(kp, dtype), table[b], int(total[b]))
+            v, _ = op.gather(on.from_storage(vp, dtype), table[b], int(total[b]))
+            want, tol = P.rows_want(q[at].transpose(1, 0, 2), k, v, lens[b] + np.arange(new[b]), there, 0, 0, D ** -0.5, dtype)
+            P.check(f"packed without pages {dtype} sequence {b}", got[at].transpose(1, 0, 2), want, tol)
 
 
 def test_packed_many_sequences():

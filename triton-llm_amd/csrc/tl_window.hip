@@ -19,8 +19,7 @@
 //
 // Bound by the matrix products and, at d_k 64, as much by exp and the conversions: 8192 tokens, window 1024, 24 / 8 heads
 // of 128, bf16: 126 to 137 us; 4 x 500 rows on prefixes of 2875 to 3835, 15 / 5 heads of 64, fp16: 40.7 to 43 us, by device.
-#include "tl_attn_tile.h"
-#include "tl_paged.h"
+#include "tl_attn_narrow.h"
 
 #include <math.h>
 
@@ -206,7 +205,63 @@ __device__ __forceinline__ Seq seq_of_lane(const Seq& s, int li) {
 template <int D>
 constexpr size_t part_floats() { return (size_t)4 * (64 + 64 * (D / 2)); }
 
-template <typename T, int D, bool PAGED>
+// The only row tile of a sequence of at most 16 NRB rows: the first wave's lanes get what they would hold after the tiles t_lo .. t_hi - 1.
+template <typename T, int D, int NRB>
+__device__ __forceinline__ void narrow_tile(const WinParams& p, int b, int hkv, const Rows& rw, const Keys& ks, int t_lo, int t_hi,
+                                            char* smem, float2 (&s_ml)[4][32], f32x16 (&o)[D / 32], float& m, float& l) {
+  using N = Narrow<T, D>;
+  using B = typename T::bits;
+  constexpr int BN = tile_keys<T>(), TB = BN / kBlk;
+  constexpr int NB = 4 * BN / (8 * kBlk) < 1 ? 1 : 4 * BN / (8 * kBlk);  // blocks in a wave's ring: 4 tiles of LDS
+  const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6);
+  const int lr = lane & 15, g = lane >> 4;
+  const int rows = rw.nq * p.group;
+  NarrowKeys k{p.pm, b, (const char*)((const B*)p.k + hkv * p.k_sh), (const char*)((const B*)p.v + hkv * p.v_sh),
+               p.k_sb * T::size, p.v_sb * T::size, (uint32_t)(p.k_ss * T::size), (uint32_t)(p.v_ss * T::size), ks.end,
+               ((t_hi - t_lo) * TB - wave + 3) >> 2};
+  auto pos_of = [&](int t) {
+    const int i = wave + 4 * t, tile = t_lo + i / TB;
+    return ks.key0(tile) * BN + kBlk * (i % TB);
+  };
+  int pages = narrow_pages(k, 0, pos_of);
+  typename N::Q q[NRB];
+  int pos[NRB];
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const int row = 16 * rb + lr, tok = token_of(p, row);
+    const bool there = row < rows;
+    pos[rb] = rw.base + tok;
+    N::load_q(q[rb], (const char*)((const B*)p.q + (there ? hkv * p.group + (row - tok * p.group) : 0) * p.q_sh +
+                                   (int64_t)(rw.first + (there ? tok : 0)) * p.q_ss),
+              there && p.scale_log2 != 0.f, g, p.scale_log2 < 0.f ? 0x80000000u : 0u);
+  }
+  NarrowState<D, NRB> st;
+  auto whole = [&](int at) {
+    return at + kBlk - 1 <= rw.base && at + kBlk <= ks.end &&
+           (p.window <= 0 || at > rw.base + rw.nq - 1 - p.window || at + kBlk <= p.sinks);
+  };
+  auto seen = [&](int key, int rb) {
+    return key <= pos[rb] && key < ks.end && (p.window <= 0 || key > pos[rb] - p.window || key < p.sinks);
+  };
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  narrow_stream<T, D, NRB, NB>(st, q, k, pages, smem, wave, lane, scale, true, pos_of, whole, seen);
+  narrow_join<T, D, NRB>(st, smem, s_ml, wave, lane);
+  const int lq = lane & 31, h = lane >> 5;
+  if (wave == 0 && lq < rows) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const f32x4 x = narrow_result<D, NRB>(smem, s_ml, lq, 8 * db + 2 * a + h, m, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[db][4 * a + e] = x[e];
+      }
+  }
+}
+
+// PACKED (and PAGED): the rows are packed (p.starts), and a row tile of few rows goes by 16 x 16 products: a packed batch is mostly
+// single tokens, whose 128-row tiles would be empty but for a few rows.
+template <typename T, int D, bool PAGED, bool PACKED>
 __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   using TL = Tile<T, D>;
   using B = typename T::bits;
@@ -420,30 +475,40 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     __builtin_amdgcn_s_setprio(0);
   };
 
-  if (t_lo < t_hi) {
-    look_up(t_lo);
-    load_tile(t_lo, 0);
-  }
-  for (int t = t_lo; t < t_hi; ++t) {
-    wait_vmcnt<0>();  // this wave's rows of tile t are in LDS
-    lds_barrier();    // everybody's are, and tile t - 1 has been read
-    const int buf = (t - t_lo) & 1;
-    const uint32_t gone = PAGED ? (uint32_t)(gone_lanes >> ((t - pages_t) * TB)) & ((1u << TB) - 1) : 0;
-    if (t + 1 < t_hi) {
-      if (PAGED && t + 1 - pages_t == 64 / TB) look_up(t + 1);
-      load_tile(t + 1, buf ^ 1);
+  bool narrow = false;
+  if constexpr (PACKED) {
+    narrow = rw.nq * p.group <= 32;
+    if (narrow) {
+      __shared__ float2 s_ml[4][32];
+      if (rw.nq * p.group <= 16) narrow_tile<T, D, 1>(p, b, hkv, rw, ks, t_lo, t_hi, smem, s_ml, o, m, l);
+      else narrow_tile<T, D, 2>(p, b, hkv, rw, ks, t_lo, t_hi, smem, s_ml, o, m, l);
     }
-    const int k0 = ks.key0(t) * BN;
-    // does any row of this wave see a key of the tile, and does every row see all of them
-    const bool any = wave_rows && k0 <= wp1 && (p.window <= 0 || k0 + BN - 1 > wp0 - p.window || k0 < p.sinks);
-    if (!any) continue;
-    const bool all = k0 + BN - 1 <= wp0 && k0 + BN <= ks.end && gone == 0 &&
-                     (p.window <= 0 || k0 > wp1 - p.window || k0 + BN <= p.sinks);
-    const char* kt = smem + buf * 2 * TILEB;
-    step(k0, kt, gone, all);
   }
-
-  l = TL::kSumMfma ? la[0] : tlp::sum_xor32(l);
+  if (!narrow) {
+    if (t_lo < t_hi) {
+      look_up(t_lo);
+      load_tile(t_lo, 0);
+    }
+    for (int t = t_lo; t < t_hi; ++t) {
+      wait_vmcnt<0>();  // this wave's rows of tile t are in LDS
+      lds_barrier();    // everybody's are, and tile t - 1 has been read
+      const int buf = (t - t_lo) & 1;
+      const uint32_t gone = PAGED ? (uint32_t)(gone_lanes >> ((t - pages_t) * TB)) & ((1u << TB) - 1) : 0;
+      if (t + 1 < t_hi) {
+        if (PAGED && t + 1 - pages_t == 64 / TB) look_up(t + 1);
+        load_tile(t + 1, buf ^ 1);
+      }
+      const int k0 = ks.key0(t) * BN;
+      // does any row of this wave see a key of the tile, and does every row see all of them
+      const bool any = wave_rows && k0 <= wp1 && (p.window <= 0 || k0 + BN - 1 > wp0 - p.window || k0 < p.sinks);
+      if (!any) continue;
+      const bool all = k0 + BN - 1 <= wp0 && k0 + BN <= ks.end && gone == 0 &&
+                       (p.window <= 0 || k0 > wp1 - p.window || k0 + BN <= p.sinks);
+      const char* kt = smem + buf * 2 * TILEB;
+      step(k0, kt, gone, all);
+    }
+    l = TL::kSumMfma ? la[0] : tlp::sum_xor32(l);
+  }
   // Divided keys: a wave leaves its part's results.  Where a row tile has few parts (p.tag: see window_entry) it waits for
   // its stores and then leaves the call's tag.  A wave that
   // finds the tags of all parts there (the last one does; several may, and write the same) adds them up in the
@@ -633,8 +698,9 @@ int launch_window(WinParams& p, bool paged, hipStream_t st) {
   p.n_lvl = (p.n_qt + (1 << p.q_shift) - 1) >> p.q_shift;
   p.xcd_groups = (int)((units << p.q_shift) / 8);
   const dim3 grid(p.slots > 0 ? (unsigned)((p.room + 7) / 8 * 8) : (unsigned)(8 * p.xcd_groups * p.n_lvl));
-  if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true>), grid, dim3(kThreads), 0, st, p);
-  else hipLaunchKernelGGL((window_fwd_kernel<T, D, false>), grid, dim3(kThreads), 0, st, p);
+  if (p.starts) hipLaunchKernelGGL((window_fwd_kernel<T, D, true, true>), grid, dim3(kThreads), 0, st, p);
+  else if (paged) hipLaunchKernelGGL((window_fwd_kernel<T, D, true, false>), grid, dim3(kThreads), 0, st, p);
+  else hipLaunchKernelGGL((window_fwd_kernel<T, D, false, false>), grid, dim3(kThreads), 0, st, p);
   const int e = tl_launch_status();
   if (e || p.slots == 0 || p.tag) return e;
   const dim3 join((unsigned)tiles, D / 32);
