@@ -124,9 +124,9 @@ __device__ __forceinline__ Scan block_scan(int64_t x, int64_t (&sums)[kScanWaves
   return Scan{x + (wave ? before : 0), __shfl(s, kScanWaves - 1)};
 }
 
-// The same of N numbers at once, whose sums fit in 32 bits.
-template <int N>
-__device__ __forceinline__ void block_scan(int (&x)[N], int (&total)[N], int (&sums)[N][kScanWaves]) {
+// The same of N numbers at once, whose sums fit in 32 bits, of a workgroup of W waves.
+template <int N, int W>
+__device__ __forceinline__ void block_scan(int (&x)[N], int (&total)[N], int (&sums)[N][W]) {
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6);
   __syncthreads();  // the sums of the scan before have been read
 #pragma unroll
@@ -137,7 +137,7 @@ __device__ __forceinline__ void block_scan(int (&x)[N], int (&total)[N], int (&s
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int s = wave_scan(lane < kScanWaves ? sums[i][lane] : 0);
+    const int s = wave_scan(lane < W ? sums[i][lane] : 0);
     total[i] = last_lane(s);
     if (wave) x[i] += __builtin_amdgcn_readlane(s, wave - 1);
   }

@@ -95,18 +95,22 @@ __device__ __forceinline__ int tiles_of(int lo, int hi, int bn) {
 __device__ __forceinline__ int share_of(int64_t work, int slots) {
   return (int)min(max((work + slots - 1) / slots, (int64_t)kMinTiles), (int64_t)1 << 30);
 }
-// The items of a sequence's own positions lo .. len - 1, t tiles in `parts` parts: at, at + 1, ..; base: their rows' place, -1: o.
-__device__ __forceinline__ void own_items(const PlanParams& p, Item* at, int b, int lo, int len, int t, int parts, int base) {
-  const int lo16 = lo & ~(kBlk - 1);
-  const int each = parts ? t / parts : 0, more = parts ? t - each * parts : 0;
-  for (int h = 0; h < p.d.n_kv; ++h) {
-    int t0 = 0;
-    for (int k = 0; k < parts; ++k) {
-      const int t1 = t0 + each + (k < more ? 1 : 0);
-      *at++ = Item{b, h, t0 ? lo16 + t0 * p.bn : lo, min(len, lo16 + t1 * p.bn), -1, 0, p.d.group,
-                   base < 0 ? -1 : base + (h * parts + k) * p.d.group};
-      t0 = t1;
-    }
+// A sequence's own positions lo .. len - 1: t tiles in `parts` parts a KV head, items `at` on, whose rows are `base` on in the
+// workspace (-1: o).
+struct Own {
+  int b, lo, len, t;
+  int parts, base, at, spare;
+};
+// Its items of KV head h.
+__device__ __forceinline__ void own_items(const PlanParams& p, Item* items, const Own& x, int h) {
+  const int lo16 = x.lo & ~(kBlk - 1);
+  const int each = x.parts ? x.t / x.parts : 0, more = x.parts ? x.t - each * x.parts : 0;
+  int t0 = 0;
+  for (int k = 0; k < x.parts; ++k) {
+    const int t1 = t0 + each + (k < more ? 1 : 0);
+    items[x.at + h * x.parts + k] = Item{x.b, h, t0 ? lo16 + t0 * p.bn : x.lo, min(x.len, lo16 + t1 * p.bn), -1, 0, p.d.group,
+                                         x.base < 0 ? -1 : x.base + (h * x.parts + k) * p.d.group};
+    t0 = t1;
   }
 }
 // Item e of those of shared positions.  Workgroups are dealt to the 8 XCDs in turn: the row tiles of one range of keys stand 8
@@ -137,13 +141,16 @@ __device__ __forceinline__ Item group_item(const PlanParams& p, const Group* gro
   return Item{order[g.i0], h, t0 * p.bn, min(g.shared, t1 * p.bn), g.i0, tile * kBM, g.R, g.row + range * g.R + tile * kBM};
 }
 
-constexpr int kOneBatch = 1024;  // sequences and groups that the plan of one pass holds: a thread each
-
-// Up to 1024 sequences and groups, a thread each of either: what the threads need of one another is in LDS.
-__global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
-  __shared__ int s_start[kOneBatch + 1], s_shared[kOneBatch], s_before[kOneBatch + 1], s_order[kOneBatch], s_named[kOneBatch];
-  __shared__ Group s_group[kOneBatch];
-  __shared__ int s_sums[4][kScanWaves], s_bucket[64];
+// As many sequences and groups as threads at most, a thread each of either: what the threads need of one another is in LDS.  Few
+// waves where they do: a step of the plan is a barrier more than anything (16 sequences, 6.4 us with 16 waves, 5.6 with 4).
+template <int W>
+__global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
+  constexpr int kThreads = 64 * W;
+  __shared__ int s_start[kThreads + 1], s_shared[kThreads], s_before[kThreads + 1], s_order[kThreads], s_named[kThreads],
+      s_len[kThreads];
+  __shared__ Group s_group[kThreads];
+  __shared__ Own s_own[kThreads];
+  __shared__ int s_sums[4][W], s_bucket[64];
   const PlanDims& d = p.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = tid < d.batch ? p.members[tid] : -1;
@@ -154,8 +161,10 @@ __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
     s_shared[tid] = min(max(p.shared[tid], 0), p.cap);
   }
   if (tid == 0) s_start[d.n_groups] = min(max(p.starts[d.n_groups], 0), d.batch);
-  const int64_t n = (unsigned)b < (unsigned)d.batch ? (int64_t)p.lens[b] + p.len_add : 0;
-  const int len = (int)(n < 0 ? 0 : n > p.cap ? p.cap : n);
+  if (tid < d.batch) {
+    const int64_t n = (int64_t)p.lens[tid] + p.len_add;
+    s_len[tid] = (int)(n < 0 ? 0 : n > p.cap ? p.cap : n);
+  }
   auto scan4 = [&](int (&x)[4], int (&total)[4]) { block_scan(x, total, s_sums); };
   __syncthreads();
   // this thread's sequence: its group, and whether it shares if the group does
@@ -167,7 +176,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
     if (s_start[mid] <= tid) g = mid;
     else hi = mid;
   }
-  const int shared = s_shared[g];
+  const int shared = s_shared[g], len = listed ? s_len[b] : 0;
   __syncthreads();
   listed = listed && s_named[b] == tid;  // a sequence named twice is its last place's
   const bool in = listed && shared > 0 && len >= shared;
@@ -222,14 +231,18 @@ __global__ __launch_bounds__(kScanThreads) void plan_one_kernel(PlanParams p) {
   const int own_at = oi ? atomicAdd(&s_bucket[bucket], oi) : 0;
   Item* const items = (Item*)(p.plan + d.items_at());
   Join* const joins = (Join*)(p.plan + d.joins_at());
-  for (int e = tid; e < total[0]; e += kScanThreads) items[e] = group_item(p, s_group, s_order, e);
+  for (int e = tid; e < total[0]; e += kThreads) items[e] = group_item(p, s_group, s_order, e);
   if (tid < d.batch && s_named[tid] < 0) joins[tid] = Join{0, 0, 0, 0, 0, 0, 1, 0};
   if (listed) {
     const int base = total[1] + x[3] - on;
     const Group& of = s_group[g];
     joins[b] = shares ? Join{of.R, of.row, of.parts, place * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
-    own_items(p, items + total[0] + own_at, b, shares ? shared : 0, len, t, parts, direct ? -1 : base);
+    s_own[tid] = Own{b, shares ? shared : 0, len, t, parts, direct ? -1 : base, total[0] + own_at, 0};
+  } else {
+    s_own[tid] = Own{0, 0, 0, 0, 0, 0, 0, 0};
   }
+  __syncthreads();
+  for (int i = tid; i < d.batch * d.n_kv; i += kThreads) own_items(p, items, s_own[i / d.n_kv], i % d.n_kv);
   if (tid == 0) *(Head*)p.plan = Head{p.check, total[0] + total[2]};
 }
 
@@ -361,7 +374,8 @@ __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
       const int base = (int)(row + sn.incl - on);
       const Group& of = groups[m.g];
       joins[m.b] = j >= 0 ? Join{of.R, of.row, of.parts, j * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
-      own_items(p, items + item + si.incl - oi, m.b, lo, m.len, t, parts, direct ? -1 : base);
+      const Own x{m.b, lo, m.len, t, parts, direct ? -1 : base, (int)(item + si.incl) - oi, 0};
+      for (int h = 0; h < d.n_kv; ++h) own_items(p, items, x, h);
     }
     item += si.total;
     row += sn.total;
@@ -763,7 +777,9 @@ int tl_shared_plan(const int32_t* cache_lens, int len_add, const int32_t* member
   p.bn = esize == 4 ? tile_keys<F32>() : tile_keys<BF16>();
   p.check = p.d.check(p.cap, esize, d_k);
   hipStream_t st = tl_resolve_stream(stream);
-  if (batch <= kOneBatch && n_groups <= kOneBatch) hipLaunchKernelGGL(plan_one_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
+  const int most = batch > n_groups ? batch : n_groups;
+  if (most <= 256) hipLaunchKernelGGL(plan_one_kernel<4>, dim3(1), dim3(256), 0, st, p);
+  else if (most <= 1024) hipLaunchKernelGGL(plan_one_kernel<16>, dim3(1), dim3(1024), 0, st, p);
   else hipLaunchKernelGGL(plan_many_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
   return tl_launch_status();
 }
