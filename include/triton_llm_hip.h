@@ -505,7 +505,8 @@ int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
  * tl_paged_attention_packed: tl_paged_attention_prefill_counted for packed rows: query i of sequence b is row starts[b] + i of
  * q / o (n_rows, n_head, d_k) {row, head}, at position cache_lens[b] + i.  max_new: the most rows of a
  * sequence; those behind are left as they were, as are rows of no sequence.  Workspace: tl_paged_packed_workspace_bytes (with n_rows
- * = 0 what tl_paged_prefill_workspace_bytes gives).  host_new_lens as there, and with the same promise.
+ * = 0 what tl_paged_prefill_workspace_bytes gives).  host_new_lens as there, and with the same promise.  Weights are rounded to a
+ * 16-bit type as there, but for sequences of at most 32 query rows a KV head, as single tokens are.
  * ------------------------------------------------------------------------- */
 size_t tl_pages_workspace_bytes(int batch);
 int tl_release_pages(const int32_t* page_table, int max_pages, int page_size, const int32_t* lens,
@@ -558,8 +559,8 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * in time need one each.  o overlaps none of q and the pools.
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; batch and n_groups <= 65535, n_head / n_kv_head <= 128, max_pages *
  * page_size <= 2^30.  Hidden positions are not read.
- * With 16-bit types the weights of shared keys are rounded to the type for the product with V, as for
- * tl_paged_attention_prefill; those of a sequence's own keys are not.
+ * With 16-bit types the weights of keys that more than 32 query rows of a KV head share (sequences times n_head / n_kv_head) are
+ * rounded to the type for the product with V, as for tl_paged_attention_prefill; others are not.
  * Deterministic.
  * ------------------------------------------------------------------------- */
 size_t tl_shared_plan_bytes(int batch, int n_groups, int n_head, int n_kv_head, int d_k);

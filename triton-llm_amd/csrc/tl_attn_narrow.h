@@ -5,6 +5,10 @@
 // keeps the running maximum and sum of the softmax over its keys (fp32, log2 domain); the waves' states are joined through LDS at the
 // end.  Against 32 x 32 blocks on one wave, the tile shared by all four: a short call waits for a quarter of the products (4
 // sequences, fp32: 13.1 -> 5.1 us), and a wave that computes is not always the same SIMD's.
+//
+// With 16-bit types a weight goes into the product with V in two words, its rounding and what that left out (2^-16 of it in bf16,
+// less in fp16), so that no weight's rounding shows: the products are not what these calls wait for (256 sequences behind 8
+// prefixes, 243.5 us either way; 64 behind one of 8192, 68.5 and 69.4).
 #pragma once
 
 #include "tl_attn_tile.h"
@@ -67,16 +71,24 @@ struct Narrow16 {
       }
     }
   }
+  typedef short v4s __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f32x4 product(v4s a, v4s b, f32x4 c) {
+    if constexpr (T::code == TL_DTYPE_BF16) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+  }
   template <int NRB>
   static __device__ __forceinline__ void values(f32x4 (&o)[NRB][D / 16], const f32x4 (&w)[NRB], const char* vt, int lane) {
-    typedef short v4s __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) v4s lds_v4s;
     const int g = lane >> 4, e = (lane >> 2) & 3, c = lane & 3;
-    u32x2 pw[NRB];
+    u32x2 pw[NRB], rest[NRB];
 #pragma unroll
     for (int rb = 0; rb < NRB; ++rb) {
-      const float x[2] = {w[rb][0], w[rb][1]}, y[2] = {w[rb][2], w[rb][3]};
+      float x[2] = {w[rb][0], w[rb][1]}, y[2] = {w[rb][2], w[rb][3]}, r[4];
       pw[rb] = u32x2{pack2<T>(x), pack2<T>(y)};
+      unpack2<T>(pw[rb].x, r[0], r[1]);
+      unpack2<T>(pw[rb].y, r[2], r[3]);
+      x[0] -= r[0], x[1] -= r[1], y[0] -= r[2], y[1] -= r[3];
+      rest[rb] = u32x2{pack2<T>(x), pack2<T>(y)};
     }
     const auto* row = (const __attribute__((address_space(3))) char*)vt + (4 * g + e) * ROWB + 8 * (c & 1);
 #pragma unroll
@@ -84,10 +96,8 @@ struct Narrow16 {
       const v4s a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(row + (((2 * db + (c >> 1)) ^ vswz(e)) << 4)));
 #pragma unroll
       for (int rb = 0; rb < NRB; ++rb) {
-        if constexpr (T::code == TL_DTYPE_BF16)
-          o[rb][db] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, __builtin_bit_cast(v4s, pw[rb]), o[rb][db], 0, 0, 0);
-        else
-          o[rb][db] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, pw[rb]), o[rb][db], 0, 0, 0);
+        o[rb][db] = product(a, __builtin_bit_cast(v4s, pw[rb]), o[rb][db]);
+        o[rb][db] = product(a, __builtin_bit_cast(v4s, rest[rb]), o[rb][db]);
       }
     }
   }
