@@ -39,6 +39,7 @@ struct AppendParams {
   const int32_t* new_lens;  // NULL: n_new for every sequence
   const int32_t* slots;      // SLOTS: by token (batch 1), and positions (NULL without rotary positions)
   const int32_t* positions;
+  int past_caches;  // SLOTS: rows are read without keeping them in the caches
   const float* cos_t;
   const float* sin_t;
   int rope_rows, rot_half;
@@ -127,7 +128,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
 // and in the other layouts two neighbours (an interleaved chunk is turned in itself).  A thread takes
 // rows g, g + R, ... of its token and loads its angles once for all of them.  8 prompts of up to 1999 tokens, 15 / 5 heads
 // of 64, fp16, 72 MB: 18.4 us, 3.9 TB/s; by pairs of elements (paged_append_kernel) 51 us.
-template <typename T, int MODE, bool SLOTS>
+// PAST: rows are read without keeping them in the caches.
+template <typename T, int MODE, bool SLOTS, bool PAST>
 __global__ __launch_bounds__(256) void paged_append_vec_kernel(AppendParams p, int R) {
   using B = typename T::bits;
   constexpr int VEC = 16 / T::size;
@@ -185,8 +187,13 @@ __global__ __launch_bounds__(256) void paged_append_vec_kernel(AppendParams p, i
       if (r + u * R < rows) {
         const B* src;
         token_row(p, b, s, row, page, r + u * R, src, out[u]);
-        wa[u] = *(const u32x4*)(src + ca * VEC);
-        wb[u] = *(const u32x4*)(src + cb * VEC);
+        if constexpr (PAST) {
+          wa[u] = __builtin_nontemporal_load((const u32x4*)(src + ca * VEC));
+          wb[u] = __builtin_nontemporal_load((const u32x4*)(src + cb * VEC));
+        } else {
+          wa[u] = *(const u32x4*)(src + ca * VEC);
+          wb[u] = *(const u32x4*)(src + cb * VEC);
+        }
       }
     }
 #pragma unroll
@@ -242,7 +249,10 @@ int launch_append_mode(const AppendParams& p, hipStream_t st) {
     groups = groups < 1 ? 1 : groups > rows ? rows : groups;
     const int64_t blocks = (lanes * groups + 255) / 256;
     if (blocks > INT32_MAX) return TL_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((paged_append_vec_kernel<T, MODE, SLOTS>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)groups);
+    if (SLOTS && p.past_caches)
+      hipLaunchKernelGGL((paged_append_vec_kernel<T, MODE, SLOTS, SLOTS>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)groups);
+    else
+      hipLaunchKernelGGL((paged_append_vec_kernel<T, MODE, SLOTS, false>), dim3((unsigned)blocks), dim3(256), 0, st, p, (int)groups);
     return tl_launch_status();
   }
   const int64_t blocks = ((int64_t)p.batch * p.n_new * rows * (p.d_k / 2) + 255) / 256;
@@ -1055,6 +1065,12 @@ int tl_paged_kv_append_slots(const void* q, void* q_out, const void* k_new, cons
   p.pm = PageMap{nullptr, 0, n_pages, shift};
   p.slots = slots;
   p.positions = positions;
+  // Rows are read once, and what is written is what attention reads next: more rows than the L2s hold are read past them.  us alone, and
+  // with the attention after it, kept in the caches / past them: 17000 tokens, 9 / 3 heads of 64, fp32 (65 MB) 34.0 / 29.8, 479 / 479;
+  // 8000 tokens, 24 / 8 heads of 128, bf16 (82 MB) with attention 173 / 166; 6000 tokens, 15 / 5 heads of 64, fp16 (19 MB) 10.6 / 12.2.
+  // (Writing past them too: 24.6 alone in the first case, and attention loses it again: 482; 177.)
+  constexpr int64_t kL2s = 32ll << 20;
+  p.past_caches = (int64_t)n_tokens * (p.n_head + 2 * n_kv_head) * d_k * esize > kL2s;
   p.cos_t = cos_table;
   p.sin_t = sin_table;
   p.rope_rows = rope_rows;
