@@ -11,7 +11,7 @@ from triton_llm import _lib, gpu
 from triton_llm.kernels import (SharedPlan, assign_kv_pages, paged_attention_packed, paged_attention_shared,
                                 paged_kv_append_slots, pages_workspace_bytes, plan_shared_attention, release_kv_pages,
                                 shared_workspace_bytes)
-from triton_llm.paged_cache import PageTables
+from triton_llm.paged_cache import PagedKVCache, PageTables
 
 F32, BF16, BAD = _lib.DTYPE_F32, _lib.DTYPE_BF16, 99
 
@@ -307,3 +307,50 @@ def test_assign_and_release_deal_pages_as_the_host_tables_do():
                 assert positions[t] == lens[b] - new[b] + t - starts[b]
                 assert places[t] == host.tables[b][positions[t] // page] * page + positions[t] % page
         assert (places[starts[-1]:] == -1).all()
+
+
+# ---- which slots share -------------------------------------------------------------------
+
+def test_sharing_follows_forks_writes_and_orders():
+    t = PageTables(200, 4, 6, 400)
+    a, b = t.open(), t.open()
+    t.begin([10, 3, 0, 0, 0, 0])
+    t.advance()
+    assert t.sharing() == []
+    c, d, e = t.fork(a), t.fork(a), t.fork(b)
+    assert t.sharing() == [([a, c, d], 3), ([b, e], 1)]
+    before = t.version
+    t.begin([1, 0, 1, 0, 1, 0])  # a, c and e write: the last pages part
+    t.advance()
+    assert t.version > before and t.sharing() == [([a, c, d], 2)]
+    before = t.version
+    for _ in range(3):
+        t.begin([0, 1, 0, 0, 0, 0])
+        t.advance()
+    assert t.version == before
+    t.reorder([d], [b])
+    assert t.sharing() == [([a, c], 2), ([b, d], 2)]
+    t.close(c)
+    assert t.sharing() == [([b, d], 2)]
+    t.compact()
+    assert t.sharing() == [([b, d], 2)]
+
+
+def test_sharing_of_long_tables():
+    t = PageTables(500, 1, 3, 400)
+    a = t.open()
+    t.begin([100, 0, 0])
+    t.advance()
+    b, c = t.fork(a), t.fork(a)
+    t.begin([1, 1, 0])
+    t.advance()
+    assert t.sharing() == [([a, b, c], 100)]
+    for n in (0, 1, 31, 32, 33, 64, 99):
+        t.tables[b][n], keep = -7, t.tables[b][n]
+        assert t.sharing() == [([a, c], 100)] if n == 0 else t.sharing() == [([a, b, c], n)]
+        t.tables[b][n] = keep
+
+
+def test_share_reads_goes_without_a_window():
+    with pytest.raises(ValueError, match="without a window"):
+        PagedKVCache(1, 4, 2, 64, n_pages=4, max_batch=2, max_seq=64, window=16, share_reads=True)

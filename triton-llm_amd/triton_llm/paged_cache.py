@@ -29,6 +29,7 @@ from triton_llm import gpu
 from triton_llm.kernels.paged import (allocate_kv_pages, check_page_size, check_window, copy_kv_pages,
                                       paged_attention_decode, paged_attention_prefill, paged_decode_workspace,
                                       paged_kv_append, write_i32)
+from triton_llm.kernels.shared import paged_attention_shared, plan_shared_attention, shared_workspace_bytes
 
 __all__ = ["PageTables", "PagedKVCache"]
 
@@ -46,13 +47,22 @@ def _differing(a: list[int], b: list[int]) -> list[int]:
     return out
 
 
+def _alike(a: list[int], b: list[int], most: int) -> int:
+    """How many pages, up to `most`, two lists begin with in common."""
+    for lo in range(0, most, 32):
+        hi = min(lo + 32, most)
+        if a[lo:hi] != b[lo:hi]:
+            return next((i for i in range(lo, hi) if i >= len(a) or i >= len(b) or a[i] != b[i]), hi)
+    return most
+
+
 class PageTables:
     """Which pages every slot's sequence has, and which are free.  Host only.
 
     ``tables[slot]`` lists a slot's pages in order (-1: given back behind the window),
     ``lens[slot]`` its cached tokens.  Changes that the GPU has to follow are collected in
     ``table_edits`` ``{(slot, column): page}`` and ``copies`` ``[(source, destination)]``
-    until :meth:`take_edits`.
+    until :meth:`take_edits`.  ``version`` grows when pages that slots may share change.
     """
 
     def __init__(self, n_pages: int, page_size: int, max_batch: int, max_seq: int, window: int = 0, sinks: int = 0):
@@ -74,6 +84,7 @@ class PageTables:
         self._free = list(range(n_pages - 1, -1, -1))
         self.table_edits: dict[tuple[int, int], int] = {}
         self.copies: list[tuple[int, int]] = []
+        self.version = 0
 
     @property
     def free_pages(self) -> int:
@@ -104,6 +115,7 @@ class PageTables:
         for c in _differing(old, new):
             self.table_edits[slot, c] = new[c] if c < len(new) else -1
         self.tables[slot] = pages
+        self.version += 1
 
     def open(self) -> int:
         """An empty sequence in the lowest closed slot."""
@@ -144,6 +156,7 @@ class PageTables:
         for s in slots + parents:
             self._check_slot(s)
         parents, slots = [p for s, p in zip(slots, parents) if s != p], [s for s, p in zip(slots, parents) if s != p]
+        self.version += 1
         # pages that a slot and its parent have in the same place keep their references
         taken = []
         for s, p in zip(slots, parents):
@@ -201,6 +214,7 @@ class PageTables:
             pages = self.tables[slot]
             at = self.lens[slot]
             if slot in copied:
+                self.version += 1
                 page = self._take()
                 self.copies.append((pages[at // ps], page))
                 self._drop(pages[at // ps])
@@ -224,6 +238,7 @@ class PageTables:
                 first = (self.lens[slot] - self.window + 1) // self.page_size  # pages before it are out of sight
                 pages = self.tables[slot]
                 for c in range(max(self._gone[slot], -(-self.sinks // self.page_size)), min(first, len(pages))):
+                    self.version += 1
                     self._drop(pages[c])
                     pages[c] = self.table_edits[slot, c] = -1
                     self._gone[slot] = c + 1
@@ -244,6 +259,22 @@ class PageTables:
         self._free = list(range(self.n_pages - 1, len(used) - 1, -1))
         return len(moved)
 
+    def sharing(self) -> list[tuple[list[int], int]]:
+        """The slots whose sequences begin with the same page, and how many pages all of them begin with."""
+        by_first: dict[int, list[int]] = {}
+        for slot, pages in enumerate(self.tables):
+            if pages and pages[0] >= 0:
+                by_first.setdefault(pages[0], []).append(slot)
+        out = []
+        for slots in by_first.values():
+            if len(slots) > 1:
+                first = self.tables[slots[0]]
+                n = len(first)
+                for s in slots[1:]:
+                    n = _alike(first, self.tables[s], min(n, len(self.tables[s])))
+                out.append((slots, n))
+        return out
+
     def take_edits(self):
         """(copies, table edits) since the last call."""
         out = self.copies, self.table_edits
@@ -256,11 +287,20 @@ class PagedKVCache:
 
     ``layers[i]`` is ``{"k": DeviceTensor, "v": DeviceTensor}``, each
     ``(n_pages, n_kv_head, page_size, d_k)``.  With ``window`` > 0 a token sees the last ``window``
-    positions up to its own and the first ``sinks``.
+    positions up to its own and the first ``sinks``.  With ``share_reads`` a step of one token a slot reads the pages that
+    slots begin with in common once for all of them, where that is at least ``SHARE_LEAST`` positions (results then differ by
+    roundings); it goes without a window.
     """
 
+    # Shared positions from which one read for all is faster than one each.  us a layer, each / once, 2 sequences and 32: 15 / 5 heads of
+    # 64, fp16, 256 positions 9.3 / 10.0 (8 sequences) and 9.2 / 10.2, 1024 12.5 / 10.2 (8) and 16.1 / 11.1; 24 / 8 heads of 128, bf16,
+    # 512 10.6 / 10.0 (2), 256 10.6 / 13.5, 1024 15.4 / 12.2 (8) and 21.9 / 15.0; 9 / 3 heads of 64, fp32, 512 9.5 / 10.0 (2),
+    # 1024 12.3 / 12.2 (8) and 17.7 / 15.0.
+    SHARE_LEAST = 1024
+
     def __init__(self, n_layer: int, n_head: int, n_kv_head: int, d_k: int, *, n_pages: int, max_batch: int,
-                 max_seq: int, page_size: int = 16, window: int = 0, sinks: int = 0, dtype=np.float32):
+                 max_seq: int, page_size: int = 16, window: int = 0, sinks: int = 0, dtype=np.float32,
+                 share_reads: bool = False):
         if n_layer <= 0 or n_kv_head <= 0 or n_head <= 0 or n_head % n_kv_head:
             raise ValueError(f"bad head counts: n_layer={n_layer} n_head={n_head} n_kv_head={n_kv_head}")
         if d_k not in (64, 128):
@@ -270,6 +310,8 @@ class PagedKVCache:
         check_window(window, sinks)
         if max_batch > 65535:
             raise ValueError(f"max_batch must be at most 65535, got {max_batch}")
+        if share_reads and window:
+            raise ValueError("share_reads goes without a window")
         self.tables = PageTables(n_pages, page_size, max_batch, max_seq, window, sinks)
         if self.tables.max_pages * page_size > 1 << 30:
             raise ValueError(f"max_seq must be at most 2^30, got {max_seq}")
@@ -297,11 +339,48 @@ class PagedKVCache:
         self._told = [0] * (3 * max_batch)  # what the device has in it
         self._lens, self._new, self._ends = (self._row(i) for i in range(3))
         self._decode_ws = paged_decode_workspace(max_batch, n_head, n_kv_head, max_seq, d_k)
+        self._plan = None  # share_reads: the step's, where it is read by
+        self._shares = False
+        if share_reads:
+            # groups of slots that share, and one of the others
+            self._n_groups = max_batch // 2 + 1
+            self._groups = gpu.zeros((max_batch + 2 * self._n_groups + 1,), np.int32)
+            parts = (max_batch, self._n_groups + 1, self._n_groups)
+            self._members, self._starts, self._shared = (self._part(self._groups, sum(parts[:i]), n) for i, n in enumerate(parts))
+            self._groups_told = [0] * (max_batch + 2 * self._n_groups + 1)
+            self._groups_of = -1  # the tables' version that they are of
+            self._most_shared = 0
+            need = shared_workspace_bytes(max_batch, self._n_groups, n_head, n_kv_head, d_k)
+            if need == 0:
+                raise ValueError(f"share_reads does not support {max_batch} slots with {n_head} / {n_kv_head} heads")
+            self._shared_ws = gpu.allocate((need,), np.uint8)
+        self._share_reads = share_reads
 
     def _row(self, i: int):
         n = self.tables.max_batch
-        return gpu.DeviceTensor(ctypes.c_void_p(self._counts.data_ptr() + 4 * n * i), (n,), np.int32, 4 * n,
-                                defer_free=False)
+        return self._part(self._counts, n * i, n)
+
+    @staticmethod
+    def _part(t, first: int, n: int):
+        return gpu.DeviceTensor(ctypes.c_void_p(t.data_ptr() + 4 * first), (n,), np.int32, 4 * n, defer_free=False)
+
+    def _publish_groups(self) -> None:
+        """Bring the GPU up to date: which slots begin with the same pages."""
+        t = self.tables
+        if self._groups_of == t.version:
+            return
+        groups = [(slots, n * t.page_size) for slots, n in t.sharing() if n]
+        self._most_shared = max((n for _, n in groups), default=0)
+        inside = {s for slots, _ in groups for s in slots}
+        groups.append(([s for s in range(t.max_batch) if s not in inside], 0))
+        members, starts, shared = [s for slots, _ in groups for s in slots], [0], [n for _, n in groups]
+        for slots, _ in groups:
+            starts.append(starts[-1] + len(slots))
+        empty = self._n_groups - len(groups)
+        now = members + starts + [t.max_batch] * empty + shared + [0] * empty
+        changed = [i for i, n in enumerate(now) if n != self._groups_told[i]]
+        write_i32(self._groups, changed, [now[i] for i in changed])
+        self._groups_told, self._groups_of = now, t.version
 
     @property
     def lens(self) -> list[int]:
@@ -366,6 +445,13 @@ class PagedKVCache:
         self._host_new[:] = t.new  # in place: a recorded call finds the step's counts there
         self._longest = max(a + b for a, b in zip(t.lens, t.new) if b)
         self._publish()
+        self._shares = False
+        if self._share_reads and self._most_new == 1:
+            self._publish_groups()
+            self._shares = self._most_shared >= self.SHARE_LEAST
+            if self._shares:
+                self._plan = plan_shared_attention(self._table, self._ends, self._members, self._starts, self._shared, self.n_head,
+                                                   self.n_kv_head, self.d_k, t.page_size, self.dtype, plan=self._plan)
 
     def advance(self) -> None:
         """End the step: its tokens are cached."""
@@ -396,6 +482,9 @@ class PagedKVCache:
         pool = self.layers[layer]
         paged_kv_append(q_dev, k_dev, v_dev, pool["k"], pool["v"], self._table, self._lens, cos_dev, sin_dev,
                         new_lens=self._new, interleaved=interleaved)
+        if n_new == 1 and self._shares:
+            return paged_attention_shared(q_dev, pool["k"], pool["v"], self._table, self._plan, self.n_head, self.n_kv_head,
+                                          sm_scale=sm_scale, out=out, workspace=self._shared_ws)
         if n_new == 1:
             return paged_attention_decode(q_dev, pool["k"], pool["v"], self._table, self._ends, self.n_head,
                                           self.n_kv_head, sm_scale=sm_scale, window=self.window, sinks=self.sinks,
