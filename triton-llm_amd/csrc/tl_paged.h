@@ -124,11 +124,11 @@ __device__ __forceinline__ Scan block_scan(int64_t x, int64_t (&sums)[kScanWaves
   return Scan{x + (wave ? before : 0), __shfl(s, kScanWaves - 1)};
 }
 
-// The same of N numbers at once, whose sums fit in 32 bits, of a workgroup of W waves.
-template <int N, int W>
+// The same of N numbers at once, whose sums fit in 32 bits, of a workgroup of W waves.  FRESH: nobody has used `sums` since a barrier.
+template <bool FRESH = false, int N, int W>
 __device__ __forceinline__ void block_scan(int (&x)[N], int (&total)[N], int (&sums)[N][W]) {
   const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6);
-  __syncthreads();  // the sums of the scan before have been read
+  if (!FRESH) __syncthreads();  // the sums of the scan before have been read
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     x[i] = wave_scan(x[i]);

@@ -26,7 +26,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kBM = 128;  // query rows of an item at most
 constexpr int kMostBatch = 65535;
-constexpr int kMinTiles = 2;  // key tiles of an item at least, if there are more
+// Key tiles of an item at least, if there are more: 2 / 4 / 8, with 4 sequences behind 496 positions, 9 / 3 heads of 64, fp32,
+// plan and call 19.0 / 23.3 / 32.0 us; 2 groups of 8 behind 2000 each, 15 / 5 heads of 64, fp16, four layers, 50.7 / 53.2 / 64.2.
+constexpr int kMinTiles = 2;
 constexpr int kScanThreads = 64 * kScanWaves;
 
 // Rows row0 .. of R: row r is query head hkv * group + r % group of the i0 + r / group-th sequence that shares (i0 < 0: of sequence
@@ -93,6 +95,7 @@ __device__ __forceinline__ int tiles_of(int lo, int hi, int bn) {
 }
 // Key tiles of an item at most: as many as `slots` workgroups have each if all end together.
 __device__ __forceinline__ int share_of(int64_t work, int slots) {
+  if (work < 1 << 30) return max((int)((unsigned)(work + slots - 1) / (unsigned)slots), kMinTiles);
   return (int)min(max((work + slots - 1) / slots, (int64_t)kMinTiles), (int64_t)1 << 30);
 }
 // A sequence's own positions lo .. len - 1: t tiles in `parts` parts a KV head, items `at` on, whose rows are `base` on in the
@@ -142,7 +145,8 @@ __device__ __forceinline__ Item group_item(const PlanParams& p, const Group* gro
 }
 
 // As many sequences and groups as threads at most, a thread each of either: what the threads need of one another is in LDS.  Few
-// waves where they do: a step of the plan is a barrier more than anything (16 sequences, 6.4 us with 16 waves, 5.6 with 4).
+// waves where they do: a step of the plan is a barrier more than anything (16 sequences, 6.4 us with 16 waves, 5.6
+// with 4, 4.9 since three of its scans share no sums and wait for nobody's reads).
 template <int W>
 __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   constexpr int kThreads = 64 * W;
@@ -150,7 +154,7 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
       s_len[kThreads];
   __shared__ Group s_group[kThreads];
   __shared__ Own s_own[kThreads];
-  __shared__ int s_sums[4][W], s_bucket[64];
+  __shared__ int s_in[1][W], s_work[3][W], s_places[4][W], s_bucket[64];
   const PlanDims& d = p.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = tid < d.batch ? p.members[tid] : -1;
@@ -165,7 +169,6 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
     const int64_t n = (int64_t)p.lens[tid] + p.len_add;
     s_len[tid] = (int)(n < 0 ? 0 : n > p.cap ? p.cap : n);
   }
-  auto scan4 = [&](int (&x)[4], int (&total)[4]) { block_scan(x, total, s_sums); };
   __syncthreads();
   // this thread's sequence: its group, and whether it shares if the group does
   int g = 0;
@@ -180,13 +183,13 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   __syncthreads();
   listed = listed && s_named[b] == tid;  // a sequence named twice is its last place's
   const bool in = listed && shared > 0 && len >= shared;
-  int x[4] = {in ? 1 : 0, 0, 0, 0}, total[4];
-  scan4(x, total);
-  if (tid < d.batch) s_before[tid] = x[0] - (in ? 1 : 0);
-  if (tid == 0) s_before[d.batch] = total[0];
+  int n_in[1] = {in ? 1 : 0}, all_in[1];
+  block_scan<true>(n_in, all_in, s_in);
+  if (tid < d.batch) s_before[tid] = n_in[0] - (in ? 1 : 0);
+  if (tid == 0) s_before[d.batch] = all_in[0];
   if (in) {
-    s_order[x[0] - 1] = b;
-    ((int*)(p.plan + d.order_at()))[x[0] - 1] = b;
+    s_order[n_in[0] - 1] = b;
+    ((int*)(p.plan + d.order_at()))[n_in[0] - 1] = b;
   }
   __syncthreads();
   auto sharing = [&](int i) { return s_before[max(s_start[i + 1], s_start[i])] - s_before[s_start[i]]; };
@@ -199,36 +202,41 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   // work in 64 bits: the tiles' upper and lower halves
   auto own_tiles = [&] { return listed ? tiles_of(shares ? shared : 0, len, p.bn) : 0; };
   const int64_t both = (int64_t)row_tiles * gr.tiles + own_tiles();
-  x[0] = (int)(both & 0xFFFF), x[1] = (int)(both >> 16), x[2] = gr.R / d.group, x[3] = 0;
-  scan4(x, total);
-  if (total[2] > d.batch) {  // starts that go back: groups overlap, and nobody shares
+  int w[3] = {(int)(both & 0xFFFF), (int)(both >> 16), gr.R / d.group}, work[3];
+  block_scan<true>(w, work, s_work);
+  if (work[2] > d.batch) {  // starts that go back: groups overlap, and nobody shares
     shares = false;
     gr = Group{};
-    x[0] = own_tiles() & 0xFFFF, x[1] = own_tiles() >> 16, x[2] = x[3] = 0;
-    scan4(x, total);
+    w[0] = own_tiles() & 0xFFFF, w[1] = own_tiles() >> 16, w[2] = 0;
+    block_scan(w, work, s_work);
   }
-  const int share = share_of((((int64_t)total[1] << 16) + total[0]) * d.n_kv, d.slots);
+  const int share = share_of((((int64_t)work[1] << 16) + work[0]) * d.n_kv, d.slots);
   gr.parts = gr.R ? (gr.tiles + share - 1) / share : 0;
   const int t = own_tiles(), parts = (t + share - 1) / share;
   const bool direct = !shares && parts == 1;
   const int gi = d.n_kv * gr.parts * ((gr.R + kBM - 1) / kBM), gn = d.n_kv * gr.parts * gr.R;
   const int oi = d.n_kv * parts, on = direct ? 0 : oi * d.group;
-  x[0] = gi, x[1] = gn, x[2] = oi, x[3] = on;
-  scan4(x, total);
+  int x[4] = {gi, gn, oi, on}, total[4];
+  block_scan<true>(x, total, s_places);
   gr.item = x[0] - gi;
   gr.row = x[1] - gn;
   if (tid < d.n_groups) s_group[tid] = gr;
-  // The longest own items first, by 64ths of a share: a launch of more items than workgroups ends with short ones (64 sequences of 1
-  // to 500 own positions, 24 / 8 heads of 128, bf16: 27.9 -> 22.6 us).  Among equals whoever comes first.
-  const int bucket = parts ? 63 - min(63, (int)((int64_t)(t / parts) * 64 / share)) : 0;
-  if (oi) atomicAdd(&s_bucket[bucket], oi);
-  __syncthreads();
-  if (wave == 0) {
-    const int n = s_bucket[lane];
-    s_bucket[lane] = wave_scan(n) - n;
+  // Where there are more items than workgroups the longest own ones come first, by 64ths of a share, so that the launch ends with short
+  // ones (64 sequences of 1 to 500 own positions, 24 / 8 heads of 128, bf16: 27.9 -> 24.7 us).  Among equals whoever comes first.
+  int own_at = x[2] - oi;
+  if (total[0] + total[2] > d.slots) {
+    const int bucket = parts ? 63 - min(63, (int)((int64_t)(t / parts) * 64 / share)) : 0;
+    if (oi) atomicAdd(&s_bucket[bucket], oi);
+    __syncthreads();
+    if (wave == 0) {
+      const int n = s_bucket[lane];
+      s_bucket[lane] = wave_scan(n) - n;
+    }
+    __syncthreads();
+    if (oi) own_at = atomicAdd(&s_bucket[bucket], oi);
+  } else {
+    __syncthreads();
   }
-  __syncthreads();
-  const int own_at = oi ? atomicAdd(&s_bucket[bucket], oi) : 0;
   Item* const items = (Item*)(p.plan + d.items_at());
   Join* const joins = (Join*)(p.plan + d.joins_at());
   for (int e = tid; e < total[0]; e += kThreads) items[e] = group_item(p, s_group, s_order, e);
@@ -439,8 +447,8 @@ __device__ __forceinline__ void narrow_item(const SharedParams& p, const Item& i
   auto whole = [&](int pos) { return pos >= it.lo && pos + kBlk <= it.hi; };
   auto seen = [&](int key, int) { return key >= it.lo && key < it.hi; };
   const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
-  // a sequence's own keys are read once in the launch: they need not stay in the caches (64 sequences of up to 1000 own
-  // positions, 24 / 8 heads of 128, bf16: 130 -> 115 us)
+  // a sequence's own keys are read once in the launch: they need not stay in the caches (8 groups of 32 sequences with up to 1000 own
+  // positions behind 4096 shared ones, 24 / 8 heads of 128, bf16: 140 -> 130 us a layer)
   narrow_stream<T, D, NRB, NB>(st, q, k, pages, smem, wave, lane, scale, it.i0 < 0, pos_of, whole, seen);
   narrow_join<T, D, NRB>(st, smem, s_ml, wave, lane);
   constexpr int CH = D / 4;
