@@ -172,6 +172,46 @@ def test_packed_starts_outside_the_rows():
         P.check(f"packed starts sequence {b}", got[lo:hi].transpose(1, 0, 2), want, tol)
 
 
+def test_packed_starts_that_go_back():
+    """A start far below the one before it: the sequence before has no rows, and none are read or written for it."""
+    rng = np.random.default_rng(17)
+    Hq, Hkv, D, page, rows = 2, 1, 64, 16, 30
+    q, before = P.values(rng, (rows, Hq, D), "float32"), P.values(rng, (rows, Hq, D), "float32")
+    kp, vp = P.values(rng, (9, Hkv, page, D), "float32"), P.values(rng, (9, Hkv, page, D), "float32")
+    table = np.array([[0, 1, 2], [3, 4, 5]], np.int32)
+    out = P.dev(before, "float32")
+    paged_attention_packed(P.dev(q, "float32"), P.dev(kp, "float32"), P.dev(vp, "float32"), P.int32(table), P.int32([0, 9]),
+                           P.int32([7, -2 ** 31, 11]), Hq, Hkv, 30, out=out)
+    got = P.back(out, "float32")
+    k, there = op.gather(on.from_storage(kp, "float32"), table[1], 20)
+    v, _ = op.gather(on.from_storage(vp, "float32"), table[1], 20)
+    want, tol = P.rows_want(q[:11].transpose(1, 0, 2), k, v, 9 + np.arange(11), there, 0, 0, D ** -0.5, "float32")
+    P.check("packed starts that go back", got[:11].transpose(1, 0, 2), want, tol)
+    np.testing.assert_array_equal(got[11:], before[11:])
+
+
+def test_append_slots_of_more_rows_than_the_caches():
+    """40 MB of rows in one call, bit for bit what calls of a third of them leave."""
+    rng = np.random.default_rng(18)
+    Hq, Hkv, D, page, n, rows = 24, 8, 128, 64, 3900, 500
+    n_pages = -(-n // page) + 2
+    q, k, v = (P.values(rng, (n, h, D), "bfloat16") for h in (Hq, Hkv, Hkv))
+    slots = rng.permutation(n_pages * page)[:n].astype(np.int32)
+    positions = rng.integers(0, rows, n).astype(np.int32)
+    tab = [gpu.to_device(x) for x in precompute_cos_sin(rows, D)]
+    shape = (n_pages, Hkv, page, D)
+    got = []
+    for pieces in (1, 3):
+        kp, vp = (P.dev(np.zeros(shape, np.uint16), "bfloat16") for _ in range(2))
+        outs = []
+        for at in np.array_split(np.arange(n), pieces):
+            outs.append(gpu.to_host(paged_kv_append_slots(*(P.dev(x[at], "bfloat16") for x in (q, k, v)), kp, vp, P.int32(slots[at]),
+                                                          P.int32(positions[at]), *tab)))
+        got.append((np.concatenate(outs), gpu.to_host(kp), gpu.to_host(vp)))
+    for a, b in zip(*got):
+        np.testing.assert_array_equal(a.view(np.uint16), b.view(np.uint16))
+
+
 @pytest.mark.parametrize("dtype,D", [("bfloat16", 128), ("float32", 64)])
 def test_packed_is_padded(dtype, D):
     """The same rows padded: equal where both divide the keys alike, which sequences of one length do not change."""

@@ -193,6 +193,29 @@ def test_starts_that_go_back():
     c.run()
     c.lists = lambda: ([0, 1, 2, 3], [-3, 2, 77], [32, -5])
     c.run()
+    # in all no more than there are sequences, and some of them in two groups
+    c = Case("float16", 4, 2, 64, 16, [96, 130, 70, 50, 64, 33, 90, 41], [(list(range(8)), 32)], blind=False)
+    c.lists = lambda: (list(range(8)), [0, 4, 2, 6, 8], [32, 16, 32, 16])
+    c.run()
+
+
+@pytest.mark.parametrize("batch,n_groups", [(6, 1500), (1, 1), (300, 2), (1030, 1)])
+def test_more_groups_than_a_workgroup_plans_at_once(batch, n_groups):
+    """Groups without members among those with some; a thread a group, and more groups or sequences than threads."""
+    rng = np.random.default_rng(23)
+    members = rng.permutation(batch)
+    cuts = np.sort(rng.integers(0, batch + 1, n_groups - 1))
+    groups = [(at.tolist(), 40) for at in np.split(members, cuts)]
+    Case("float16", 2, 1, 64, 16, 40 + rng.integers(0, 20, batch), groups).run()
+
+
+@pytest.mark.parametrize("batch", [5, 1100])
+def test_lengths_below_zero(batch):
+    """Sequences of no positions, as a padded batch's: zeros, and no part in what the others share."""
+    rng = np.random.default_rng(24)
+    lens = np.where(np.arange(batch) % 3 == 1, -7, 50 + rng.integers(0, 9, batch))
+    got = Case("bfloat16", 2, 1, 64, 16, lens, [(list(range(batch)), 48)]).run()
+    assert not got[lens < 0].any()
 
 
 def test_a_prefix_beyond_32_bit_offsets():

@@ -83,7 +83,7 @@ __device__ __forceinline__ Rows rows_of(const WinParams& p, int b) {
     r.base = min(max(p.lens[b], -p.seq_q), 1 << 30);
     if (p.starts) {
       r.first = min(max(p.starts[b], 0), p.packed_rows);
-      r.nq = min(max(min(p.starts[b + 1], p.packed_rows) - r.first, 0), p.seq_q);
+      r.nq = min(max(min(max(p.starts[b + 1], 0), p.packed_rows) - r.first, 0), p.seq_q);
     } else {
       r.nq = p.new_lens ? min(max(p.new_lens[b], 0), p.seq_q) : p.seq_q;
     }
