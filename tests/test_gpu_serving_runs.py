@@ -181,6 +181,45 @@ def test_paged_cache_shares_reads(every_shared_page, dtype, Hq, Hkv, D, page):
     assert r.cache.free_pages == 90
 
 
+def test_paged_cache_recorded_while_it_shares(every_shared_page):
+    """A layer's call, recorded while slots share, replayed after most of them have ended and nothing is shared any more."""
+    Hq, Hkv, D, batch = 4, 2, 64, 4
+    r = Run("bfloat16", Hq, Hkv, D, batch=batch, n_layer=1, n_pages=60, max_seq=200, share_reads=True)
+    a = r.open()
+    r.step([70, 0, 0, 0])
+    others = [r.fork(a) for _ in range(3)]
+    q_d, k_d, v_d, out = (P.dev(np.zeros((batch, 1, h, D), np.uint16), "bfloat16") for h in (Hq, Hkv, Hkv, Hq))
+    attention = r.cache.attention
+    graph = None
+
+    def recorded(layer, q, k, v, *tab):
+        nonlocal graph
+        for to, x in ((q_d, q), (k_d, k), (v_d, v)):
+            gpu.copy_(to, x)
+        if graph is None:
+            with gpu.capture() as graph:
+                attention(layer, q_d, k_d, v_d, *tab, out=out)
+        graph.replay()
+        return out
+
+    r.cache.attention = recorded
+    r.step([1, 1, 1, 1])
+    assert r.cache._shares
+    r.step([1, 1, 0, 1])
+    for s in others:
+        r.cache.close(s)
+        del r.hist[s]
+    r.step([1, 0, 0, 0])
+    assert not r.cache._shares
+    b = r.open()
+    r.step([1, 1, 0, 0])
+    r.cache.close(a)
+    del r.hist[a]
+    r.step([0, 1, 0, 0])
+    r.fork(b)
+    r.step([1, 1, 0, 0])
+
+
 def test_paged_cache_reads_short_prefixes_each():
     r = Run("bfloat16", 4, 2, 64, batch=3, n_layer=1, n_pages=60, max_seq=400, share_reads=True)
     a = r.open()

@@ -449,7 +449,7 @@ class PagedKVCache:
         if self._share_reads and self._most_new == 1:
             self._publish_groups()
             self._shares = self._most_shared >= self.SHARE_LEAST
-            if self._shares:
+            if self._shares or self._plan:  # a recorded call goes by the plan, also where nothing is shared any more
                 self._plan = plan_shared_attention(self._table, self._ends, self._members, self._starts, self._shared, self.n_head,
                                                    self.n_kv_head, self.d_k, t.page_size, self.dtype, plan=self._plan)
 
