@@ -283,7 +283,8 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
   // Workgroups are dealt to the 8 XCDs in turn, and an XCD's L2 should hold the keys of few (sequence, KV head)s.
   // Undivided: these are cut into every 2^q_shift-th row tile, so that a multiple of 8 groups is dealt to the XCDs;
   // within an XCD the longest rows come first.  Divided: an XCD takes a contiguous range of the parts; packed rows' parts, which are
-  // not equal work, are dealt in turn.
+  // not equal work, are dealt in turn, the KV head first, so that with 8 of them an XCD reads one head's keys (30 tokens and 2 prompts
+  // of up to 500 rows, 24 / 8 heads of 128, bf16: 82.5 -> 77 us).
   const int xcd = blockIdx.x % 8, at = blockIdx.x / 8;
   int b, hkv, qt, part = 0, parts = 1, place = 0, stride = 0;  // stride: places from part to part
   Rows rw;
@@ -306,8 +307,15 @@ __global__ __launch_bounds__(kThreads, 2) void window_fwd_kernel(WinParams p) {
     const int in = place - before;
     parts = s.parts;
     stride = s.tiles;
-    hkv = (int)((unsigned)in / (unsigned)(parts * s.tiles));
-    const int r = in - hkv * parts * s.tiles;
+    int r;
+    if constexpr (PACKED) {
+      r = (int)((unsigned)in / (unsigned)p.n_kv);
+      hkv = in - r * p.n_kv;
+      place = before + hkv * parts * s.tiles + r;
+    } else {
+      hkv = (int)((unsigned)in / (unsigned)(parts * s.tiles));
+      r = in - hkv * parts * s.tiles;
+    }
     part = (int)((unsigned)r / (unsigned)s.tiles);
     qt = s.tiles - 1 - (r - part * s.tiles);
   } else {
