@@ -126,6 +126,20 @@ def test_many_rows(dtype, D, batch):
     Case(dtype, 6, 2, D, 16, 700 + rng.integers(0, 60, batch), [(rng.permutation(batch).tolist(), 699)]).run()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("batch,group,page,shared", [(11, 3, 16, 401), (16, 3, 16, 33), (16, 4, 64, 1000), (21, 3, 32, 95), (13, 5, 16, 64),
+                                                     (63, 3, 16, 130)])
+def test_up_to_64_rows(dtype, D, batch, group, page, shared):
+    """33 to 64 rows in a tile, over few keys and many; tiles with a page that is not there, in their first half and their second."""
+    rng = np.random.default_rng(25)
+
+    def edit(table, n_pages):
+        if shared > 90 and page == 16:
+            table[:, 1], table[:, 6] = -1, n_pages
+    Case(dtype, group, 1, D, page, shared + rng.integers(0, 40, batch), [(rng.permutation(batch).tolist(), shared)], edit=edit).run()
+
+
 def test_more_sequences_than_a_workgroup_plans_at_once():
     rng = np.random.default_rng(3)
     B = 1100
