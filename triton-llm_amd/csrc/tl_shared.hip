@@ -657,14 +657,15 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
   else wide_item<T, D>(p, it, smem);
 }
 
-// A wave a query head of a sequence: the states of its items, shared ones first.  Every load that goes by the plan alone is on its way
-// before the first is waited for.  (A join by the last of a sequence's items to end, in the same launch: the shared keys' last item joins a whole
-// tile's rows, one after the other; 64 sequences behind 8192 positions took 57 us for 25 + 5.8, 16 beams 14.7 for 6.4 + 4.9.)
+// A wave a query head of a sequence: the states of its items, shared ones first, several at a time side by side in the wave, 16 bytes a
+// lane.  Every load that goes by the plan alone, of up to 32 states (16 at d_k 128), is on its way before the first is waited for.  (A join by the last of a sequence's items to end, in the same launch: the shared keys' last item joins a whole
+// tile's rows, one after the other; 64 sequences behind 8192 positions took 57 us for 25 + 5.8, 16 beams 14.7 for 6.4 + 4.9, which is 6.3 + 3.5
+// since states are read side by side.)
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   using B = typename T::bits;
-  constexpr int NJ = D / 64, U = 16;
-  const int lane = threadIdx.x & 63;
+  constexpr int LPR = D / 4, G = 64 / LPR, U = 8;  // lanes of a row, rows of a load, loads on their way
+  const int lane = threadIdx.x & 63, sub = lane / LPR, c = lane % LPR;
   const int b = blockIdx.y, hq = (int)blockIdx.x * (kThreads / 64) + uni((int)threadIdx.x >> 6);
   if (hq >= p.n_head) return;
   const Head head = *(const Head*)p.plan;
@@ -672,20 +673,18 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   if (head.check != p.check || x.done) return;
   const int hkv = hq / p.d.group, g = hq - hkv * p.d.group;
   const int parts = x.p_parts + x.s_parts;
-  auto row_of = [&](int k) {
-    return k < x.p_parts ? (int64_t)x.p_base + (int64_t)(hkv * x.p_parts + k) * x.R + x.r0 + g
-                         : (int64_t)x.s_base + (hkv * x.s_parts + k - x.p_parts) * p.d.group + g;
-  };
+  const int p_row = x.p_base + hkv * x.p_parts * x.R + x.r0 + g;
+  const int s_row = x.s_base + (hkv * x.s_parts - x.p_parts) * p.d.group + g;
+  auto row_of = [&](int k) { return k < x.p_parts ? p_row + k * x.R : s_row + k * p.d.group; };
   auto ml_at = [&](int k) { return k < parts ? p.ml[row_of(k)] : make_float2(-INFINITY, 0.f); };
-  float r[U][NJ];
+  f32x4 r[U];
   auto load = [&](int k0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k0 + u < parts) {
-        const float* at = p.acc + row_of(k0 + u) * D + NJ * lane;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) r[u][j] = at[j];
-      }
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * G + sub;
+      r[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (k0 + u * G < parts && k < parts) r[u] = *(const f32x4*)(p.acc + (int64_t)row_of(k) * D + 4 * c);
+    }
   };
   const float2 e0 = ml_at(lane);
   load(0);
@@ -694,10 +693,9 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
 #pragma unroll
   for (int off = 32; off; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
   const float base = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, w = 0.f, a[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) a[j] = 0.f;
-  for (int k0 = 0; k0 < parts; k0 += U) {
+  float l = 0.f, w = 0.f;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < parts; k0 += U * G) {
     if ((k0 & 63) == 0) {
       const float2 e = k0 ? ml_at(k0 + lane) : e0;
       w = fast_exp2(e.x - base);
@@ -706,17 +704,21 @@ __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
     if (k0) load(k0);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (k0 + u < parts) {
-        const float wu = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (k0 + u) & 63));
+      if (k0 + u * G < parts) {
+        const float wu = __shfl(w, (k0 + u * G + sub) & 63);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) a[j] = fmaf(r[u][j], wu, a[j]);
+        for (int i = 0; i < 4; ++i) a[i] = fmaf(r[u][i], wu, a[i]);
       }
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) l += __shfl_xor(l, off);
-  B* o = (B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh;
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) o[NJ * lane + j] = from_f32<T>(l == 0.f ? 0.f : a[j] / l);
+  for (int off = LPR; off < 64; off <<= 1)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] += __shfl_xor(a[i], off);
+  if (sub) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store4<T>((B*)p.o + b * p.o_sb + (int64_t)hq * p.o_sh + 4 * c, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv, p.vec_out);
 }
 
 template <typename T, int D>
