@@ -657,10 +657,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
   else wide_item<T, D>(p, it, smem);
 }
 
-// A wave a query head of a sequence: the states of its items, shared ones first, several at a time side by side in the wave, 16 bytes a
-// lane.  Every load that goes by the plan alone, of up to 32 states (16 at d_k 128), is on its way before the first is waited for.  (A join by the last of a sequence's items to end, in the same launch: the shared keys' last item joins a whole
-// tile's rows, one after the other; 64 sequences behind 8192 positions took 57 us for 25 + 5.8, 16 beams 14.7 for 6.4 + 4.9, which is 6.3 + 3.5
-// since states are read side by side.)
+// A wave a query head of a sequence: the states of its items, shared ones first, 4 (d_k 128: 2) at a time side by side in the wave, 16
+// bytes a lane (17 states of 64 features: 3.6 us, one by one 4.9).  Every load that goes by the plan alone, of up to 32 states (16), is
+// on its way before the first is waited for; twice as many at d_k 128 took the registers of half the waves (256 sequences, 7.0 us for
+// 5.4).  (A join by the last of a sequence's items to end, in the same launch: the shared keys' last item joins a whole tile's rows,
+// one after the other; 64 sequences behind 8192 positions took 57 us for 25 + 5.8, 16 beams 14.7 for 6.4 + 4.9.)
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void shared_join_kernel(SharedParams p) {
   using B = typename T::bits;
