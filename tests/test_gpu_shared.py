@@ -213,7 +213,7 @@ def test_starts_that_go_back():
     c.run()
 
 
-@pytest.mark.parametrize("batch,n_groups", [(6, 1500), (1, 1), (300, 2), (1030, 1)])
+@pytest.mark.parametrize("batch,n_groups", [(6, 1500), (1, 1), (300, 2), (130, 3), (500, 40), (513, 2), (1030, 1)])
 def test_more_groups_than_a_workgroup_plans_at_once(batch, n_groups):
     """Groups without members among those with some; a thread a group, and more groups or sequences than threads."""
     rng = np.random.default_rng(23)

@@ -146,7 +146,8 @@ __device__ __forceinline__ Item group_item(const PlanParams& p, const Group* gro
 
 // As many sequences and groups as threads at most, a thread each of either: what the threads need of one another is in LDS.  Few
 // waves where they do: a step of the plan is a barrier more than anything (16 sequences, 6.4 us with 16 waves, 5.6
-// with 4, 4.9 since three of its scans share no sums and wait for nobody's reads).
+// with 4, 4.9 since three of its scans share no sums and wait for nobody's reads).  Items are many waves' work: 256 sequences of 8 KV
+// heads, 4 / 8 / 16 waves 9.2 / 8.5 / 9.6 us.
 template <int W>
 __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   constexpr int kThreads = 64 * W;
@@ -789,7 +790,8 @@ int tl_shared_plan(const int32_t* cache_lens, int len_add, const int32_t* member
   p.check = p.d.check(p.cap, esize, d_k);
   hipStream_t st = tl_resolve_stream(stream);
   const int most = batch > n_groups ? batch : n_groups;
-  if (most <= 256) hipLaunchKernelGGL(plan_one_kernel<4>, dim3(1), dim3(256), 0, st, p);
+  if (most <= 128) hipLaunchKernelGGL(plan_one_kernel<4>, dim3(1), dim3(256), 0, st, p);
+  else if (most <= 512) hipLaunchKernelGGL(plan_one_kernel<8>, dim3(1), dim3(512), 0, st, p);
   else if (most <= 1024) hipLaunchKernelGGL(plan_one_kernel<16>, dim3(1), dim3(1024), 0, st, p);
   else hipLaunchKernelGGL(plan_many_kernel, dim3(1), dim3(kScanThreads), 0, st, p);
   return tl_launch_status();
