@@ -223,6 +223,19 @@ def test_more_groups_than_a_workgroup_plans_at_once(batch, n_groups):
     Case("float16", 2, 1, 64, 16, 40 + rng.integers(0, 20, batch), groups).run()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D,Hq,Hkv,batch,shared", [(64, 6, 2, 130, 48), (128, 20, 10, 60, 37), (64, 28, 7, 90, 16), (128, 40, 2, 150, 0), (64, 3, 3, 1100, 21),
+                                                   (64, 66, 2, 140, 16)])
+def test_many_short_sequences(dtype, D, Hq, Hkv, batch, shared):
+    """Own parts of one tile and fewer, of two now and then, in such numbers that they fill the device."""
+    rng = np.random.default_rng(26)
+    lens = shared + rng.integers(0, 17, batch)
+    lens[::9] += rng.integers(14, 60, lens[::9].size)
+    def edit(table, n_pages):
+        table[3::7, -1] = -1
+    Case(dtype, Hq, Hkv, D, 16, lens, [(rng.permutation(batch).tolist(), shared)], edit=edit).run()
+
+
 @pytest.mark.parametrize("batch", [5, 1100])
 def test_lengths_below_zero(batch):
     """Sequences of no positions, as a padded batch's: zeros, and no part in what the others share."""

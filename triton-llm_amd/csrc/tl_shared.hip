@@ -37,6 +37,7 @@ struct Item {
   int b, hkv, lo, hi;
   int i0, row0, R, out;  // out: the first row's place in the workspace, -1: the rows go to o, as these are all their keys
 };
+constexpr int kFour = -2;  // i0: of sequence b, rows 0 .. R of KV heads hkv .. hkv + 3, a wave each
 // Where the results of a sequence's heads are: of head hkv * group + g, the shared keys' at p_base + (hkv * p_parts + k) * R +
 // r0 + g and its own ones' at s_base + (hkv * s_parts + k) * group + g.
 struct Join {
@@ -86,6 +87,7 @@ struct PlanParams {
   char* plan;
   PlanDims d;
   int len_add, cap, bn;
+  int fours;  // one item for four KV heads is possible
   uint32_t check;
 };
 
@@ -98,15 +100,23 @@ __device__ __forceinline__ int share_of(int64_t work, int slots) {
   if (work < 1 << 30) return max((int)((unsigned)(work + slots - 1) / (unsigned)slots), kMinTiles);
   return (int)min(max((work + slots - 1) / slots, (int64_t)kMinTiles), (int64_t)1 << 30);
 }
+// Sequences of one own tile: an item for four KV heads where an item a head would be half a round of the device.  195 sequences of 11 to 16
+// own positions, 24 / 8 heads of 128, bf16, 22.9 -> 20.3 us a layer; 120 of up to 60, 15 / 5 heads of 64, fp16, 15.1 -> 14.9; but 64
+// of up to 500 behind 8192, of which eight have one tile, 32.2 -> 32.8.
+__device__ __forceinline__ bool by_fours(const PlanParams& p, int64_t ones) { return p.fours && 2 * ones * p.d.n_kv >= p.d.slots; }
 // A sequence's own positions lo .. len - 1: t tiles in `parts` parts a KV head, items `at` on, whose rows are `base` on in the
 // workspace (-1: o).
 struct Own {
   int b, lo, len, t;
-  int parts, base, at, spare;
+  int parts, base, at, four;
 };
 // Its items of KV head h.
 __device__ __forceinline__ void own_items(const PlanParams& p, Item* items, const Own& x, int h) {
   const int lo16 = x.lo & ~(kBlk - 1);
+  if (x.four) {
+    if (h % 4 == 0) items[x.at + h / 4] = Item{x.b, h, x.lo, x.len, kFour, 0, p.d.group, x.base < 0 ? -1 : x.base + h * p.d.group};
+    return;
+  }
   const int each = x.parts ? x.t / x.parts : 0, more = x.parts ? x.t - each * x.parts : 0;
   int t0 = 0;
   for (int k = 0; k < x.parts; ++k) {
@@ -155,7 +165,7 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
       s_len[kThreads];
   __shared__ Group s_group[kThreads];
   __shared__ Own s_own[kThreads];
-  __shared__ int s_in[1][W], s_work[3][W], s_places[4][W], s_bucket[64];
+  __shared__ int s_in[1][W], s_work[4][W], s_places[4][W], s_bucket[64];
   const PlanDims& d = p.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = tid < d.batch ? p.members[tid] : -1;
@@ -203,12 +213,12 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   // work in 64 bits: the tiles' upper and lower halves
   auto own_tiles = [&] { return listed ? tiles_of(shares ? shared : 0, len, p.bn) : 0; };
   const int64_t both = (int64_t)row_tiles * gr.tiles + own_tiles();
-  int w[3] = {(int)(both & 0xFFFF), (int)(both >> 16), gr.R / d.group}, work[3];
+  int w[4] = {(int)(both & 0xFFFF), (int)(both >> 16), gr.R / d.group, own_tiles() == 1}, work[4];
   block_scan<true>(w, work, s_work);
   if (work[2] > d.batch) {  // starts that go back: groups overlap, and nobody shares
     shares = false;
     gr = Group{};
-    w[0] = own_tiles() & 0xFFFF, w[1] = own_tiles() >> 16, w[2] = 0;
+    w[0] = own_tiles() & 0xFFFF, w[1] = own_tiles() >> 16, w[2] = 0, w[3] = own_tiles() == 1;
     block_scan(w, work, s_work);
   }
   const int share = share_of((((int64_t)work[1] << 16) + work[0]) * d.n_kv, d.slots);
@@ -216,7 +226,8 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   const int t = own_tiles(), parts = (t + share - 1) / share;
   const bool direct = !shares && parts == 1;
   const int gi = d.n_kv * gr.parts * ((gr.R + kBM - 1) / kBM), gn = d.n_kv * gr.parts * gr.R;
-  const int oi = d.n_kv * parts, on = direct ? 0 : oi * d.group;
+  const bool four = t == 1 && by_fours(p, work[3]);
+  const int oi = four ? (d.n_kv + 3) / 4 : d.n_kv * parts, on = direct ? 0 : d.n_kv * parts * d.group;
   int x[4] = {gi, gn, oi, on}, total[4];
   block_scan<true>(x, total, s_places);
   gr.item = x[0] - gi;
@@ -226,7 +237,7 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   // ones (64 sequences of 1 to 500 own positions, 24 / 8 heads of 128, bf16: 27.9 -> 24.7 us).  Among equals whoever comes first.
   int own_at = x[2] - oi;
   if (total[0] + total[2] > d.slots) {
-    const int bucket = parts ? 63 - min(63, (int)((int64_t)(t / parts) * 64 / share)) : 0;
+    const int bucket = parts ? 63 - min(63, (int)((int64_t)(four ? 4 : t / parts) * 64 / share)) : 0;
     if (oi) atomicAdd(&s_bucket[bucket], oi);
     __syncthreads();
     if (wave == 0) {
@@ -246,7 +257,7 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
     const int base = total[1] + x[3] - on;
     const Group& of = s_group[g];
     joins[b] = shares ? Join{of.R, of.row, of.parts, place * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
-    s_own[tid] = Own{b, shares ? shared : 0, len, t, parts, direct ? -1 : base, total[0] + own_at, 0};
+    s_own[tid] = Own{b, shares ? shared : 0, len, t, parts, direct ? -1 : base, total[0] + own_at, four};
   } else {
     s_own[tid] = Own{0, 0, 0, 0, 0, 0, 0, 0};
   }
@@ -345,9 +356,12 @@ __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
     const int j = before[i] - groups[m.g].i0;
     return j >= 0 && j < groups[m.g].R / d.group ? j : -1;
   };
+  int64_t ones = 0;
   for (int i0 = 0; i0 < d.batch; i0 += kScanThreads) {
     const Member m = member(i0 + tid);
-    work += block_scan(m.b >= 0 ? tiles_of(place(m, i0 + tid) >= 0 ? m.shared : 0, m.len, p.bn) : 0, sums).total;
+    const int t = m.b >= 0 ? tiles_of(place(m, i0 + tid) >= 0 ? m.shared : 0, m.len, p.bn) : 0;
+    work += block_scan(t, sums).total;
+    ones += block_scan(t == 1, sums).total;
   }
   const int share = share_of(work * d.n_kv, d.slots);
   int64_t item = 0, row = 0;
@@ -377,13 +391,14 @@ __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
     const int j = m.b >= 0 ? place(m, i0 + tid) : -1;
     const int lo = j >= 0 ? m.shared : 0, t = m.b >= 0 ? tiles_of(lo, m.len, p.bn) : 0, parts = (t + share - 1) / share;
     const bool direct = j < 0 && parts == 1;
-    const int oi = d.n_kv * parts, on = direct ? 0 : oi * d.group;
+    const bool four = t == 1 && by_fours(p, ones);
+    const int oi = four ? (d.n_kv + 3) / 4 : d.n_kv * parts, on = direct ? 0 : d.n_kv * parts * d.group;
     const Scan si = block_scan(oi, sums), sn = block_scan(on, sums);
     if (m.b >= 0) {
       const int base = (int)(row + sn.incl - on);
       const Group& of = groups[m.g];
       joins[m.b] = j >= 0 ? Join{of.R, of.row, of.parts, j * d.group, base, parts, 0, 0} : Join{0, 0, 0, 0, base, parts, direct, 0};
-      const Own x{m.b, lo, m.len, t, parts, direct ? -1 : base, (int)(item + si.incl) - oi, 0};
+      const Own x{m.b, lo, m.len, t, parts, direct ? -1 : base, (int)(item + si.incl) - oi, four};
       for (int h = 0; h < d.n_kv; ++h) own_items(p, items, x, h);
     }
     item += si.total;
@@ -466,6 +481,57 @@ __device__ __forceinline__ void narrow_item(const SharedParams& p, const Item& i
       const int64_t at = it.out + r;
       if (c == 0) p.ml[at] = make_float2(m, l);
       *(f32x4*)(p.acc + at * D + 4 * c) = a;
+    }
+  }
+}
+
+// One key tile of a sequence's own, a wave a KV head: no join, and a fourth of the workgroups.
+template <typename T, int D, int NRB>
+__device__ __forceinline__ void four_item(const SharedParams& p, const Item& it, char* smem) {
+  using N = Narrow<T, D>;
+  using B = typename T::bits;
+  constexpr int NB = lds_bytes<T, D>() / (8 * kBlk * D * T::size);
+  const int lane = threadIdx.x & 63, wave = uni((int)threadIdx.x >> 6);
+  const int lr = lane & 15, g = lane >> 4;
+  const int hkv = it.hkv + wave;
+  if (hkv >= p.d.n_kv) return;
+  const int b0 = it.lo >> kBlkShift;
+  NarrowKeys k{p.pm, it.b, (const char*)((const B*)p.k + hkv * p.k_sh), (const char*)((const B*)p.v + hkv * p.v_sh),
+               p.k_sp * T::size, p.v_sp * T::size, (uint32_t)(p.k_sr * T::size), (uint32_t)(p.v_sr * T::size), it.hi,
+               ((it.hi + kBlk - 1) >> kBlkShift) - b0};
+  auto pos_of = [&](int t) { return (b0 + t) << kBlkShift; };
+  const int pages = narrow_pages(k, 0, pos_of);
+  typename N::Q q[NRB];
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const int r = 16 * rb + lr;
+    const bool there = r < it.R;
+    N::load_q(q[rb], (const char*)((const B*)p.q + it.b * p.q_sb + (hkv * p.d.group + (there ? r : 0)) * p.q_sh),
+              there && p.scale_log2 != 0.f, g, p.scale_log2 < 0.f ? 0x80000000u : 0u);
+  }
+  NarrowState<D, NRB> st;
+  auto whole = [&](int pos) { return pos >= it.lo && pos + kBlk <= it.hi; };
+  auto seen = [&](int key, int) { return key >= it.lo && key < it.hi; };
+  const float scale = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  narrow_stream<T, D, NRB, NB>(st, q, k, pages, smem, wave, lane, scale, true, pos_of, whole, seen);
+#pragma unroll
+  for (int rb = 0; rb < NRB; ++rb) {
+    const float l = tlp::sum_xor32(sum_xor16(st.l[rb]));
+    const int r = 16 * rb + lr;
+    if (r >= it.R) continue;
+    if (it.out < 0) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      B* out = (B*)p.o + it.b * p.o_sb + (int64_t)(hkv * p.d.group + r) * p.o_sh + 4 * g;
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) {
+        const f32x4 a = st.o[rb][db];
+        store4<T>(out + 16 * db, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv, p.vec_out);
+      }
+    } else {
+      const int64_t at = it.out + wave * p.d.group + r;
+      if (g == 0) p.ml[at] = make_float2(st.m[rb] - Tile<T, D>::kLift, l);
+#pragma unroll
+      for (int db = 0; db < D / 16; ++db) *(f32x4*)(p.acc + at * D + 16 * db + 4 * g) = st.o[rb][db];
     }
   }
 }
@@ -653,6 +719,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_kernel(SharedParams p) {
   const Item it = ((const Item*)(p.plan + p.d.items_at()))[blockIdx.x];  // the grid is no larger than the room for them
   if (head.check != p.check || (int)blockIdx.x >= head.n_items) return;
   const int rows = it.R - it.row0;
+  if (it.i0 == kFour) {
+    if (rows <= 16) four_item<T, D, 1>(p, it, smem);
+    else four_item<T, D, 2>(p, it, smem);
+    return;
+  }
   if (rows <= 16) narrow_item<T, D, 1>(p, it, smem, s_ml);
   else if (rows <= 32) narrow_item<T, D, 2>(p, it, smem, s_ml);
   else wide_item<T, D>(p, it, smem);
@@ -787,6 +858,7 @@ int tl_shared_plan(const int32_t* cache_lens, int len_add, const int32_t* member
   p.cap = (int)cap;
   const int esize = dtype == TL_DTYPE_F32 ? 4 : 2;
   p.bn = esize == 4 ? tile_keys<F32>() : tile_keys<BF16>();
+  p.fours = n_kv_head > 1 && p.d.group <= 32;
   p.check = p.d.check(p.cap, esize, d_k);
   hipStream_t st = tl_resolve_stream(stream);
   const int most = batch > n_groups ? batch : n_groups;
