@@ -292,11 +292,11 @@ class PagedKVCache:
     roundings); it goes without a window.
     """
 
-    # Shared positions from which one read for all is faster than one each.  us a layer, each / once, 2 sequences and 32: 15 / 5 heads of
-    # 64, fp16, 256 positions 9.3 / 10.0 (8 sequences) and 9.2 / 10.2, 1024 12.5 / 10.2 (8) and 16.1 / 11.1; 24 / 8 heads of 128, bf16,
-    # 512 10.6 / 10.0 (2), 256 10.6 / 13.5, 1024 15.4 / 12.2 (8) and 21.9 / 15.0; 9 / 3 heads of 64, fp32, 512 9.5 / 10.0 (2),
-    # 1024 12.3 / 12.2 (8) and 17.7 / 15.0.
-    SHARE_LEAST = 1024
+    # Shared positions from which one read for all is faster than one each.  us a layer of eight, each / once: 2, 8, 32 sequences behind 256
+    # of 15 / 5 heads of 64, fp16, 7.2 / 9.1, 9.2 / 9.4, 9.1 / 9.9, behind 512 9.1 / 8.9, 10.7 / 9.5, 11.4 / 10.1; 24 / 8 heads of 128, bf16,
+    # 9.7 / 9.3, 10.6 / 10.9, 10.8 / 12.9, and 10.4 / 9.6, 13.8 / 11.2, 17.9 / 13.3; 9 / 3 heads of 64, fp32, 8.9 / 8.6, 9.2 / 9.8,
+    # 10.6 / 12.8, and 9.4 / 8.9, 10.0 / 10.0, 13.1 / 13.1.
+    SHARE_LEAST = 512
 
     def __init__(self, n_layer: int, n_head: int, n_kv_head: int, d_k: int, *, n_pages: int, max_batch: int,
                  max_seq: int, page_size: int = 16, window: int = 0, sinks: int = 0, dtype=np.float32,
