@@ -26,7 +26,7 @@ import ctypes
 import numpy as np
 
 from triton_llm import gpu
-from triton_llm.kernels.paged import (allocate_kv_pages, check_page_size, check_window, copy_kv_pages,
+from triton_llm.kernels.paged import (_same_output, allocate_kv_pages, check_page_size, check_window, copy_kv_pages,
                                       paged_attention_decode, paged_attention_prefill, paged_decode_workspace,
                                       paged_kv_append, write_i32)
 from triton_llm.kernels.shared import paged_attention_shared, plan_shared_attention, shared_workspace_bytes
@@ -54,6 +54,12 @@ def _alike(a: list[int], b: list[int], most: int) -> int:
         if a[lo:hi] != b[lo:hi]:
             return next((i for i in range(lo, hi) if i >= len(a) or i >= len(b) or a[i] != b[i]), hi)
     return most
+
+
+def _overlap(a, b) -> bool:
+    """Whether two device tensors have a byte in common."""
+    at, to = a.data_ptr(), b.data_ptr()
+    return at < to + b.nbytes and to < at + a.nbytes
 
 
 class PageTables:
@@ -464,7 +470,8 @@ class PagedKVCache:
         n_kv_head, d_k)`` in the cache's dtype, n_new at least the step's largest count; a slot's tokens are the first
         of its rows.  q is rotated in place.  cos/sin as in ``paged_kv_append``, of at least as many rows as the
         longest sequence has tokens.  Returns the attention output, like q; the rows that are no tokens
-        hold nothing of meaning.  A slot that rests costs nothing: its pages are not read.
+        hold nothing of meaning.  A slot that rests costs nothing: its pages are not read.  ``out`` overlaps neither the
+        pools nor, but in place of it in a one-token step, q; such a step reads the slots' pages each, also with ``share_reads``.
         """
         t = self.tables
         if not 0 <= layer < self.n_layer:
@@ -480,9 +487,17 @@ class PagedKVCache:
         if cos_dev is not None and self._longest > cos_dev.shape[0]:
             raise ValueError(f"{self._longest} positions exceed the cos/sin table size ({cos_dev.shape[0]})")
         pool = self.layers[layer]
+        in_place = False
+        if out is not None:  # refused before q is turned and the pages are written, so that the step can go on
+            _same_output(out, q_dev)
+            if _overlap(out, pool["k"]) or _overlap(out, pool["v"]):
+                raise ValueError("out lies over the layer's pages")
+            in_place = _overlap(out, q_dev)
+            if in_place and (n_new > 1 or out.data_ptr() != q_dev.data_ptr()):
+                raise ValueError("out lies over q: only a one-token step's may, and only in place of it")
         paged_kv_append(q_dev, k_dev, v_dev, pool["k"], pool["v"], self._table, self._lens, cos_dev, sin_dev,
                         new_lens=self._new, interleaved=interleaved)
-        if n_new == 1 and self._shares:
+        if n_new == 1 and self._shares and not in_place:  # items of one launch read q after others have written out
             return paged_attention_shared(q_dev, pool["k"], pool["v"], self._table, self._plan, self.n_head, self.n_kv_head,
                                           sm_scale=sm_scale, out=out, workspace=self._shared_ws)
         if n_new == 1:
