@@ -548,7 +548,9 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * batch entries, those outside [0, batch) name no sequence.  Sequence b sees L = cache_lens[b] + len_add positions (at
  * least 0, at most max_pages * page_size); its first shared_lens[g] ones lie in the same pages for every sequence of the group
  * (any number of them, whole pages or not).  The caller promises that: only the first sequence's entries of the
- * table are read.  A sequence with L < shared_lens[g], or the only one of its group, is taken as one that shares nothing.  One
+ * table are read.  A sequence with L < shared_lens[g], or the only one of its group, is taken as one that shares nothing.
+ * group_starts ascend, within [0, batch] (others count as the nearer end); where one lies below the one before it groups would overlap:
+ * then nobody shares, and the sequences are those from members[group_starts[0]] to members[group_starts[n_groups] - 1].  One
  * that is in no group keeps its row of o; one that sees nothing gets zeros.  One that is named twice counts where it
  * is named last.
  *

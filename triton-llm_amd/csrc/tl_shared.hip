@@ -165,7 +165,7 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
       s_len[kThreads];
   __shared__ Group s_group[kThreads];
   __shared__ Own s_own[kThreads];
-  __shared__ int s_in[1][W], s_work[4][W], s_places[4][W], s_bucket[64];
+  __shared__ int s_in[1][W], s_work[3][W], s_places[4][W], s_bucket[64], s_back;
   const PlanDims& d = p.d;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = tid < d.batch ? p.members[tid] : -1;
@@ -175,7 +175,10 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
     s_start[tid] = min(max(p.starts[tid], 0), d.batch);
     s_shared[tid] = min(max(p.shared[tid], 0), p.cap);
   }
-  if (tid == 0) s_start[d.n_groups] = min(max(p.starts[d.n_groups], 0), d.batch);
+  if (tid == 0) {
+    s_start[d.n_groups] = min(max(p.starts[d.n_groups], 0), d.batch);
+    s_back = 0;
+  }
   if (tid < d.batch) {
     const int64_t n = (int64_t)p.lens[tid] + p.len_add;
     s_len[tid] = (int)(n < 0 ? 0 : n > p.cap ? p.cap : n);
@@ -185,13 +188,15 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
   int g = 0;
   bool listed = (unsigned)b < (unsigned)d.batch && tid >= s_start[0] && tid < s_start[d.n_groups];
   if (listed) atomicMax(&s_named[b], tid);
+  if (tid < d.n_groups && s_start[tid + 1] < s_start[tid]) s_back = 1;
   for (int hi = d.n_groups; hi - g > 1;) {
     const int mid = (g + hi) >> 1;
     if (s_start[mid] <= tid) g = mid;
     else hi = mid;
   }
-  const int shared = s_shared[g], len = listed ? s_len[b] : 0;
+  const int len = listed ? s_len[b] : 0;
   __syncthreads();
+  const int shared = s_back ? 0 : s_shared[g];  // starts that go back: groups overlap, and nobody shares
   listed = listed && s_named[b] == tid;  // a sequence named twice is its last place's
   const bool in = listed && shared > 0 && len >= shared;
   int n_in[1] = {in ? 1 : 0}, all_in[1];
@@ -209,24 +214,18 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
     gr = Group{s_shared[tid], s_before[s_start[tid]], sharing(tid) * d.group, tiles_of(0, s_shared[tid], p.bn), 0, 0, 0, 0};
   const int row_tiles = (gr.R + kBM - 1) / kBM;
   const int peers = sharing(g), place = s_before[tid < d.batch ? tid : 0] - s_before[s_start[g]];
-  bool shares = in && peers >= 2 && place >= 0 && place < peers;
+  const bool shares = in && peers >= 2;
   // work in 64 bits: the tiles' upper and lower halves
-  auto own_tiles = [&] { return listed ? tiles_of(shares ? shared : 0, len, p.bn) : 0; };
-  const int64_t both = (int64_t)row_tiles * gr.tiles + own_tiles();
-  int w[4] = {(int)(both & 0xFFFF), (int)(both >> 16), gr.R / d.group, own_tiles() == 1}, work[4];
+  const int t = listed ? tiles_of(shares ? shared : 0, len, p.bn) : 0;
+  const int64_t both = (int64_t)row_tiles * gr.tiles + t;
+  int w[3] = {(int)(both & 0xFFFF), (int)(both >> 16), t == 1}, work[3];
   block_scan<true>(w, work, s_work);
-  if (work[2] > d.batch) {  // starts that go back: groups overlap, and nobody shares
-    shares = false;
-    gr = Group{};
-    w[0] = own_tiles() & 0xFFFF, w[1] = own_tiles() >> 16, w[2] = 0, w[3] = own_tiles() == 1;
-    block_scan(w, work, s_work);
-  }
   const int share = share_of((((int64_t)work[1] << 16) + work[0]) * d.n_kv, d.slots);
   gr.parts = gr.R ? (gr.tiles + share - 1) / share : 0;
-  const int t = own_tiles(), parts = (t + share - 1) / share;
+  const int parts = (t + share - 1) / share;
   const bool direct = !shares && parts == 1;
   const int gi = d.n_kv * gr.parts * ((gr.R + kBM - 1) / kBM), gn = d.n_kv * gr.parts * gr.R;
-  const bool four = t == 1 && by_fours(p, work[3]);
+  const bool four = t == 1 && by_fours(p, work[2]);
   const int oi = four ? (d.n_kv + 3) / 4 : d.n_kv * parts, on = direct ? 0 : d.n_kv * parts * d.group;
   int x[4] = {gi, gn, oi, on}, total[4];
   block_scan<true>(x, total, s_places);
@@ -269,6 +268,7 @@ __global__ __launch_bounds__(64 * W) void plan_one_kernel(PlanParams p) {
 // Any number of them, 1024 at a time, with what the threads need of one another in the plan itself.
 __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
   __shared__ int64_t sums[kScanWaves];
+  __shared__ int s_back;
   const PlanDims& d = p.d;
   Item* const items = (Item*)(p.plan + d.items_at());
   Join* const joins = (Join*)(p.plan + d.joins_at());
@@ -297,13 +297,16 @@ __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
     m.b = b;
     const int64_t len = (int64_t)p.lens[b] + p.len_add;
     m.len = (int)(len < 0 ? 0 : len > p.cap ? p.cap : len);
-    const int sh = min(max(p.shared[lo], 0), p.cap);
+    const int sh = s_back ? 0 : min(max(p.shared[lo], 0), p.cap);
     m.shared = m.len >= sh ? sh : 0;
     return m;
   };
 
   for (int b = tid; b < d.batch; b += kScanThreads) named[b] = -1;
+  if (tid == 0) s_back = 0;
   __syncthreads();
+  for (int g = tid; g < d.n_groups; g += kScanThreads)
+    if (start_of(g + 1) < start_of(g)) s_back = 1;  // starts that go back: groups overlap, and nobody shares
   for (int i = tid; i < d.batch; i += kScanThreads) {
     const int b = p.members[i];
     if (i >= start_of(0) && i < start_of(d.n_groups) && (unsigned)b < (unsigned)d.batch) atomicMax(&named[b], i);
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
   if (tid == 0) before[d.batch] = (int)n;
   __syncthreads();
   // the groups' key tiles, and where their items and results begin
-  int64_t work = 0, rows = 0;
+  int64_t work = 0;
   for (int g0 = 0; g0 < d.n_groups; g0 += kScanThreads) {
     const int g = g0 + tid;
     int64_t w = 0;
@@ -343,18 +346,11 @@ __global__ __launch_bounds__(kScanThreads) void plan_many_kernel(PlanParams p) {
       groups[g] = x;
     }
     work += block_scan(w, sums).total;
-    rows += block_scan(x.R, sums).total;
-  }
-  if (rows > (int64_t)d.batch * d.group) {  // starts that go back: groups overlap, and nobody shares
-    for (int g = tid; g < d.n_groups; g += kScanThreads) groups[g].R = groups[g].tiles = 0;
-    work = 0;
   }
   __syncthreads();
   // place of a sequence among its group's that share, -1: it shares nothing
   auto place = [&](const Member& m, int i) {
-    if (m.shared <= 0 || groups[m.g].R == 0) return -1;
-    const int j = before[i] - groups[m.g].i0;
-    return j >= 0 && j < groups[m.g].R / d.group ? j : -1;
+    return m.shared <= 0 || groups[m.g].R == 0 ? -1 : before[i] - groups[m.g].i0;
   };
   int64_t ones = 0;
   for (int i0 = 0; i0 < d.batch; i0 += kScanThreads) {

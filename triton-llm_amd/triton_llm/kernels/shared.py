@@ -59,7 +59,7 @@ def plan_shared_attention(page_table, cache_lens, members, group_starts, shared_
     page_table: int32 ``(batch, max_pages)``; cache_lens and members: int32 ``(batch,)``; group_starts: int32 ``(n_groups + 1,)``;
     shared_lens: int32 ``(n_groups,)``, all on the device.  Sequence b sees ``cache_lens[b] + len_add`` positions.  A member outside ``[0,
     batch)`` is none; a sequence in no group is not computed, one that is named twice counts where it is named last.  One that is shorter than ``shared_lens[g]``, or the only one
-    of its group, shares nothing.  The plan holds for every layer, for as long as lengths, groups and table stay.  ``plan``: an
+    of its group, shares nothing, and nobody does where a group's start lies below the one before it.  The plan holds for every layer, for as long as lengths, groups and table stay.  ``plan``: an
     earlier plan, which is written over if its sizes fit (it may be in use by calls issued before).
     """
     if not (page_table.dtype.char == cache_lens.dtype.char == members.dtype.char == group_starts.dtype.char
