@@ -561,8 +561,7 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * in time need one each.  o overlaps none of q and the pools.
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; batch and n_groups <= 65535, n_head / n_kv_head <= 128, max_pages *
  * page_size <= 2^30.  Hidden positions are not read.
- * With 16-bit types the weights of keys that more than 32 query rows of a KV head share (sequences times n_head / n_kv_head) are
- * rounded to the type for the product with V, as for tl_paged_attention_prefill; others are not.
+ * No weight is rounded to a 16-bit type.
  * Deterministic.
  * ------------------------------------------------------------------------- */
 size_t tl_shared_plan_bytes(int batch, int n_groups, int n_head, int n_kv_head, int d_k);

@@ -665,7 +665,9 @@ __device__ __forceinline__ void wide_item(const SharedParams& p, const Item& it,
         if (!TL::kSumMfma) l += s[mb][r];
       }
     __builtin_amdgcn_s_setprio(1);
-    TL::values(o, la, s, kt + TILEB, lane);
+    // whole weights, as paged_attention_decode has them: these items wait for memory more than for the products (64 sequences behind
+    // 8192 positions 67.4 -> 70.0 us for two layers and their plan, 256 behind 8 prefixes 242.9 -> 242.5)
+    TL::template values<true>(o, la, s, kt + TILEB, lane);
     __builtin_amdgcn_s_setprio(0);
   };
 

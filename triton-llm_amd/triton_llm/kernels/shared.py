@@ -98,8 +98,8 @@ def paged_attention_shared(q_dev, k_pages, v_pages, page_table, plan: SharedPlan
                            sm_scale: float | None = None, out=None, workspace=None):
     """One query per sequence, ``(batch, n_head, d_k)``, over its pages, by a plan of the step.
 
-    Results are those of ``paged_attention_decode`` without a window, to rounding (in 16 bits the weights of keys that more than 32 query rows of a KV head share are rounded to the type, as in
-    ``paged_attention_prefill``).  A sequence that sees nothing gives zeros; the rows of sequences in no group are left
+    Results are those of ``paged_attention_decode`` without a window, to the rounding of sums in
+    32 bits.  A sequence that sees nothing gives zeros; the rows of sequences in no group are left
     as they were.  ``out`` overlaps no input.
     """
     if not _is_int32(page_table):

@@ -294,8 +294,8 @@ class PagedKVCache:
     ``layers[i]`` is ``{"k": DeviceTensor, "v": DeviceTensor}``, each
     ``(n_pages, n_kv_head, page_size, d_k)``.  With ``window`` > 0 a token sees the last ``window``
     positions up to its own and the first ``sinks``.  With ``share_reads`` a step of one token a slot reads the pages that
-    slots begin with in common once for all of them, where that is at least ``SHARE_LEAST`` positions (results then differ by
-    roundings); it goes without a window.
+    slots begin with in common once for all of them, where that is at least ``SHARE_LEAST`` positions (results then differ by the
+    order of sums in 32 bits); it goes without a window.
     """
 
     # Shared positions from which one read for all is faster than one each.  us a layer of eight, each / once: 2, 8, 32 sequences behind 256
