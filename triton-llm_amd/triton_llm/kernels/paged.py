@@ -388,6 +388,7 @@ def _packed_plan(pool, v_pool, table, lens, starts, q, n_head, n_kv_head, max_ne
         raise ValueError(f"q shape {q} is not (rows, n_head={n_head}, d_k={d_k})")
     if max_new < 0:
         raise ValueError(f"max_new must be >= 0, got {max_new}")
+    max_new = min(max_new, q[0])  # no sequence has more rows than there are; a C int holds it
     p_str = _lib.strides(n_kv * page_size * d_k, page_size * d_k, d_k)
     q_str = _lib.strides(n_head * d_k, d_k)
     ws = [_lib.load().tl_paged_packed_workspace_bytes(None, q[0], batch, n_head, n_kv_head, max_new, max_pages * page_size,
@@ -401,8 +402,8 @@ def paged_attention_packed(q_dev, k_pages, v_pages, page_table, cache_lens, star
     """:func:`paged_attention_prefill` for packed rows: query i of sequence b is row ``starts[b] + i`` of q ``(rows, n_head,
     d_k)``, at position ``cache_lens[b] + i``.
 
-    ``starts``: int32 ``(batch + 1,)`` on the device.  ``max_new``: the most rows that a sequence may have; rows behind them,
-    and rows of no sequence, are left as they were.  ``host_new_lens`` as there: the sequences' rows, where the host has them.
+    ``starts``: int32 ``(batch + 1,)`` on the device.  ``max_new``: the most rows that a sequence may have (any number from q's rows on
+    sets no bound); rows behind them, and rows of no sequence, are left as they were.  ``host_new_lens`` as there: the sequences' rows, where the host has them.
     """
     _check_int32(page_table, cache_lens, starts)
     pages, sizes, ws_bytes = _packed_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape, starts.shape,
@@ -416,7 +417,7 @@ def paged_attention_packed(q_dev, k_pages, v_pages, page_table, cache_lens, star
         host_new_lens = _host_counts(host_new_lens, sizes[0])
         # the plan without the counts has its room too: a captured call goes by that
         need = max(need, _lib.load().tl_paged_packed_workspace_bytes(
-            host_new_lens, sizes[1], sizes[0], n_head, n_kv_head, max_new, pages[0] * pages[2], sizes[5], window, sinks, code))
+            host_new_lens, sizes[1], sizes[0], n_head, n_kv_head, sizes[2], pages[0] * pages[2], sizes[5], window, sinks, code))
     ws = scratch(need, workspace, key="window")
     if sm_scale is None:
         sm_scale = default_scale(k_pages.shape[3])
