@@ -70,6 +70,8 @@ def plan_shared_attention(page_table, cache_lens, members, group_starts, shared_
                 raise ValueError(f"{name} must be int32, got {gpu.dtype_name(t.dtype)} {t.shape}")
     sizes, need = _plan_sizes(page_table.shape, cache_lens.shape, members.shape, group_starts.shape, shared_lens.shape, n_head,
                               n_kv_head, d_k, page_size, _BF16 if dtype is gpu.bfloat16 else gpu.dtype_code(dtype))
+    if not -(1 << 31) <= len_add < 1 << 31:
+        raise ValueError(f"len_add must fit in int32, got {len_add}")
     if plan is None or plan.sizes != sizes or plan.buffer.nbytes < need:
         plan = SharedPlan(sizes, need)
     launch(gpu.runtime().tl_shared_plan, cache_lens.ptr, int(len_add), members.ptr, group_starts.ptr, shared_lens.ptr, sizes[0],
