@@ -490,7 +490,7 @@ int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
  * new pages are written to its row of the table.  For row t < max_tokens of the packed batch slots[t] = page * page_size + row in
  * page and positions[t] its position, or -1 and -1 for rows of sequences not granted and behind the last; a page number
  * outside [0, n_pages) on the stack gives slot -1 and table entry -1.  starts (batch + 1):
- * the first row of each sequence, at most max_tokens; ends[b]: lens[b] and what was granted.  counts_out: pages
+ * the first row of each sequence, at most max_tokens, granted or not; ends[b]: lens[b] and what was granted.  counts_out: pages
  * left on the stack, and how many sequences with new tokens were not granted.  counts_out may be counts; otherwise no
  * output overlaps an input or another.
  * Its workspace (tl_pages_workspace_bytes, 16-byte aligned) needs no initialisation; calls that overlap in time need one
@@ -504,7 +504,9 @@ int tl_write_i32(int32_t* dst, int64_t dst_count, const int32_t* host_index,
  *
  * tl_paged_attention_packed: tl_paged_attention_prefill_counted for packed rows: query i of sequence b is row starts[b] + i of
  * q / o (n_rows, n_head, d_k) {row, head}, at position cache_lens[b] + i.  max_new: the most rows of a
- * sequence; those behind are left as they were, as are rows of no sequence.  Workspace: tl_paged_packed_workspace_bytes (with n_rows
+ * sequence; those behind are left as they were, as are rows of no sequence.  Rows of a sequence that tl_assign_pages did not grant are
+ * rows of one here (its starts name them), over positions that were not written and what its row of the table still names: they
+ * hold nothing of meaning.  Workspace: tl_paged_packed_workspace_bytes (with n_rows
  * = 0 what tl_paged_prefill_workspace_bytes gives).  host_new_lens as there, and with the same promise.  Weights are rounded to a
  * 16-bit type as there, but for sequences of at most 32 query rows a KV head, as single tokens are.
  * ------------------------------------------------------------------------- */

@@ -404,6 +404,11 @@ def paged_attention_packed(q_dev, k_pages, v_pages, page_table, cache_lens, star
 
     ``starts``: int32 ``(batch + 1,)`` on the device.  ``max_new``: the most rows that a sequence may have (any number from q's rows on
     sets no bound); rows behind them, and rows of no sequence, are left as they were.  ``host_new_lens`` as there: the sequences' rows, where the host has them.
+    Rows of a sequence that :func:`assign_kv_pages` did not grant its pages come out without meaning: drop them.
+
+    Whether keys are divided, and how many workgroups start, goes by ``max_new`` and the rows of q, before the lengths are looked at: q
+    of no more rows than a step may have, and a ``max_new`` near the longest sequence's, are faster (32 sequences with 742 rows, 24 / 8
+    heads of 128, bf16: 74 us; in a q of 2048 rows 90, with max_new 2048 too 100; of 4096 rows 89 and 114).
     """
     _check_int32(page_table, cache_lens, starts)
     pages, sizes, ws_bytes = _packed_plan(k_pages.shape, v_pages.shape, page_table.shape, cache_lens.shape, starts.shape,

@@ -116,7 +116,9 @@ def assign_kv_pages(cache_lens, new_lens, page_table, free_pages, counts, page_s
     needs none), its tokens fit in its row of the table and its rows below ``max_tokens``.  New pages are written to
     the rows of ``page_table``.  ``slots`` and ``positions`` ``(max_tokens,)``: ``page * page_size + row`` and the position of every row of
     the packed batch, -1 for rows of a sequence that was not granted and behind the last; ``starts`` ``(batch + 1,)``: each
-    sequence's first row; ``ends`` ``(batch,)``: ``cache_lens`` and what was granted.  ``counts_out`` (default: ``counts`` itself):
+    sequence's first row, also of one that was not granted: :func:`~triton_llm.kernels.paged_attention_packed` goes by ``starts``
+    alone, so what it leaves in rows of slot -1 holds nothing of meaning (their keys were not written, and a row of ``page_table`` that was released
+    still names pages that others may hold) and is to be dropped.  ``ends`` ``(batch,)``: ``cache_lens`` and what was granted.  ``counts_out`` (default: ``counts`` itself):
     pages left, and the sequences with new tokens that were not granted.  ``out``: the four tensors, which
     overlap no input.
     """
