@@ -550,7 +550,8 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * batch entries, those outside [0, batch) name no sequence.  Sequence b sees L = cache_lens[b] + len_add positions (at
  * least 0, at most max_pages * page_size); its first shared_lens[g] ones lie in the same pages for every sequence of the group
  * (any number of them, whole pages or not).  The caller promises that: only the first sequence's entries of the
- * table are read.  A sequence with L < shared_lens[g], or the only one of its group, is taken as one that shares nothing.
+ * table are read, but for a block of 16 positions that shared_lens[g] ends inside, which is read through each sequence's own entry too (its
+ * shared rows with weight zero: a NaN there shows).  A sequence with L < shared_lens[g], or the only one of its group, is taken as one that shares nothing.
  * group_starts ascend, within [0, batch] (others count as the nearer end); where one lies below the one before it groups would overlap:
  * then nobody shares, and the sequences are those from members[group_starts[0]] to members[group_starts[n_groups] - 1].  One
  * that is in no group keeps its row of o; one that sees nothing gets zeros.  One that is named twice counts where it
@@ -563,7 +564,7 @@ int tl_paged_attention_packed(const void* q, const void* k_pages, const void* v_
  * in time need one each.  o overlaps none of q and the pools.
  * d_k 64 or 128, rows of q, k and v 16-byte aligned; batch and n_groups <= 65535, n_head / n_kv_head <= 128, max_pages *
  * page_size <= 2^30.  Hidden positions are not read.
- * No weight is rounded to a 16-bit type.
+ * No weight is rounded to a 16-bit type; as its two words are multiplied one by one, an infinity in V makes NaN of its feature.
  * Deterministic.
  * ------------------------------------------------------------------------- */
 size_t tl_shared_plan_bytes(int batch, int n_groups, int n_head, int n_kv_head, int d_k);

@@ -54,7 +54,7 @@ def plan_shared_attention(page_table, cache_lens, members, group_starts, shared_
                           page_size: int, dtype, len_add: int = 0, plan: SharedPlan | None = None) -> SharedPlan:
     """The plan of a step: group g is the sequences ``members[group_starts[g] : group_starts[g + 1]]``, whose first
     ``shared_lens[g]`` positions lie in the same pages (any number of positions; only the first sequence's entries of the
-    table are read for them).
+    table are read for whole blocks of 16 of them).
 
     page_table: int32 ``(batch, max_pages)``; cache_lens and members: int32 ``(batch,)``; group_starts: int32 ``(n_groups + 1,)``;
     shared_lens: int32 ``(n_groups,)``, all on the device.  Sequence b sees ``cache_lens[b] + len_add`` positions.  A member outside ``[0,
