@@ -300,12 +300,13 @@ class PagedKVCache:
     in common with it, and groups inside a group are not looked for.
     """
 
-    # Shared positions from which one read for all is faster than one each.  us a layer of eight, each / once: 2, 8, 32 sequences behind 256
-    # of 15 / 5 heads of 64, fp16, 7.2 / 9.1, 9.2 / 9.4, 9.1 / 9.9, behind 512 9.1 / 8.9, 10.7 / 9.5, 11.4 / 10.1; 24 / 8 heads of 128, bf16,
-    # 9.7 / 9.3, 10.6 / 10.9, 10.8 / 12.9, and 10.4 / 9.6, 13.8 / 11.2, 17.9 / 13.3; 9 / 3 heads of 64, fp32, 8.9 / 8.6, 9.2 / 9.8,
-    # 10.6 / 12.8, and 9.4 / 8.9, 10.0 / 10.0, 13.1 / 13.1.  One group that is long enough is reason for all slots: two of 64 behind 512, the
-    # others of 4000 positions of their own, 24 / 8 heads of 128, bf16, four layers, append and plan in it, 182 / 158, of 400 37 / 30, of 20
-    # 17.0 / 18.2; two of 8, the others of 4000, 34 / 27.5, of 100 14.4 / 18.0.
+    # Shared positions from which one read for all is about as fast as one each, and beyond which it is the faster.  us a layer of eight, the
+    # plan in it, up to 60 own positions, each / once: 2, 8, 32 sequences behind 256 of 15 / 5 heads of 64, fp16, 6.5 / 10.2, 7.9 / 10.4,
+    # 7.9 / 10.4, behind 512 9.1 / 10.2, 10.7 / 9.9, 10.2 / 10.6; 24 / 8 heads of 128, bf16, 9.5 / 9.8, 9.3 / 10.9, 9.6 / 12.6, and 10.1 / 9.8,
+    # 12.2 / 11.1, 16.6 / 13.1; 9 / 3 heads of 64, fp32, 8.9 / 10.1, 9.4 / 10.2, 9.2 / 12.8, and 9.4 / 10.1, 10.1 / 10.3, 11.9 / 13.0.
+    # One group that is long enough is reason for all slots: two of 64 behind 512, the others of 4000 positions of their own, 24 / 8 heads of
+    # 128, bf16, four layers, append and plan in it, 182 / 158, of 400 37 / 30, of 20 17.0 / 18.2; two of 8, the others of 4000, 34 / 27.5,
+    # of 100 14.4 / 18.0.
     SHARE_LEAST = 512
 
     def __init__(self, n_layer: int, n_head: int, n_kv_head: int, d_k: int, *, n_pages: int, max_batch: int,
